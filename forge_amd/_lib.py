@@ -18,6 +18,8 @@ FORGE_ERANGE = -3
 
 _P = ctypes.c_void_p
 _I = ctypes.c_int
+_L = ctypes.c_longlong
+_F = ctypes.c_float
 
 # name -> (restype, argtypes); mirrors include/forge_amd.h one to one.
 SIGNATURES = {
@@ -56,6 +58,13 @@ SIGNATURES = {
     "forge_int8_conv_transpose2d_k2s2_workspace_size": (ctypes.c_size_t, [_I] * 4),
     "forge_int8_conv_transpose2d_k2s2_forward": (_I, [_P] * 5 + [_I] * 5 + [_P, _P]),
     "forge_int8_depthwise_conv2d_forward": (_I, [_P] * 5 + [_I] * 12 + [_P]),
+    "forge_quantize_weight_int4": (_I, [_P, _I, _P, _P, _I, _I, _I, _P]),
+    "forge_pack_weight_int4": (_I, [_P, _P, _I, _I, _P]),
+    "forge_int4_linear": (_I, [_P] * 5 + [_I] * 5 + [_P]),
+    "forge_qk_norm_rope": (_I, [_P] * 13 + [_L] + [_I] * 6 + [_L] * 6 + [_F, _I, _I, _P]),
+    "forge_prompt_attention": (_I, [_P] * 5 + [_I] * 5 + [_L] * 6 + [_F, _I, _I, _P]),
+    "forge_cache_attention_workspace_size": (ctypes.c_size_t, [_I] * 5 + [_L]),
+    "forge_cache_attention": (_I, [_P] * 7 + [_I] * 8 + [_F, _I, _P, ctypes.c_size_t, _P]),
 }
 
 _lib = None

@@ -51,6 +51,10 @@ SOURCES = [
     "conv_depthwise.hip",
     "linear_backward.hip",
     "noalloc.hip",
+    "int4_linear.hip",
+    "qk_norm_rope.hip",
+    "prompt_attention.hip",
+    "cache_attention.hip",
     "forge_api.cpp",
 ]
 

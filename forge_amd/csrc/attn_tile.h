@@ -1,0 +1,225 @@
+// One wave's attention over a tile of keys that lies in LDS, for FP16 and BF16.
+//
+// The wave owns 32 query rows (a second set of 32 in the cache kernel). It multiplies S^T = K Q^T on
+// 32 x 32 x 16 products: keys are the A operand's rows, queries the B operand's columns, and a lane
+// ends up with 16 of a block's 32 scores of ONE query (lane l: query l % 32; register e: key 8 (e / 4) +
+// 4 (l / 32) + e % 4). Row maxima and sums are then mostly inside a lane (one exchange with lane l ^ 32),
+// and the probabilities, rounded in pairs, are as they stand the B operand of O^T = V^T P^T: a
+// product's sum over keys may take them in any order, if V^T's operand takes the same one. That operand
+// is 4 + 4 keys of one column of V, which the transposing LDS read gathers from V's rows.
+// The running maximum m, sum l and O follow the usual recurrence, FP32; P is rounded to 16 bits for
+// its product (its sum is not). O is rescaled only when some row's maximum has grown by more than
+// 2^8 since the last time: until then P stays below 2^8, well inside both types.
+//
+// K and V tiles are rows of DP values (D padded with zeros) in 16-byte chunks, permuted in each row so that the
+// 16 rows of a K read and the 4 rows of a V read fall on different banks.
+#pragma once
+
+#include "float16_types.h"
+#include "mfma_tile.h"
+
+namespace forge_amd {
+
+constexpr float kNoScore = -1e30f;   // running maximum of a row that has seen nothing
+constexpr float kRescale = 8.0f;
+
+// s_waitcnt lgkmcnt(0) only.
+__device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+
+typedef short v4s __attribute__((ext_vector_type(4)));
+
+// Four values of one column from four rows: each lane of 16 passes the address of 4 values of row
+// (lane / 4), columns 4 (lane % 4) on; lane i receives column i of the four rows.
+__device__ __forceinline__ v2u lds_read_tr(const int8_t* p) {
+    return __builtin_bit_cast(v2u, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                       (__attribute__((address_space(3))) v4s*)p));
+}
+
+// The value of lane l ^ 32 combined with this lane's.
+__device__ __forceinline__ float half_max(float x) {
+    const v2u r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float half_sum(float x) {
+    const v2u r = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+
+// Tile rows of DP values; physical chunk = logical chunk ^ swz(row).
+template <int DP>
+struct KvRows {
+    static_assert(DP == 64 || DP == 96 || DP == 128 || DP == 256, "row lengths with a permutation");
+    static constexpr int kChunks = DP / 8, kBytes = DP * 2;
+    static __device__ __forceinline__ int swz_k(int r) {
+        return DP == 64 ? (r >> 1) & 7 : DP == 96 ? (r >> 2) & 3 : r & 15;
+    }
+    static __device__ __forceinline__ int swz_v(int r) {
+        return DP == 64 ? 2 * ((r >> 1) & 3) : DP == 96 ? 2 * ((r >> 2) & 1) : 2 * (r & 7);
+    }
+};
+
+template <class T, int DP, int RB, int KB>
+struct AttnWave {
+    using Rows = KvRows<DP>;
+    static constexpr int kSteps = DP / 16, kOut = DP / 32;
+    v4u q[RB][kSteps];
+    v16f o[RB][kOut];
+    float m[RB], l[RB];      // of query lane % 32; l: this lane's keys only
+    int lane, k_at, v_at;    // byte addresses in a tile, before the chunk permutation
+    int k_x, v_x;            // the permutations, as byte masks
+
+    __device__ __forceinline__ void init() {
+        lane = threadIdx.x & (kWave - 1);
+        const int half = lane >> 5, r = lane & 31, i = lane & 15, vr = 4 * half + i / 4;
+        k_at = r * Rows::kBytes;
+        k_x = (half ^ Rows::swz_k(r)) * 16;
+        v_at = vr * Rows::kBytes + (i & 1) * 8;
+        v_x = ((2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ Rows::swz_v(vr)) * 16;
+#pragma unroll
+        for (int b = 0; b < RB; b++) {
+            m[b] = kNoScore;
+            l[b] = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kOut; j++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) o[b][j][e] = 0.0f;
+        }
+    }
+
+    // Query row of set b; D values at p, or zeros.
+    __device__ __forceinline__ void load_q(int b, const uint16_t* p, bool live, int D) {
+#pragma unroll
+        for (int s = 0; s < kSteps; s++) {
+            const int d = 16 * s + 8 * (lane >> 5);
+            q[b][s] = live && d < D ? *reinterpret_cast<const v4u*>(p + d) : v4u{0u, 0u, 0u, 0u};
+        }
+    }
+
+    // One tile of 32 KB keys. seen(b, key in tile) says whether row b sees the key; called only if MASK.
+    template <bool MASK, class Seen>
+    __device__ __forceinline__ void step(const int8_t* ks, const int8_t* vs, float scale2, const Seen& seen) {
+        v16f s[RB][KB];
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++) {
+#pragma unroll
+            for (int b = 0; b < RB; b++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) s[b][kb][e] = 0.0f;
+#pragma unroll
+            for (int st = 0; st < kSteps; st++) {
+                const v4u k = *reinterpret_cast<const v4u*>(ks + 32 * kb * Rows::kBytes + k_at + ((32 * st) ^ k_x));
+#pragma unroll
+                for (int b = 0; b < RB; b++) s[b][kb] = T::mfma32(k, q[b][st], s[b][kb]);
+            }
+        }
+        v4u p[RB][KB][2];
+#pragma unroll
+        for (int b = 0; b < RB; b++) {
+            if constexpr (MASK) {
+#pragma unroll
+                for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++)
+                        if (!seen(b, 32 * kb + 8 * (e / 4) + 4 * (lane >> 5) + e % 4)) s[b][kb][e] = -INFINITY;
+            }
+            float mx = s[b][0][0];
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[b][kb][e]);
+            mx = half_max(mx) * scale2;
+            if (__any(mx > m[b] + kRescale)) {
+                const float mn = fmaxf(m[b], mx), f = __builtin_amdgcn_exp2f(m[b] - mn);
+                m[b] = mn;
+                l[b] *= f;
+#pragma unroll
+                for (int j = 0; j < kOut; j++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[b][j][e] *= f;
+            }
+            float sum = 0.0f;
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
+#pragma unroll
+                for (int e = 0; e < 16; e++) {
+                    s[b][kb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][kb][e], scale2, -m[b]));
+                    sum += s[b][kb][e];
+                }
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int d = 0; d < 4; d++) p[b][kb][h][d] = T::pack(s[b][kb][8 * h + 2 * d], s[b][kb][8 * h + 2 * d + 1]);
+            }
+            l[b] += sum;
+        }
+#pragma unroll
+        for (int j = 0; j < kOut; j++)
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+                    const int8_t* at = vs + (32 * kb + 16 * h) * Rows::kBytes + v_at + ((64 * j) ^ v_x);
+                    const v2u lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * Rows::kBytes);
+                    const v4u v = {lo[0], lo[1], hi[0], hi[1]};
+#pragma unroll
+                    for (int b = 0; b < RB; b++) o[b][j] = T::mfma32(v, p[b][kb][h], o[b][j]);
+                }
+    }
+
+    // Whether some value of the rows `live` is no finite number.
+    __device__ __forceinline__ bool odd(int b, bool live) const {
+        float z = 0.0f;
+#pragma unroll
+        for (int j = 0; j < kOut; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) z = __builtin_fmaf(o[b][j][e], 0.0f, z);
+        z = __builtin_fmaf(l[b], 0.0f, z);
+        return __any(live && z != 0.0f);
+    }
+};
+
+// One query row over keys [0, n) by a whole wave, key by key, reading nothing that the row does not
+// see: for rows whose tile result is not finite, as a product takes a masked key's value times zero,
+// which is NaN where that value is infinite or NaN. key(j) / value(j): the rows of key j; seen(j).
+// Returns m and l, and in acc the columns lane + 64 i.
+template <class T, int DP, class Key, class Value, class Seen>
+__device__ __forceinline__ void attn_row(const uint16_t* q, int D, int n, float scale2, const Key& key, const Value& value,
+                                         const Seen& seen, float& m, float& l, float (&acc)[(DP + 63) / 64]) {
+    const int lane = threadIdx.x & (kWave - 1);
+    auto score = [&](int j) {
+        const uint16_t* k = key(j);
+        float s = 0.0f;
+#pragma unroll 1
+        for (int d = 0; d < D; d++) s = __builtin_fmaf(T::widen(q[d]), T::widen(k[d]), s);
+        return s * scale2;
+    };
+    m = kNoScore;
+    l = 0.0f;
+#pragma unroll
+    for (int i = 0; i < (DP + 63) / 64; i++) acc[i] = 0.0f;
+#pragma unroll 1
+    for (int j0 = 0; j0 < n; j0 += kWave) {
+        const int j = j0 + lane;
+        if (j < n && seen(j)) m = fmaxf(m, score(j));
+    }
+    m = wave_max(m);
+#pragma unroll 1
+    for (int j0 = 0; j0 < n; j0 += kWave) {
+        const int j = j0 + lane;
+        const bool on = j < n && seen(j);
+        const float p = on ? __builtin_amdgcn_exp2f(score(j) - m) : 0.0f;
+        unsigned long long left = __ballot(on);
+        while (left) {
+            const int i = __builtin_ctzll(left);
+            left &= left - 1;
+            const float pj = __shfl(p, i, kWave);
+            l += pj;
+            const uint16_t* v = value(j0 + i);
+#pragma unroll
+            for (int c = 0; c < (DP + 63) / 64; c++)
+                if (lane + 64 * c < D) acc[c] = __builtin_fmaf(pj, T::widen(v[lane + 64 * c]), acc[c]);
+        }
+    }
+}
+
+}  // namespace forge_amd

@@ -1,0 +1,198 @@
+// Attention over whole prompts packed without padding: softmax(scale Q K^T) V within each sequence, causal
+// or not, with grouped heads.
+//
+// A workgroup takes 32 W query rows of one sequence and head, a wave 32 of them (attn_tile.h), and
+// walks the keys in tiles of 64 that all waves share: K and V rows come by LDS DMA into two buffers,
+// the next tile's while this one is multiplied, one barrier a tile. Tiles past the diagonal are not
+// loaded, only those that cross it are masked.
+//
+// The grid is laid out without reading cu_seqlens on the host: sequence b's tiles start at
+// cu[b] / rows + b, which leaves room for each sequence's last partial tile.
+#include "attn_tile.h"
+#include "ring_tile.h"
+
+#include <climits>
+
+namespace forge_amd {
+
+struct PromptArgs {
+    const uint16_t *q, *k, *v;
+    uint16_t* out;
+    const int32_t* cu;
+    long long q_token, q_head, k_token, k_head, v_token, v_head;
+    int sequences, tokens, Hq, Hkv, D, tiles;
+    float scale;
+};
+
+constexpr int kPromptKeys = 64;
+
+template <class T, int DP, int W, bool CAUSAL>
+__global__ __launch_bounds__(64 * W) void prompt_attention_kernel(PromptArgs a)
+{
+    using Rows = KvRows<DP>;
+    constexpr int kRows = 32 * W, kTile = kPromptKeys * Rows::kBytes;
+    constexpr int kIns = kPromptKeys * Rows::kChunks / kWave / W;   // DMA instructions per wave, tile and tensor
+    static_assert(kPromptKeys * Rows::kChunks % (kWave * W) == 0, "a tile splits evenly over the waves");
+    extern __shared__ __align__(1024) int8_t lds[];                 // K, V of buffer 0, then of buffer 1
+
+    const int group = a.Hq / a.Hkv;
+    // Query tiles from the last (the longest in a causal prompt) on; units (tile, KV head) go round
+    // the 8 XCDs, whose workgroups are dealt in turn, so that the heads of a group meet in one L2.
+    const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
+    const int unit = (i / group) * 8 + xcd, hk = unit % a.Hkv, hq = hk * group + i % group;
+    const int id = a.tiles - 1 - unit / a.Hkv;
+    if (id < 0) return;
+
+    auto cu = [&](int b) { return min(max(a.cu[b], 0), a.tokens); };
+    int b = 0;
+    for (int hi = a.sequences; b < hi;) {                           // the last b whose first tile is <= id
+        const int mid = (b + hi + 1) >> 1;
+        if (cu(mid) / kRows + mid <= id) b = mid;
+        else hi = mid - 1;
+    }
+    const int start = cu(b);
+    const int len = (b < a.sequences ? cu(b + 1) : a.tokens) - start;
+    const int row0 = (id - (start / kRows + b)) * kRows;
+    if (row0 < 0 || row0 >= len) return;
+
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int lane = threadIdx.x & (kWave - 1);
+    const int row = row0 + 32 * wave + (lane & 31);
+    uint16_t* out = a.out + (static_cast<size_t>(start + row) * a.Hq + hq) * a.D;
+    if (b == a.sequences) {                                          // rows after the last sequence
+        for (int d = 4 * (lane >> 5); d < a.D; d += 8)
+            if (row < len) *reinterpret_cast<v2u*>(out + d) = v2u{0u, 0u};
+        return;
+    }
+
+    AttnWave<T, DP, 1, kPromptKeys / 32> w;
+    w.init();
+    w.load_q(0, a.q + static_cast<size_t>(start + row) * a.q_token + hq * a.q_head, row < len, a.D);
+
+    const uint16_t* kbase = a.k + static_cast<size_t>(start) * a.k_token + hk * a.k_head;
+    const uint16_t* vbase = a.v + static_cast<size_t>(start) * a.v_token + hk * a.v_head;
+    int dma_row[kIns];
+    uint32_t koff[kIns], voff[kIns];
+#pragma unroll
+    for (int n = 0; n < kIns; n++) {
+        const int c = (wave * kIns + n) * kWave + lane, r = c / Rows::kChunks, p = c % Rows::kChunks;
+        const int ck = p ^ Rows::swz_k(r), cv = p ^ Rows::swz_v(r);
+        dma_row[n] = r;
+        koff[n] = 8 * ck < a.D ? static_cast<uint32_t>(r * a.k_token * 2 + 16 * ck) : kOutOfRange;
+        voff[n] = 8 * cv < a.D ? static_cast<uint32_t>(r * a.v_token * 2 + 16 * cv) : kOutOfRange;
+    }
+    const int end = CAUSAL ? min(row0 + kRows, len) : len;
+    const int tiles = (end + kPromptKeys - 1) / kPromptKeys;
+    auto load = [&](int t) {                                         // rows past the sequence's end read as zeros
+        const int left = len - t * kPromptKeys;
+        const auto kr = buf_rsrc(kbase + static_cast<size_t>(t) * kPromptKeys * a.k_token,
+                                 static_cast<uint32_t>((kPromptKeys - 1) * a.k_token * 2 + 2 * a.D));
+        const auto vr = buf_rsrc(vbase + static_cast<size_t>(t) * kPromptKeys * a.v_token,
+                                 static_cast<uint32_t>((kPromptKeys - 1) * a.v_token * 2 + 2 * a.D));
+        int8_t* ks = lds + (t & 1) * 2 * kTile;
+#pragma unroll
+        for (int n = 0; n < kIns; n++)
+            dma16_buf(kr, dma_row[n] < left ? koff[n] : kOutOfRange, 0, ks + (wave * kIns + n) * 1024);
+#pragma unroll
+        for (int n = 0; n < kIns; n++)
+            dma16_buf(vr, dma_row[n] < left ? voff[n] : kOutOfRange, 0, ks + kTile + (wave * kIns + n) * 1024);
+    };
+    const float scale2 = a.scale * 1.44269504f;
+    load(0);
+    for (int t = 0; t < tiles; t++) {
+        wait_vm_lgkm<0>();
+        lds_barrier();                                               // tile t is whole, tile t - 1 is read
+        if (t + 1 < tiles) load(t + 1);
+        const int8_t* ks = lds + (t & 1) * 2 * kTile;
+        const int k0 = t * kPromptKeys, first = row0 + 32 * wave;
+        if (CAUSAL && k0 > first + 31) continue;                     // wave-uniform
+        if ((CAUSAL && k0 + kPromptKeys - 1 > first) || k0 + kPromptKeys > len)
+            w.template step<true>(ks, ks + kTile, scale2,
+                                  [&](int, int j) { return k0 + j < len && (!CAUSAL || k0 + j <= row); });
+        else
+            w.template step<false>(ks, ks + kTile, scale2, [](int, int) { return true; });
+    }
+    const bool live = row < len;
+    if (w.odd(0, live)) {
+        for (int r = 0; r < 32; r++) {
+            const int rr = row0 + 32 * wave + r;
+            if (rr >= len) break;
+            float m, l, acc[(DP + 63) / 64];
+            attn_row<T, DP>(
+                a.q + static_cast<size_t>(start + rr) * a.q_token + hq * a.q_head, a.D, CAUSAL ? rr + 1 : len, scale2,
+                [&](int j) { return kbase + static_cast<size_t>(j) * a.k_token; },
+                [&](int j) { return vbase + static_cast<size_t>(j) * a.v_token; }, [](int) { return true; }, m, l, acc);
+            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+            uint16_t* o = a.out + (static_cast<size_t>(start + rr) * a.Hq + hq) * a.D;
+#pragma unroll
+            for (int c = 0; c < (DP + 63) / 64; c++)
+                if (lane + 64 * c < a.D) o[lane + 64 * c] = narrow<T>(acc[c] * inv);
+        }
+        return;
+    }
+    const float l = half_sum(w.l[0]);
+    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+    if (!live) return;
+#pragma unroll
+    for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4) {
+            const int d = 32 * j + 2 * e + 4 * (lane >> 5);
+            if (d < a.D)
+                *reinterpret_cast<v2u*>(out + d) = v2u{T::pack(w.o[0][j][e] * inv, w.o[0][j][e + 1] * inv),
+                                                       T::pack(w.o[0][j][e + 2] * inv, w.o[0][j][e + 3] * inv)};
+        }
+}
+
+template <class T, int DP, int W, bool CAUSAL>
+int launch_prompt(PromptArgs a, hipStream_t s) {
+    constexpr int kLds = 4 * kPromptKeys * KvRows<DP>::kBytes;
+    const long long tiles = a.tokens / (32 * W) + static_cast<long long>(a.sequences) + 1;
+    const long long units = tiles * a.Hkv, wgs = divupll(units, 8) * 8 * (a.Hq / a.Hkv);
+    if (units > INT_MAX - 8 || wgs > INT_MAX) return FORGE_EINVAL;
+    a.tiles = static_cast<int>(tiles);
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&prompt_attention_kernel<T, DP, W, CAUSAL>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+    if (attr != hipSuccess) return static_cast<int>(attr);
+    prompt_attention_kernel<T, DP, W, CAUSAL><<<static_cast<unsigned>(wgs), 64 * W, kLds, s>>>(a);
+    return launch_status();
+}
+
+template <class T, int DP, int W>
+int launch_prompt(const PromptArgs& a, bool causal, hipStream_t s) {
+    return causal ? launch_prompt<T, DP, W, true>(a, s) : launch_prompt<T, DP, W, false>(a, s);
+}
+
+template <class T>
+int launch_prompt(const PromptArgs& a, bool causal, hipStream_t s) {
+    if (a.D <= 64) return launch_prompt<T, 64, 4>(a, causal, s);
+    if (a.D <= 96) return launch_prompt<T, 96, 4>(a, causal, s);
+    if (a.D <= 128) return launch_prompt<T, 128, 4>(a, causal, s);
+    return launch_prompt<T, 256, 4>(a, causal, s);
+}
+
+}  // namespace forge_amd
+
+using namespace forge_amd;
+
+extern "C" int forge_prompt_attention(const uint16_t* q, const uint16_t* k, const uint16_t* v, const int32_t* cu_seqlens,
+                                      uint16_t* out, int sequences, int tokens, int Hq, int Hkv, int D,
+                                      long long q_token, long long q_head, long long k_token, long long k_head,
+                                      long long v_token, long long v_head, float scale, int causal, int dtype,
+                                      void* stream)
+{
+    if (sequences <= 0 || tokens <= 0 || Hq <= 0 || D <= 0) return FORGE_OK;
+    if (!q || !k || !v || !cu_seqlens || !out || Hkv <= 0 || Hq % Hkv != 0 || D % 8 != 0 || D > 256 ||
+        !(scale > 0.0f && scale < INFINITY) || (dtype != FORGE_FP16 && dtype != FORGE_BF16))
+        return FORGE_EINVAL;
+    for (const void* p : {static_cast<const void*>(q), static_cast<const void*>(k), static_cast<const void*>(v),
+                          static_cast<const void*>(out)})
+        if (!aligned(p, 16)) return FORGE_EINVAL;
+    // a tile's 64 rows are addressed in 32 bits
+    for (long long st : {q_token, q_head, k_token, k_head, v_token, v_head})
+        if (st < 0 || st % 8 != 0 || st > (1 << 23)) return FORGE_EINVAL;
+    const PromptArgs a{q, k, v, out, cu_seqlens, q_token, q_head, k_token, k_head, v_token, v_head,
+                       sequences, tokens, Hq, Hkv, D, 0, scale};
+    hipStream_t s = as_stream(stream);
+    return dtype == FORGE_FP16 ? launch_prompt<Fp16>(a, causal != 0, s) : launch_prompt<Bf16>(a, causal != 0, s);
+}

@@ -520,3 +520,292 @@ def prepare_sparse_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, 
     scale = torch.empty((N,), dtype=torch.float16, device=w.device)
     _call("forge_prepare_sparse_weight", _p(w), f16, _p(comp), _p(meta), _p(scale), N, K, _stream())
     return comp, meta, scale
+
+
+# ---- decoder attention (extension; include/forge_amd.h "decoder attention") -----------
+
+_DTYPE = {torch.float16: 0, torch.bfloat16: 1}   # FORGE_FP16, FORGE_BF16
+
+
+def _act_type(t: torch.Tensor, name: str) -> int:
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    code = _DTYPE.get(t.dtype)
+    if code is None:
+        raise TypeError(f"{name} must be torch.float16 or torch.bfloat16, got {t.dtype}")
+    return code
+
+
+def _need_shape(t: torch.Tensor, dtype: torch.dtype, name: str, shape: Tuple[int, ...]) -> None:
+    """A contiguous device tensor of this type and shape, 16-byte aligned."""
+    _need(t, dtype, name)
+    if t.shape != shape:
+        raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    if t.data_ptr() % 16:
+        raise ValueError(f"{name} must be 16-byte aligned")
+
+
+def _need_heads(t: torch.Tensor, dtype: torch.dtype, name: str, tokens: int) -> Tuple[int, int]:
+    """A (tokens, heads, D) device tensor whose heads are contiguous; its token and head strides, of
+    dimensions of one element too (torch gives those any)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError(f"{name} must be a torch.Tensor")
+    if t.dtype is not dtype:
+        raise TypeError(f"{name} must be {dtype}, got {t.dtype}")
+    if not t.is_cuda:
+        raise ValueError(f"{name} must be a device tensor")
+    if t.dim() != 3 or t.shape[0] != tokens:
+        raise ValueError(f"{name} must be ({tokens}, heads, D), got {tuple(t.shape)}")
+    D = t.shape[2]
+    if D % 8 or D > 256 or D == 0:
+        raise ValueError(f"{name}: a head must have a multiple of 8 values up to 256, got {D}")
+    token, head, one = t.stride()
+    token = token if tokens > 1 else 0
+    head = head if t.shape[1] > 1 else 0
+    if one != 1 or token % 8 or head % 8 or t.data_ptr() % 16:
+        raise ValueError(f"{name}: heads must be contiguous and 16-byte aligned, got strides {t.stride()}")
+    return token, head
+
+
+def _same_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
+    """Calls run on the current device's stream: every operand has to be there."""
+    dev = torch._C._cuda_getDevice()
+    for t in (first,) + others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"operands must be on the current device (cuda:{dev}), got {t.device}")
+
+
+def _softmax_scale(scale: Optional[float], D: int) -> float:
+    if scale is None:
+        return D ** -0.5
+    if not 0.0 < scale < float("inf"):
+        raise ValueError(f"scale must be positive and finite, got {scale}")
+    return scale
+
+
+def int4_row_bytes(K: int) -> int:
+    """Bytes of a row of K 4-bit weights as stored (blocks of 128 values)."""
+    return (K + 127) // 128 * 64
+
+
+def quantize_weight_int4(weight: torch.Tensor, group_size: int = 128) -> Tuple[torch.Tensor, torch.Tensor]:
+    """forge_quantize_weight_int4: a float32 or float16 weight (N, K) -> (w_int4 (N, row bytes) uint8,
+    w_scale (N, K / group_size) float16); group_size 32, 64 or 128 and K a multiple of it."""
+    f16 = _weight_arg(weight)
+    N, K = weight.shape
+    if group_size not in (32, 64, 128) or K % group_size or K == 0:
+        raise ValueError(f"group_size must be 32, 64 or 128 and divide K, got {group_size} and K = {K}")
+    _same_device(weight)
+    w_int4 = torch.empty((N, int4_row_bytes(K)), dtype=torch.uint8, device=weight.device)
+    w_scale = torch.empty((N, K // group_size), dtype=torch.float16, device=weight.device)
+    _call("forge_quantize_weight_int4", _p(weight), f16, _p(w_int4), _p(w_scale), N, K, group_size, _stream())
+    return w_int4, w_scale
+
+
+def pack_weight_int4(q: torch.Tensor) -> torch.Tensor:
+    """forge_pack_weight_int4: (N, K) int8 values -8..7 -> w_int4 (N, row bytes) uint8; K % 32 == 0."""
+    _need(q, torch.int8, "q")
+    if q.dim() != 2 or q.shape[1] % 32 or q.shape[1] == 0:
+        raise ValueError(f"q must be (N, K) with K a multiple of 32, got {tuple(q.shape)}")
+    _same_device(q)
+    N, K = q.shape
+    out = torch.empty((N, int4_row_bytes(K)), dtype=torch.uint8, device=q.device)
+    _call("forge_pack_weight_int4", _p(q), _p(out), N, K, _stream())
+    return out
+
+
+def int4_linear(x: torch.Tensor, w_int4: torch.Tensor, w_scale: torch.Tensor, bias: Optional[torch.Tensor] = None,
+                out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """forge_int4_linear: x (M, K) float16 or bfloat16 times the transpose of the 4-bit weights of
+    quantize_weight_int4 / pack_weight_int4 with their scales, plus bias (N,); `out` may be passed to reuse an (M, N) buffer."""
+    code = _act_type(x, "x")
+    if x.dim() != 2:
+        raise ValueError(f"x must be (M, K), got {tuple(x.shape)}")
+    M, K = x.shape
+    _need(x, x.dtype, "x")
+    _need(w_scale, torch.float16, "w_scale")
+    if w_scale.dim() != 2:
+        raise ValueError(f"w_scale must be (N, K / group size), got {tuple(w_scale.shape)}")
+    N, groups = w_scale.shape
+    group = K // groups if groups else 0
+    if group not in (32, 64, 128) or group * groups != K:
+        raise ValueError(f"w_scale must hold a scale per 32, 64 or 128 of K = {K} values, got {tuple(w_scale.shape)}")
+    _need_shape(w_int4, torch.uint8, "w_int4", (N, int4_row_bytes(K)))
+    if x.data_ptr() % 16:
+        raise ValueError("x must be 16-byte aligned")
+    if bias is not None:
+        _need(bias, x.dtype, "bias", N)
+    if out is None:
+        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
+    else:
+        _need(out, x.dtype, "out", M * N)
+    _same_device(x, w_int4, w_scale, bias, out)
+    _call("forge_int4_linear", _p(x), _p(w_int4), _p(w_scale), _p(bias), _p(out), M, K, N, group, code, _stream())
+    return out
+
+
+def _qk_norm_rope(q, k, v, q_weight, k_weight, cos, sin, positions, k_cache, v_cache, slots, eps, interleaved, q_out,
+                  k_out):
+    code = _act_type(q, "q")
+    dt = q.dtype
+    T = q.shape[0] if q.dim() else 0
+    q_token, q_head = _need_heads(q, dt, "q", T)
+    k_token, k_head = _need_heads(k, dt, "k", T)
+    Hq, Hkv, D = q.shape[1], k.shape[1], q.shape[2]
+    if k.shape[2] != D:
+        raise ValueError(f"q and k must have heads of one size, got {D} and {k.shape[2]}")
+    for w, name in ((q_weight, "q_weight"), (k_weight, "k_weight")):
+        if w is not None:
+            _need_shape(w, dt, name, (D,))
+    _need(cos, torch.float32, "cos")
+    _need(sin, torch.float32, "sin")
+    if cos.dim() != 2 or cos.shape != sin.shape:
+        raise ValueError(f"cos and sin must be (positions, R / 2) tables of one shape, got {tuple(cos.shape)} and "
+                         f"{tuple(sin.shape)}")
+    P, R = cos.shape[0], 2 * cos.shape[1]
+    if R % 16 or R > D:
+        raise ValueError(f"the rotated part must be a multiple of 16 up to {D} values, got {R}")
+    _need(positions, torch.int32, "positions")
+    if positions.shape != (T,):
+        raise ValueError(f"positions must have shape ({T},), got {tuple(positions.shape)}")
+    if R and not P and T:
+        raise ValueError("cos and sin hold no position")
+    _need_shape(q_out, dt, "q_out", (T, Hq, D))
+    v_token = v_head = rows = 0
+    if k_out is not None:
+        _need_shape(k_out, dt, "k_out", (T, Hkv, D))
+    else:
+        v_token, v_head = _need_heads(v, dt, "v", T)
+        if v.shape != k.shape:
+            raise ValueError(f"v must have k's shape {tuple(k.shape)}, got {tuple(v.shape)}")
+        if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4 or tuple(k_cache.shape[2:]) != (Hkv, D):
+            raise ValueError(f"k_cache must be (pages, page size, {Hkv}, {D})")
+        _need_shape(k_cache, dt, "k_cache", tuple(k_cache.shape))
+        _need_shape(v_cache, dt, "v_cache", tuple(k_cache.shape))
+        _need(slots, torch.int32, "slots")
+        if slots.shape != (T,):
+            raise ValueError(f"slots must have shape ({T},), got {tuple(slots.shape)}")
+        rows = k_cache.shape[0] * k_cache.shape[1]
+    _same_device(q, k, v, q_weight, k_weight, cos, sin, positions, k_cache, v_cache, slots, q_out, k_out)
+    _call("forge_qk_norm_rope", _p(q), _p(k), _p(v), _p(q_weight), _p(k_weight), _p(cos), _p(sin), _p(positions),
+          _p(q_out), _p(k_out), _p(k_cache), _p(v_cache), _p(slots), rows, T, Hq, Hkv, D, R, P, q_token, q_head, k_token,
+          k_head, v_token, v_head, eps, 1 if interleaved else 0, code, _stream())
+
+
+def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tensor], k_weight: Optional[torch.Tensor],
+                 cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor, eps: float = 1e-6,
+                 interleaved: bool = False, q_out: Optional[torch.Tensor] = None, k_out: Optional[torch.Tensor] = None
+                 ) -> Tuple[torch.Tensor, torch.Tensor]:
+    """forge_qk_norm_rope: RMS norm of each head of q (T, Hq, D) and k (T, Hkv, D) with its weight (D,)
+    (None: no norm), and the rotation of the first R values by row positions[t] (int32) of cos and sin (positions, R / 2).
+    q and k may be views into a larger projection output; q_out and k_out may be passed to reuse buffers."""
+    _act_type(q, "q")
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if k_out is None:
+        _act_type(k, "k")
+        k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+    _qk_norm_rope(q, k, None, q_weight, k_weight, cos, sin, positions, None, None, None, eps, interleaved, q_out, k_out)
+    return q_out, k_out
+
+
+def qk_norm_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: Optional[torch.Tensor],
+                       k_weight: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
+                       k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, eps: float = 1e-6,
+                       interleaved: bool = False, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """qk_norm_rope whose keys go straight into a paged cache (pages, page size, Hkv, D) with the values v, token t
+    into row slots[t] (int32, page * page size + offset; a slot outside the cache writes nothing). Returns the queries."""
+    _act_type(q, "q")
+    if q_out is None:
+        q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    _qk_norm_rope(q, k, v, q_weight, k_weight, cos, sin, positions, k_cache, v_cache, slots, eps, interleaved, q_out, None)
+    return q_out
+
+
+def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqlens: torch.Tensor,
+                     scale: Optional[float] = None, causal: bool = True, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """forge_prompt_attention: softmax(scale q k^T) v within each of the packed sequences of q (tokens, Hq, D)
+    and k, v (tokens, Hkv, D), sequence b being tokens cu_seqlens[b] to cu_seqlens[b + 1] - 1 (int32, the first 0). Query
+    head h reads KV head h // (Hq // Hkv). scale: 1 / sqrt(D) unless given. q, k and v may be strided views."""
+    code = _act_type(q, "q")
+    dt = q.dtype
+    T = q.shape[0] if q.dim() else 0
+    qs, ks, vs = _need_heads(q, dt, "q", T), _need_heads(k, dt, "k", T), _need_heads(v, dt, "v", T)
+    Hq, D, Hkv = q.shape[1], q.shape[2], k.shape[1]
+    if k.shape != v.shape or k.shape[2] != D:
+        raise ValueError(f"k and v must be ({T}, KV heads, {D}), got {tuple(k.shape)} and {tuple(v.shape)}")
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"query heads must be a multiple of the KV heads, got {Hq} and {Hkv}")
+    _need(cu_seqlens, torch.int32, "cu_seqlens")
+    if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
+        raise ValueError(f"cu_seqlens must hold the sequences' boundaries, got shape {tuple(cu_seqlens.shape)}")
+    scale = _softmax_scale(scale, D)
+    if out is None:
+        out = torch.empty((T, Hq, D), dtype=dt, device=q.device)
+    else:
+        _need_shape(out, dt, "out", (T, Hq, D))
+    _same_device(q, k, v, cu_seqlens, out)
+    _call("forge_prompt_attention", _p(q), _p(k), _p(v), _p(cu_seqlens), _p(out), cu_seqlens.shape[0] - 1, T, Hq, Hkv, D,
+          *qs, *ks, *vs, scale, 1 if causal else 0, code, _stream())
+    return out
+
+
+def cache_attention_workspace_size(B: int, T: int, Hq: int, Hkv: int, D: int, max_keys: int) -> int:
+    """Bytes of cache_attention's workspace; max_keys = page_table.shape[1] * page size."""
+    return _lib.load().forge_cache_attention_workspace_size(B, T, Hq, Hkv, D, max_keys)
+
+
+def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor, page_table: torch.Tensor,
+                    cache_lens: torch.Tensor, tree: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                    workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """forge_cache_attention: attention of the T (1 to 64) newest tokens of each sequence, q (B, T, Hq, D), over a
+    paged cache (pages, page size, Hkv, D) that page_table (B, width) and cache_lens (B,) (int32) describe. The new
+    tokens' keys and values are in the cache at positions cache_lens[b] on (qk_norm_rope_cache). Token t sees the
+    positions before cache_lens[b] and the new tokens whose bit is set in tree[b, t] (int64 (B, T)), or tokens 0..t
+    without a tree (T = 1: plain decode)."""
+    code = _act_type(q, "q")
+    dt = q.dtype
+    if q.dim() != 4:
+        raise ValueError(f"q must be (B, T, Hq, D), got {tuple(q.shape)}")
+    B, T, Hq, D = q.shape
+    if not 1 <= T <= 64:
+        raise ValueError(f"1 to 64 new tokens per sequence, got {T}")
+    if D % 8 or D > 256 or D == 0:
+        raise ValueError(f"a head must have a multiple of 8 values up to 256, got {D}")
+    _need_shape(q, dt, "q", (B, T, Hq, D))
+    if not isinstance(k_cache, torch.Tensor) or k_cache.dim() != 4 or k_cache.shape[3] != D:
+        raise ValueError(f"k_cache must be (pages, page size, KV heads, {D})")
+    pages, page, Hkv, _ = k_cache.shape
+    _need_shape(k_cache, dt, "k_cache", (pages, page, Hkv, D))
+    _need_shape(v_cache, dt, "v_cache", (pages, page, Hkv, D))
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"query heads must be a multiple of the KV heads, got {Hq} and {Hkv}")
+    if pages == 0 or page == 0 or page & (page - 1):
+        raise ValueError(f"the cache must hold pages of a power of two of positions, got {tuple(k_cache.shape)}")
+    _need(page_table, torch.int32, "page_table")
+    if page_table.dim() != 2 or page_table.shape[0] != B or page_table.shape[1] == 0:
+        raise ValueError(f"page_table must be ({B}, pages of the longest sequence), got {tuple(page_table.shape)}")
+    _need(cache_lens, torch.int32, "cache_lens")
+    if cache_lens.shape != (B,):
+        raise ValueError(f"cache_lens must have shape ({B},), got {tuple(cache_lens.shape)}")
+    if tree is not None:
+        _need(tree, torch.int64, "tree")
+        if tree.shape != (B, T):
+            raise ValueError(f"tree must have shape ({B}, {T}), got {tuple(tree.shape)}")
+    scale = _softmax_scale(scale, D)
+    width = page_table.shape[1]
+    size = cache_attention_workspace_size(B, T, Hq, Hkv, D, width * page)
+    if workspace is None and size:
+        workspace = torch.empty((size,), dtype=torch.uint8, device=q.device)
+    elif workspace is not None:
+        _need(workspace, torch.uint8, "workspace", size)
+        if workspace.data_ptr() % 16:
+            raise ValueError("workspace must be 16-byte aligned")
+    if out is None:
+        out = torch.empty((B, T, Hq, D), dtype=dt, device=q.device)
+    else:
+        _need_shape(out, dt, "out", (B, T, Hq, D))
+    _same_device(q, k_cache, v_cache, page_table, cache_lens, tree, workspace, out)
+    _call("forge_cache_attention", _p(q), _p(k_cache), _p(v_cache), _p(page_table), _p(cache_lens), _p(tree), _p(out), B, T,
+          Hq, Hkv, D, pages, page, width, scale, code, _p(workspace) if size else None, size, _stream())
+    return out

@@ -304,6 +304,70 @@ int forge_int8_depthwise_conv2d_forward(const uint16_t* input, const int8_t* wei
                                         int kH, int kW, int padH, int padW, int strideH,
                                         int strideW, int dilH, int dilW, void* stream);
 
+/* ---- decoder attention ----------------------------------------------------------------
+ *
+ * No counterparts in the reference's INT8 path: what a decoder runs between and beside its linear
+ * layers. Activations, queries, keys, values and caches are FP16 or BF16 (dtype); sums and softmax
+ * statistics are FP32 and results are rounded once, except for the softmax weights, which are rounded to the
+ * 16-bit type for their product with V. 16-bit tensors are 16-byte aligned, strides are in elements, not negative and
+ * multiples of 8, head sizes D are multiples of 8 up to 256. */
+#define FORGE_FP16 0
+#define FORGE_BF16 1
+
+/* 4-bit weights with one FP16 scale per `group` (32, 64 or 128) consecutive values of a row:
+ * w_scale (N, K/group), K % group == 0. w_int4: N rows of ceil(K / 128) * 64 bytes, 16-byte aligned, in blocks of
+ * 128 values (the last filled up with zeros). A block is a 4 x 4 transpose of its sixteen 32-bit words: word
+ * 4 g + j holds values 32 j + 8 g to 32 j + 8 g + 7 of the block, of these value 2 i at bits 4 i and value 2 i + 1 at
+ * bits 16 + 4 i, as q + 8 with q in -8..7.
+ * forge_quantize_weight_int4: scale = fp16(amax|w| / 7), at least the smallest positive FP16, and
+ * q = clamp(round_half_even(w / scale), -8, 7); w: (N, K) fp32, or fp16 when w_fp16 != 0.
+ * forge_pack_weight_int4: (N, K) integers (clamped to -8..7) into the same storage; K % 32 == 0. */
+int forge_quantize_weight_int4(const void* w, int w_fp16, uint8_t* w_int4, uint16_t* w_scale, int N, int K,
+                               int group, void* stream);
+int forge_pack_weight_int4(const int8_t* q, uint8_t* w_int4, int N, int K, void* stream);
+
+/* out (M,N) = x (M,K) times the weights' transpose, plus bias (N, of x's type, or NULL):
+ * sum over groups of w_scale[n,g] * (sum over the group of x q). Any M; made for the tokens of a decode
+ * step (up to 64 in one pass over the weights). */
+int forge_int4_linear(const uint16_t* x, const uint8_t* w_int4, const uint16_t* w_scale, const uint16_t* bias,
+                      uint16_t* out, int M, int K, int N, int group, int dtype, void* stream);
+
+/* Norm and rotation of the query heads (T, Hq, D) and key heads (T, Hkv, D) of T tokens. Per head
+ * y = x / sqrt(mean(x^2) + eps) * weight (D; a NULL weight: that side is not normed), then each pair
+ * (a, b) of the first R values (R % 16 == 0) turns: (a cos - b sin, b cos + a sin), with row positions[t]
+ * of the FP32 tables cos, sin (table_rows, R/2); pair i is (y[i], y[i + R/2]), or (y[2i], y[2i + 1]) when
+ * interleaved. A position outside the table gives NaN. q_out (T,Hq,D), contiguous; the keys go to k_out (T,Hkv,D)
+ * and / or, with v (T,Hkv,D) as it is, to rows slots[t] of k_cache, v_cache (cache_rows, Hkv, D); a slot
+ * outside 0..cache_rows-1 writes nothing. q_out may be q itself. */
+int forge_qk_norm_rope(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* q_weight,
+                       const uint16_t* k_weight, const float* cos, const float* sin, const int32_t* positions,
+                       uint16_t* q_out, uint16_t* k_out, uint16_t* k_cache, uint16_t* v_cache,
+                       const int32_t* slots, long long cache_rows, int T, int Hq, int Hkv, int D, int R,
+                       int table_rows, long long q_token, long long q_head, long long k_token, long long k_head,
+                       long long v_token, long long v_head, float eps, int interleaved, int dtype, void* stream);
+
+/* Attention within each of the sequences packed into q (tokens,Hq,D) and k, v (tokens,Hkv,D):
+ * sequence b is tokens cu_seqlens[b] to cu_seqlens[b+1] - 1 (sequences + 1 ascending values on the device, the first 0;
+ * values outside 0..tokens are clamped), empty ones allowed. out (tokens,Hq,D), contiguous; tokens
+ * after the last sequence are zeros. Query head h reads KV head h / (Hq / Hkv). scale > 0. */
+int forge_prompt_attention(const uint16_t* q, const uint16_t* k, const uint16_t* v, const int32_t* cu_seqlens,
+                           uint16_t* out, int sequences, int tokens, int Hq, int Hkv, int D, long long q_token,
+                           long long q_head, long long k_token, long long k_head, long long v_token,
+                           long long v_head, float scale, int causal, int dtype, void* stream);
+
+/* Attention of T (1 to 64) new tokens per sequence, q and out (B,T,Hq,D), over a paged cache:
+ * k_cache, v_cache (pages,page_size,Hkv,D), page_size a power of two; position j of sequence b is row
+ * j % page_size of page page_table[b, j / page_size] (B,table_width). The new tokens' own keys and values are in
+ * the cache already, at positions cache_lens[b] to cache_lens[b] + T - 1. Token t sees every position before
+ * cache_lens[b] and the new tokens whose bit is set in tree[b,t] (B,T), or tokens 0..t when
+ * tree is NULL; positions past the table are not seen, pages outside the cache read as zeros, and a token
+ * that sees nothing gives zeros. workspace: scratch of the size below at max_keys = table_width * page_size. */
+size_t forge_cache_attention_workspace_size(int B, int T, int Hq, int Hkv, int D, long long max_keys);
+int forge_cache_attention(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
+                          const int32_t* page_table, const int32_t* cache_lens, const int64_t* tree, uint16_t* out,
+                          int B, int T, int Hq, int Hkv, int D, int pages, int page_size, int table_width,
+                          float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
