@@ -23,8 +23,29 @@ namespace forge_amd {
 constexpr float kNoScore = -1e30f;   // running maximum of a row that has seen nothing
 constexpr float kRescale = 8.0f;
 
-// s_waitcnt lgkmcnt(0) only.
-__device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+// LDS DMA of 16 bytes a lane to lds + 16 * lane, as in mfma_tile.h but written out: the compiler makes
+// every transposing LDS read wait for all DMAs that it knows of, which would end the prefetch of the next
+// tile at the first read of V. Nothing is returned in registers; the callers wait by count (wait_vmcnt). M0 has
+// no other use in these kernels.
+__device__ __forceinline__ uint32_t lds_address(const int8_t* p) {
+    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const int8_t*)p));
+}
+__device__ __forceinline__ void dma16_rows(v4i rsrc, uint32_t voff, uint32_t lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds) : "memory");
+#endif
+}
+__device__ __forceinline__ void dma16_at(const void* p, uint32_t lds) {
+#if defined(__HIP_DEVICE_COMPILE__)
+    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory");
+#endif
+}
+// A raw buffer resource over `bytes` from p, both wave-uniform.
+__device__ __forceinline__ v4i row_rsrc(const void* p, uint32_t bytes) {
+    const uint64_t a = reinterpret_cast<uint64_t>(p);
+    return v4i{__builtin_amdgcn_readfirstlane(static_cast<int>(a)),
+               __builtin_amdgcn_readfirstlane(static_cast<int>(a >> 32) & 0xFFFF), static_cast<int>(bytes), 0x00020000};
+}
 
 typedef short v4s __attribute__((ext_vector_type(4)));
 
@@ -57,6 +78,11 @@ struct KvRows {
         return DP == 64 ? 2 * ((r >> 1) & 3) : DP == 96 ? 2 * ((r >> 2) & 1) : 2 * (r & 7);
     }
 };
+
+// Bits 0 to last.
+__device__ __forceinline__ uint32_t bits_to(int last) {
+    return last >= 31 ? ~0u : last < 0 ? 0u : (2u << last) - 1u;
+}
 
 template <class T, int DP, int RB, int KB>
 struct AttnWave {
@@ -95,9 +121,10 @@ struct AttnWave {
         }
     }
 
-    // One tile of 32 KB keys. seen(b, key in tile) says whether row b sees the key; called only if MASK.
-    template <bool MASK, class Seen>
-    __device__ __forceinline__ void step(const int8_t* ks, const int8_t* vs, float scale2, const Seen& seen) {
+    // One tile of 32 KB keys. If `mask` (uniform), seen(b, kb) has a bit for each key of block kb that this lane's
+    // row of set b sees.
+    template <class Seen>
+    __device__ __forceinline__ void step(const int8_t* ks, const int8_t* vs, float scale2, bool mask, const Seen& seen) {
         v16f s[RB][KB];
 #pragma unroll
         for (int kb = 0; kb < KB; kb++) {
@@ -115,12 +142,14 @@ struct AttnWave {
         v4u p[RB][KB][2];
 #pragma unroll
         for (int b = 0; b < RB; b++) {
-            if constexpr (MASK) {
+            if (mask) {
 #pragma unroll
-                for (int kb = 0; kb < KB; kb++)
+                for (int kb = 0; kb < KB; kb++) {
+                    const uint32_t bits = seen(b, kb) >> (4 * (lane >> 5));
 #pragma unroll
                     for (int e = 0; e < 16; e++)
-                        if (!seen(b, 32 * kb + 8 * (e / 4) + 4 * (lane >> 5) + e % 4)) s[b][kb][e] = -INFINITY;
+                        if (!(bits & (1u << (8 * (e / 4) + e % 4)))) s[b][kb][e] = -INFINITY;
+                }
             }
             float mx = s[b][0][0];
 #pragma unroll

@@ -5,11 +5,11 @@
 // the cache at cache_lens[b] + j, whose bit j is set in tree[b, t] (without a tree: j <= t). A row that
 // sees nothing gives zeros.
 //
-// Bound: reading the cache. A KV head's rows (T tokens x Hq / Hkv heads) are taken together, 32 or 64
-// to a wave, so that K and V are read once for them; the keys are split over workgroups in chunks
-// of equal length, whatever the sequence's, and in a chunk over the waves, each with tiles of 32
-// keys in two LDS buffers of its own (no barrier while it streams). The waves' results are joined in
-// LDS; the chunks' go as FP32 to the workspace and are joined by a second kernel, in chunk order.
+// Bound: reading the cache. A KV head's rows (T tokens x Hq / Hkv heads) are taken together, up to 256 in a
+// workgroup of RS x KS waves (32 rows each), so that K and V are read once for them; the keys are split
+// over workgroups in chunks of equal length, whatever the sequence's, and a chunk's tiles, which come by
+// LDS DMA into two buffers, over the KS waves of a row set. The waves' results are joined in LDS; the chunks'
+// go as FP32 to the workspace and are joined by a second kernel, in a fixed order.
 #include "attn_tile.h"
 
 #include <algorithm>
@@ -22,7 +22,7 @@ constexpr int kCacheMaxTokens = 64;
 
 struct CachePlan {
     int chunk, chunks;   // keys of a chunk; chunks of the longest sequence
-    int sets;            // 32-row sets per wave
+    int sets;            // 32-row sets of a workgroup: 1, 2, 4 or 8
 };
 
 struct CacheArgs {
@@ -43,19 +43,19 @@ __device__ __forceinline__ int cache_keys(const CacheArgs& a, int b) {
     return static_cast<int>(min(static_cast<long long>(max(a.lens[b], 0)) + a.T, cap));
 }
 
-template <class T, int DP, int RB, int W>
-__global__ __launch_bounds__(64 * W) void cache_attention_kernel(CacheArgs a)
+template <class T, int DP, int RS, int KS, int KB>
+__global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attention_kernel(CacheArgs a)
 {
     using Rows = KvRows<DP>;
-    constexpr int kKeys = 32, kTile = kKeys * Rows::kBytes, kIns = kKeys * Rows::kChunks / kWave;
-    constexpr int kWaveLds = 4 * kTile, kPitch = DP + 4;
-    static_assert(32 * RB * kPitch * 4 <= kWaveLds + 32 * RB * 16, "the waves' sums fit the tiles' LDS and its pad");
+    constexpr int W = RS * KS, kKeys = 32 * KS * KB, kTile = kKeys * Rows::kBytes;
+    constexpr int kIns = kKeys * Rows::kChunks / kWave / W, kPitch = DP + 4;
+    static_assert(kKeys * Rows::kChunks % (kWave * W) == 0, "a tile splits evenly over the waves");
     extern __shared__ __align__(1024) int8_t lds[];
     __shared__ int page_of[kCacheMaxChunk + 2];
-    __shared__ float stat_m[W][32 * RB], stat_l[W][32 * RB];
+    __shared__ float stat_m[W][32], stat_l[W][32];
     __shared__ int odd_rows;
 
-    const int group = a.Hq / a.Hkv, rows = a.T * group, sets = (rows + 32 * RB - 1) / (32 * RB);
+    const int group = a.Hq / a.Hkv, rows = a.T * group, sets = (rows + 32 * RS - 1) / (32 * RS);
     int id = blockIdx.x;
     const int hk = id % a.Hkv; id /= a.Hkv;
     const int set = id % sets; id /= sets;
@@ -66,6 +66,7 @@ __global__ __launch_bounds__(64 * W) void cache_attention_kernel(CacheArgs a)
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x & (kWave - 1);
+    const int rs = wave / KS, ks = wave % KS;
     const int page_mask = (1 << a.page_shift) - 1, page0 = key0 >> a.page_shift;
     const int last_page = (key0 + n - 1) >> a.page_shift;
     for (int p = page0 + threadIdx.x; p <= last_page; p += 64 * W) {
@@ -83,191 +84,220 @@ __global__ __launch_bounds__(64 * W) void cache_attention_kernel(CacheArgs a)
                       : static_cast<long long>((((static_cast<size_t>(pg) << a.page_shift) + ((key0 + j) & page_mask)) *
                                                 token) + static_cast<size_t>(hk) * a.D);
     };
-
-    AttnWave<T, DP, RB, 1> w;
-    w.init();
-    unsigned long long bits[RB];
-#pragma unroll
-    for (int s = 0; s < RB; s++) {
-        const int r = (set * RB + s) * 32 + (lane & 31), t = r / group, g = r - t * group;
-        const bool live = r < rows;
-        w.load_q(s, a.q + ((static_cast<size_t>(b) * a.T + t) * a.Hq + hk * group + g) * a.D, live, a.D);
-        bits[s] = !live ? 0ull
-                        : a.tree ? static_cast<unsigned long long>(a.tree[static_cast<size_t>(b) * a.T + t])
-                                 : ~0ull >> (63 - t);
-    }
-    const int open = len - key0;                                     // keys of this chunk that every row sees
-    auto sees = [&](int s, int j) {
-        const int d = j - open;
-        return j < n && (d < 0 || (bits[s] >> (d & 63)) & 1ull);
+    auto row_of = [&](auto* base, int r) {                     // of q and out
+        const int t = r / group;
+        return base + ((static_cast<size_t>(b) * a.T + t) * a.Hq + hk * group + (r - t * group)) * a.D;
+    };
+    auto drafts_of = [&](int r) {                                    // the new tokens that row r sees
+        const int t = r / group;
+        return a.tree ? static_cast<unsigned long long>(a.tree[static_cast<size_t>(b) * a.T + t]) : ~0ull >> (63 - t);
     };
 
-    int8_t* mine = lds + wave * kWaveLds;
-    auto load = [&](int t, int buf) {
+    AttnWave<T, DP, 1, KB> w;
+    w.init();
+    const int row = (set * RS + rs) * 32 + (lane & 31);
+    const bool live = row < rows;
+    w.load_q(0, row_of(a.q, row), live, a.D);
+    const unsigned long long drafts = live ? drafts_of(row) : 0ull;
+    const int open = len - key0;                                     // keys of this chunk that every row sees
+
+    int dma_row[kIns];
+    int ck[kIns], cv[kIns];
+#pragma unroll
+    for (int i = 0; i < kIns; i++) {
+        const int c = (wave * kIns + i) * kWave + lane, p = c % Rows::kChunks;
+        dma_row[i] = c / Rows::kChunks;
+        ck[i] = 8 * (p ^ Rows::swz_k(dma_row[i]));
+        cv[i] = 8 * (p ^ Rows::swz_v(dma_row[i]));
+    }
+    const uint32_t lds0 = lds_address(lds);
+    auto load = [&](int t) {
+        const uint32_t to = lds0 + (t & 1) * 2 * kTile + wave * kIns * 1024;
+        const uint16_t* zero = reinterpret_cast<const uint16_t*>(kZeroRow);
 #pragma unroll
         for (int i = 0; i < kIns; i++) {
-            const int c = i * kWave + lane, r = c / Rows::kChunks, p = c % Rows::kChunks;
-            const int j = t * kKeys + r;
+            const int j = t * kKeys + dma_row[i];
             const long long at = j < n ? row_at(j) : -1LL;
-            const int ck = p ^ Rows::swz_k(r), cv = p ^ Rows::swz_v(r);
-            const int8_t* zero = reinterpret_cast<const int8_t*>(kZeroRow);
-            const int8_t* ks = at >= 0 && 8 * ck < a.D ? reinterpret_cast<const int8_t*>(a.k + at + 8 * ck) : zero;
-            const int8_t* vs = at >= 0 && 8 * cv < a.D ? reinterpret_cast<const int8_t*>(a.v + at + 8 * cv) : zero;
-            dma16(ks, mine + buf * 2 * kTile + i * 1024);
-            dma16(vs, mine + buf * 2 * kTile + kTile + i * 1024);
+            dma16_at(at >= 0 && ck[i] < a.D ? a.k + at + ck[i] : zero, to + i * 1024);
+            dma16_at(at >= 0 && cv[i] < a.D ? a.v + at + cv[i] : zero, to + kTile + i * 1024);
         }
     };
     const float scale2 = a.scale * 1.44269504f;
     const int tiles = (n + kKeys - 1) / kKeys;
-    if (wave < tiles) load(wave, 0);
-    int buf = 0;
-    for (int t = wave; t < tiles; t += W, buf ^= 1) {
-        // the reads of the buffer that the next tile goes to are complete
-        wait_lgkm0();
-        compiler_fence();
-        if (t + W < tiles) {
-            load(t + W, buf ^ 1);
-            wait_vmcnt<2 * kIns>();
-        } else {
-            wait_vmcnt<0>();
-        }
-        compiler_fence();
-        const int8_t* ks = mine + buf * 2 * kTile;
-        const int k0 = t * kKeys;
-        if (k0 + kKeys > open || k0 + kKeys > n)
-            w.template step<true>(ks, ks + kTile, scale2, [&](int s, int j) { return sees(s, k0 + j); });
-        else
-            w.template step<false>(ks, ks + kTile, scale2, [](int, int) { return true; });
+    load(0);
+    for (int t = 0; t < tiles; t++) {
+        wait_vm_lgkm<0>();
+        lds_barrier();                                               // tile t is whole, tile t - 1 is read
+        if (t + 1 < tiles) load(t + 1);
+        const int k0 = t * kKeys + 32 * KB * ks;                     // this wave's keys of the tile
+        const int8_t* at = lds + (t & 1) * 2 * kTile + 32 * KB * ks * Rows::kBytes;
+        w.step(at, at + kTile, scale2, k0 + 32 * KB > min(open, n), [&](int, int kb) {
+            const int d = open - (k0 + 32 * kb);                     // bits below d: the cache; from d on: drafts
+            uint32_t bits = bits_to(d - 1);
+            if (d < 32) bits |= d >= 0 ? static_cast<uint32_t>(drafts << d) : d > -64 ? static_cast<uint32_t>(drafts >> -d) : 0u;
+            return bits & bits_to(n - 1 - (k0 + 32 * kb));
+        });
     }
 
-    // ---- join the waves, in wave order
+    // ---- join the waves of a row set, in wave order
+    wait_vm_lgkm<0>();
     __syncthreads();
+    if (w.odd(0, live) && lane == 0) atomicOr(&odd_rows, 1);
     float* sums = reinterpret_cast<float*>(lds);
-#pragma unroll
-    for (int s = 0; s < RB; s++) {
-        const int r = 32 * s + (lane & 31);
-        if (w.odd(s, (set * RB + s) * 32 + (lane & 31) < rows) && lane == 0) atomicOr(&odd_rows, 1);
-        const float l = half_sum(w.l[s]);
+    if constexpr (KS > 1) {
+        const float l = half_sum(w.l[0]);
         if (lane < 32) {
-            stat_m[wave][r] = w.m[s];
-            stat_l[wave][r] = l;
+            stat_m[wave][lane] = w.m[0];
+            stat_l[wave][lane] = l;
         }
 #pragma unroll
         for (int j = 0; j < DP / 32; j++)
 #pragma unroll
             for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<v4f*>(sums + (wave * 32 * RB + r) * kPitch + 32 * j + 2 * e + 4 * (lane >> 5)) =
-                    v4f{w.o[s][j][e], w.o[s][j][e + 1], w.o[s][j][e + 2], w.o[s][j][e + 3]};
+                *reinterpret_cast<v4f*>(sums + (wave * 32 + (lane & 31)) * kPitch + 32 * j + 2 * e + 4 * (lane >> 5)) =
+                    v4f{w.o[0][j][e], w.o[0][j][e + 1], w.o[0][j][e + 2], w.o[0][j][e + 3]};
     }
     __syncthreads();
     const bool whole = keys <= a.chunk;                              // the only chunk: the result itself
-    const size_t part0 = (static_cast<size_t>(b) * a.Hkv + hk) * a.chunks + chunk;
-    auto out_row = [&](int r) {
-        const int t = r / group;
-        return a.out + ((static_cast<size_t>(b) * a.T + t) * a.Hq + hk * group + (r - t * group)) * a.D;
+    const size_t part0 = ((static_cast<size_t>(b) * a.Hkv + hk) * a.chunks + chunk) * rows;
+    auto put = [&](int r, int d, v4f s, float m, float l) {
+        if (whole) {
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            *reinterpret_cast<v2u*>(row_of(a.out, r) + d) = v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
+        } else {
+            *reinterpret_cast<v4f*>(a.part + (part0 + r) * a.D + d) = s;
+            if (d == 0) {
+                a.stat[(part0 + r) * 2] = m;
+                a.stat[(part0 + r) * 2 + 1] = l;
+            }
+        }
     };
     if (odd_rows) {
         // some row's sum is not finite: every row again, key by key
-        for (int i = wave; i < 32 * RB; i += W) {
-            const int r = set * RB * 32 + i;
+        for (int i = wave; i < 32 * RS; i += W) {
+            const int r = set * RS * 32 + i;
             if (r >= rows) break;
-            const int t = r / group;
-            const unsigned long long rb = a.tree ? static_cast<unsigned long long>(a.tree[static_cast<size_t>(b) * a.T + t])
-                                                 : ~0ull >> (63 - t);
+            const unsigned long long rb = drafts_of(r);
             float m, l, acc[(DP + 63) / 64];
             auto at = [&](const uint16_t* base, int j) {
                 const long long o = row_at(j);
                 return o < 0 ? reinterpret_cast<const uint16_t*>(kZeroRow) : base + o;
             };
             attn_row<T, DP>(
-                a.q + ((static_cast<size_t>(b) * a.T + t) * a.Hq + hk * group + (r - t * group)) * a.D, a.D, n, scale2,
-                [&](int j) { return at(a.k, j); }, [&](int j) { return at(a.v, j); },
+                row_of(a.q, r), a.D, n, scale2, [&](int j) { return at(a.k, j); }, [&](int j) { return at(a.v, j); },
                 [&](int j) {
                     const int d = j - open;
                     return d < 0 || ((rb >> (d & 63)) & 1ull);
                 },
                 m, l, acc);
+            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+#pragma unroll
             for (int c = 0; c < (DP + 63) / 64; c++) {
                 const int d = lane + 64 * c;
                 if (d >= a.D) break;
-                if (whole) out_row(r)[d] = narrow<T>(acc[c] * (l != 0.0f ? 1.0f / l : 0.0f));
-                else a.part[(part0 * rows + r) * a.D + d] = acc[c];
+                if (whole) row_of(a.out, r)[d] = narrow<T>(acc[c] * inv);
+                else a.part[(part0 + r) * a.D + d] = acc[c];
             }
             if (!whole && lane == 0) {
-                a.stat[(part0 * rows + r) * 2] = m;
-                a.stat[(part0 * rows + r) * 2 + 1] = l;
+                a.stat[(part0 + r) * 2] = m;
+                a.stat[(part0 + r) * 2 + 1] = l;
             }
         }
         return;
     }
-    const int quads = a.D / 4;
-    for (int i = threadIdx.x; i < 32 * RB * quads; i += 64 * W) {
-        const int lr = i / quads, d = 4 * (i - lr * quads), r = set * RB * 32 + lr;
-        if (r >= rows) break;
-        float m = kNoScore, l = 0.0f;
+    if constexpr (KS > 1) {
+        const int quads = a.D / 4;
+        for (int i = threadIdx.x; i < 32 * RS * quads; i += 64 * W) {
+            const int lr = i / quads, d = 4 * (i - lr * quads), r = set * RS * 32 + lr;
+            if (r >= rows) break;
+            const int w0 = (lr / 32) * KS, x = lr % 32;
+            float m = kNoScore, l = 0.0f;
 #pragma unroll
-        for (int v = 0; v < W; v++) m = fmaxf(m, stat_m[v][lr]);
-        v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
+            for (int v = 0; v < KS; v++) m = fmaxf(m, stat_m[w0 + v][x]);
+            v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int v = 0; v < W; v++) {
-            const float f = __builtin_amdgcn_exp2f(stat_m[v][lr] - m);
-            l = __builtin_fmaf(f, stat_l[v][lr], l);
-            const v4f x = *reinterpret_cast<const v4f*>(sums + (v * 32 * RB + lr) * kPitch + d);
+            for (int v = 0; v < KS; v++) {
+                const float f = __builtin_amdgcn_exp2f(stat_m[w0 + v][x] - m);
+                l = __builtin_fmaf(f, stat_l[w0 + v][x], l);
+                const v4f y = *reinterpret_cast<const v4f*>(sums + ((w0 + v) * 32 + x) * kPitch + d);
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[e] = __builtin_fmaf(f, x[e], s[e]);
-        }
-        if (whole) {
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            *reinterpret_cast<v2u*>(out_row(r) + d) = v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
-        } else {
-            *reinterpret_cast<v4f*>(a.part + (part0 * rows + r) * a.D + d) = s;
-            if (d == 0) {
-                a.stat[(part0 * rows + r) * 2] = m;
-                a.stat[(part0 * rows + r) * 2 + 1] = l;
+                for (int e = 0; e < 4; e++) s[e] = __builtin_fmaf(f, y[e], s[e]);
             }
+            put(r, d, s, m, l);
         }
+    } else {
+        const float l = half_sum(w.l[0]);
+#pragma unroll
+        for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int d = 32 * j + 2 * e + 4 * (lane >> 5);
+                if (live && d < a.D)
+                    put(row, d, v4f{w.o[0][j][e], w.o[0][j][e + 1], w.o[0][j][e + 2], w.o[0][j][e + 3]}, w.m[0], l);
+            }
     }
 }
 
-// A wave joins one row's chunks.
-template <class T>
+// A wave joins one row's chunks: LPR lanes of 4 values take every (64 / LPR)-th chunk, four in flight.
+template <class T, int LPR>
 __global__ __launch_bounds__(256) void cache_join_kernel(CacheArgs a)
 {
-    const int lane = threadIdx.x & (kWave - 1);
+    constexpr int kSets = kWave / LPR;
+    const int lane = threadIdx.x & (kWave - 1), sub = lane / LPR, d = 4 * (lane % LPR);
     const long long id = static_cast<long long>(blockIdx.x) * 4 + threadIdx.x / kWave;
     const int group = a.Hq / a.Hkv, rows = a.T * group;
     if (id >= static_cast<long long>(a.B) * a.T * a.Hq) return;
     const int h = static_cast<int>(id % a.Hq), t = static_cast<int>(id / a.Hq % a.T);
     const int b = static_cast<int>(id / (static_cast<long long>(a.Hq) * a.T));
-    const int keys = cache_keys(a, b);
-    if (keys <= a.chunk && keys > 0) return;
-    const int used = (keys + a.chunk - 1) / a.chunk, hk = h / group, r = t * group + h - hk * group;
+    const int keys = cache_keys(a, b), used = (keys + a.chunk - 1) / a.chunk;
+    if (used <= 1) return;                                           // the only chunk has written the result
+    const int hk = h / group, r = t * group + h - hk * group;
     const size_t first = (static_cast<size_t>(b) * a.Hkv + hk) * a.chunks;
+    auto at = [&](int c) { return (first + c) * rows + r; };
     float m = kNoScore;
-    for (int c = 0; c < used; c++) m = fmaxf(m, a.stat[((first + c) * rows + r) * 2]);
+    for (int c = lane; c < used; c += kWave) m = fmaxf(m, a.stat[at(c) * 2]);
+    m = wave_max(m);
     float l = 0.0f, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
-    const bool in = 4 * lane < a.D;
-    for (int c = 0; c < used; c++) {
-        const size_t at = (first + c) * rows + r;
-        const float f = __builtin_amdgcn_exp2f(a.stat[at * 2] - m);
-        l = __builtin_fmaf(f, a.stat[at * 2 + 1], l);
-        if (!in) continue;
-        const v4f x = *reinterpret_cast<const v4f*>(a.part + at * a.D + 4 * lane);
+    const bool in = d < a.D;
+    for (int c0 = sub; c0 < used; c0 += 4 * kSets) {
+        v4f x[4];
+        float cm[4], cl[4];
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[e] = __builtin_fmaf(f, x[e], s[e]);
+        for (int u = 0; u < 4; u++) {
+            const int c = c0 + u * kSets;
+            const bool on = c < used;
+            cm[u] = on ? a.stat[at(c) * 2] : kNoScore;
+            cl[u] = on ? a.stat[at(c) * 2 + 1] : 0.0f;
+            x[u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            if (on && in) x[u] = *reinterpret_cast<const v4f*>(a.part + at(c) * a.D + d);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            const float f = __builtin_amdgcn_exp2f(cm[u] - m);
+            l = __builtin_fmaf(f, cl[u], l);
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[e] = __builtin_fmaf(f, x[u][e], s[e]);
+        }
+    }
+#pragma unroll
+    for (int o = LPR; o < kWave; o <<= 1) {
+        l += __shfl_xor(l, o, kWave);
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[e] += __shfl_xor(s[e], o, kWave);
     }
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-    if (in)
-        *reinterpret_cast<v2u*>(a.out + id * a.D + 4 * lane) =
-            v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
+    if (in && sub == 0)
+        *reinterpret_cast<v2u*>(a.out + id * a.D + d) = v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
 }
 
 // Chunks such that the longest sequences make about three workgroups per CU, of 128 keys (one tile for
 // each of four waves) at least.
-CachePlan cache_plan(int B, int T, int Hq, int Hkv, long long max_keys) {
+inline int cache_row(int D) { return D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256; }
+
+CachePlan cache_plan(int B, int T, int Hq, int Hkv, int D, long long max_keys) {
     CachePlan p;
-    const int rows = T * (Hq / Hkv);
-    p.sets = rows > 32 ? 2 : 1;
+    const int rows = T * (Hq / Hkv), most = cache_row(D) == 64 || cache_row(D) == 128 ? 8 : 4;
+    for (p.sets = 1; 32 * p.sets < rows && p.sets < most;) p.sets *= 2;
     const long long heads = static_cast<long long>(B) * Hkv * divup(rows, 32 * p.sets);
     const long long want = std::max<long long>(1, divupll(768, heads));
     const long long chunk = divupll(divupll(max_keys, want), 128) * 128;
@@ -280,29 +310,44 @@ size_t cache_floats(int B, int T, int Hq, int D, const CachePlan& p) {
     return p.chunks == 1 ? 0 : static_cast<size_t>(B) * T * Hq * p.chunks * (D + 2);
 }
 
-template <class T, int DP, int RB, int W>
+template <class T, int DP, int RS, int KS, int KB>
 int launch_cache(const CacheArgs& a, hipStream_t s) {
-    constexpr int kLds = W * (4 * 32 * KvRows<DP>::kBytes + 32 * RB * 16);
+    constexpr int kTiles = 4 * 32 * KS * KB * KvRows<DP>::kBytes, kSums = KS > 1 ? RS * KS * 32 * (DP + 4) * 4 : 0;
+    constexpr int kLds = kTiles > kSums ? kTiles : kSums, LPR = DP <= 64 ? 16 : DP <= 128 ? 32 : 64;
     const int rows = a.T * (a.Hq / a.Hkv);
-    const long long wgs = static_cast<long long>(a.B) * a.Hkv * divup(rows, 32 * RB) * a.chunks;
+    const long long wgs = static_cast<long long>(a.B) * a.Hkv * divup(rows, 32 * RS) * a.chunks;
     if (wgs > INT_MAX) return FORGE_EINVAL;
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&cache_attention_kernel<T, DP, RB, W>),
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&cache_attention_kernel<T, DP, RS, KS, KB>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (attr != hipSuccess) return static_cast<int>(attr);
-    cache_attention_kernel<T, DP, RB, W><<<static_cast<unsigned>(wgs), 64 * W, kLds, s>>>(a);
-    int st = launch_status();
+    cache_attention_kernel<T, DP, RS, KS, KB><<<static_cast<unsigned>(wgs), 64 * RS * KS, kLds, s>>>(a);
+    const int st = launch_status();
     if (st != FORGE_OK || a.chunks == 1) return st;
     const long long all = static_cast<long long>(a.B) * a.T * a.Hq;
-    cache_join_kernel<T><<<static_cast<unsigned>(divupll(all, 4)), 256, 0, s>>>(a);
+    cache_join_kernel<T, LPR><<<static_cast<unsigned>(divupll(all, 4)), 256, 0, s>>>(a);
     return launch_status();
 }
 
-template <class T, int RB>
-int launch_cache(const CacheArgs& a, hipStream_t s) {
-    if (a.D <= 64) return launch_cache<T, 64, RB, 4>(a, s);
-    if (a.D <= 96) return launch_cache<T, 96, RB, 4>(a, s);
-    if (a.D <= 128) return launch_cache<T, 128, RB, 4>(a, s);
-    return launch_cache<T, 256, RB, 2>(a, s);
+// Waves by 32-row sets, then by keys, up to 8 (4 at 256 values a head, whose sums take 128 registers a lane);
+// tiles of 64 or 128 keys, 128 KB of LDS at most for two of K and V.
+template <class T>
+int launch_cache(const CacheArgs& a, int sets, hipStream_t s) {
+    switch (cache_row(a.D)) {
+    case 64:
+        if (sets == 1) return launch_cache<T, 64, 1, 4, 1>(a, s);
+        if (sets == 2) return launch_cache<T, 64, 2, 4, 1>(a, s);
+        return sets == 4 ? launch_cache<T, 64, 4, 2, 2>(a, s) : launch_cache<T, 64, 8, 1, 2>(a, s);
+    case 96:
+        if (sets == 1) return launch_cache<T, 96, 1, 4, 1>(a, s);
+        return sets == 2 ? launch_cache<T, 96, 2, 4, 1>(a, s) : launch_cache<T, 96, 4, 2, 2>(a, s);
+    case 128:
+        if (sets == 1) return launch_cache<T, 128, 1, 4, 1>(a, s);
+        if (sets == 2) return launch_cache<T, 128, 2, 4, 1>(a, s);
+        return sets == 4 ? launch_cache<T, 128, 4, 2, 2>(a, s) : launch_cache<T, 128, 8, 1, 2>(a, s);
+    default:
+        if (sets == 1) return launch_cache<T, 256, 1, 2, 1>(a, s);
+        return sets == 2 ? launch_cache<T, 256, 2, 2, 1>(a, s) : launch_cache<T, 256, 4, 1, 2>(a, s);
+    }
 }
 
 bool cache_shape_ok(int B, int T, int Hq, int Hkv, int D) {
@@ -316,7 +361,7 @@ using namespace forge_amd;
 
 extern "C" size_t forge_cache_attention_workspace_size(int B, int T, int Hq, int Hkv, int D, long long max_keys) {
     if (!cache_shape_ok(B, T, Hq, Hkv, D) || max_keys <= 0) return 0;
-    return 4 * cache_floats(B, T, Hq, D, cache_plan(B, T, Hq, Hkv, max_keys));
+    return 4 * cache_floats(B, T, Hq, D, cache_plan(B, T, Hq, Hkv, D, max_keys));
 }
 
 extern "C" int forge_cache_attention(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
@@ -335,7 +380,7 @@ extern "C" int forge_cache_attention(const uint16_t* q, const uint16_t* k_cache,
         if (!aligned(p, 16)) return FORGE_EINVAL;
     const long long max_keys = static_cast<long long>(table_width) * page_size;
     if (max_keys > INT_MAX - kCacheMaxChunk) return FORGE_EINVAL;
-    const CachePlan p = cache_plan(B, T, Hq, Hkv, max_keys);
+    const CachePlan p = cache_plan(B, T, Hq, Hkv, D, max_keys);
     const size_t floats = cache_floats(B, T, Hq, D, p);
     if (floats && (!workspace || workspace_bytes < 4 * floats)) return FORGE_EINVAL;
     float* part = static_cast<float*>(workspace);
@@ -344,6 +389,5 @@ extern "C" int forge_cache_attention(const uint16_t* q, const uint16_t* k_cache,
                       B, T, Hq, Hkv, D, pages, __builtin_ctz(static_cast<unsigned>(page_size)), table_width,
                       p.chunk, p.chunks, scale};
     hipStream_t s = as_stream(stream);
-    if (dtype == FORGE_FP16) return p.sets == 1 ? launch_cache<Fp16, 1>(a, s) : launch_cache<Fp16, 2>(a, s);
-    return p.sets == 1 ? launch_cache<Bf16, 1>(a, s) : launch_cache<Bf16, 2>(a, s);
+    return dtype == FORGE_FP16 ? launch_cache<Fp16>(a, p.sets, s) : launch_cache<Bf16>(a, p.sets, s);
 }

@@ -27,7 +27,7 @@ struct PromptArgs {
 constexpr int kPromptKeys = 64;
 
 template <class T, int DP, int W, bool CAUSAL>
-__global__ __launch_bounds__(64 * W) void prompt_attention_kernel(PromptArgs a)
+__global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void prompt_attention_kernel(PromptArgs a)
 {
     using Rows = KvRows<DP>;
     constexpr int kRows = 32 * W, kTile = kPromptKeys * Rows::kBytes;
@@ -83,35 +83,39 @@ __global__ __launch_bounds__(64 * W) void prompt_attention_kernel(PromptArgs a)
     }
     const int end = CAUSAL ? min(row0 + kRows, len) : len;
     const int tiles = (end + kPromptKeys - 1) / kPromptKeys;
+    const uint32_t lds0 = lds_address(lds);
     auto load = [&](int t) {                                         // rows past the sequence's end read as zeros
         const int left = len - t * kPromptKeys;
-        const auto kr = buf_rsrc(kbase + static_cast<size_t>(t) * kPromptKeys * a.k_token,
-                                 static_cast<uint32_t>((kPromptKeys - 1) * a.k_token * 2 + 2 * a.D));
-        const auto vr = buf_rsrc(vbase + static_cast<size_t>(t) * kPromptKeys * a.v_token,
-                                 static_cast<uint32_t>((kPromptKeys - 1) * a.v_token * 2 + 2 * a.D));
-        int8_t* ks = lds + (t & 1) * 2 * kTile;
+        const v4i kr = row_rsrc(kbase + static_cast<size_t>(t) * kPromptKeys * a.k_token,
+                                static_cast<uint32_t>((kPromptKeys - 1) * a.k_token * 2 + 2 * a.D));
+        const v4i vr = row_rsrc(vbase + static_cast<size_t>(t) * kPromptKeys * a.v_token,
+                                static_cast<uint32_t>((kPromptKeys - 1) * a.v_token * 2 + 2 * a.D));
+        const uint32_t ks = lds0 + (t & 1) * 2 * kTile;
 #pragma unroll
         for (int n = 0; n < kIns; n++)
-            dma16_buf(kr, dma_row[n] < left ? koff[n] : kOutOfRange, 0, ks + (wave * kIns + n) * 1024);
+            dma16_rows(kr, dma_row[n] < left ? koff[n] : kOutOfRange, ks + (wave * kIns + n) * 1024);
 #pragma unroll
         for (int n = 0; n < kIns; n++)
-            dma16_buf(vr, dma_row[n] < left ? voff[n] : kOutOfRange, 0, ks + kTile + (wave * kIns + n) * 1024);
+            dma16_rows(vr, dma_row[n] < left ? voff[n] : kOutOfRange, ks + kTile + (wave * kIns + n) * 1024);
     };
     const float scale2 = a.scale * 1.44269504f;
-    load(0);
-    for (int t = 0; t < tiles; t++) {
+    const int first = row0 + 32 * wave;
+    const int mine = CAUSAL ? min(tiles, first / kPromptKeys + 1) : tiles;   // tiles that reach this wave's rows
+    auto next = [&](int t) {
         wait_vm_lgkm<0>();
         lds_barrier();                                               // tile t is whole, tile t - 1 is read
         if (t + 1 < tiles) load(t + 1);
+    };
+    load(0);
+    int t = 0;
+    for (; t < mine; t++) {
+        next(t);
         const int8_t* ks = lds + (t & 1) * 2 * kTile;
-        const int k0 = t * kPromptKeys, first = row0 + 32 * wave;
-        if (CAUSAL && k0 > first + 31) continue;                     // wave-uniform
-        if ((CAUSAL && k0 + kPromptKeys - 1 > first) || k0 + kPromptKeys > len)
-            w.template step<true>(ks, ks + kTile, scale2,
-                                  [&](int, int j) { return k0 + j < len && (!CAUSAL || k0 + j <= row); });
-        else
-            w.template step<false>(ks, ks + kTile, scale2, [](int, int) { return true; });
+        const int k0 = t * kPromptKeys;
+        w.step(ks, ks + kTile, scale2, (CAUSAL && k0 + kPromptKeys - 1 > first) || k0 + kPromptKeys > len,
+               [&](int, int kb) { return bits_to((CAUSAL ? min(row, len - 1) : len - 1) - k0 - 32 * kb); });
     }
+    for (; t < tiles; t++) next(t);
     const bool live = row < len;
     if (w.odd(0, live)) {
         for (int r = 0; r < 32; r++) {
