@@ -16,36 +16,12 @@
 #pragma once
 
 #include "float16_types.h"
-#include "mfma_tile.h"
+#include "lds_dma.h"
 
 namespace forge_amd {
 
 constexpr float kNoScore = -1e30f;   // running maximum of a row that has seen nothing
 constexpr float kRescale = 8.0f;
-
-// LDS DMA of 16 bytes a lane to lds + 16 * lane, as in mfma_tile.h but written out: the compiler makes
-// every transposing LDS read wait for all DMAs that it knows of, which would end the prefetch of the next
-// tile at the first read of V. Nothing is returned in registers; the callers wait by count (wait_vmcnt). M0 has
-// no other use in these kernels.
-__device__ __forceinline__ uint32_t lds_address(const int8_t* p) {
-    return static_cast<uint32_t>(reinterpret_cast<uintptr_t>((__attribute__((address_space(3))) const int8_t*)p));
-}
-__device__ __forceinline__ void dma16_rows(v4i rsrc, uint32_t voff, uint32_t lds) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    asm volatile("s_mov_b32 m0, %2\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds) : "memory");
-#endif
-}
-__device__ __forceinline__ void dma16_at(const void* p, uint32_t lds) {
-#if defined(__HIP_DEVICE_COMPILE__)
-    asm volatile("s_mov_b32 m0, %1\n\tglobal_load_lds_dwordx4 %0, off" ::"v"(p), "s"(lds) : "memory");
-#endif
-}
-// A raw buffer resource over `bytes` from p, both wave-uniform.
-__device__ __forceinline__ v4i row_rsrc(const void* p, uint32_t bytes) {
-    const uint64_t a = reinterpret_cast<uint64_t>(p);
-    return v4i{__builtin_amdgcn_readfirstlane(static_cast<int>(a)),
-               __builtin_amdgcn_readfirstlane(static_cast<int>(a >> 32) & 0xFFFF), static_cast<int>(bytes), 0x00020000};
-}
 
 typedef short v4s __attribute__((ext_vector_type(4)));
 

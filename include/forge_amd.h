@@ -315,7 +315,7 @@ int forge_int8_depthwise_conv2d_forward(const uint16_t* input, const int8_t* wei
 #define FORGE_BF16 1
 
 /* 4-bit weights with one FP16 scale per `group` (32, 64 or 128) consecutive values of a row:
- * w_scale (N, K/group), K % group == 0. w_int4: N rows of ceil(K / 128) * 64 bytes, 16-byte aligned, in blocks of
+ * w_scale (N, K/group), K % group == 0, K <= 2^23. w_int4: N rows of ceil(K / 128) * 64 bytes, 16-byte aligned, in blocks of
  * 128 values (the last filled up with zeros). A block is a 4 x 4 transpose of its sixteen 32-bit words: word
  * 4 g + j holds values 32 j + 8 g to 32 j + 8 g + 7 of the block, of these value 2 i at bits 4 i and value 2 i + 1 at
  * bits 16 + 4 i, as q + 8 with q in -8..7.

@@ -64,6 +64,19 @@ def make(M, K, N, G, dt, bias, dev, seed):
     (16, 2880, 47, 32), (17, 2880, 48, 64), (31, 1152, 130, 128), (33, 416, 15, 32), (64, 640, 257, 64),
     (65, 384, 40, 128), (200, 256, 20, 64), (5, 8192, 40, 128), (48, 6144, 100, 32)])
 def test_int4_linear(dev, dt, M, K, N, G):
+    linear_case(dev, dt, M, K, N, G)
+
+
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("M,K,N,G", [
+    (1, 256, 16400, 128), (4, 544, 17001, 32), (7, 288, 8200, 32), (16, 384, 11008, 128), (20, 320, 11001, 64),
+    (32, 256, 8193, 32), (40, 416, 12289, 32), (64, 512, 11008, 128), (130, 256, 9000, 64)])
+def test_wide_layers(dev, dt, M, K, N, G):
+    """Row counts that take the other tiles."""
+    linear_case(dev, dt, M, K, N, G)
+
+
+def linear_case(dev, dt, M, K, N, G):
     from forge_amd import ops
     q, s, x, b = make(M, K, N, G, dt, (M + N) % 2 == 0, dev, M + K + N)
     say(f"int4_linear {dt} M={M} K={K} N={N} G={G}")
