@@ -10,6 +10,7 @@ import os
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.path.join(HERE, "lib", "libforge_amd.so")
+BINDING_PATH = os.path.join(HERE, "lib", "forge_torch.so")
 
 FORGE_OK = 0
 FORGE_EINVAL = -1
@@ -89,6 +90,27 @@ def load() -> ctypes.CDLL:
             fn.argtypes = args
         _lib = lib
     return _lib
+
+
+_calls = None
+
+
+def calls():
+    """The compiled calls of the decoder-attention operators (csrc/torch_calls.cpp), linked to the library."""
+    global _calls
+    if _calls is None:
+        import importlib.machinery
+        import importlib.util
+
+        import torch  # noqa: F401  (its libraries, which the module needs)
+        load()
+        if not os.path.exists(BINDING_PATH):
+            raise ForgeError(f"forge_amd binding not found at {BINDING_PATH}; build it with `python -m forge_amd.build`")
+        loader = importlib.machinery.ExtensionFileLoader("forge_torch", BINDING_PATH)
+        module = importlib.util.module_from_spec(importlib.util.spec_from_loader("forge_torch", loader))
+        loader.exec_module(module)
+        _calls = module
+    return _calls
 
 
 def check(status: int, what: str = "") -> None:

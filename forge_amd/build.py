@@ -21,6 +21,7 @@ LIB = os.path.join(LIBDIR, "libforge_amd.so")
 # Measurement probes (bench.py --probes), a library of their own: not part of the product.
 PROBE_LIB = os.path.join(LIBDIR, "libforge_probes.so")
 PROBE_SOURCES = ["probes.hip"]
+BINDING = os.path.join(LIBDIR, "forge_torch.so")
 
 ARCH = "gfx950"
 HIPCC = os.environ.get("HIPCC", "/opt/rocm/bin/hipcc")
@@ -81,6 +82,24 @@ def _link(objs: list, lib: str) -> None:
     os.replace(tmp, lib)
 
 
+def _bind(lib: str) -> None:
+    """The host-only module that takes the decoder-attention calls from PyTorch tensors (torch_calls.cpp)."""
+    import sysconfig
+
+    import torch
+    root = os.path.dirname(torch.__file__)
+    tmp = lib + ".tmp"
+    cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-shared", "-Wall",
+           f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}", f"-I{os.path.join(ROOT, 'include')}",
+           f"-I{root}/include", f"-I{root}/include/torch/csrc/api/include", f"-I{sysconfig.get_paths()['include']}",
+           os.path.join(CSRC, "torch_calls.cpp"), "-o", tmp, f"-L{LIBDIR}", "-lforge_amd", f"-L{root}/lib",
+           "-ltorch_python", "-ltorch_cpu", "-lc10", "-Wl,-rpath,$ORIGIN"]
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        raise RuntimeError(f"building the binding failed:\n{' '.join(cmd)}\n{r.stdout}\n{r.stderr}")
+    os.replace(tmp, lib)
+
+
 def build(jobs: int | None = None) -> str:
     os.makedirs(BUILD, exist_ok=True)
     os.makedirs(LIBDIR, exist_ok=True)
@@ -90,6 +109,7 @@ def build(jobs: int | None = None) -> str:
         objs = dict(zip(srcs, ex.map(_compile, srcs)))
     _link([objs[s] for s in SOURCES], LIB)
     _link([objs[s] for s in PROBE_SOURCES], PROBE_LIB)
+    _bind(BINDING)
     return LIB
 
 

@@ -523,8 +523,31 @@ def prepare_sparse_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, 
 
 
 # ---- decoder attention (extension; include/forge_amd.h "decoder attention") -----------
+# A call whose operands are all in order goes through csrc/torch_calls.cpp, which checks them and calls the library in
+# about a microsecond; any other takes the checks below, which say what is wrong.
 
 _DTYPE = {torch.float16: 0, torch.bfloat16: 1}   # FORGE_FP16, FORGE_BF16
+_NOT_IN_ORDER = -1000
+_device = torch._C._cuda_getDevice
+_raw_stream = torch._C._cuda_getCurrentRawStream
+_calls = None
+
+
+def _fast(name: str, *args) -> bool:
+    """Whether the compiled call was made; raises what the library or a launch reports."""
+    global _calls
+    if _calls is None:
+        _calls = _lib.calls()
+    try:
+        dev = _device()
+    except RuntimeError:                          # no device: the checks say so
+        return False
+    status = getattr(_calls, name)(*args, dev, _raw_stream(dev))
+    if status == 0:
+        return True
+    if status > 0:
+        _lib_check(status, "forge_" + name)
+    return False
 
 
 def _act_type(t: torch.Tensor, name: str) -> int:
@@ -536,13 +559,13 @@ def _act_type(t: torch.Tensor, name: str) -> int:
     return code
 
 
-def _need_shape(t: torch.Tensor, dtype: torch.dtype, name: str, shape: Tuple[int, ...]) -> None:
-    """A contiguous device tensor of this type and shape, 16-byte aligned."""
+def _need_shape(t: torch.Tensor, dtype: torch.dtype, name: str, shape: Tuple[int, ...], align: int = 16) -> None:
+    """A contiguous device tensor of this type, shape and alignment in bytes."""
     _need(t, dtype, name)
     if t.shape != shape:
         raise ValueError(f"{name} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if t.data_ptr() % 16:
-        raise ValueError(f"{name} must be 16-byte aligned")
+    if t.data_ptr() % align:
+        raise ValueError(f"{name} must be {align}-byte aligned")
 
 
 def _need_heads(t: torch.Tensor, dtype: torch.dtype, name: str, tokens: int) -> Tuple[int, int]:
@@ -618,6 +641,10 @@ def int4_linear(x: torch.Tensor, w_int4: torch.Tensor, w_scale: torch.Tensor, bi
                 out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """forge_int4_linear: x (M, K) float16 or bfloat16 times the transpose of the 4-bit weights of
     quantize_weight_int4 / pack_weight_int4 with their scales, plus bias (N,); `out` may be passed to reuse an (M, N) buffer."""
+    if out is None and isinstance(x, torch.Tensor) and isinstance(w_scale, torch.Tensor) and x.dim() == 2 == w_scale.dim():
+        out = torch.empty((x.shape[0], w_scale.shape[0]), dtype=x.dtype, device=x.device)
+    if _fast("int4_linear", x, w_int4, w_scale, bias, out):
+        return out
     code = _act_type(x, "x")
     if x.dim() != 2:
         raise ValueError(f"x must be (M, K), got {tuple(x.shape)}")
@@ -634,11 +661,8 @@ def int4_linear(x: torch.Tensor, w_int4: torch.Tensor, w_scale: torch.Tensor, bi
     if x.data_ptr() % 16:
         raise ValueError("x must be 16-byte aligned")
     if bias is not None:
-        _need(bias, x.dtype, "bias", N)
-    if out is None:
-        out = torch.empty((M, N), dtype=x.dtype, device=x.device)
-    else:
-        _need(out, x.dtype, "out", M * N)
+        _need_shape(bias, x.dtype, "bias", (N,), align=1)
+    _need_shape(out, x.dtype, "out", (M, N), align=1)
     _same_device(x, w_int4, w_scale, bias, out)
     _call("forge_int4_linear", _p(x), _p(w_int4), _p(w_scale), _p(bias), _p(out), M, K, N, group, code, _stream())
     return out
@@ -646,6 +670,9 @@ def int4_linear(x: torch.Tensor, w_int4: torch.Tensor, w_scale: torch.Tensor, bi
 
 def _qk_norm_rope(q, k, v, q_weight, k_weight, cos, sin, positions, k_cache, v_cache, slots, eps, interleaved, q_out,
                   k_out):
+    if _fast("qk_norm_rope", q, k, v, q_weight, k_weight, cos, sin, positions, q_out, k_out, k_cache, v_cache, slots, eps,
+             interleaved):
+        return
     code = _act_type(q, "q")
     dt = q.dtype
     T = q.shape[0] if q.dim() else 0
@@ -728,6 +755,10 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     and k, v (tokens, Hkv, D), sequence b being tokens cu_seqlens[b] to cu_seqlens[b + 1] - 1 (int32, the first 0). Query
     head h reads KV head h // (Hq // Hkv). scale: 1 / sqrt(D) unless given. q, k and v may be strided views."""
     code = _act_type(q, "q")
+    if out is None:
+        out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
+    if _fast("prompt_attention", q, k, v, cu_seqlens, out, q.shape[-1] ** -0.5 if scale is None else scale, causal):
+        return out
     dt = q.dtype
     T = q.shape[0] if q.dim() else 0
     qs, ks, vs = _need_heads(q, dt, "q", T), _need_heads(k, dt, "k", T), _need_heads(v, dt, "v", T)
@@ -740,10 +771,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     if cu_seqlens.dim() != 1 or cu_seqlens.shape[0] < 2:
         raise ValueError(f"cu_seqlens must hold the sequences' boundaries, got shape {tuple(cu_seqlens.shape)}")
     scale = _softmax_scale(scale, D)
-    if out is None:
-        out = torch.empty((T, Hq, D), dtype=dt, device=q.device)
-    else:
-        _need_shape(out, dt, "out", (T, Hq, D))
+    _need_shape(out, dt, "out", (T, Hq, D))
     _same_device(q, k, v, cu_seqlens, out)
     _call("forge_prompt_attention", _p(q), _p(k), _p(v), _p(cu_seqlens), _p(out), cu_seqlens.shape[0] - 1, T, Hq, Hkv, D,
           *qs, *ks, *vs, scale, 1 if causal else 0, code, _stream())
@@ -763,6 +791,10 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     tokens' keys and values are in the cache at positions cache_lens[b] on (qk_norm_rope_cache). Token t sees the
     positions before cache_lens[b] and the new tokens whose bit is set in tree[b, t] (int64 (B, T)), or tokens 0..t
     without a tree (T = 1: plain decode)."""
+    if workspace is not None and out is not None and isinstance(q, torch.Tensor):
+        if _fast("cache_attention", q, k_cache, v_cache, page_table, cache_lens, tree, workspace, out,
+                 q.shape[-1] ** -0.5 if scale is None else scale):
+            return out
     code = _act_type(q, "q")
     dt = q.dtype
     if q.dim() != 4:
