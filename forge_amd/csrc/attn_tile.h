@@ -8,11 +8,11 @@
 // product's sum over keys may take them in any order, if V^T's operand takes the same one. That operand
 // is 4 + 4 keys of one column of V, which the transposing LDS read gathers from V's rows.
 // The running maximum m, sum l and O follow the usual recurrence, FP32; P is rounded to 16 bits for
-// its product (its sum is not). O is rescaled only when some row's maximum has grown by more than
+// its product, and l sums the rounded weights, so that they add up to one. O is rescaled only when some row's maximum has grown by more than
 // 2^8 since the last time: until then P stays below 2^8, well inside both types.
 //
-// K and V tiles are rows of DP values (D padded with zeros) in 16-byte chunks, permuted in each row so that the
-// 16 rows of a K read and the 4 rows of a V read fall on different banks.
+// K and V tiles are rows of DP values (D padded with zeros) in 16-byte chunks, permuted in each row so that what
+// LDS serves in one clock falls on different banks: one chunk of 16 rows of K, four chunks of 4 rows of V.
 #pragma once
 
 #include "float16_types.h"
@@ -51,7 +51,7 @@ struct KvRows {
         return DP == 64 ? (r >> 1) & 7 : DP == 96 ? (r >> 2) & 3 : r & 15;
     }
     static __device__ __forceinline__ int swz_v(int r) {
-        return DP == 64 ? 2 * ((r >> 1) & 3) : DP == 96 ? 2 * ((r >> 2) & 1) : 2 * (r & 7);
+        return DP == 64 ? 4 * ((r >> 1) & 1) : DP == 96 ? 0 : 4 * (r & 3);
     }
 };
 
@@ -97,78 +97,131 @@ struct AttnWave {
         }
     }
 
-    // One tile of 32 KB keys. If `mask` (uniform), seen(b, kb) has a bit for each key of block kb that this lane's
-    // row of set b sees.
-    template <class Seen>
-    __device__ __forceinline__ void step(const int8_t* ks, const int8_t* vs, float scale2, bool mask, const Seen& seen) {
-        v16f s[RB][KB];
+    // The order of a block's N products and the LDS reads of their operands, R each: those of the first
+    // `ahead` products, then one product and the reads of the one `ahead` further on. Left to itself the compiler
+    // reads one or two ahead and each product waits for LDS.
+    static constexpr int kAhead = 6;
+    template <int N, int R, int AHEAD>
+    static __device__ __forceinline__ void interleave() {
+        __builtin_amdgcn_sched_group_barrier(0x100, R * (AHEAD < N ? AHEAD : N), 0);
 #pragma unroll
-        for (int kb = 0; kb < KB; kb++) {
-#pragma unroll
-            for (int b = 0; b < RB; b++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) s[b][kb][e] = 0.0f;
-#pragma unroll
-            for (int st = 0; st < kSteps; st++) {
-                const v4u k = *reinterpret_cast<const v4u*>(ks + 32 * kb * Rows::kBytes + k_at + ((32 * st) ^ k_x));
-#pragma unroll
-                for (int b = 0; b < RB; b++) s[b][kb] = T::mfma32(k, q[b][st], s[b][kb]);
-            }
+        for (int i = 0; i < N; i++) {
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (i + AHEAD < N) __builtin_amdgcn_sched_group_barrier(0x100, R, 0);
         }
-        v4u p[RB][KB][2];
+    }
+
+    using Scores = v16f[RB][KB];
+    using Weights = v4u[RB][KB][2];
+
+    // Scores of a tile of 32 KB keys; products in a row go to different sums.
+    __device__ __forceinline__ void scores(const int8_t* ks, Scores& s) const {
 #pragma unroll
-        for (int b = 0; b < RB; b++) {
-            if (mask) {
-#pragma unroll
-                for (int kb = 0; kb < KB; kb++) {
-                    const uint32_t bits = seen(b, kb) >> (4 * (lane >> 5));
-#pragma unroll
-                    for (int e = 0; e < 16; e++)
-                        if (!(bits & (1u << (8 * (e / 4) + e % 4)))) s[b][kb][e] = -INFINITY;
-                }
-            }
-            float mx = s[b][0][0];
-#pragma unroll
-            for (int kb = 0; kb < KB; kb++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) mx = fmaxf(mx, s[b][kb][e]);
-            mx = half_max(mx) * scale2;
-            if (__any(mx > m[b] + kRescale)) {
-                const float mn = fmaxf(m[b], mx), f = __builtin_amdgcn_exp2f(m[b] - mn);
-                m[b] = mn;
-                l[b] *= f;
-#pragma unroll
-                for (int j = 0; j < kOut; j++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) o[b][j][e] *= f;
-            }
-            float sum = 0.0f;
+        for (int st = 0; st < kSteps; st++)
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
+                const v4u k = *reinterpret_cast<const v4u*>(ks + 32 * kb * Rows::kBytes + k_at + ((32 * st) ^ k_x));
 #pragma unroll
-                for (int e = 0; e < 16; e++) {
-                    s[b][kb][e] = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][kb][e], scale2, -m[b]));
-                    sum += s[b][kb][e];
+                for (int b = 0; b < RB; b++) {
+                    const v16f zero = {};
+                    s[b][kb] = T::mfma32(k, q[b][st], st == 0 ? zero : s[b][kb]);
                 }
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int d = 0; d < 4; d++) p[b][kb][h][d] = T::pack(s[b][kb][8 * h + 2 * d], s[b][kb][8 * h + 2 * d + 1]);
             }
-            l[b] += sum;
-        }
+        if constexpr (RB == 1) interleave<KB * kSteps, 1, kAhead>();
+    }
+
+    // seen(b, kb) has a bit for each key of block kb that this lane's row of set b sees.
+    template <class Seen>
+    __device__ __forceinline__ void mask(Scores& s, const Seen& seen) const {
 #pragma unroll
-        for (int j = 0; j < kOut; j++)
+        for (int b = 0; b < RB; b++)
+#pragma unroll
+            for (int kb = 0; kb < KB; kb++) {
+                const uint32_t bits = seen(b, kb) >> (4 * (lane >> 5));
+#pragma unroll
+                for (int e = 0; e < 16; e++)
+                    if (!(bits & (1u << (8 * (e / 4) + e % 4)))) s[b][kb][e] = -INFINITY;
+            }
+    }
+
+    // The largest score of set b's row, in the exponent's units.
+    __device__ __forceinline__ float largest(const Scores& s, int b, float scale2) const {
+        float mx[4];
+#pragma unroll
+        for (int c = 0; c < 4; c++) {                                // four chains of maxima of three
+            mx[c] = s[b][0][4 * c];
 #pragma unroll
             for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-                for (int h = 0; h < 2; h++) {
+                for (int e = 0; e < 4; e++) mx[c] = fmaxf(mx[c], s[b][kb][4 * c + e]);
+        }
+        return half_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))) * scale2;
+    }
+
+    // The weights of set b against its maximum as it stands; returns their sum.
+    __device__ __forceinline__ float weights(const Scores& s, int b, float scale2, Weights& p) const {
+        float sum[2] = {0.0f, 0.0f};
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int d = 0; d < 4; d++) {
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][kb][8 * h + 2 * d], scale2, -m[b]));
+                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][kb][8 * h + 2 * d + 1], scale2, -m[b]));
+                    p[b][kb][h][d] = T::pack(x, y);
+                    sum[h] = T::add_pair(p[b][kb][h][d], sum[h]);
+                }
+        return sum[0] + sum[1];
+    }
+
+    // O += P V of a tile.
+    __device__ __forceinline__ void values(const int8_t* vs, const Weights& p) {
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int j = 0; j < kOut; j++) {
                     const int8_t* at = vs + (32 * kb + 16 * h) * Rows::kBytes + v_at + ((64 * j) ^ v_x);
                     const v2u lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * Rows::kBytes);
                     const v4u v = {lo[0], lo[1], hi[0], hi[1]};
 #pragma unroll
                     for (int b = 0; b < RB; b++) o[b][j] = T::mfma32(v, p[b][kb][h], o[b][j]);
                 }
+        if constexpr (RB == 1) interleave<2 * KB * kOut, 2, kAhead>();
+    }
+
+    // A tile from its scores on; masked if `masked` (uniform).
+    template <class Seen>
+    __device__ __forceinline__ void finish(Scores& s, const int8_t* vs, float scale2, bool masked, const Seen& seen) {
+        if (masked) mask(s, seen);
+        Weights p;
+        float sum[RB], mx[RB];
+        bool grown = false;
+#pragma unroll
+        for (int b = 0; b < RB; b++) {
+            sum[b] = weights(s, b, scale2, p);
+            mx[b] = largest(s, b, scale2);
+            grown |= mx[b] > m[b] + kRescale;
+        }
+        // A maximum that has grown is met seldom, and so the weights do not wait for it: they are taken again.
+        if (__any(grown)) {
+#pragma unroll
+            for (int b = 0; b < RB; b++) {
+                const float mn = fmaxf(m[b], mx[b]), f = __builtin_amdgcn_exp2f(m[b] - mn);
+                m[b] = mn;
+                l[b] *= f;
+#pragma unroll
+                for (int j = 0; j < kOut; j++)
+#pragma unroll
+                    for (int e = 0; e < 16; e++) o[b][j][e] *= f;
+                sum[b] = weights(s, b, scale2, p);
+            }
+        }
+#pragma unroll
+        for (int b = 0; b < RB; b++) l[b] += sum[b];
+        values(vs, p);
     }
 
     // Whether some value of the rows `live` is no finite number.

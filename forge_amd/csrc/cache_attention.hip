@@ -60,21 +60,17 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
     const int hk = id % a.Hkv; id /= a.Hkv;
     const int set = id % sets; id /= sets;
     const int chunk = id % a.chunks, b = id / a.chunks;
-    const int keys = cache_keys(a, b), len = max(a.lens[b], 0);
-    const int key0 = chunk * a.chunk, n = min(keys - key0, a.chunk);
-    if (n <= 0) return;
-
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x & (kWave - 1);
     const int rs = wave / KS, ks = wave % KS;
-    const int page_mask = (1 << a.page_shift) - 1, page0 = key0 >> a.page_shift;
-    const int last_page = (key0 + n - 1) >> a.page_shift;
+    const int key0 = chunk * a.chunk, page_mask = (1 << a.page_shift) - 1, page0 = key0 >> a.page_shift;
+    // the chunk's whole part of the table, so that its loads need not wait for the length
+    const int last_page = min((key0 + a.chunk - 1) >> a.page_shift, a.width - 1);
     for (int p = page0 + threadIdx.x; p <= last_page; p += 64 * W) {
         const int pg = a.table[static_cast<size_t>(b) * a.width + p];
         page_of[p - page0] = pg >= 0 && pg < a.pages ? pg : -1;
     }
     if (threadIdx.x == 0) odd_rows = 0;
-    __syncthreads();
 
     const size_t token = static_cast<size_t>(a.Hkv) * a.D;
     // element offset of key j's row (of both tensors), or -1
@@ -99,6 +95,9 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
     const bool live = row < rows;
     w.load_q(0, row_of(a.q, row), live, a.D);
     const unsigned long long drafts = live ? drafts_of(row) : 0ull;
+    const int keys = cache_keys(a, b), len = max(a.lens[b], 0), n = min(keys - key0, a.chunk);
+    if (n <= 0) return;
+    __syncthreads();
     const int open = len - key0;                                     // keys of this chunk that every row sees
 
     int dma_row[kIns];
@@ -131,7 +130,9 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
         if (t + 1 < tiles) load(t + 1);
         const int k0 = t * kKeys + 32 * KB * ks;                     // this wave's keys of the tile
         const int8_t* at = lds + (t & 1) * 2 * kTile + 32 * KB * ks * Rows::kBytes;
-        w.step(at, at + kTile, scale2, k0 + 32 * KB > min(open, n), [&](int, int kb) {
+        v16f s[1][KB];
+        w.scores(at, s);
+        w.finish(s, at + kTile, scale2, k0 + 32 * KB > min(open, n), [&](int, int kb) {
             const int d = open - (k0 + 32 * kb);                     // bits below d: the cache; from d on: drafts
             uint32_t bits = bits_to(d - 1);
             if (d < 32) bits |= d >= 0 ? static_cast<uint32_t>(drafts << d) : d > -64 ? static_cast<uint32_t>(drafts >> -d) : 0u;
@@ -144,34 +145,20 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
     __syncthreads();
     if (w.odd(0, live) && lane == 0) atomicOr(&odd_rows, 1);
     float* sums = reinterpret_cast<float*>(lds);
-    if constexpr (KS > 1) {
-        const float l = half_sum(w.l[0]);
-        if (lane < 32) {
-            stat_m[wave][lane] = w.m[0];
-            stat_l[wave][lane] = l;
-        }
-#pragma unroll
-        for (int j = 0; j < DP / 32; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<v4f*>(sums + (wave * 32 + (lane & 31)) * kPitch + 32 * j + 2 * e + 4 * (lane >> 5)) =
-                    v4f{w.o[0][j][e], w.o[0][j][e + 1], w.o[0][j][e + 2], w.o[0][j][e + 3]};
+    const float lane_l = half_sum(w.l[0]);
+    if (lane < 32) {
+        stat_m[wave][lane] = w.m[0];
+        stat_l[wave][lane] = lane_l;
     }
+#pragma unroll
+    for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+        for (int e = 0; e < 16; e += 4)
+            *reinterpret_cast<v4f*>(sums + (wave * 32 + (lane & 31)) * kPitch + 32 * j + 2 * e + 4 * (lane >> 5)) =
+                v4f{w.o[0][j][e], w.o[0][j][e + 1], w.o[0][j][e + 2], w.o[0][j][e + 3]};
     __syncthreads();
     const bool whole = keys <= a.chunk;                              // the only chunk: the result itself
     const size_t part0 = ((static_cast<size_t>(b) * a.Hkv + hk) * a.chunks + chunk) * rows;
-    auto put = [&](int r, int d, v4f s, float m, float l) {
-        if (whole) {
-            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            *reinterpret_cast<v2u*>(row_of(a.out, r) + d) = v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
-        } else {
-            *reinterpret_cast<v4f*>(a.part + (part0 + r) * a.D + d) = s;
-            if (d == 0) {
-                a.stat[(part0 + r) * 2] = m;
-                a.stat[(part0 + r) * 2 + 1] = l;
-            }
-        }
-    };
     if (odd_rows) {
         // some row's sum is not finite: every row again, key by key
         for (int i = wave; i < 32 * RS; i += W) {
@@ -205,36 +192,33 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
         }
         return;
     }
-    if constexpr (KS > 1) {
-        const int quads = a.D / 4;
-        for (int i = threadIdx.x; i < 32 * RS * quads; i += 64 * W) {
-            const int lr = i / quads, d = 4 * (i - lr * quads), r = set * RS * 32 + lr;
-            if (r >= rows) break;
-            const int w0 = (lr / 32) * KS, x = lr % 32;
-            float m = kNoScore, l = 0.0f;
+    const int quads = a.D / 4;
+    for (int i = threadIdx.x; i < 32 * RS * quads; i += 64 * W) {
+        const int lr = i / quads, d = 4 * (i - lr * quads), r = set * RS * 32 + lr;
+        if (r >= rows) break;
+        const int w0 = (lr / 32) * KS, x = lr % 32;
+        float m = kNoScore, l = 0.0f;
 #pragma unroll
-            for (int v = 0; v < KS; v++) m = fmaxf(m, stat_m[w0 + v][x]);
-            v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
+        for (int v = 0; v < KS; v++) m = fmaxf(m, stat_m[w0 + v][x]);
+        v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-            for (int v = 0; v < KS; v++) {
-                const float f = __builtin_amdgcn_exp2f(stat_m[w0 + v][x] - m);
-                l = __builtin_fmaf(f, stat_l[w0 + v][x], l);
-                const v4f y = *reinterpret_cast<const v4f*>(sums + ((w0 + v) * 32 + x) * kPitch + d);
+        for (int v = 0; v < KS; v++) {
+            const float f = __builtin_amdgcn_exp2f(stat_m[w0 + v][x] - m);
+            l = __builtin_fmaf(f, stat_l[w0 + v][x], l);
+            const v4f y = *reinterpret_cast<const v4f*>(sums + ((w0 + v) * 32 + x) * kPitch + d);
 #pragma unroll
-                for (int e = 0; e < 4; e++) s[e] = __builtin_fmaf(f, y[e], s[e]);
-            }
-            put(r, d, s, m, l);
+            for (int e = 0; e < 4; e++) s[e] = __builtin_fmaf(f, y[e], s[e]);
         }
-    } else {
-        const float l = half_sum(w.l[0]);
-#pragma unroll
-        for (int j = 0; j < DP / 32; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int d = 32 * j + 2 * e + 4 * (lane >> 5);
-                if (live && d < a.D)
-                    put(row, d, v4f{w.o[0][j][e], w.o[0][j][e + 1], w.o[0][j][e + 2], w.o[0][j][e + 3]}, w.m[0], l);
+        if (whole) {
+            const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+            *reinterpret_cast<v2u*>(row_of(a.out, r) + d) = v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
+        } else {
+            *reinterpret_cast<v4f*>(a.part + (part0 + r) * a.D + d) = s;
+            if (d == 0) {
+                a.stat[(part0 + r) * 2] = m;
+                a.stat[(part0 + r) * 2 + 1] = l;
             }
+        }
     }
 }
 
@@ -312,7 +296,7 @@ size_t cache_floats(int B, int T, int Hq, int D, const CachePlan& p) {
 
 template <class T, int DP, int RS, int KS, int KB>
 int launch_cache(const CacheArgs& a, hipStream_t s) {
-    constexpr int kTiles = 4 * 32 * KS * KB * KvRows<DP>::kBytes, kSums = KS > 1 ? RS * KS * 32 * (DP + 4) * 4 : 0;
+    constexpr int kTiles = 4 * 32 * KS * KB * KvRows<DP>::kBytes, kSums = RS * KS * 32 * (DP + 4) * 4;
     constexpr int kLds = kTiles > kSums ? kTiles : kSums, LPR = DP <= 64 ? 16 : DP <= 128 ? 32 : 64;
     const int rows = a.T * (a.Hq / a.Hkv);
     const long long wgs = static_cast<long long>(a.B) * a.Hkv * divup(rows, 32 * RS) * a.chunks;

@@ -7,6 +7,7 @@
 
 namespace forge_amd {
 
+typedef float v2f __attribute__((ext_vector_type(2)));
 typedef float v4f __attribute__((ext_vector_type(4)));
 typedef float v16f __attribute__((ext_vector_type(16)));
 typedef uint32_t v2u __attribute__((ext_vector_type(2)));
@@ -17,11 +18,14 @@ struct Fp16 {
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     static constexpr uint32_t kOnes = 0x3C003C00u;
     static __device__ __forceinline__ float widen(uint16_t b) { return h2f(b); }
-    // two values rounded to nearest even, the first in the low half
+    // Two values rounded to nearest even, the first in the low half. (No inline asm: the wait state between an
+    // exponential and its use is the compiler's to keep.)
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
-        uint32_t r;
-        asm("v_cvt_pk_f16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-        return r;
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2));
+    }
+    // c + both values of the pair
+    static __device__ __forceinline__ float add_pair(uint32_t p, float c) {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, p), __builtin_bit_cast(v2, kOnes), c, false);
     }
     static __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
@@ -32,13 +36,15 @@ struct Fp16 {
 };
 
 struct Bf16 {
+    typedef __bf16 v2 __attribute__((ext_vector_type(2)));
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     static constexpr uint32_t kOnes = 0x3F803F80u;
     static __device__ __forceinline__ float widen(uint16_t b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
-        uint32_t r;
-        asm("v_cvt_pk_bf16_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
-        return r;
+        return __builtin_bit_cast(uint32_t, __builtin_convertvector((v2f{a, b}), v2));
+    }
+    static __device__ __forceinline__ float add_pair(uint32_t p, float c) {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, p), __builtin_bit_cast(v2, kOnes), c, false);
     }
     static __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);

@@ -2,8 +2,8 @@
 // or not, with grouped heads.
 //
 // A workgroup takes 32 W query rows of one sequence and head, a wave 32 of them (attn_tile.h), and
-// walks the keys in tiles of 64 that all waves share: K and V rows come by LDS DMA into two buffers,
-// the next tile's while this one is multiplied, one barrier a tile. Tiles past the diagonal are not
+// walks the keys in tiles of 64 that all waves share: K and V rows come by LDS DMA into NS buffers each,
+// the next tiles' while this one is multiplied, one barrier a tile. Tiles past the diagonal are not
 // loaded, only those that cross it are masked.
 //
 // The grid is laid out without reading cu_seqlens on the host: sequence b's tiles start at
@@ -26,7 +26,7 @@ struct PromptArgs {
 
 constexpr int kPromptKeys = 64;
 
-template <class T, int DP, int W, bool CAUSAL>
+template <class T, int DP, int W, int NS, bool CAUSAL>
 __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void prompt_attention_kernel(PromptArgs a)
 {
     using Rows = KvRows<DP>;
@@ -44,12 +44,14 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void prompt_attention_ker
     if (id < 0) return;
 
     auto cu = [&](int b) { return min(max(a.cu[b], 0), a.tokens); };
-    int b = 0;
-    for (int hi = a.sequences; b < hi;) {                           // the last b whose first tile is <= id
-        const int mid = (b + hi + 1) >> 1;
-        if (cu(mid) / kRows + mid <= id) b = mid;
-        else hi = mid - 1;
+    int b = 0;                                                       // the last b whose first tile is <= id,
+    for (int span = a.sequences + 1; span > 1;) {                    // 64 candidates at a time
+        const int step = (span + 63) / 64, c = b + static_cast<int>(threadIdx.x & (kWave - 1)) * step;
+        const bool on = c < min(b + span, a.sequences + 1) && cu(c) / kRows + c <= id;
+        b += max(__popcll(__ballot(on)) - 1, 0) * step;
+        span = step;
     }
+    b = __builtin_amdgcn_readfirstlane(min(b, a.sequences));
     const int start = cu(b);
     const int len = (b < a.sequences ? cu(b + 1) : a.tokens) - start;
     const int row0 = (id - (start / kRows + b)) * kRows;
@@ -84,13 +86,14 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void prompt_attention_ker
     const int end = CAUSAL ? min(row0 + kRows, len) : len;
     const int tiles = (end + kPromptKeys - 1) / kPromptKeys;
     const uint32_t lds0 = lds_address(lds);
-    auto load = [&](int t) {                                         // rows past the sequence's end read as zeros
+    // rows past the sequence's end read as zeros
+    auto load = [&](int t) {
         const int left = len - t * kPromptKeys;
         const v4i kr = row_rsrc(kbase + static_cast<size_t>(t) * kPromptKeys * a.k_token,
                                 static_cast<uint32_t>((kPromptKeys - 1) * a.k_token * 2 + 2 * a.D));
         const v4i vr = row_rsrc(vbase + static_cast<size_t>(t) * kPromptKeys * a.v_token,
                                 static_cast<uint32_t>((kPromptKeys - 1) * a.v_token * 2 + 2 * a.D));
-        const uint32_t ks = lds0 + (t & 1) * 2 * kTile;
+        const uint32_t ks = lds0 + (t % NS) * 2 * kTile;
 #pragma unroll
         for (int n = 0; n < kIns; n++)
             dma16_rows(kr, dma_row[n] < left ? koff[n] : kOutOfRange, ks + (wave * kIns + n) * 1024);
@@ -102,18 +105,23 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void prompt_attention_ker
     const int first = row0 + 32 * wave;
     const int mine = CAUSAL ? min(tiles, first / kPromptKeys + 1) : tiles;   // tiles that reach this wave's rows
     auto next = [&](int t) {
-        wait_vm_lgkm<0>();
+        if (t + NS - 1 <= tiles) wait_vm_lgkm<2 * kIns*(NS - 2)>();
+        else wait_vm_lgkm<0>();
         lds_barrier();                                               // tile t is whole, tile t - 1 is read
-        if (t + 1 < tiles) load(t + 1);
+        if (t + NS - 1 < tiles) load(t + NS - 1);
     };
-    load(0);
+#pragma unroll
+    for (int t = 0; t < NS - 1; t++)
+        if (t < tiles) load(t);
     int t = 0;
     for (; t < mine; t++) {
         next(t);
-        const int8_t* ks = lds + (t & 1) * 2 * kTile;
+        const int8_t* ks = lds + (t % NS) * 2 * kTile;
         const int k0 = t * kPromptKeys;
-        w.step(ks, ks + kTile, scale2, (CAUSAL && k0 + kPromptKeys - 1 > first) || k0 + kPromptKeys > len,
-               [&](int, int kb) { return bits_to((CAUSAL ? min(row, len - 1) : len - 1) - k0 - 32 * kb); });
+        v16f s[1][kPromptKeys / 32];
+        w.scores(ks, s);
+        w.finish(s, ks + kTile, scale2, (CAUSAL && k0 + kPromptKeys - 1 > first) || k0 + kPromptKeys > len,
+                 [&](int, int kb) { return bits_to((CAUSAL ? min(row, len - 1) : len - 1) - k0 - 32 * kb); });
     }
     for (; t < tiles; t++) next(t);
     const bool live = row < len;
@@ -148,31 +156,31 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void prompt_attention_ker
         }
 }
 
-template <class T, int DP, int W, bool CAUSAL>
+template <class T, int DP, int W, int NS, bool CAUSAL>
 int launch_prompt(PromptArgs a, hipStream_t s) {
-    constexpr int kLds = 4 * kPromptKeys * KvRows<DP>::kBytes;
+    constexpr int kLds = NS * 2 * kPromptKeys * KvRows<DP>::kBytes;
     const long long tiles = a.tokens / (32 * W) + static_cast<long long>(a.sequences) + 1;
     const long long units = tiles * a.Hkv, wgs = divupll(units, 8) * 8 * (a.Hq / a.Hkv);
     if (units > INT_MAX - 8 || wgs > INT_MAX) return FORGE_EINVAL;
     a.tiles = static_cast<int>(tiles);
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&prompt_attention_kernel<T, DP, W, CAUSAL>),
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&prompt_attention_kernel<T, DP, W, NS, CAUSAL>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (attr != hipSuccess) return static_cast<int>(attr);
-    prompt_attention_kernel<T, DP, W, CAUSAL><<<static_cast<unsigned>(wgs), 64 * W, kLds, s>>>(a);
+    prompt_attention_kernel<T, DP, W, NS, CAUSAL><<<static_cast<unsigned>(wgs), 64 * W, kLds, s>>>(a);
     return launch_status();
 }
 
-template <class T, int DP, int W>
+template <class T, int DP, int W, int NS>
 int launch_prompt(const PromptArgs& a, bool causal, hipStream_t s) {
-    return causal ? launch_prompt<T, DP, W, true>(a, s) : launch_prompt<T, DP, W, false>(a, s);
+    return causal ? launch_prompt<T, DP, W, NS, true>(a, s) : launch_prompt<T, DP, W, NS, false>(a, s);
 }
 
 template <class T>
 int launch_prompt(const PromptArgs& a, bool causal, hipStream_t s) {
-    if (a.D <= 64) return launch_prompt<T, 64, 4>(a, causal, s);
-    if (a.D <= 96) return launch_prompt<T, 96, 4>(a, causal, s);
-    if (a.D <= 128) return launch_prompt<T, 128, 4>(a, causal, s);
-    return launch_prompt<T, 256, 4>(a, causal, s);
+    if (a.D <= 64) return launch_prompt<T, 64, 4, 4>(a, causal, s);
+    if (a.D <= 96) return launch_prompt<T, 96, 4, 3>(a, causal, s);
+    if (a.D <= 128) return launch_prompt<T, 128, 4, 2>(a, causal, s);
+    return launch_prompt<T, 256, 4, 2>(a, causal, s);
 }
 
 }  // namespace forge_amd
