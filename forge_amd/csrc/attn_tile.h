@@ -192,10 +192,14 @@ struct AttnWave {
         if constexpr (RB == 1) interleave<2 * KB * kOut, 2, kAhead>();
     }
 
-    // A tile from its scores on; masked if `masked` (uniform).
+    // A tile from its scores on; masked if `masked`. `first`: nothing has been summed yet. (Both uniform.)
     template <class Seen>
-    __device__ __forceinline__ void finish(Scores& s, const int8_t* vs, float scale2, bool masked, const Seen& seen) {
+    __device__ __forceinline__ void finish(Scores& s, const int8_t* vs, float scale2, bool first, bool masked, const Seen& seen) {
         if (masked) mask(s, seen);
+        if (first) {
+#pragma unroll
+            for (int b = 0; b < RB; b++) m[b] = fmaxf(m[b], largest(s, b, scale2));
+        }
         Weights p;
         float sum[RB], mx[RB];
         bool grown = false;

@@ -31,7 +31,8 @@ struct CacheArgs {
     const int64_t* tree;
     uint16_t* out;
     float *part, *stat;  // (B, Hkv, chunks, rows, D) sums and (.., rows, 2) maxima and sums of the chunks
-    int B, T, Hq, Hkv, D, pages, page_shift, width, chunk, chunks;
+    int B, T, Hq, Hkv, D, pages, page_shift, width, chunk, chunks, group, sets;
+    uint32_t mg_group, mg_sets;   // udiv_magic multipliers
     float scale;
 };
 
@@ -55,11 +56,8 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
     __shared__ float stat_m[W][32], stat_l[W][32];
     __shared__ int odd_rows;
 
-    const int group = a.Hq / a.Hkv, rows = a.T * group, sets = (rows + 32 * RS - 1) / (32 * RS);
-    int id = blockIdx.x;
-    const int hk = id % a.Hkv; id /= a.Hkv;
-    const int set = id % sets; id /= sets;
-    const int chunk = id % a.chunks, b = id / a.chunks;
+    const int group = a.group, rows = a.T * group;
+    const int hk = blockIdx.x, chunk = blockIdx.y, b = udiv_magic(blockIdx.z, a.mg_sets), set = blockIdx.z - b * a.sets;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x & (kWave - 1);
     const int rs = wave / KS, ks = wave % KS;
@@ -81,11 +79,11 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
                                                 token) + static_cast<size_t>(hk) * a.D);
     };
     auto row_of = [&](auto* base, int r) {                     // of q and out
-        const int t = r / group;
+        const int t = udiv_magic(r, a.mg_group);
         return base + ((static_cast<size_t>(b) * a.T + t) * a.Hq + hk * group + (r - t * group)) * a.D;
     };
     auto drafts_of = [&](int r) {                                    // the new tokens that row r sees
-        const int t = r / group;
+        const int t = udiv_magic(r, a.mg_group);
         return a.tree ? static_cast<unsigned long long>(a.tree[static_cast<size_t>(b) * a.T + t]) : ~0ull >> (63 - t);
     };
 
@@ -132,7 +130,7 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
         const int8_t* at = lds + (t & 1) * 2 * kTile + 32 * KB * ks * Rows::kBytes;
         v16f s[1][KB];
         w.scores(at, s);
-        w.finish(s, at + kTile, scale2, k0 + 32 * KB > min(open, n), [&](int, int kb) {
+        w.finish(s, at + kTile, scale2, t == 0, k0 + 32 * KB > min(open, n), [&](int, int kb) {
             const int d = open - (k0 + 32 * kb);                     // bits below d: the cache; from d on: drafts
             uint32_t bits = bits_to(d - 1);
             if (d < 32) bits |= d >= 0 ? static_cast<uint32_t>(drafts << d) : d > -64 ? static_cast<uint32_t>(drafts >> -d) : 0u;
@@ -146,16 +144,18 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
     if (w.odd(0, live) && lane == 0) atomicOr(&odd_rows, 1);
     float* sums = reinterpret_cast<float*>(lds);
     const float lane_l = half_sum(w.l[0]);
-    if (lane < 32) {
-        stat_m[wave][lane] = w.m[0];
-        stat_l[wave][lane] = lane_l;
+    if constexpr (KS > 1) {
+        if (lane < 32) {
+            stat_m[wave][lane] = w.m[0];
+            stat_l[wave][lane] = lane_l;
+        }
+#pragma unroll
+        for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<v4f*>(sums + (wave * 32 + (lane & 31)) * kPitch + 32 * j + 2 * e + 4 * (lane >> 5)) =
+                    v4f{w.o[0][j][e], w.o[0][j][e + 1], w.o[0][j][e + 2], w.o[0][j][e + 3]};
     }
-#pragma unroll
-    for (int j = 0; j < DP / 32; j++)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4)
-            *reinterpret_cast<v4f*>(sums + (wave * 32 + (lane & 31)) * kPitch + 32 * j + 2 * e + 4 * (lane >> 5)) =
-                v4f{w.o[0][j][e], w.o[0][j][e + 1], w.o[0][j][e + 2], w.o[0][j][e + 3]};
     __syncthreads();
     const bool whole = keys <= a.chunk;                              // the only chunk: the result itself
     const size_t part0 = ((static_cast<size_t>(b) * a.Hkv + hk) * a.chunks + chunk) * rows;
@@ -192,10 +192,31 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
         }
         return;
     }
-    const int quads = a.D / 4;
-    for (int i = threadIdx.x; i < 32 * RS * quads; i += 64 * W) {
-        const int lr = i / quads, d = 4 * (i - lr * quads), r = set * RS * 32 + lr;
+    if constexpr (KS == 1) {
+        if (!live) return;
+        const float inv = lane_l > 0.0f ? 1.0f / lane_l : 0.0f;
+        float* part = a.part + (part0 + row) * a.D;
+        uint16_t* out = row_of(a.out, row);
+#pragma unroll
+        for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int d = 32 * j + 2 * e + 4 * (lane >> 5);
+                if (d >= a.D) continue;
+                const v4f s = {w.o[0][j][e], w.o[0][j][e + 1], w.o[0][j][e + 2], w.o[0][j][e + 3]};
+                if (whole) *reinterpret_cast<v2u*>(out + d) = v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
+                else *reinterpret_cast<v4f*>(part + d) = s;
+            }
+        if (!whole && lane < 32) {
+            a.stat[(part0 + row) * 2] = w.m[0];
+            a.stat[(part0 + row) * 2 + 1] = lane_l;
+        }
+        return;
+    }
+    for (int i = threadIdx.x; i < 32 * RS * (DP / 4); i += 64 * W) {
+        const int lr = i / (DP / 4), d = 4 * (i % (DP / 4)), r = set * RS * 32 + lr;
         if (r >= rows) break;
+        if (d >= a.D) continue;
         const int w0 = (lr / 32) * KS, x = lr % 32;
         float m = kNoScore, l = 0.0f;
 #pragma unroll
@@ -222,60 +243,62 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
     }
 }
 
-// A wave joins one row's chunks: LPR lanes of 4 values take every (64 / LPR)-th chunk, four in flight.
+// A wave joins one row's chunks: LPR lanes of 4 values take every (64 / LPR)-th chunk, four in flight, with the
+// running maximum of a softmax, and the lanes' sums are joined in a fixed order. The first ones are loaded before the
+// sequence's length is there.
 template <class T, int LPR>
 __global__ __launch_bounds__(256) void cache_join_kernel(CacheArgs a)
 {
     constexpr int kSets = kWave / LPR;
     const int lane = threadIdx.x & (kWave - 1), sub = lane / LPR, d = 4 * (lane % LPR);
-    const long long id = static_cast<long long>(blockIdx.x) * 4 + threadIdx.x / kWave;
-    const int group = a.Hq / a.Hkv, rows = a.T * group;
-    if (id >= static_cast<long long>(a.B) * a.T * a.Hq) return;
-    const int h = static_cast<int>(id % a.Hq), t = static_cast<int>(id / a.Hq % a.T);
-    const int b = static_cast<int>(id / (static_cast<long long>(a.Hq) * a.T));
-    const int keys = cache_keys(a, b), used = (keys + a.chunk - 1) / a.chunk;
-    if (used <= 1) return;                                           // the only chunk has written the result
-    const int hk = h / group, r = t * group + h - hk * group;
+    const int t = blockIdx.y, b = blockIdx.z, h = blockIdx.x * 4 + threadIdx.x / kWave;
+    if (h >= a.Hq) return;
+    const int rows = a.T * a.group;
+    const int hk = udiv_magic(h, a.mg_group), r = t * a.group + h - hk * a.group;
     const size_t first = (static_cast<size_t>(b) * a.Hkv + hk) * a.chunks;
-    auto at = [&](int c) { return (first + c) * rows + r; };
-    float m = kNoScore;
-    for (int c = lane; c < used; c += kWave) m = fmaxf(m, a.stat[at(c) * 2]);
-    m = wave_max(m);
-    float l = 0.0f, s[4] = {0.0f, 0.0f, 0.0f, 0.0f};
     const bool in = d < a.D;
-    for (int c0 = sub; c0 < used; c0 += 4 * kSets) {
+    float m = kNoScore, l = 0.0f;
+    v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
+    int used = a.chunks;
+    for (int c0 = sub; c0 - sub < used; c0 += 4 * kSets) {
         v4f x[4];
-        float cm[4], cl[4];
+        v2f st[4];
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const int c = c0 + u * kSets;
-            const bool on = c < used;
-            cm[u] = on ? a.stat[at(c) * 2] : kNoScore;
-            cl[u] = on ? a.stat[at(c) * 2 + 1] : 0.0f;
-            x[u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-            if (on && in) x[u] = *reinterpret_cast<const v4f*>(a.part + at(c) * a.D + d);
+            const size_t at = (first + min(c0 + u * kSets, a.chunks - 1)) * rows + r;
+            st[u] = *reinterpret_cast<const v2f*>(a.stat + at * 2);
+            x[u] = *reinterpret_cast<const v4f*>(a.part + at * a.D + (in ? d : 0));
+        }
+        if (c0 == sub) {
+            used = (cache_keys(a, b) + a.chunk - 1) / a.chunk;
+            if (used <= 1) return;                                   // the only chunk has written the result
         }
 #pragma unroll
         for (int u = 0; u < 4; u++) {
-            const float f = __builtin_amdgcn_exp2f(cm[u] - m);
-            l = __builtin_fmaf(f, cl[u], l);
+            if (c0 + u * kSets >= used) continue;
+            const float mn = fmaxf(m, st[u][0]);
+            const float f = __builtin_amdgcn_exp2f(m - mn), g = __builtin_amdgcn_exp2f(st[u][0] - mn);
+            m = mn;
+            l = __builtin_fmaf(l, f, st[u][1] * g);
 #pragma unroll
-            for (int e = 0; e < 4; e++) s[e] = __builtin_fmaf(f, x[u][e], s[e]);
+            for (int e = 0; e < 4; e++) s[e] = __builtin_fmaf(s[e], f, x[u][e] * g);
         }
     }
 #pragma unroll
     for (int o = LPR; o < kWave; o <<= 1) {
-        l += __shfl_xor(l, o, kWave);
+        const float om = __shfl_xor(m, o, kWave), mn = fmaxf(m, om);
+        const float f = __builtin_amdgcn_exp2f(m - mn), g = __builtin_amdgcn_exp2f(om - mn);
+        m = mn;
+        l = l * f + __shfl_xor(l, o, kWave) * g;
 #pragma unroll
-        for (int e = 0; e < 4; e++) s[e] += __shfl_xor(s[e], o, kWave);
+        for (int e = 0; e < 4; e++) s[e] = s[e] * f + __shfl_xor(s[e], o, kWave) * g;
     }
     const float inv = l != 0.0f ? 1.0f / l : 0.0f;
     if (in && sub == 0)
-        *reinterpret_cast<v2u*>(a.out + id * a.D + d) = v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
+        *reinterpret_cast<v2u*>(a.out + ((static_cast<size_t>(b) * a.T + t) * a.Hq + h) * a.D + d) =
+            v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
 }
 
-// Chunks such that the longest sequences make about three workgroups per CU, of 128 keys (one tile for
-// each of four waves) at least.
 inline int cache_row(int D) { return D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256; }
 
 CachePlan cache_plan(int B, int T, int Hq, int Hkv, int D, long long max_keys) {
@@ -295,20 +318,23 @@ size_t cache_floats(int B, int T, int Hq, int D, const CachePlan& p) {
 }
 
 template <class T, int DP, int RS, int KS, int KB>
-int launch_cache(const CacheArgs& a, hipStream_t s) {
-    constexpr int kTiles = 4 * 32 * KS * KB * KvRows<DP>::kBytes, kSums = RS * KS * 32 * (DP + 4) * 4;
+int launch_cache(CacheArgs a, hipStream_t s) {
+    constexpr int kTiles = 4 * 32 * KS * KB * KvRows<DP>::kBytes, kSums = KS > 1 ? RS * KS * 32 * (DP + 4) * 4 : 0;
     constexpr int kLds = kTiles > kSums ? kTiles : kSums, LPR = DP <= 64 ? 16 : DP <= 128 ? 32 : 64;
     const int rows = a.T * (a.Hq / a.Hkv);
-    const long long wgs = static_cast<long long>(a.B) * a.Hkv * divup(rows, 32 * RS) * a.chunks;
-    if (wgs > INT_MAX) return FORGE_EINVAL;
+    a.sets = divup(rows, 32 * RS);
+    a.mg_sets = udiv_multiplier(a.sets);
+    const long long z = static_cast<long long>(a.B) * a.sets;
+    if (a.chunks > 65535 || z > 65535) return FORGE_EINVAL;
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&cache_attention_kernel<T, DP, RS, KS, KB>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (attr != hipSuccess) return static_cast<int>(attr);
-    cache_attention_kernel<T, DP, RS, KS, KB><<<static_cast<unsigned>(wgs), 64 * RS * KS, kLds, s>>>(a);
+    const dim3 grid(static_cast<unsigned>(a.Hkv), static_cast<unsigned>(a.chunks), static_cast<unsigned>(z));
+    cache_attention_kernel<T, DP, RS, KS, KB><<<grid, 64 * RS * KS, kLds, s>>>(a);
     const int st = launch_status();
     if (st != FORGE_OK || a.chunks == 1) return st;
-    const long long all = static_cast<long long>(a.B) * a.T * a.Hq;
-    cache_join_kernel<T, LPR><<<static_cast<unsigned>(divupll(all, 4)), 256, 0, s>>>(a);
+    const dim3 rows_grid(static_cast<unsigned>(divup(a.Hq, 4)), static_cast<unsigned>(a.T), static_cast<unsigned>(a.B));
+    cache_join_kernel<T, LPR><<<rows_grid, 256, 0, s>>>(a);
     return launch_status();
 }
 
@@ -363,7 +389,7 @@ extern "C" int forge_cache_attention(const uint16_t* q, const uint16_t* k_cache,
                           static_cast<const void*>(out), static_cast<const void*>(workspace)})
         if (!aligned(p, 16)) return FORGE_EINVAL;
     const long long max_keys = static_cast<long long>(table_width) * page_size;
-    if (max_keys > INT_MAX - kCacheMaxChunk) return FORGE_EINVAL;
+    if (max_keys > 1 << 27) return FORGE_EINVAL;
     const CachePlan p = cache_plan(B, T, Hq, Hkv, D, max_keys);
     const size_t floats = cache_floats(B, T, Hq, D, p);
     if (floats && (!workspace || workspace_bytes < 4 * floats)) return FORGE_EINVAL;
@@ -371,7 +397,7 @@ extern "C" int forge_cache_attention(const uint16_t* q, const uint16_t* k_cache,
     const size_t parts = static_cast<size_t>(B) * T * Hq * p.chunks;
     const CacheArgs a{q, k_cache, v_cache, page_table, cache_lens, tree, out, part, part ? part + parts * D : nullptr,
                       B, T, Hq, Hkv, D, pages, __builtin_ctz(static_cast<unsigned>(page_size)), table_width,
-                      p.chunk, p.chunks, scale};
+                      p.chunk, p.chunks, Hq / Hkv, 1, udiv_multiplier(Hq / Hkv), 0u, scale};
     hipStream_t s = as_stream(stream);
     return dtype == FORGE_FP16 ? launch_cache<Fp16>(a, p.sets, s) : launch_cache<Bf16>(a, p.sets, s);
 }

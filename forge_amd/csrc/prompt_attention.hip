@@ -1,8 +1,8 @@
 // Attention over whole prompts packed without padding: softmax(scale Q K^T) V within each sequence, causal
 // or not, with grouped heads.
 //
-// A workgroup takes 32 W query rows of one sequence and head, a wave 32 of them (attn_tile.h), and
-// walks the keys in tiles of 64 that all waves share: K and V rows come by LDS DMA into NS buffers each,
+// A workgroup of RS x KS waves takes 32 RS query rows of one sequence and head, a wave 32 of them (attn_tile.h)
+// and 64 keys of each tile of 64 KS, which all waves share: K and V rows come by LDS DMA into NS buffers each,
 // the next tiles' while this one is multiplied, one barrier a tile. Tiles past the diagonal are not
 // loaded, only those that cross it are masked.
 //
@@ -20,27 +20,29 @@ struct PromptArgs {
     uint16_t* out;
     const int32_t* cu;
     long long q_token, q_head, k_token, k_head, v_token, v_head;
-    int sequences, tokens, Hq, Hkv, D, tiles;
+    int sequences, tokens, Hq, Hkv, D, tiles, group;
+    uint32_t mg_group, mg_hkv;   // udiv_magic multipliers
     float scale;
 };
 
 constexpr int kPromptKeys = 64;
 
-template <class T, int DP, int W, int NS, bool CAUSAL>
-__global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void prompt_attention_kernel(PromptArgs a)
+template <class T, int DP, int RS, int KS, int NS, bool CAUSAL>
+__global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void prompt_attention_kernel(PromptArgs a)
 {
     using Rows = KvRows<DP>;
-    constexpr int kRows = 32 * W, kTile = kPromptKeys * Rows::kBytes;
-    constexpr int kIns = kPromptKeys * Rows::kChunks / kWave / W;   // DMA instructions per wave, tile and tensor
-    static_assert(kPromptKeys * Rows::kChunks % (kWave * W) == 0, "a tile splits evenly over the waves");
-    extern __shared__ __align__(1024) int8_t lds[];                 // K, V of buffer 0, then of buffer 1
+    constexpr int W = RS * KS, kRows = 32 * RS, kKeys = kPromptKeys * KS, kTile = kKeys * Rows::kBytes;
+    constexpr int kIns = kKeys * Rows::kChunks / kWave / W, kPitch = DP + 4;   // DMA instructions per wave, tile and tensor
+    static_assert(kKeys * Rows::kChunks % (kWave * W) == 0, "a tile splits evenly over the waves");
+    extern __shared__ __align__(1024) int8_t lds[];                 // K, V of buffer 0, then of buffer 1 ...
 
-    const int group = a.Hq / a.Hkv;
+    const int group = a.group;
     // Query tiles from the last (the longest in a causal prompt) on; units (tile, KV head) go round
     // the 8 XCDs, whose workgroups are dealt in turn, so that the heads of a group meet in one L2.
     const int xcd = blockIdx.x & 7, i = blockIdx.x >> 3;
-    const int unit = (i / group) * 8 + xcd, hk = unit % a.Hkv, hq = hk * group + i % group;
-    const int id = a.tiles - 1 - unit / a.Hkv;
+    const int ig = udiv_magic(i, a.mg_group), unit = ig * 8 + xcd, tile = udiv_magic(unit, a.mg_hkv);
+    const int hk = unit - tile * a.Hkv, hq = hk * group + i - ig * group;
+    const int id = a.tiles - 1 - tile;
     if (id < 0) return;
 
     auto cu = [&](int b) { return min(max(a.cu[b], 0), a.tokens); };
@@ -59,11 +61,11 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void prompt_attention_ker
 
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x & (kWave - 1);
-    const int row = row0 + 32 * wave + (lane & 31);
+    const int rs = wave / KS, ks = wave % KS, row = row0 + 32 * rs + (lane & 31);
     uint16_t* out = a.out + (static_cast<size_t>(start + row) * a.Hq + hq) * a.D;
     if (b == a.sequences) {                                          // rows after the last sequence
         for (int d = 4 * (lane >> 5); d < a.D; d += 8)
-            if (row < len) *reinterpret_cast<v2u*>(out + d) = v2u{0u, 0u};
+            if (row < len && ks == 0) *reinterpret_cast<v2u*>(out + d) = v2u{0u, 0u};
         return;
     }
 
@@ -84,26 +86,27 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void prompt_attention_ker
         voff[n] = 8 * cv < a.D ? static_cast<uint32_t>(r * a.v_token * 2 + 16 * cv) : kOutOfRange;
     }
     const int end = CAUSAL ? min(row0 + kRows, len) : len;
-    const int tiles = (end + kPromptKeys - 1) / kPromptKeys;
+    const int tiles = (end + kKeys - 1) / kKeys;
     const uint32_t lds0 = lds_address(lds);
     // rows past the sequence's end read as zeros
     auto load = [&](int t) {
-        const int left = len - t * kPromptKeys;
-        const v4i kr = row_rsrc(kbase + static_cast<size_t>(t) * kPromptKeys * a.k_token,
-                                static_cast<uint32_t>((kPromptKeys - 1) * a.k_token * 2 + 2 * a.D));
-        const v4i vr = row_rsrc(vbase + static_cast<size_t>(t) * kPromptKeys * a.v_token,
-                                static_cast<uint32_t>((kPromptKeys - 1) * a.v_token * 2 + 2 * a.D));
-        const uint32_t ks = lds0 + (t % NS) * 2 * kTile;
+        const int left = len - t * kKeys;
+        const v4i kr = row_rsrc(kbase + static_cast<size_t>(t) * kKeys * a.k_token,
+                                static_cast<uint32_t>((kKeys - 1) * a.k_token * 2 + 2 * a.D));
+        const v4i vr = row_rsrc(vbase + static_cast<size_t>(t) * kKeys * a.v_token,
+                                static_cast<uint32_t>((kKeys - 1) * a.v_token * 2 + 2 * a.D));
+        const uint32_t to = lds0 + (t % NS) * 2 * kTile;
 #pragma unroll
         for (int n = 0; n < kIns; n++)
-            dma16_rows(kr, dma_row[n] < left ? koff[n] : kOutOfRange, ks + (wave * kIns + n) * 1024);
+            dma16_rows(kr, dma_row[n] < left ? koff[n] : kOutOfRange, to + (wave * kIns + n) * 1024);
 #pragma unroll
         for (int n = 0; n < kIns; n++)
-            dma16_rows(vr, dma_row[n] < left ? voff[n] : kOutOfRange, ks + kTile + (wave * kIns + n) * 1024);
+            dma16_rows(vr, dma_row[n] < left ? voff[n] : kOutOfRange, to + kTile + (wave * kIns + n) * 1024);
     };
     const float scale2 = a.scale * 1.44269504f;
-    const int first = row0 + 32 * wave;
-    const int mine = CAUSAL ? min(tiles, first / kPromptKeys + 1) : tiles;   // tiles that reach this wave's rows
+    const int first = row0 + 32 * rs, ahead = first - kPromptKeys * ks;
+    // tiles that reach this wave's rows
+    const int mine = !CAUSAL ? tiles : ahead < 0 ? 0 : min(tiles, ahead / kKeys + 1);
     auto next = [&](int t) {
         if (t + NS - 1 <= tiles) wait_vm_lgkm<2 * kIns*(NS - 2)>();
         else wait_vm_lgkm<0>();
@@ -116,71 +119,128 @@ __global__ __launch_bounds__(64 * W, DP > 128 ? 1 : 2) void prompt_attention_ker
     int t = 0;
     for (; t < mine; t++) {
         next(t);
-        const int8_t* ks = lds + (t % NS) * 2 * kTile;
-        const int k0 = t * kPromptKeys;
+        const int8_t* at = lds + (t % NS) * 2 * kTile + kPromptKeys * ks * Rows::kBytes;
+        const int k0 = t * kKeys + kPromptKeys * ks;
         v16f s[1][kPromptKeys / 32];
-        w.scores(ks, s);
-        w.finish(s, ks + kTile, scale2, (CAUSAL && k0 + kPromptKeys - 1 > first) || k0 + kPromptKeys > len,
+        w.scores(at, s);
+        w.finish(s, at + kTile, scale2, t == 0, (CAUSAL && k0 + kPromptKeys - 1 > first) || k0 + kPromptKeys > len,
                  [&](int, int kb) { return bits_to((CAUSAL ? min(row, len - 1) : len - 1) - k0 - 32 * kb); });
     }
     for (; t < tiles; t++) next(t);
     const bool live = row < len;
-    if (w.odd(0, live)) {
-        for (int r = 0; r < 32; r++) {
-            const int rr = row0 + 32 * wave + r;
-            if (rr >= len) break;
+    auto out_row = [&](int r) { return a.out + (static_cast<size_t>(start + r) * a.Hq + hq) * a.D; };
+    // some row's sum is not finite: rows r0, r0 + step, ... of the workgroup again, key by key
+    auto again = [&](int r0, int end, int step) {
+        for (int r = row0 + r0; r < min(row0 + end, len); r += step) {
             float m, l, acc[(DP + 63) / 64];
             attn_row<T, DP>(
-                a.q + static_cast<size_t>(start + rr) * a.q_token + hq * a.q_head, a.D, CAUSAL ? rr + 1 : len, scale2,
+                a.q + static_cast<size_t>(start + r) * a.q_token + hq * a.q_head, a.D, CAUSAL ? r + 1 : len, scale2,
                 [&](int j) { return kbase + static_cast<size_t>(j) * a.k_token; },
                 [&](int j) { return vbase + static_cast<size_t>(j) * a.v_token; }, [](int) { return true; }, m, l, acc);
             const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-            uint16_t* o = a.out + (static_cast<size_t>(start + rr) * a.Hq + hq) * a.D;
 #pragma unroll
             for (int c = 0; c < (DP + 63) / 64; c++)
-                if (lane + 64 * c < a.D) o[lane + 64 * c] = narrow<T>(acc[c] * inv);
+                if (lane + 64 * c < a.D) out_row(r)[lane + 64 * c] = narrow<T>(acc[c] * inv);
         }
-        return;
-    }
+    };
     const float l = half_sum(w.l[0]);
-    const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-    if (!live) return;
-#pragma unroll
-    for (int j = 0; j < DP / 32; j++)
-#pragma unroll
-        for (int e = 0; e < 16; e += 4) {
-            const int d = 32 * j + 2 * e + 4 * (lane >> 5);
-            if (d < a.D)
-                *reinterpret_cast<v2u*>(out + d) = v2u{T::pack(w.o[0][j][e] * inv, w.o[0][j][e + 1] * inv),
-                                                       T::pack(w.o[0][j][e + 2] * inv, w.o[0][j][e + 3] * inv)};
+    if constexpr (KS == 1) {
+        if (w.odd(0, live)) {
+            again(32 * rs, 32 * rs + 32, 1);
+            return;
         }
+        const float inv = l > 0.0f ? 1.0f / l : 0.0f;
+        if (!live) return;
+#pragma unroll
+        for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4) {
+                const int d = 32 * j + 2 * e + 4 * (lane >> 5);
+                if (d < a.D)
+                    *reinterpret_cast<v2u*>(out + d) = v2u{T::pack(w.o[0][j][e] * inv, w.o[0][j][e + 1] * inv),
+                                                           T::pack(w.o[0][j][e + 2] * inv, w.o[0][j][e + 3] * inv)};
+            }
+    } else {
+        // join the waves of a row set, in wave order
+        __shared__ float stat_m[W][32], stat_l[W][32];
+        __shared__ int odd_rows;
+        float* sums = reinterpret_cast<float*>(lds);
+        if (threadIdx.x == 0) odd_rows = 0;
+        wait_vm_lgkm<0>();
+        __syncthreads();
+        if (w.odd(0, live) && lane == 0) atomicOr(&odd_rows, 1);
+        if (lane < 32) {
+            stat_m[wave][lane] = w.m[0];
+            stat_l[wave][lane] = l;
+        }
+#pragma unroll
+        for (int j = 0; j < DP / 32; j++)
+#pragma unroll
+            for (int e = 0; e < 16; e += 4)
+                *reinterpret_cast<v4f*>(sums + (wave * 32 + (lane & 31)) * kPitch + 32 * j + 2 * e + 4 * (lane >> 5)) =
+                    v4f{w.o[0][j][e], w.o[0][j][e + 1], w.o[0][j][e + 2], w.o[0][j][e + 3]};
+        __syncthreads();
+        if (odd_rows) {
+            again(wave, kRows, W);
+            return;
+        }
+        for (int i = threadIdx.x; i < kRows * (DP / 4); i += 64 * W) {
+            const int lr = i / (DP / 4), d = 4 * (i % (DP / 4)), w0 = (lr / 32) * KS, x = lr % 32;
+            if (row0 + lr >= len) break;
+            if (d >= a.D) continue;
+            float m = kNoScore, sum = 0.0f;
+#pragma unroll
+            for (int v = 0; v < KS; v++) m = fmaxf(m, stat_m[w0 + v][x]);
+            v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int v = 0; v < KS; v++) {
+                const float f = __builtin_amdgcn_exp2f(stat_m[w0 + v][x] - m);
+                sum = __builtin_fmaf(f, stat_l[w0 + v][x], sum);
+                const v4f y = *reinterpret_cast<const v4f*>(sums + ((w0 + v) * 32 + x) * kPitch + d);
+#pragma unroll
+                for (int e = 0; e < 4; e++) s[e] = __builtin_fmaf(f, y[e], s[e]);
+            }
+            const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
+            *reinterpret_cast<v2u*>(out_row(row0 + lr) + d) =
+                v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
+        }
+    }
 }
 
-template <class T, int DP, int W, int NS, bool CAUSAL>
+template <class T, int DP, int RS, int KS, int NS, bool CAUSAL>
 int launch_prompt(PromptArgs a, hipStream_t s) {
-    constexpr int kLds = NS * 2 * kPromptKeys * KvRows<DP>::kBytes;
-    const long long tiles = a.tokens / (32 * W) + static_cast<long long>(a.sequences) + 1;
+    constexpr int kTiles = NS * 2 * kPromptKeys * KS * KvRows<DP>::kBytes, kSums = KS > 1 ? RS * KS * 32 * (DP + 4) * 4 : 0;
+    constexpr int kLds = kTiles > kSums ? kTiles : kSums;
+    const long long tiles = a.tokens / (32 * RS) + static_cast<long long>(a.sequences) + 1;
     const long long units = tiles * a.Hkv, wgs = divupll(units, 8) * 8 * (a.Hq / a.Hkv);
-    if (units > INT_MAX - 8 || wgs > INT_MAX) return FORGE_EINVAL;
+    // udiv_magic's range; 2^31 / 65536 tiles of heads at least
+    if ((units + 8) * a.Hkv >= 1LL << 32 || wgs * a.group >= 1LL << 32 || wgs > INT_MAX) return FORGE_EINVAL;
+    a.mg_group = udiv_multiplier(a.group);
+    a.mg_hkv = udiv_multiplier(a.Hkv);
     a.tiles = static_cast<int>(tiles);
-    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&prompt_attention_kernel<T, DP, W, NS, CAUSAL>),
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&prompt_attention_kernel<T, DP, RS, KS, NS, CAUSAL>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
     if (attr != hipSuccess) return static_cast<int>(attr);
-    prompt_attention_kernel<T, DP, W, NS, CAUSAL><<<static_cast<unsigned>(wgs), 64 * W, kLds, s>>>(a);
+    prompt_attention_kernel<T, DP, RS, KS, NS, CAUSAL><<<static_cast<unsigned>(wgs), 64 * RS * KS, kLds, s>>>(a);
     return launch_status();
 }
 
-template <class T, int DP, int W, int NS>
+template <class T, int DP, int RS, int KS, int NS>
 int launch_prompt(const PromptArgs& a, bool causal, hipStream_t s) {
-    return causal ? launch_prompt<T, DP, W, NS, true>(a, s) : launch_prompt<T, DP, W, NS, false>(a, s);
+    return causal ? launch_prompt<T, DP, RS, KS, NS, true>(a, s) : launch_prompt<T, DP, RS, KS, NS, false>(a, s);
 }
 
+// While workgroups of 128 rows are fewer than the CUs, the time is that of the longest sequence's chain of
+// tiles: 64 rows a workgroup then, and two waves for each 32 that take 64 keys each of a tile. us, 128 rows /
+// 64, heads of 64: 16 heads of 512 tokens 11.3 / 9.0, 1024 19.1 / 13.6, 2048 34.7 / 27.4; 32 heads of 2048 (544
+// workgroups) 39.7 / 51.4; 64 tokens 4.7 / 5.7.
 template <class T>
 int launch_prompt(const PromptArgs& a, bool causal, hipStream_t s) {
-    if (a.D <= 64) return launch_prompt<T, 64, 4, 4>(a, causal, s);
-    if (a.D <= 96) return launch_prompt<T, 96, 4, 3>(a, causal, s);
-    if (a.D <= 128) return launch_prompt<T, 128, 4, 2>(a, causal, s);
-    return launch_prompt<T, 256, 4, 2>(a, causal, s);
+    const bool few = a.tokens >= 256 && (a.tokens / 128 + static_cast<long long>(a.sequences)) * a.Hq < default_cu_count();
+    if (a.D <= 64) return few ? launch_prompt<T, 64, 2, 2, 3>(a, causal, s) : launch_prompt<T, 64, 4, 1, 4>(a, causal, s);
+    if (a.D <= 96) return few ? launch_prompt<T, 96, 2, 2, 2>(a, causal, s) : launch_prompt<T, 96, 4, 1, 3>(a, causal, s);
+    if (a.D <= 128) return few ? launch_prompt<T, 128, 2, 2, 2>(a, causal, s) : launch_prompt<T, 128, 4, 1, 2>(a, causal, s);
+    return launch_prompt<T, 256, 4, 1, 2>(a, causal, s);
 }
 
 }  // namespace forge_amd
@@ -204,7 +264,7 @@ extern "C" int forge_prompt_attention(const uint16_t* q, const uint16_t* k, cons
     for (long long st : {q_token, q_head, k_token, k_head, v_token, v_head})
         if (st < 0 || st % 8 != 0 || st > (1 << 23)) return FORGE_EINVAL;
     const PromptArgs a{q, k, v, out, cu_seqlens, q_token, q_head, k_token, k_head, v_token, v_head,
-                       sequences, tokens, Hq, Hkv, D, 0, scale};
+                       sequences, tokens, Hq, Hkv, D, 0, Hq / Hkv, 0u, 0u, scale};
     hipStream_t s = as_stream(stream);
     return dtype == FORGE_FP16 ? launch_prompt<Fp16>(a, causal != 0, s) : launch_prompt<Bf16>(a, causal != 0, s);
 }
