@@ -96,7 +96,7 @@ PyObject* int4_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // qk_norm_rope(q, k, v, q_weight, k_weight, cos, sin, positions, q_out, k_out, k_cache, v_cache, slots, eps,
-// interleaved, device, stream): with k_out, or with v, k_cache, v_cache and slots
+// interleaved, device, stream): with k_out, with v, k_cache, v_cache and slots, or with both
 PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return call<17>(args, n, [](const Call& c) -> long {
         const at::Tensor* q0 = tensor(c.a[0]);
@@ -116,9 +116,9 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (!c.none(3) && !dense(qw = tensor(c.a[3]), type, c.device, {D})) return kNotInOrder;
         if (!c.none(4) && !dense(kw = tensor(c.a[4]), type, c.device, {D})) return kNotInOrder;
         int64_t rows = 0;
-        if (!c.none(9)) {
-            if (!dense(k_out = tensor(c.a[9]), type, c.device, {T, k.heads, D})) return kNotInOrder;
-        } else {
+        if (c.none(9) && c.none(10)) return kNotInOrder;
+        if (!c.none(9) && !dense(k_out = tensor(c.a[9]), type, c.device, {T, k.heads, D})) return kNotInOrder;
+        if (!c.none(10)) {
             kc = tensor(c.a[10]);
             if (!kc || kc->dim() != 4 || !v.take(c.a[2], type, c.device) || v.tokens != T || v.heads != k.heads || v.D != D)
                 return kNotInOrder;

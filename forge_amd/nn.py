@@ -14,6 +14,10 @@ reference's outputs. w_meta_from_reference / w_meta_to_reference convert a whole
 device.
 
 Forward runs the library (forge_int8_linear / forge_sparse_int8_linear); there is no other path.
+
+Without a counterpart in the reference: Int4Linear (4-bit weights with group scales, for the few tokens of a
+decode step) and DecoderAttention (the attention block of a decoder on it: projection, norm and rotation of the heads,
+attention over prompts or over a paged cache). Both serve only: no backward.
 """
 from __future__ import annotations
 
@@ -200,6 +204,120 @@ class SparseLinear(nn.Module):
     def extra_repr(self) -> str:
         return (f"in_features={self.in_features}, out_features={self.out_features}, "
                 f"bias={self.bias is not None}, sparse=2:4")
+
+
+class _Int4LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, w_int4, w_scale, bias):
+        return ops.int4_linear(x, w_int4, w_scale, bias)
+
+    @staticmethod
+    def backward(ctx, grad_output):
+        raise NotImplementedError("Int4Linear has no backward")
+
+
+class Int4Linear(nn.Module):
+    """Linear layer with 4-bit weights and an FP16 scale per group_size (32, 64 or 128) values of a row:
+    y = x @ (q * scale)^T + bias, x of `dtype` (float16 or bfloat16), FP32 sums (ops.int4_linear)."""
+
+    def __init__(self, in_features: int, out_features: int, bias: bool = True, group_size: int = 128,
+                 dtype: torch.dtype = torch.float16):
+        super().__init__()
+        if group_size not in (32, 64, 128) or in_features % group_size != 0:
+            raise ValueError("Int4Linear needs group_size 32, 64 or 128 and in_features % group_size == 0")
+        if dtype not in (torch.float16, torch.bfloat16):
+            raise TypeError(f"dtype must be torch.float16 or torch.bfloat16, got {dtype}")
+        self.in_features = in_features
+        self.out_features = out_features
+        self.group_size = group_size
+        # 0x88: eight weights of zero
+        self.register_buffer("w_int4", torch.full((out_features, ops.int4_row_bytes(in_features)), 0x88, dtype=torch.uint8))
+        self.register_buffer("w_scale", torch.ones((out_features, in_features // group_size), dtype=torch.float16))
+        if bias:
+            self.bias = nn.Parameter(torch.zeros(out_features, dtype=dtype))
+        else:
+            self.register_parameter("bias", None)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        y = _Int4LinearFn.apply(x.reshape(-1, self.in_features), self.w_int4, self.w_scale, self.bias)
+        return y.view(*x.shape[:-1], self.out_features)
+
+    @torch.no_grad()
+    def quantize_weight(self, weight_fp: torch.Tensor) -> None:
+        """Symmetric quantization of each group of a row on the device (ops.quantize_weight_int4)."""
+        q, scale = ops.quantize_weight_int4(_as_weight(weight_fp, _prep_device(self.w_int4)), self.group_size)
+        self.w_int4.copy_(q)
+        self.w_scale.copy_(scale)
+
+    def extra_repr(self) -> str:
+        return (f"in_features={self.in_features}, out_features={self.out_features}, bias={self.bias is not None}, "
+                f"group_size={self.group_size}")
+
+
+def tree_masks(parents: torch.Tensor) -> torch.Tensor:
+    """ops.cache_attention's tree of drafted tokens from each token's parent, (B, T) integers on the host: -1 for a
+    token that follows the cache, else an earlier token of its row. Token t sees itself, its parent, and so on."""
+    if parents.dim() != 2 or not 1 <= parents.shape[1] <= 64:
+        raise ValueError(f"parents must be (B, 1 to 64), got {tuple(parents.shape)}")
+    rows = []
+    for row in parents.tolist():
+        masks = []
+        for t, p in enumerate(row):
+            if not -1 <= p < t:
+                raise ValueError(f"token {t}'s parent must be -1 or an earlier token, got {p}")
+            masks.append((1 << t) | (masks[p] if p >= 0 else 0))
+        rows.append([m - (1 << 64) if m >> 63 else m for m in masks])
+    return torch.tensor(rows, dtype=torch.int64)
+
+
+class DecoderAttention(nn.Module):
+    """The attention block of a decoder: one 4-bit projection to queries, keys and values, RMS norm and rotation of
+    the query and key heads, attention, and the 4-bit output projection.
+
+    Keys and values live in a paged cache of the caller's, (pages, page size, kv_heads, head_dim) each; `slots` says
+    where each token's go (page * page size + offset)."""
+
+    def __init__(self, hidden: int, heads: int, kv_heads: int, head_dim: int, positions: int, group_size: int = 128,
+                 theta: float = 10000.0, eps: float = 1e-6, dtype: torch.dtype = torch.float16):
+        super().__init__()
+        if heads % kv_heads != 0 or head_dim % 16 != 0 or head_dim > 256:
+            raise ValueError("DecoderAttention needs heads % kv_heads == 0 and a head_dim of a multiple of 16 up to 256")
+        self.heads, self.kv_heads, self.head_dim, self.eps = heads, kv_heads, head_dim, eps
+        self.qkv = Int4Linear(hidden, (heads + 2 * kv_heads) * head_dim, False, group_size, dtype)
+        self.out = Int4Linear(heads * head_dim, hidden, False, group_size, dtype)
+        self.q_norm = nn.Parameter(torch.ones(head_dim, dtype=dtype), requires_grad=False)
+        self.k_norm = nn.Parameter(torch.ones(head_dim, dtype=dtype), requires_grad=False)
+        angle = torch.arange(positions)[:, None] * theta ** (-torch.arange(0, head_dim, 2) / head_dim)
+        self.register_buffer("cos", angle.cos().float(), persistent=False)
+        self.register_buffer("sin", angle.sin().float(), persistent=False)
+
+    def _heads(self, x):
+        """The projections of (tokens, hidden): views of queries, keys and values in one output."""
+        return self.qkv(x).view(x.shape[0], -1, self.head_dim).split((self.heads, self.kv_heads, self.kv_heads), 1)
+
+    @torch.no_grad()
+    def prompt(self, x: torch.Tensor, cu_seqlens: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tensor,
+               v_cache: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
+        """Whole prompts packed into x (tokens, hidden), sequence b being tokens cu_seqlens[b] to cu_seqlens[b + 1] - 1; their
+        keys and values go into the cache too."""
+        q, k, v = self._heads(x)
+        keys = torch.empty(k.shape, dtype=k.dtype, device=k.device)
+        q = ops.qk_norm_rope_cache(q, k, v, self.q_norm, self.k_norm, self.cos, self.sin, positions, k_cache, v_cache, slots,
+                                   eps=self.eps, k_out=keys)
+        return self.out(ops.prompt_attention(q, keys, v, cu_seqlens).view(x.shape[0], -1))
+
+    @torch.no_grad()
+    def cached(self, x: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+               slots: torch.Tensor, page_table: torch.Tensor, cache_lens: torch.Tensor,
+               tree: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """The newest T tokens of each sequence, x (B, T, hidden), over the cache: one token, or a tree of drafts
+        (tree_masks). positions and slots are (B * T,); token t of sequence b is at cache position cache_lens[b] + t."""
+        B, T, hidden = x.shape
+        q, k, v = self._heads(x.reshape(B * T, hidden))
+        q = ops.qk_norm_rope_cache(q, k, v, self.q_norm, self.k_norm, self.cos, self.sin, positions, k_cache, v_cache, slots,
+                                   eps=self.eps)
+        o = ops.cache_attention(q.view(B, T, self.heads, self.head_dim), k_cache, v_cache, page_table, cache_lens, tree)
+        return self.out(o.view(B, T, -1))
 
 
 def _gfx950_word_positions(N: int, W: int, device) -> torch.Tensor:

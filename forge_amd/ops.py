@@ -701,7 +701,7 @@ def _qk_norm_rope(q, k, v, q_weight, k_weight, cos, sin, positions, k_cache, v_c
     v_token = v_head = rows = 0
     if k_out is not None:
         _need_shape(k_out, dt, "k_out", (T, Hkv, D))
-    else:
+    if k_out is None or k_cache is not None:
         v_token, v_head = _need_heads(v, dt, "v", T)
         if v.shape != k.shape:
             raise ValueError(f"v must have k's shape {tuple(k.shape)}, got {tuple(v.shape)}")
@@ -739,13 +739,15 @@ def qk_norm_rope(q: torch.Tensor, k: torch.Tensor, q_weight: Optional[torch.Tens
 def qk_norm_rope_cache(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, q_weight: Optional[torch.Tensor],
                        k_weight: Optional[torch.Tensor], cos: torch.Tensor, sin: torch.Tensor, positions: torch.Tensor,
                        k_cache: torch.Tensor, v_cache: torch.Tensor, slots: torch.Tensor, eps: float = 1e-6,
-                       interleaved: bool = False, q_out: Optional[torch.Tensor] = None) -> torch.Tensor:
+                       interleaved: bool = False, q_out: Optional[torch.Tensor] = None,
+                       k_out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """qk_norm_rope whose keys go straight into a paged cache (pages, page size, Hkv, D) with the values v, token t
-    into row slots[t] (int32, page * page size + offset; a slot outside the cache writes nothing). Returns the queries."""
+    into row slots[t] (int32, page * page size + offset; a slot outside the cache writes nothing), and to k_out as
+    well if it is given. Returns the queries."""
     _act_type(q, "q")
     if q_out is None:
         q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    _qk_norm_rope(q, k, v, q_weight, k_weight, cos, sin, positions, k_cache, v_cache, slots, eps, interleaved, q_out, None)
+    _qk_norm_rope(q, k, v, q_weight, k_weight, cos, sin, positions, k_cache, v_cache, slots, eps, interleaved, q_out, k_out)
     return q_out
 
 

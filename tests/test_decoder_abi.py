@@ -77,3 +77,17 @@ def test_workspace_size(lib):
     n = size(2, 3, 8, 2, 128, 5000)
     row = 2 * 3 * 8 * (128 + 2) * 4
     assert n > 0 and n % row == 0 and 2 <= n // row <= (5000 + 127) // 128
+
+
+def test_tree_masks():
+    import torch
+    from forge_amd.nn import tree_masks
+    got = tree_masks(torch.tensor([[-1, 0, 0, 2], [-1, -1, 1, 1]]))
+    assert got.tolist() == [[0b1, 0b11, 0b101, 0b1101], [0b1, 0b10, 0b110, 0b1010]]
+    chain = tree_masks(torch.arange(-1, 63)[None])
+    assert chain[0, 63] == -1 and chain[0, 62] == (1 << 63) - 1
+    for bad in ([[0]], [[-1, 1]], [[-2]]):
+        with pytest.raises(ValueError):
+            tree_masks(torch.tensor(bad))
+    with pytest.raises(ValueError):
+        tree_masks(torch.zeros((1, 65), dtype=torch.int64))
