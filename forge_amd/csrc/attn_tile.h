@@ -228,6 +228,55 @@ struct AttnWave {
         values(vs, p);
     }
 
+    // Joining KS waves (wave, wave + 1, .. from a multiple of KS on) that have the same rows and other keys, in
+    // wave order: each leaves its state in LDS, and after a barrier wave ks takes every KS-th block of 32
+    // columns from ks on. put(j, e, sums of columns 32 j + 8 e + 4 (lane / 32) .. + 3, maximum, sum of the weights).
+    template <int W>
+    struct Shared {
+        v4f sums[W][kOut * 4][kWave];
+        v2f stat[W][32];
+    };
+    template <int W>
+    __device__ __forceinline__ void leave(Shared<W>* sh, int wave) const {
+        const float sum = half_sum(l[0]);
+        if (lane < 32) sh->stat[wave][lane] = v2f{m[0], sum};
+#pragma unroll
+        for (int j = 0; j < kOut; j++)
+#pragma unroll
+            for (int e = 0; e < 4; e++)
+                sh->sums[wave][4 * j + e][lane] = v4f{o[0][j][4 * e], o[0][j][4 * e + 1], o[0][j][4 * e + 2], o[0][j][4 * e + 3]};
+    }
+    template <int KS, int W, class Put>
+    __device__ __forceinline__ void join(const Shared<W>* sh, int wave, const Put& put) const {
+        const int ks = wave % KS, w0 = wave - ks;
+        float top = kNoScore, sum = 0.0f, f[KS];
+#pragma unroll
+        for (int v = 0; v < KS; v++) {
+            f[v] = sh->stat[w0 + v][lane & 31][0];
+            top = fmaxf(top, f[v]);
+        }
+#pragma unroll
+        for (int v = 0; v < KS; v++) {
+            f[v] = __builtin_amdgcn_exp2f(f[v] - top);
+            sum = __builtin_fmaf(f[v], sh->stat[w0 + v][lane & 31][1], sum);
+        }
+#pragma unroll
+        for (int j = 0; j < kOut; j++) {
+            if (j % KS != ks) continue;
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int v = 0; v < KS; v++) {
+                    const v4f y = sh->sums[w0 + v][4 * j + e][lane];
+#pragma unroll
+                    for (int c = 0; c < 4; c++) s[c] = __builtin_fmaf(f[v], y[c], s[c]);
+                }
+                put(j, e, s, top, sum);
+            }
+        }
+    }
+
     // Whether some value of the rows `live` is no finite number.
     __device__ __forceinline__ bool odd(int b, bool live) const {
         float z = 0.0f;

@@ -5,7 +5,7 @@
 // the cache at cache_lens[b] + j, whose bit j is set in tree[b, t] (without a tree: j <= t). A row that
 // sees nothing gives zeros.
 //
-// Bound: reading the cache. A KV head's rows (T tokens x Hq / Hkv heads) are taken together, up to 256 in a
+// Bound: reading the cache. A KV head's rows (T tokens x Hq / Hkv heads) are taken together, up to 128 in a
 // workgroup of RS x KS waves (32 rows each), so that K and V are read once for them; the keys are split
 // over workgroups in chunks of equal length, whatever the sequence's, and a chunk's tiles, which come by
 // LDS DMA into two buffers, over the KS waves of a row set. The waves' results are joined in LDS; the chunks'
@@ -22,7 +22,7 @@ constexpr int kCacheMaxTokens = 64;
 
 struct CachePlan {
     int chunk, chunks;   // keys of a chunk; chunks of the longest sequence
-    int sets;            // 32-row sets of a workgroup: 1, 2, 4 or 8
+    int sets;            // 32-row sets of a workgroup: 1, 2 or 4
 };
 
 struct CacheArgs {
@@ -44,17 +44,21 @@ __device__ __forceinline__ int cache_keys(const CacheArgs& a, int b) {
     return static_cast<int>(min(static_cast<long long>(max(a.lens[b], 0)) + a.T, cap));
 }
 
+// LDS of the tiles, in which the waves' sums are left afterwards; the chunk's page numbers follow.
+template <class T, int DP, int RS, int KS, int KB>
+constexpr int kCacheLds = std::max<int>(4 * 32 * KS * KB * KvRows<DP>::kBytes,
+                                        sizeof(typename AttnWave<T, DP, 1, KB>::template Shared<RS * KS>));
+
 template <class T, int DP, int RS, int KS, int KB>
 __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attention_kernel(CacheArgs a)
 {
     using Rows = KvRows<DP>;
     constexpr int W = RS * KS, kKeys = 32 * KS * KB, kTile = kKeys * Rows::kBytes;
-    constexpr int kIns = kKeys * Rows::kChunks / kWave / W, kPitch = DP + 4;
+    constexpr int kIns = kKeys * Rows::kChunks / kWave / W;
     static_assert(kKeys * Rows::kChunks % (kWave * W) == 0, "a tile splits evenly over the waves");
     extern __shared__ __align__(1024) int8_t lds[];
-    __shared__ int page_of[kCacheMaxChunk + 2];
-    __shared__ float stat_m[W][32], stat_l[W][32];
     __shared__ int odd_rows;
+    int* page_of = reinterpret_cast<int*>(lds + kCacheLds<T, DP, RS, KS, KB>);
 
     const int group = a.group, rows = a.T * group;
     const int hk = blockIdx.x, chunk = blockIdx.y, b = udiv_magic(blockIdx.z, a.mg_sets), set = blockIdx.z - b * a.sets;
@@ -138,24 +142,11 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
         });
     }
 
-    // ---- join the waves of a row set, in wave order
     wait_vm_lgkm<0>();
     __syncthreads();
+    auto* sh = reinterpret_cast<typename AttnWave<T, DP, 1, KB>::template Shared<W>*>(lds);
     if (w.odd(0, live) && lane == 0) atomicOr(&odd_rows, 1);
-    float* sums = reinterpret_cast<float*>(lds);
-    const float lane_l = half_sum(w.l[0]);
-    if constexpr (KS > 1) {
-        if (lane < 32) {
-            stat_m[wave][lane] = w.m[0];
-            stat_l[wave][lane] = lane_l;
-        }
-#pragma unroll
-        for (int j = 0; j < DP / 32; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<v4f*>(sums + (wave * 32 + (lane & 31)) * kPitch + 32 * j + 2 * e + 4 * (lane >> 5)) =
-                    v4f{w.o[0][j][e], w.o[0][j][e + 1], w.o[0][j][e + 2], w.o[0][j][e + 3]};
-    }
+    w.leave(sh, wave);
     __syncthreads();
     const bool whole = keys <= a.chunk;                              // the only chunk: the result itself
     const size_t part0 = ((static_cast<size_t>(b) * a.Hkv + hk) * a.chunks + chunk) * rows;
@@ -192,55 +183,23 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
         }
         return;
     }
-    if constexpr (KS == 1) {
-        if (!live) return;
-        const float inv = lane_l > 0.0f ? 1.0f / lane_l : 0.0f;
-        float* part = a.part + (part0 + row) * a.D;
-        uint16_t* out = row_of(a.out, row);
-#pragma unroll
-        for (int j = 0; j < DP / 32; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4) {
-                const int d = 32 * j + 2 * e + 4 * (lane >> 5);
-                if (d >= a.D) continue;
-                const v4f s = {w.o[0][j][e], w.o[0][j][e + 1], w.o[0][j][e + 2], w.o[0][j][e + 3]};
-                if (whole) *reinterpret_cast<v2u*>(out + d) = v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
-                else *reinterpret_cast<v4f*>(part + d) = s;
-            }
-        if (!whole && lane < 32) {
-            a.stat[(part0 + row) * 2] = w.m[0];
-            a.stat[(part0 + row) * 2 + 1] = lane_l;
-        }
-        return;
-    }
-    for (int i = threadIdx.x; i < 32 * RS * (DP / 4); i += 64 * W) {
-        const int lr = i / (DP / 4), d = 4 * (i % (DP / 4)), r = set * RS * 32 + lr;
-        if (r >= rows) break;
-        if (d >= a.D) continue;
-        const int w0 = (lr / 32) * KS, x = lr % 32;
-        float m = kNoScore, l = 0.0f;
-#pragma unroll
-        for (int v = 0; v < KS; v++) m = fmaxf(m, stat_m[w0 + v][x]);
-        v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-        for (int v = 0; v < KS; v++) {
-            const float f = __builtin_amdgcn_exp2f(stat_m[w0 + v][x] - m);
-            l = __builtin_fmaf(f, stat_l[w0 + v][x], l);
-            const v4f y = *reinterpret_cast<const v4f*>(sums + ((w0 + v) * 32 + x) * kPitch + d);
-#pragma unroll
-            for (int e = 0; e < 4; e++) s[e] = __builtin_fmaf(f, y[e], s[e]);
-        }
+    if (!live) return;
+    float* part = a.part + (part0 + row) * a.D;
+    uint16_t* out = row_of(a.out, row);
+    w.template join<KS>(sh, wave, [&](int j, int e, v4f s, float m, float l) {
+        const int d = 32 * j + 8 * e + 4 * (lane >> 5);
+        if (d >= a.D) return;
         if (whole) {
             const float inv = l > 0.0f ? 1.0f / l : 0.0f;
-            *reinterpret_cast<v2u*>(row_of(a.out, r) + d) = v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
+            *reinterpret_cast<v2u*>(out + d) = v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
         } else {
-            *reinterpret_cast<v4f*>(a.part + (part0 + r) * a.D + d) = s;
+            *reinterpret_cast<v4f*>(part + d) = s;
             if (d == 0) {
-                a.stat[(part0 + r) * 2] = m;
-                a.stat[(part0 + r) * 2 + 1] = l;
+                a.stat[(part0 + row) * 2] = m;
+                a.stat[(part0 + row) * 2 + 1] = l;
             }
         }
-    }
+    });
 }
 
 // A wave joins one row's chunks: LPR lanes of 4 values take every (64 / LPR)-th chunk, four in flight, with the
@@ -301,14 +260,18 @@ __global__ __launch_bounds__(256) void cache_join_kernel(CacheArgs a)
 
 inline int cache_row(int D) { return D <= 64 ? 64 : D <= 96 ? 96 : D <= 128 ? 128 : 256; }
 
-CachePlan cache_plan(int B, int T, int Hq, int Hkv, int D, long long max_keys) {
+// Chunks such that sequences of the table's length make about a workgroup per CU, of as many keys as there are
+// rows at least (a chunk's sums are as large as its keys and values then), in whole tiles of 128. us, with a
+// third of that length / this: one token of 32 heads over 16000 27.8 / 21.0, 61 tokens of 32 heads over 16000 51 / 32.5;
+// 4 trees of 61 over 3001, 17, 0 and 2048 with chunks of 128 19.7, of the 488 rows 15.
+CachePlan cache_plan(int B, int T, int Hq, int Hkv, long long max_keys) {
     CachePlan p;
-    const int rows = T * (Hq / Hkv), most = cache_row(D) == 64 || cache_row(D) == 128 ? 8 : 4;
-    for (p.sets = 1; 32 * p.sets < rows && p.sets < most;) p.sets *= 2;
+    const int rows = T * (Hq / Hkv);
+    for (p.sets = 1; 32 * p.sets < rows && p.sets < 4;) p.sets *= 2;
     const long long heads = static_cast<long long>(B) * Hkv * divup(rows, 32 * p.sets);
-    const long long want = std::max<long long>(1, divupll(768, heads));
-    const long long chunk = divupll(divupll(max_keys, want), 128) * 128;
-    p.chunk = static_cast<int>(std::min<long long>(std::max<long long>(chunk, 128), kCacheMaxChunk));
+    const long long want = std::max<long long>(1, divupll(default_cu_count(), heads));
+    const long long chunk = divupll(std::max<long long>(divupll(max_keys, want), rows), 128) * 128;
+    p.chunk = static_cast<int>(std::min<long long>(chunk, kCacheMaxChunk));
     p.chunks = static_cast<int>(std::max<long long>(1, divupll(max_keys, p.chunk)));
     return p;
 }
@@ -319,18 +282,19 @@ size_t cache_floats(int B, int T, int Hq, int D, const CachePlan& p) {
 
 template <class T, int DP, int RS, int KS, int KB>
 int launch_cache(CacheArgs a, hipStream_t s) {
-    constexpr int kTiles = 4 * 32 * KS * KB * KvRows<DP>::kBytes, kSums = KS > 1 ? RS * KS * 32 * (DP + 4) * 4 : 0;
-    constexpr int kLds = kTiles > kSums ? kTiles : kSums, LPR = DP <= 64 ? 16 : DP <= 128 ? 32 : 64;
+    constexpr int LPR = DP <= 64 ? 16 : DP <= 128 ? 32 : 64, kMost = kCacheLds<T, DP, RS, KS, KB> + 4 * (kCacheMaxChunk + 2);
+    static_assert(kMost <= 159 * 1024, "tiles, sums and page numbers fit");
+    const int lds = kCacheLds<T, DP, RS, KS, KB> + 4 * ((a.chunk >> a.page_shift) + 2);
     const int rows = a.T * (a.Hq / a.Hkv);
     a.sets = divup(rows, 32 * RS);
     a.mg_sets = udiv_multiplier(a.sets);
     const long long z = static_cast<long long>(a.B) * a.sets;
     if (a.chunks > 65535 || z > 65535) return FORGE_EINVAL;
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&cache_attention_kernel<T, DP, RS, KS, KB>),
-                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kLds);
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
     if (attr != hipSuccess) return static_cast<int>(attr);
     const dim3 grid(static_cast<unsigned>(a.Hkv), static_cast<unsigned>(a.chunks), static_cast<unsigned>(z));
-    cache_attention_kernel<T, DP, RS, KS, KB><<<grid, 64 * RS * KS, kLds, s>>>(a);
+    cache_attention_kernel<T, DP, RS, KS, KB><<<grid, 64 * RS * KS, lds, s>>>(a);
     const int st = launch_status();
     if (st != FORGE_OK || a.chunks == 1) return st;
     const dim3 rows_grid(static_cast<unsigned>(divup(a.Hq, 4)), static_cast<unsigned>(a.T), static_cast<unsigned>(a.B));
@@ -345,15 +309,13 @@ int launch_cache(const CacheArgs& a, int sets, hipStream_t s) {
     switch (cache_row(a.D)) {
     case 64:
         if (sets == 1) return launch_cache<T, 64, 1, 4, 1>(a, s);
-        if (sets == 2) return launch_cache<T, 64, 2, 4, 1>(a, s);
-        return sets == 4 ? launch_cache<T, 64, 4, 2, 2>(a, s) : launch_cache<T, 64, 8, 1, 2>(a, s);
+        return sets == 2 ? launch_cache<T, 64, 2, 4, 1>(a, s) : launch_cache<T, 64, 4, 2, 2>(a, s);
     case 96:
         if (sets == 1) return launch_cache<T, 96, 1, 4, 1>(a, s);
         return sets == 2 ? launch_cache<T, 96, 2, 4, 1>(a, s) : launch_cache<T, 96, 4, 2, 2>(a, s);
     case 128:
         if (sets == 1) return launch_cache<T, 128, 1, 4, 1>(a, s);
-        if (sets == 2) return launch_cache<T, 128, 2, 4, 1>(a, s);
-        return sets == 4 ? launch_cache<T, 128, 4, 2, 2>(a, s) : launch_cache<T, 128, 8, 1, 2>(a, s);
+        return sets == 2 ? launch_cache<T, 128, 2, 4, 1>(a, s) : launch_cache<T, 128, 4, 2, 2>(a, s);
     default:
         if (sets == 1) return launch_cache<T, 256, 1, 2, 1>(a, s);
         return sets == 2 ? launch_cache<T, 256, 2, 2, 1>(a, s) : launch_cache<T, 256, 4, 1, 2>(a, s);
@@ -371,7 +333,7 @@ using namespace forge_amd;
 
 extern "C" size_t forge_cache_attention_workspace_size(int B, int T, int Hq, int Hkv, int D, long long max_keys) {
     if (!cache_shape_ok(B, T, Hq, Hkv, D) || max_keys <= 0) return 0;
-    return 4 * cache_floats(B, T, Hq, D, cache_plan(B, T, Hq, Hkv, D, max_keys));
+    return 4 * cache_floats(B, T, Hq, D, cache_plan(B, T, Hq, Hkv, max_keys));
 }
 
 extern "C" int forge_cache_attention(const uint16_t* q, const uint16_t* k_cache, const uint16_t* v_cache,
@@ -390,7 +352,7 @@ extern "C" int forge_cache_attention(const uint16_t* q, const uint16_t* k_cache,
         if (!aligned(p, 16)) return FORGE_EINVAL;
     const long long max_keys = static_cast<long long>(table_width) * page_size;
     if (max_keys > 1 << 27) return FORGE_EINVAL;
-    const CachePlan p = cache_plan(B, T, Hq, Hkv, D, max_keys);
+    const CachePlan p = cache_plan(B, T, Hq, Hkv, max_keys);
     const size_t floats = cache_floats(B, T, Hq, D, p);
     if (floats && (!workspace || workspace_bytes < 4 * floats)) return FORGE_EINVAL;
     float* part = static_cast<float*>(workspace);

@@ -32,7 +32,7 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void prompt_attenti
 {
     using Rows = KvRows<DP>;
     constexpr int W = RS * KS, kRows = 32 * RS, kKeys = kPromptKeys * KS, kTile = kKeys * Rows::kBytes;
-    constexpr int kIns = kKeys * Rows::kChunks / kWave / W, kPitch = DP + 4;   // DMA instructions per wave, tile and tensor
+    constexpr int kIns = kKeys * Rows::kChunks / kWave / W;   // DMA instructions per wave, tile and tensor
     static_assert(kKeys * Rows::kChunks % (kWave * W) == 0, "a tile splits evenly over the waves");
     extern __shared__ __align__(1024) int8_t lds[];                 // K, V of buffer 0, then of buffer 1 ...
 
@@ -143,12 +143,12 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void prompt_attenti
                 if (lane + 64 * c < a.D) out_row(r)[lane + 64 * c] = narrow<T>(acc[c] * inv);
         }
     };
-    const float l = half_sum(w.l[0]);
     if constexpr (KS == 1) {
         if (w.odd(0, live)) {
             again(32 * rs, 32 * rs + 32, 1);
             return;
         }
+        const float l = half_sum(w.l[0]);
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
         if (!live) return;
 #pragma unroll
@@ -161,55 +161,31 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void prompt_attenti
                                                            T::pack(w.o[0][j][e + 2] * inv, w.o[0][j][e + 3] * inv)};
             }
     } else {
-        // join the waves of a row set, in wave order
-        __shared__ float stat_m[W][32], stat_l[W][32];
         __shared__ int odd_rows;
-        float* sums = reinterpret_cast<float*>(lds);
+        auto* sh = reinterpret_cast<typename AttnWave<T, DP, 1, kPromptKeys / 32>::template Shared<W>*>(lds);
         if (threadIdx.x == 0) odd_rows = 0;
         wait_vm_lgkm<0>();
         __syncthreads();
         if (w.odd(0, live) && lane == 0) atomicOr(&odd_rows, 1);
-        if (lane < 32) {
-            stat_m[wave][lane] = w.m[0];
-            stat_l[wave][lane] = l;
-        }
-#pragma unroll
-        for (int j = 0; j < DP / 32; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e += 4)
-                *reinterpret_cast<v4f*>(sums + (wave * 32 + (lane & 31)) * kPitch + 32 * j + 2 * e + 4 * (lane >> 5)) =
-                    v4f{w.o[0][j][e], w.o[0][j][e + 1], w.o[0][j][e + 2], w.o[0][j][e + 3]};
+        w.leave(sh, wave);
         __syncthreads();
         if (odd_rows) {
             again(wave, kRows, W);
             return;
         }
-        for (int i = threadIdx.x; i < kRows * (DP / 4); i += 64 * W) {
-            const int lr = i / (DP / 4), d = 4 * (i % (DP / 4)), w0 = (lr / 32) * KS, x = lr % 32;
-            if (row0 + lr >= len) break;
-            if (d >= a.D) continue;
-            float m = kNoScore, sum = 0.0f;
-#pragma unroll
-            for (int v = 0; v < KS; v++) m = fmaxf(m, stat_m[w0 + v][x]);
-            v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
-#pragma unroll
-            for (int v = 0; v < KS; v++) {
-                const float f = __builtin_amdgcn_exp2f(stat_m[w0 + v][x] - m);
-                sum = __builtin_fmaf(f, stat_l[w0 + v][x], sum);
-                const v4f y = *reinterpret_cast<const v4f*>(sums + ((w0 + v) * 32 + x) * kPitch + d);
-#pragma unroll
-                for (int e = 0; e < 4; e++) s[e] = __builtin_fmaf(f, y[e], s[e]);
-            }
+        if (!live) return;
+        w.template join<KS>(sh, wave, [&](int j, int e, v4f s, float, float sum) {
+            const int d = 32 * j + 8 * e + 4 * (lane >> 5);
+            if (d >= a.D) return;
             const float inv = sum > 0.0f ? 1.0f / sum : 0.0f;
-            *reinterpret_cast<v2u*>(out_row(row0 + lr) + d) =
-                v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
-        }
+            *reinterpret_cast<v2u*>(out + d) = v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
+        });
     }
 }
 
 template <class T, int DP, int RS, int KS, int NS, bool CAUSAL>
 int launch_prompt(PromptArgs a, hipStream_t s) {
-    constexpr int kTiles = NS * 2 * kPromptKeys * KS * KvRows<DP>::kBytes, kSums = KS > 1 ? RS * KS * 32 * (DP + 4) * 4 : 0;
+    constexpr int kTiles = NS * 2 * kPromptKeys * KS * KvRows<DP>::kBytes, kSums = KS > 1 ? sizeof(typename AttnWave<T, DP, 1, 2>::template Shared<RS * KS>) : 0;
     constexpr int kLds = kTiles > kSums ? kTiles : kSums;
     const long long tiles = a.tokens / (32 * RS) + static_cast<long long>(a.sequences) + 1;
     const long long units = tiles * a.Hkv, wgs = divupll(units, 8) * 8 * (a.Hq / a.Hkv);
