@@ -237,9 +237,10 @@ struct AttnWave {
         v2f stat[W][32];
     };
     template <int W>
-    __device__ __forceinline__ void leave(Shared<W>* sh, int wave) const {
+    __device__ __forceinline__ void leave(Shared<W>* sh, int wave, bool live) const {
         const float sum = half_sum(l[0]);
         if (lane < 32) sh->stat[wave][lane] = v2f{m[0], sum};
+        if (!live) return;                                           // a row that nobody asks for
 #pragma unroll
         for (int j = 0; j < kOut; j++)
 #pragma unroll

@@ -146,7 +146,7 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
     __syncthreads();
     auto* sh = reinterpret_cast<typename AttnWave<T, DP, 1, KB>::template Shared<W>*>(lds);
     if (w.odd(0, live) && lane == 0) atomicOr(&odd_rows, 1);
-    w.leave(sh, wave);
+    w.leave(sh, wave, live);
     __syncthreads();
     const bool whole = keys <= a.chunk;                              // the only chunk: the result itself
     const size_t part0 = ((static_cast<size_t>(b) * a.Hkv + hk) * a.chunks + chunk) * rows;

@@ -167,7 +167,7 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void prompt_attenti
         wait_vm_lgkm<0>();
         __syncthreads();
         if (w.odd(0, live) && lane == 0) atomicOr(&odd_rows, 1);
-        w.leave(sh, wave);
+        w.leave(sh, wave, live);
         __syncthreads();
         if (odd_rows) {
             again(wave, kRows, W);
