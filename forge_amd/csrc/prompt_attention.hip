@@ -6,6 +6,11 @@
 // the next tiles' while this one is multiplied, one barrier a tile. Tiles past the diagonal are not
 // loaded, only those that cross it are masked.
 //
+// Bound: the matrix units at the clock that they leave (1.6 to 1.7 GHz; busy 44 to 52 %), and the softmax's vector
+// instructions that the other wave of a SIMD does not cover. Causal, 32 / 8 heads of 128: a prompt of 4096 155 us
+// (887 TFLOP/s), of 9001 + 5120 + 2263 905 to 940 (980 to 1017). Two workgroups of 4 waves a CU; 8 waves that share
+// their tiles measured the same.
+//
 // The grid is laid out without reading cu_seqlens on the host: sequence b's tiles start at
 // cu[b] / rows + b, which leaves room for each sequence's last partial tile.
 #include "attn_tile.h"

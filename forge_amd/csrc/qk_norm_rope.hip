@@ -4,7 +4,8 @@
 // Per head of D values: y = x / sqrt(mean(x^2) + eps) * weight (a side without a weight is not
 // normed), then for the pairs (a, b) of its first R values, (i, i + R/2) or neighbours (2i, 2i + 1),
 // a' = a cos - b sin, b' = b cos + a sin with the table row of the token's position. FP32 inside,
-// rounded once. Bound: memory; every value is read and written once, 16 bytes a lane.
+// rounded once. Bound: memory; every value is read and written once, 16 bytes a lane: 16384 tokens of 64 + 8
+// heads of 128 with their values into the cache 142 us, 680 MB at 4.8 TB/s, the rate of a copy; 8 tokens 3.3 us.
 #include "float16_types.h"
 
 #include <algorithm>
