@@ -2,8 +2,10 @@
 // the compiler makes every transposing LDS read wait for all DMAs that it knows of, and counts the
 // loads of a loop only where each of its paths has the same ones; either would end a prefetch. Nothing is returned
 // in registers; the callers wait by count (wait_vmcnt), and their kernels' own loads are waited for in order with
-// these, which is never too short. M0 has no other use in these kernels; a DMA may not follow its write without a
-// wait state in between.
+// these, which is never too short. M0 has no other use in these kernels. The wait
+// states that the compiler keeps for its own instructions are written out as well: one between M0 and the DMA that
+// reads it, five between a vector instruction's scalar result (an address that was kept in a vector register, or a
+// reloaded one) and a memory instruction that takes it.
 #pragma once
 
 #include "mfma_tile.h"
@@ -18,7 +20,7 @@ __device__ __forceinline__ uint32_t lds_address(const int8_t* p) {
 }
 __device__ __forceinline__ void dma16_rows(v4i rsrc, uint32_t voff, uint32_t lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tbuffer_load_dwordx4 %0, %1, 0 offen lds" ::"v"(voff), "s"(rsrc), "s"(lds) : "memory");
 #endif
 }
 __device__ __forceinline__ void dma16_at(const void* p, uint32_t lds) {
@@ -35,12 +37,12 @@ __device__ __forceinline__ v4i row_rsrc(const void* p, uint32_t bytes) {
 // From `off` bytes past a uniform base.
 __device__ __forceinline__ void dma16_off(const void* base, uint32_t off, uint32_t lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_dwordx4 %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
 #endif
 }
 __device__ __forceinline__ void dma2_off(const void* base, uint32_t off, uint32_t lds) {
 #if defined(__HIP_DEVICE_COMPILE__)
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tglobal_load_lds_ushort %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 4\n\tglobal_load_lds_ushort %0, %1" ::"v"(off), "s"(base), "s"(lds) : "memory");
 #endif
 }
 

@@ -94,6 +94,19 @@ def test_cache_attention(dev, lens, T, Hq, Hkv, D, page, dt):
     check_all(ops.cache_attention(q, c.k, c.v, c.table, c.lens, tree=tree.to(dev), scale=0.2), q, c, lens, tree, 0.2)
 
 
+@pytest.mark.parametrize("lens,T,Hq,Hkv,D,page", [
+    ([900, 5], 10, 4, 1, 96, 16), ([300], 20, 4, 1, 96, 32), ([600, 0], 10, 4, 1, 64, 16), ([500], 10, 8, 2, 256, 16),
+    ([3000, 40], 33, 8, 2, 128, 64), ([5000], 64, 8, 1, 72, 16)])
+def test_row_sets(dev, lens, T, Hq, Hkv, D, page):
+    """Two and four sets of 32 rows at each head size, and rows enough to lengthen the chunks."""
+    from forge_amd import ops
+    c = Cache(lens, T, Hkv, D, page, "bfloat16", dev, T + D)
+    q = queries(len(lens), T, Hq, D, "bfloat16", dev, D)
+    say(f"cache_attention lens={lens} T={T} Hq={Hq} Hkv={Hkv} D={D} page={page}")
+    tree = random_tree(len(lens), T, D)
+    check_all(ops.cache_attention(q, c.k, c.v, c.table, c.lens, tree=tree.to(dev)), q, c, lens, tree)
+
+
 def test_table_wider_than_the_lengths(dev):
     """A table laid out for a far longer sequence: many chunks without keys."""
     from forge_amd import ops

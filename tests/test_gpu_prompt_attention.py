@@ -57,6 +57,18 @@ def test_long(dev, tokens, Hq, Hkv):
     check_all(ops.prompt_attention(q, k, v, cu), q, k, v, [tokens, 77], True)
 
 
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens,Hq,Hkv,D", [([900], 32, 8, 64), ([901, 30], 32, 32, 80), ([450], 3, 1, 256), ([260], 2, 2, 48),
+                                           ([641, 2], 5, 5, 128)])
+def test_many_tiles(dev, lens, Hq, Hkv, D, causal, dt):
+    """Chains of tiles longer than the buffers, at every head size and both ways of sharing the keys."""
+    from forge_amd import ops
+    q, k, v, cu = make(lens, Hq, Hkv, D, dt, dev, sum(lens) + D)
+    say(f"prompt_attention {dt} lens={lens} Hq={Hq} Hkv={Hkv} D={D} causal={causal}")
+    check_all(ops.prompt_attention(q, k, v, cu, causal=causal), q, k, v, lens, causal)
+
+
 def test_scale_tail_and_growing_scores(dev):
     """A scale of the caller's, tokens after the last sequence, and scores whose maximum keeps growing along
     the keys (the sums are rescaled again and again) or falls from the first on."""
