@@ -241,7 +241,7 @@ extern "C" int forge_prompt_attention(const uint16_t* q, const uint16_t* k, cons
     for (const void* p : {static_cast<const void*>(q), static_cast<const void*>(k), static_cast<const void*>(v),
                           static_cast<const void*>(out)})
         if (!aligned(p, 16)) return FORGE_EINVAL;
-    // a tile's 64 rows are addressed in 32 bits
+    // a tile's rows, 128 at most, are addressed in 31 bits
     for (long long st : {q_token, q_head, k_token, k_head, v_token, v_head})
         if (st < 0 || st % 8 != 0 || st > (1 << 23)) return FORGE_EINVAL;
     const PromptArgs a{q, k, v, out, cu_seqlens, q_token, q_head, k_token, k_head, v_token, v_head,

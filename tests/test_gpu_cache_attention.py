@@ -267,3 +267,19 @@ def test_refusals(dev):
     wide = torch.zeros((1, 100), dtype=torch.int32, device=dev)
     with pytest.raises(ValueError):
         f(q, c.k, c.v, wide, c.lens, workspace=torch.empty((16,), dtype=torch.uint8, device=dev))
+
+
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("lens,T,Hq,Hkv", [([1000], 1, 4, 1), ([700, 3, 1500], 5, 16, 2), ([900, 2000], 12, 16, 4),
+                                           ([1200, 40], 61, 8, 2), ([3000] * 8, 1, 32, 8)])
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+def test_same_bits_every_call(dev, lens, T, Hq, Hkv, D, dt):
+    """Nothing depends on which wave or workgroup comes first."""
+    import torch
+    from forge_amd import ops
+    c = Cache(lens, T, Hkv, D, 16, dt, dev, D)
+    q = queries(len(lens), T, Hq, D, dt, dev, D)
+    want = ops.cache_attention(q, c.k, c.v, c.table, c.lens)
+    outs = [ops.cache_attention(q, c.k, c.v, c.table, c.lens) for _ in range(20)]
+    for out in outs:
+        assert torch.equal(out, want)

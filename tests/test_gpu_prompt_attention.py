@@ -217,3 +217,70 @@ def test_refusals(dev):
     with pytest.raises(ValueError):
         f(wide, wide, wide, cu)
     assert f(q[:0], k[:0], v[:0], cu).shape == (0, 4, 64)
+
+
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("lens,Hq,Hkv,D", [
+    ([1025], 4, 2, 64), ([300, 0, 1, 31], 3, 1, 40), ([1100, 33], 4, 4, 80), ([257], 1, 1, 96), ([997, 5], 4, 1, 128),
+    ([400, 260, 3], 6, 2, 128), ([1030], 10, 5, 64), ([1030], 12, 4, 128), ([1500], 9, 3, 80), ([901, 64], 4, 2, 256),
+    ([1, 290], 8, 8, 200), ([650], 32, 8, 136)])
+def test_few_workgroups(dev, lens, Hq, Hkv, D, causal, dt):
+    """Sizes that leave CUs over, whose workgroups take fewer rows (up to 128 values a head)."""
+    from forge_amd import ops
+    q, k, v, cu = make(lens, Hq, Hkv, D, dt, dev, sum(lens) + D)
+    say(f"prompt_attention {dt} lens={lens} Hq={Hq} Hkv={Hkv} D={D} causal={causal}")
+    check_all(ops.prompt_attention(q, k, v, cu, causal=causal), q, k, v, lens, causal)
+
+
+@pytest.mark.parametrize("D", [64, 128, 256])
+def test_few_workgroups_masked_places(dev, D):
+    """NaN and infinities after a row and in the next sequence, with waves that share rows."""
+    import torch
+    from attention_plain import check
+    from forge_amd import ops
+    lens = [290, 40]
+    q, k, v, cu = make(lens, 2, 1, D, "float16", dev, D + 1)
+    k, v = k.clone(), v.clone()
+    k[290:], v[290:] = float("nan"), float("inf")
+    v[201, 0, 3] = float("nan")
+    out = ops.prompt_attention(q, k, v, cu)
+    i = torch.arange(290, device=dev)
+    seen = i[None] <= i[:, None]
+    rest = [d for d in range(D) if d != 3]
+    for h in range(2):
+        check(out[:201, h], q[:201, h], k[:290, 0], v[:290, 0], seen[:201], D ** -0.5)
+        assert not torch.isfinite(out[201:290, h, 3]).any()
+        check(out[:290, h][:, rest], q[:290, h], k[:290, 0], v[:290, 0][:, rest], seen, D ** -0.5)
+
+
+@pytest.mark.parametrize("D", [64, 128])
+def test_far_rows(dev, D):
+    """The largest stride of tokens, 16 MB, with waves that share rows: tiles of 2 GB."""
+    import torch
+    from forge_amd import ops
+    n, step = 300, 1 << 23
+    q, k, v, cu = make([n], 1, 1, D, "float16", dev, 14)
+    big = torch.empty(((n - 1) * step + D,), dtype=torch.float16, device=dev)
+    far = big.as_strided((n, 1, D), (step, D, 1))
+    for causal in (True, False):
+        want = ops.prompt_attention(q, k, v, cu, causal=causal)
+        far.copy_(k)
+        assert torch.equal(ops.prompt_attention(q, far, v, cu, causal=causal), want)
+        far.copy_(v)
+        assert torch.equal(ops.prompt_attention(q, k, far, cu, causal=causal), want)
+
+
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("lens,Hq,Hkv", [([300], 1, 1), ([1025, 40], 4, 2), ([2100], 12, 4), ([900], 40, 8), ([130, 7, 61], 3, 3)])
+@pytest.mark.parametrize("D", [64, 80, 128, 256])
+def test_same_bits_every_call(dev, lens, Hq, Hkv, D, dt):
+    """Nothing depends on which wave comes first."""
+    import torch
+    from forge_amd import ops
+    q, k, v, cu = make(lens, Hq, Hkv, D, dt, dev, sum(lens))
+    for causal in (True, False):
+        want = ops.prompt_attention(q, k, v, cu, causal=causal)
+        outs = [ops.prompt_attention(q, k, v, cu, causal=causal) for _ in range(20)]
+        for out in outs:
+            assert torch.equal(out, want)
