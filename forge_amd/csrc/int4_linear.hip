@@ -86,16 +86,18 @@ __global__ __launch_bounds__(256) void pack_weight_int4_kernel(const int8_t* __r
 
 // ---- the product -----------------------------------------------------------------------------------
 
-// Eight stored values as a product's operand. FP16: nibble | 0x6400 is 1024 + nibble, and the exact
-// packed subtraction of 1032 leaves q; the odd nibbles are taken in place, 1024 + 16 nibble, by an
-// exact multiply-add. BF16 has no packed subtraction: nibble | 0x4300 is 128 + nibble = 136 + q, and
-// the caller starts its sum from -136 x.
+// Eight stored values as a product's operand, exact: q for FP16, q / 16 for BF16 (kUnit, which the group's scale takes
+// back). FP16: nibble | 0x6400 is 1024 + nibble, and the exact packed subtraction of 1032 leaves q; the odd
+// nibbles are taken in place, 1024 + 16 nibble, by an exact multiply-add (the published trick of 16-bit
+// exponent bits under a small integer). BF16 has no packed arithmetic: the nibbles, made two's complement by their top
+// bits, are converted to FP32 sixteenths one by one and packed in pairs, 14 instructions a word against FP16's 9 (us, FP16 /
+// BF16: 1 token of 8192 x 11008 12.7 / 13.5, 16 tokens 13.9 / 15.7, 64 tokens 25.8 / 25.4). A shifted weight, 136 + q in 7
+// instructions, would need -136 x beside it: sums 17 times as large, and inf - inf for an infinite x.
 template <class T>
 struct Int4Operand {
-    uint32_t top;   // the exponent bits, in a register: and-or takes one constant from elsewhere
-    __device__ __forceinline__ Int4Operand() : top(std::is_same<T, Fp16>::value ? 0x64006400u : 0x43004300u) {
-        asm volatile("" : "+v"(top));
-    }
+    static constexpr float kUnit = std::is_same<T, Fp16>::value ? 1.0f : 0.0625f;
+    uint32_t top;   // FP16's exponent bits, in a register: and-or takes one constant from elsewhere
+    __device__ __forceinline__ Int4Operand() : top(0x64006400u) { asm volatile("" : "+v"(top)); }
     __device__ __forceinline__ v4u operator()(uint32_t w) const {
         if constexpr (std::is_same<T, Fp16>::value) {
             const uint32_t hi = w >> 8;
@@ -109,8 +111,14 @@ struct Int4Operand {
             };
             return v4u{even(w), odd(w), even(hi), odd(hi)};
         } else {
-            auto at = [&](uint32_t b) { return (b & 0x000F000Fu) | top; };
-            return v4u{at(w), at(w >> 4), at(w >> 8), at(w >> 12)};
+            const uint32_t even = w ^ 0x88888888u;
+            uint32_t odd = even >> 4;
+            asm volatile("" : "+v"(odd));                            // so that the conversions select bytes of it
+            auto at = [](uint32_t b, int shift) {
+                return T::pack(__builtin_amdgcn_cvt_off_f32_i4(static_cast<int>(b >> shift & 255u)),
+                               __builtin_amdgcn_cvt_off_f32_i4(static_cast<int>(b >> (16 + shift) & 255u)));
+            };
+            return v4u{at(even, 0), at(odd, 0), at(even, 8), at(odd, 8)};
         }
     }
 };
@@ -170,7 +178,6 @@ template <class T, int G, int MT, int XR, int NT, int W, int U, int S>
 __global__ __launch_bounds__(64 * W) void int4_linear_kernel(Int4Args a)
 {
     using Ring = Int4Ring<U>;
-    constexpr bool kBf16 = std::is_same<T, Bf16>::value;
     constexpr int kGroups = U / G, kBlocks = U / kInt4Block;         // of a unit
     constexpr int kWIns = kBlocks, kSIns = (16 * kGroups + 63) / 64, kXIns = XR * Ring::kXChunks / 64;
     constexpr int kIns = NT * (kWIns + kSIns) + MT * kXIns;          // DMA instructions of a unit
@@ -251,13 +258,14 @@ __global__ __launch_bounds__(64 * W) void int4_linear_kernel(Int4Args a)
         compiler_fence();
         const int u = wave + it * W;
         const int8_t* at = lds + (wave * S + slot) * kStage;
-        v4f sum[MT][NT], base[MT];
+        v4f sum[MT][NT];
         float sc[NT][kGroups];
 #pragma unroll
         for (int n = 0; n < NT; n++)
 #pragma unroll
             for (int i = 0; i < kGroups; i++)
-                sc[n][i] = h2f(*reinterpret_cast<const uint16_t*>(at + kS0 + n * kSIns * 256 + (col * kGroups + i) * 4));
+                sc[n][i] = h2f(*reinterpret_cast<const uint16_t*>(at + kS0 + n * kSIns * 256 + (col * kGroups + i) * 4)) *
+                           (1.0f / Int4Operand<T>::kUnit);
 #pragma unroll
         for (int b = 0; b < kBlocks; b++) {
             v4u w[NT];
@@ -271,14 +279,9 @@ __global__ __launch_bounds__(64 * W) void int4_linear_kernel(Int4Args a)
                 const v4f zero = {0.0f, 0.0f, 0.0f, 0.0f};
                 v4u x[MT];
 #pragma unroll
-                for (int m = 0; m < MT; m++) {
+                for (int m = 0; m < MT; m++)
                     x[m] = *reinterpret_cast<const v4u*>(at + kX0 + m * kXIns * 1024 +
                                                          (xr + ((4 * step + g) ^ Ring::swz_x(xrow))) * 16);
-                    if constexpr (kBf16) {
-                        const v4u c = {0xC308C308u, 0xC308C308u, 0xC308C308u, 0xC308C308u};   // -136
-                        base[m] = T::mfma16(x[m], c, first ? zero : base[m]);
-                    }
-                }
 #pragma unroll
                 for (int n = 0; n < NT; n++) {
                     const v4u q = operand(w[n][j]);
@@ -292,8 +295,7 @@ __global__ __launch_bounds__(64 * W) void int4_linear_kernel(Int4Args a)
                         for (int m = 0; m < MT; m++)
 #pragma unroll
                             for (int e = 0; e < 4; e++)
-                                acc[m][n][e] = __builtin_fmaf(kBf16 ? sum[m][n][e] + base[m][e] : sum[m][n][e],
-                                                              sc[n][step / (G / 32)], acc[m][n][e]);
+                                acc[m][n][e] = __builtin_fmaf(sum[m][n][e], sc[n][step / (G / 32)], acc[m][n][e]);
                 }
             }
         }

@@ -1,0 +1,67 @@
+"""GPU: the decoder operators at the ends of their ranges: the largest and smallest values, infinities and NaN, empty
+and extreme sizes, arguments that are no numbers."""
+import pytest
+
+from helpers import say
+
+pytestmark = pytest.mark.gpu
+
+
+# ---- int4_linear ---------------------------------------------------------------------------------
+
+def int4_case(M, K, N, dt, dev, seed):
+    """x, and weights of one scale group whose rows 0 and 1 hold no zero."""
+    import torch
+    from forge_amd import ops
+    g = torch.Generator().manual_seed(seed)
+    q = torch.randint(-8, 8, (N, K), generator=g)
+    q[:2] = torch.where(q[:2] == 0, 3, q[:2])
+    s = (torch.rand((N, K // 32), generator=g) * 1e-2 + 1e-3).half().to(dev)
+    x = torch.randn((M, K), generator=g).to(getattr(torch, dt)).to(dev)
+    return x, q.to(dev), s, ops.pack_weight_int4(q.to(torch.int8).to(dev))
+
+
+SIZES = [(1, 128, 20), (3, 512, 40), (1, 1024, 16400), (16, 512, 20), (16, 512, 11008), (30, 512, 40), (30, 256, 8200), (64, 512, 50),
+         (64, 512, 11008)]
+
+
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_int4_infinite_tokens(dev, M, K, N, dt):
+    """An infinite activation times a weight of zero is NaN, times any other an infinity, as in the sum of products."""
+    import torch
+    from forge_amd import ops
+    x, q, s, w = int4_case(M, K, N, dt, dev, K + N)
+    x[M - 1, 37] = float("inf")
+    x[M // 2, K - 2] = float("-inf")
+    say(f"int4_linear infinities {dt} M={M} K={K} N={N}")
+    y = ops.int4_linear(x, w, s)
+    sign = torch.ones((M, N), device=dev)
+    hit = torch.zeros((M, N), dtype=torch.bool, device=dev)
+    nan = torch.zeros((M, N), dtype=torch.bool, device=dev)
+    for m, k, v in ((M - 1, 37, 1.0), (M // 2, K - 2, -1.0)):
+        here = v * q[:, k].sign().float()
+        nan[m] |= (here == 0) | (hit[m] & (here != sign[m]))
+        sign[m] = here
+        hit[m] = True
+    assert torch.equal(torch.isnan(y), nan)
+    assert torch.equal(torch.isinf(y), hit & ~nan)
+    assert (y[hit & ~nan].sign() == sign[hit & ~nan]).all()
+
+
+@pytest.mark.parametrize("M,K,N", SIZES)
+def test_int4_large_tokens(dev, M, K, N):
+    """BF16 values far above what a shifted weight could take: the sum of products itself stays in range.
+    Bound as in test_gpu_int4.py, of products of |q| <= 8: 2^-8 of the result and n 2^-23 of the products' magnitudes."""
+    import torch
+    from forge_amd import ops
+    x, q, s, w = int4_case(M, K, N, "bfloat16", dev, K + N + 1)
+    x[:, 5] = 1e37
+    x[:, 70] = -1e37
+    x[M // 2] = 3e36
+    say(f"int4_linear large values M={M} K={K} N={N}")
+    y = ops.int4_linear(x, w, s).double()
+    ws = q.double() * s.double().repeat_interleave(32, 1)
+    want, mag = x.double() @ ws.T.contiguous(), x.double().abs() @ ws.abs().T.contiguous()
+    assert torch.isfinite(y).all()
+    assert ((y - want).abs() <= 2.0 ** -8 * want.abs() + (K + 32) * 2.0 ** -23 * mag).all()
