@@ -83,7 +83,8 @@ PyObject* int4_linear(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (!x || x->dim() != 2 || !s || s->dim() != 2 || s->size(1) == 0) return kNotInOrder;
         const at::ScalarType type = x->scalar_type();
         const int64_t M = x->size(0), K = x->size(1), N = s->size(0), group = K / s->size(1);
-        if (code(type) < 0 || group * s->size(1) != K || !dense(x, type, c.device, {M, K}) ||
+        // (no values, K = 0, would be no work to the library, and the output nobody's)
+        if (code(type) < 0 || group <= 0 || group * s->size(1) != K || !dense(x, type, c.device, {M, K}) ||
             !dense(s, at::kHalf, c.device, {N, s->size(1)}) || !dense(w, at::kByte, c.device, {N, (K + 127) / 128 * 64}) ||
             !dense(out, type, c.device, {M, N}) || M > INT32_MAX || K > INT32_MAX || N > INT32_MAX)
             return kNotInOrder;

@@ -9,6 +9,17 @@ pytestmark = pytest.mark.gpu
 
 # ---- int4_linear ---------------------------------------------------------------------------------
 
+def test_no_values_is_refused(dev):
+    """K = 0 has no scale group: an error, not an output that nobody wrote."""
+    import torch
+    from forge_amd import ops
+    x = torch.empty((2, 0), dtype=torch.float16, device=dev)
+    w = torch.empty((8, 0), dtype=torch.uint8, device=dev)
+    for groups in (0, 1, 3):
+        with pytest.raises(ValueError):
+            ops.int4_linear(x, w, torch.ones((8, groups), dtype=torch.float16, device=dev))
+
+
 def int4_case(M, K, N, dt, dev, seed):
     """x, and weights of one scale group whose rows 0 and 1 hold no zero."""
     import torch
