@@ -56,6 +56,12 @@ struct Call {
     Call(PyObject* const* args, Py_ssize_t n)
         : a(args), device(PyLong_AsLong(args[n - 2])), stream(PyLong_AsVoidPtr(args[n - 1])) {}
     bool none(int i) const { return a[i] == Py_None; }
+    // Numbers and flags, before the library is called: what is none leaves its error for call() to clear.
+    bool number(int i, float* to) const {
+        *to = static_cast<float>(PyFloat_AsDouble(a[i]));
+        return !PyErr_Occurred();
+    }
+    bool flag(int i, int* to) const { return (*to = PyObject_IsTrue(a[i])) >= 0; }
 };
 
 // Runs f (Call -> status) if the argument count is right; no exception leaves.
@@ -104,6 +110,9 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (!q0) return kNotInOrder;
         const at::ScalarType type = q0->scalar_type();
         Heads q, k, v = {};
+        float eps;
+        int interleaved;
+        if (!c.number(13, &eps) || !c.flag(14, &interleaved)) return kNotInOrder;
         if (code(type) < 0 || !q.take(c.a[0], type, c.device) || !k.take(c.a[1], type, c.device)) return kNotInOrder;
         const int64_t T = q.tokens, D = q.D;
         const at::Tensor *qw = nullptr, *kw = nullptr, *cos = tensor(c.a[5]), *sin = tensor(c.a[6]), *pos = tensor(c.a[7]);
@@ -135,8 +144,7 @@ PyObject* qk_norm_rope(PyObject*, PyObject* const* args, Py_ssize_t n) {
             at_<float>(sin), at_<int32_t>(pos), at_<uint16_t>(q_out), at_<uint16_t>(k_out), at_<uint16_t>(kc),
             at_<uint16_t>(vc), at_<int32_t>(slots), rows, static_cast<int>(T), static_cast<int>(q.heads),
             static_cast<int>(k.heads), static_cast<int>(D), static_cast<int>(2 * half), static_cast<int>(P), q.token, q.head,
-            k.token, k.head, v.token, v.head, static_cast<float>(PyFloat_AsDouble(c.a[13])),
-            PyObject_IsTrue(c.a[14]), code(type), c.stream);
+            k.token, k.head, v.token, v.head, eps, interleaved, code(type), c.stream);
     });
 }
 
@@ -147,6 +155,9 @@ PyObject* prompt_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (!q0 || !cu || cu->dim() != 1 || cu->size(0) < 2) return kNotInOrder;
         const at::ScalarType type = q0->scalar_type();
         Heads q, k, v;
+        float scale;
+        int causal;
+        if (!c.number(5, &scale) || !c.flag(6, &causal)) return kNotInOrder;
         if (code(type) < 0 || !q.take(c.a[0], type, c.device) || !k.take(c.a[1], type, c.device) ||
             !v.take(c.a[2], type, c.device))
             return kNotInOrder;
@@ -157,8 +168,7 @@ PyObject* prompt_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         return forge_prompt_attention(at_<uint16_t>(q.t), at_<uint16_t>(k.t), at_<uint16_t>(v.t), at_<int32_t>(cu),
                                       at_<uint16_t>(out), static_cast<int>(seqs), static_cast<int>(T),
                                       static_cast<int>(q.heads), static_cast<int>(k.heads), static_cast<int>(q.D), q.token, q.head,
-                                      k.token, k.head, v.token, v.head, static_cast<float>(PyFloat_AsDouble(c.a[5])),
-                                      PyObject_IsTrue(c.a[6]), code(type), c.stream);
+                                      k.token, k.head, v.token, v.head, scale, causal, code(type), c.stream);
     });
 }
 
@@ -171,6 +181,8 @@ PyObject* cache_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const at::ScalarType type = q->scalar_type();
         const int64_t B = q->size(0), T = q->size(1), Hq = q->size(2), D = q->size(3);
         const int64_t pages = kc->size(0), page = kc->size(1), Hkv = kc->size(2), width = table->size(1);
+        float scale;
+        if (!c.number(8, &scale)) return kNotInOrder;
         if (code(type) < 0 || T < 1 || T > 64 || !dense(q, type, c.device, {B, T, Hq, D}) || !dense(kc, type, c.device, {pages, page, Hkv, D}) ||
             !dense(vc, type, c.device, {pages, page, Hkv, D}) || !dense(table, at::kInt, c.device, {B, width}) ||
             !dense(lens, at::kInt, c.device, {B}) || !dense(out, type, c.device, {B, T, Hq, D}) || B > INT32_MAX ||
@@ -181,8 +193,8 @@ PyObject* cache_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         return forge_cache_attention(at_<uint16_t>(q), at_<uint16_t>(kc), at_<uint16_t>(vc), at_<int32_t>(table),
                                      at_<int32_t>(lens), at_<int64_t>(tree), at_<uint16_t>(out), static_cast<int>(B), static_cast<int>(T),
                                      static_cast<int>(Hq), static_cast<int>(Hkv), static_cast<int>(D), static_cast<int>(pages),
-                                     static_cast<int>(page), static_cast<int>(width), static_cast<float>(PyFloat_AsDouble(c.a[8])),
-                                     code(type), at_<void>(ws), ws ? static_cast<size_t>(ws->numel()) : 0, c.stream);
+                                     static_cast<int>(page), static_cast<int>(width), scale, code(type), at_<void>(ws),
+                                     ws ? static_cast<size_t>(ws->numel()) : 0, c.stream);
     });
 }
 

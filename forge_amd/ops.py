@@ -692,6 +692,9 @@ def _qk_norm_rope(q, k, v, q_weight, k_weight, cos, sin, positions, k_cache, v_c
     P, R = cos.shape[0], 2 * cos.shape[1]
     if R % 16 or R > D:
         raise ValueError(f"the rotated part must be a multiple of 16 up to {D} values, got {R}")
+    if not hasattr(eps, "__float__"):             # strings have none
+        raise TypeError(f"eps must be a number, got {eps!r}")
+    eps = float(eps)
     _need(positions, torch.int32, "positions")
     if positions.shape != (T,):
         raise ValueError(f"positions must have shape ({T},), got {tuple(positions.shape)}")

@@ -76,3 +76,35 @@ def test_int4_large_tokens(dev, M, K, N):
     want, mag = x.double() @ ws.T.contiguous(), x.double().abs() @ ws.abs().T.contiguous()
     assert torch.isfinite(y).all()
     assert ((y - want).abs() <= 2.0 ** -8 * want.abs() + (K + 32) * 2.0 ** -23 * mag).all()
+
+
+# ---- arguments -----------------------------------------------------------------------------------
+
+class NoBool:
+    def __bool__(self):
+        raise RuntimeError("no truth value")
+
+
+@pytest.mark.parametrize("eps,interleaved", [("small", False), (None, False), (1e-6, NoBool())])
+def test_bad_numbers_touch_nothing(dev, eps, interleaved):
+    """An eps or a flag that is no number is refused before the queries (in place here) or the cache are written."""
+    import torch
+    from forge_amd import ops
+    T, D = 4, 64
+    q, k, v = (torch.randn((T, 2, D), device=dev).half() for _ in range(3))
+    kc, vc = (torch.randn((2, 16, 2, D), device=dev).half() for _ in range(2))
+    cos, sin = torch.rand((8, D // 2), device=dev), torch.rand((8, D // 2), device=dev)
+    pos = torch.arange(T, dtype=torch.int32, device=dev)
+    w = torch.ones((D,), dtype=torch.float16, device=dev)
+    was = [t.clone() for t in (q, kc, vc)]
+    with pytest.raises(Exception):
+        ops.qk_norm_rope_cache(q, k, v, w, w, cos, sin, pos, kc, vc, pos, eps=eps, interleaved=interleaved, q_out=q)
+    torch.cuda.synchronize()
+    for t, before in zip((q, kc, vc), was):
+        assert torch.equal(t, before)
+    cu = torch.tensor([0, T], dtype=torch.int32, device=dev)
+    out = torch.full_like(q, 5.0)
+    with pytest.raises(Exception):
+        ops.prompt_attention(q, k, v, cu, causal=NoBool(), out=out)
+    torch.cuda.synchronize()
+    assert (out == 5.0).all()
