@@ -45,7 +45,7 @@ struct Heads {
         tokens = t->size(0); heads = t->size(1); D = t->size(2);
         token = tokens > 1 ? t->stride(0) : 0;
         head = heads > 1 ? t->stride(1) : 0;
-        return t->stride(2) == 1;
+        return D > 0 && t->stride(2) == 1;
     }
 };
 
@@ -183,7 +183,7 @@ PyObject* cache_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const int64_t pages = kc->size(0), page = kc->size(1), Hkv = kc->size(2), width = table->size(1);
         float scale;
         if (!c.number(8, &scale)) return kNotInOrder;
-        if (code(type) < 0 || T < 1 || T > 64 || !dense(q, type, c.device, {B, T, Hq, D}) || !dense(kc, type, c.device, {pages, page, Hkv, D}) ||
+        if (code(type) < 0 || T < 1 || T > 64 || D < 1 || !dense(q, type, c.device, {B, T, Hq, D}) || !dense(kc, type, c.device, {pages, page, Hkv, D}) ||
             !dense(vc, type, c.device, {pages, page, Hkv, D}) || !dense(table, at::kInt, c.device, {B, width}) ||
             !dense(lens, at::kInt, c.device, {B}) || !dense(out, type, c.device, {B, T, Hq, D}) || B > INT32_MAX ||
             Hq > INT32_MAX || pages > INT32_MAX || page > INT32_MAX || width > INT32_MAX)

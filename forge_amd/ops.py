@@ -598,6 +598,14 @@ def _same_device(first: torch.Tensor, *others: Optional[torch.Tensor]) -> None:
             raise ValueError(f"operands must be on the current device (cuda:{dev}), got {t.device}")
 
 
+def _scale_of(scale: Optional[float], q: torch.Tensor) -> float:
+    """The scale for the compiled call, of any q (heads of no values are refused later)."""
+    if scale is not None:
+        return scale
+    D = q.shape[-1] if q.dim() else 0
+    return D ** -0.5 if D else 1.0
+
+
 def _softmax_scale(scale: Optional[float], D: int) -> float:
     if scale is None:
         return D ** -0.5
@@ -762,7 +770,7 @@ def prompt_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, cu_seqle
     code = _act_type(q, "q")
     if out is None:
         out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    if _fast("prompt_attention", q, k, v, cu_seqlens, out, q.shape[-1] ** -0.5 if scale is None else scale, causal):
+    if _fast("prompt_attention", q, k, v, cu_seqlens, out, _scale_of(scale, q), causal):
         return out
     dt = q.dtype
     T = q.shape[0] if q.dim() else 0
@@ -798,7 +806,7 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     without a tree (T = 1: plain decode)."""
     if workspace is not None and out is not None and isinstance(q, torch.Tensor):
         if _fast("cache_attention", q, k_cache, v_cache, page_table, cache_lens, tree, workspace, out,
-                 q.shape[-1] ** -0.5 if scale is None else scale):
+                 _scale_of(scale, q)):
             return out
     code = _act_type(q, "q")
     dt = q.dtype

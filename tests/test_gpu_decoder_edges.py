@@ -108,3 +108,24 @@ def test_bad_numbers_touch_nothing(dev, eps, interleaved):
         ops.prompt_attention(q, k, v, cu, causal=NoBool(), out=out)
     torch.cuda.synchronize()
     assert (out == 5.0).all()
+
+
+def test_heads_of_no_values_are_refused(dev):
+    import torch
+    from forge_amd import ops
+    q = torch.empty((4, 2, 0), dtype=torch.float16, device=dev)
+    cu = torch.tensor([0, 4], dtype=torch.int32, device=dev)
+    with pytest.raises(ValueError):
+        ops.prompt_attention(q, q, q, cu)
+    w = torch.empty((0,), dtype=torch.float16, device=dev)
+    table = torch.empty((4, 0), device=dev)
+    with pytest.raises(ValueError):
+        ops.qk_norm_rope(q, q, w, w, table, table, cu.new_zeros(4))
+    with pytest.raises(ValueError):
+        ops.prompt_attention(q.new_zeros(()), q, q, cu)
+    cache = torch.empty((1, 16, 2, 0), dtype=torch.float16, device=dev)
+    one = torch.zeros((1, 1), dtype=torch.int32, device=dev)
+    ws = torch.empty((16,), dtype=torch.uint8, device=dev)
+    q4 = q.view(1, 4, 2, 0)
+    with pytest.raises(ValueError):
+        ops.cache_attention(q4, cache, cache, one, one[0], workspace=ws, out=torch.empty_like(q4))
