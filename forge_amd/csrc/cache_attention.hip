@@ -18,8 +18,10 @@
 
 namespace forge_amd {
 
-constexpr int kCacheMaxChunk = 2048;   // keys; a chunk's pages are looked up in LDS
+constexpr int kCacheMaxChunk = 2048;   // keys; a chunk's pages are looked up in LDS (128 more for the longest tables)
 constexpr int kCacheMaxTokens = 64;
+constexpr long long kCacheMaxKeys = 1LL << 27;
+constexpr int kGridRows = 65535;       // of a grid's second and third dimension
 
 struct CachePlan {
     int chunk, chunks;   // keys of a chunk; chunks of the longest sequence
@@ -272,7 +274,8 @@ CachePlan cache_plan(int B, int T, int Hq, int Hkv, long long max_keys) {
     const long long heads = static_cast<long long>(B) * Hkv * divup(rows, 32 * p.sets);
     const long long want = std::max<long long>(1, divupll(default_cu_count(), heads));
     const long long chunk = divupll(std::max<long long>(divupll(max_keys, want), rows), 128) * 128;
-    p.chunk = static_cast<int>(std::min<long long>(chunk, kCacheMaxChunk));
+    const long long most = std::max<long long>(kCacheMaxChunk, divupll(divupll(max_keys, kGridRows), 128) * 128);
+    p.chunk = static_cast<int>(std::min(chunk, most));
     p.chunks = static_cast<int>(std::max<long long>(1, divupll(max_keys, p.chunk)));
     return p;
 }
@@ -283,24 +286,42 @@ size_t cache_floats(int B, int T, int Hq, int D, const CachePlan& p) {
 
 template <class T, int DP, int RS, int KS, int KB>
 int launch_cache(CacheArgs a, hipStream_t s) {
-    constexpr int LPR = DP <= 64 ? 16 : DP <= 128 ? 32 : 64, kMost = kCacheLds<T, DP, RS, KS, KB> + 4 * (kCacheMaxChunk + 2);
+    constexpr int LPR = DP <= 64 ? 16 : DP <= 128 ? 32 : 64, kMost = kCacheLds<T, DP, RS, KS, KB> + 4 * (kCacheMaxChunk + 128 + 2);
     static_assert(kMost <= 159 * 1024, "tiles, sums and page numbers fit");
+    static_assert(divupll(kCacheMaxKeys, kGridRows) <= kCacheMaxChunk + 128, "the longest table's chunks are a grid's rows");
     const int lds = kCacheLds<T, DP, RS, KS, KB> + 4 * ((a.chunk >> a.page_shift) + 2);
     const int rows = a.T * (a.Hq / a.Hkv);
     a.sets = divup(rows, 32 * RS);
     a.mg_sets = udiv_multiplier(a.sets);
-    const long long z = static_cast<long long>(a.B) * a.sets;
-    if (a.chunks > 65535 || z > 65535) return FORGE_EINVAL;
     static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&cache_attention_kernel<T, DP, RS, KS, KB>),
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
     if (attr != hipSuccess) return static_cast<int>(attr);
-    const dim3 grid(static_cast<unsigned>(a.Hkv), static_cast<unsigned>(a.chunks), static_cast<unsigned>(z));
-    cache_attention_kernel<T, DP, RS, KS, KB><<<grid, 64 * RS * KS, lds, s>>>(a);
-    const int st = launch_status();
-    if (st != FORGE_OK || a.chunks == 1) return st;
-    const dim3 rows_grid(static_cast<unsigned>(divup(a.Hq, 4)), static_cast<unsigned>(a.T), static_cast<unsigned>(a.B));
-    cache_join_kernel<T, LPR><<<rows_grid, 256, 0, s>>>(a);
-    return launch_status();
+    // as many sequences at a time as a grid has rows
+    const long long total = a.B, most = kGridRows / a.sets;
+    const size_t parts = static_cast<size_t>(a.T) * a.Hq * a.chunks;     // of a sequence
+    for (long long b = 0; b < total; b += most) {
+        a.B = static_cast<int>(std::min(most, total - b));
+        const dim3 grid(static_cast<unsigned>(a.Hkv), static_cast<unsigned>(a.chunks), static_cast<unsigned>(a.B * a.sets));
+        cache_attention_kernel<T, DP, RS, KS, KB><<<grid, 64 * RS * KS, lds, s>>>(a);
+        int st = launch_status();
+        if (st == FORGE_OK && a.chunks > 1) {
+            const dim3 rows_grid(static_cast<unsigned>(divup(a.Hq, 4)), static_cast<unsigned>(a.T), static_cast<unsigned>(a.B));
+            cache_join_kernel<T, LPR><<<rows_grid, 256, 0, s>>>(a);
+            st = launch_status();
+        }
+        if (st != FORGE_OK) return st;
+        const size_t q = static_cast<size_t>(a.B) * a.T * a.Hq * a.D;
+        a.q += q;
+        a.out += q;
+        a.table += static_cast<size_t>(a.B) * a.width;
+        a.lens += a.B;
+        if (a.tree) a.tree += static_cast<size_t>(a.B) * a.T;
+        if (a.part) {
+            a.part += a.B * parts * a.D;
+            a.stat += a.B * parts * 2;
+        }
+    }
+    return FORGE_OK;
 }
 
 // Waves by 32-row sets, then by keys, up to 8 (4 at 256 values a head, whose sums take 128 registers a lane);
@@ -323,9 +344,13 @@ int launch_cache(const CacheArgs& a, int sets, hipStream_t s) {
     }
 }
 
+// Rows (up to the last set's end) and heads are divided by the heads of a group in udiv_magic's range. The row sets of a
+// sequence are then under 2^13, a few sequences' at least fit a grid, and their number too is divided in that range.
 bool cache_shape_ok(int B, int T, int Hq, int Hkv, int D) {
-    return B > 0 && T > 0 && T <= kCacheMaxTokens && Hq > 0 && Hkv > 0 && Hq % Hkv == 0 && D > 0 && D % 8 == 0 &&
-           D <= 256 && static_cast<long long>(B) * T * Hq <= INT_MAX;
+    if (B <= 0 || T <= 0 || T > kCacheMaxTokens || Hq <= 0 || Hkv <= 0 || Hq % Hkv != 0 || D <= 0 || D % 8 != 0 || D > 256)
+        return false;
+    const long long group = Hq / Hkv;
+    return static_cast<long long>(B) * T * Hq <= INT_MAX && (T * group + 128) * group < 1LL << 32 && (Hq + 4LL) * group < 1LL << 32;
 }
 
 }  // namespace forge_amd
@@ -333,7 +358,7 @@ bool cache_shape_ok(int B, int T, int Hq, int Hkv, int D) {
 using namespace forge_amd;
 
 extern "C" size_t forge_cache_attention_workspace_size(int B, int T, int Hq, int Hkv, int D, long long max_keys) {
-    if (!cache_shape_ok(B, T, Hq, Hkv, D) || max_keys <= 0) return 0;
+    if (!cache_shape_ok(B, T, Hq, Hkv, D) || max_keys <= 0 || max_keys > kCacheMaxKeys) return 0;
     return 4 * cache_floats(B, T, Hq, D, cache_plan(B, T, Hq, Hkv, max_keys));
 }
 
@@ -352,7 +377,7 @@ extern "C" int forge_cache_attention(const uint16_t* q, const uint16_t* k_cache,
                           static_cast<const void*>(out), static_cast<const void*>(workspace)})
         if (!aligned(p, 16)) return FORGE_EINVAL;
     const long long max_keys = static_cast<long long>(table_width) * page_size;
-    if (max_keys > 1 << 27) return FORGE_EINVAL;
+    if (max_keys > kCacheMaxKeys) return FORGE_EINVAL;
     const CachePlan p = cache_plan(B, T, Hq, Hkv, max_keys);
     const size_t floats = cache_floats(B, T, Hq, D, p);
     if (floats && (!workspace || workspace_bytes < 4 * floats)) return FORGE_EINVAL;

@@ -357,7 +357,8 @@ int forge_prompt_attention(const uint16_t* q, const uint16_t* k, const uint16_t*
 
 /* Attention of T (1 to 64) new tokens per sequence, q and out (B,T,Hq,D), over a paged cache:
  * k_cache, v_cache (pages,page_size,Hkv,D), page_size a power of two and table_width * page_size <= 2^27; position j of sequence b is row
- * j % page_size of page page_table[b, j / page_size] (B,table_width). The new tokens' own keys and values are in
+ * j % page_size of page page_table[b, j / page_size] (B,table_width). B * T * Hq is under 2^31 and, with G = Hq / Hkv,
+ * (T * G + 128) * G and (Hq + 4) * G under 2^32. The new tokens' own keys and values are in
  * the cache already, at positions cache_lens[b] to cache_lens[b] + T - 1. Token t sees every position before
  * cache_lens[b] and the new tokens whose bit is set in tree[b,t] (B,T), or tokens 0..t when
  * tree is NULL; positions past the table are not seen, pages outside the cache read as zeros, and a token

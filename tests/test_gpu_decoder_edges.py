@@ -129,3 +129,46 @@ def test_heads_of_no_values_are_refused(dev):
     q4 = q.view(1, 4, 2, 0)
     with pytest.raises(ValueError):
         ops.cache_attention(q4, cache, cache, one, one[0], workspace=ws, out=torch.empty_like(q4))
+
+
+# ---- attention -----------------------------------------------------------------------------------
+
+def normals(shape, dt, dev, seed):
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(shape, generator=g).to(getattr(torch, dt)).to(dev)
+
+
+def test_longest_table(dev):
+    """A table of 2^27 positions, the most that there may be."""
+    import torch
+    from forge_amd import ops
+    page, n, D = 4096, 5000, 64
+    q, k, v = normals((1, 1, 2, D), "float16", dev, 13), normals((2, page, 1, D), "float16", dev, 14), normals((2, page, 1, D), "float16", dev, 15)
+    table = torch.full((1, (1 << 27) // page), -1, dtype=torch.int32, device=dev)
+    table[0, :2] = torch.tensor([1, 0])
+    lens = torch.tensor([n], dtype=torch.int32, device=dev)
+    out = ops.cache_attention(q, k, v, table, lens)
+    from attention_plain import check
+    kk, vv = torch.cat([k[1], k[0]])[:n + 1, 0], torch.cat([v[1], v[0]])[:n + 1, 0]
+    for h in range(2):
+        check(out[0, :, h], q[0, :, h], kk, vv, torch.ones((1, n + 1), dtype=torch.bool, device=dev), D ** -0.5)
+
+
+@pytest.mark.parametrize("keys", [30, 3000])
+def test_many_sequences(dev, keys):
+    """More sequences than a grid has rows: each its own query over one cache that they share."""
+    import torch
+    from attention_plain import check
+    from forge_amd import ops
+    B, D = 70001, 8
+    page = 16 if keys < 100 else 4096
+    q, k, v = normals((B, 1, 1, D), "float16", dev, 16), normals((2, page, 1, D), "float16", dev, 17), normals((2, page, 1, D), "float16", dev, 18)
+    lens = keys - torch.arange(B, dtype=torch.int32, device=dev) % 3
+    table = torch.tensor([[0, 1]], dtype=torch.int32, device=dev).repeat(B, 1)
+    out = ops.cache_attention(q, k, v, table, lens)
+    for r in range(3):
+        n = keys - r + 1
+        rows = torch.arange(r, B, 3, device=dev)
+        kk, vv = k.view(-1, D)[:n], v.view(-1, D)[:n]
+        check(out[rows, 0, 0], q[rows, 0, 0], kk, vv, torch.ones((len(rows), n), dtype=torch.bool, device=dev), D ** -0.5)
