@@ -1,6 +1,6 @@
 // One wave's attention over a tile of keys that lies in LDS, for FP16 and BF16.
 //
-// The wave owns 32 query rows (a second set of 32 in the cache kernel). It multiplies S^T = K Q^T on
+// The wave owns 32 query rows. It multiplies S^T = K Q^T on
 // 32 x 32 x 16 products: keys are the A operand's rows, queries the B operand's columns, and a lane
 // ends up with 16 of a block's 32 scores of ONE query (lane l: query l % 32; register e: key 8 (e / 4) +
 // 4 (l / 32) + e % 4). Row maxima and sums are then mostly inside a lane (one exchange with lane l ^ 32),
@@ -60,13 +60,13 @@ __device__ __forceinline__ uint32_t bits_to(int last) {
     return last >= 31 ? ~0u : last < 0 ? 0u : (2u << last) - 1u;
 }
 
-template <class T, int DP, int RB, int KB>
+template <class T, int DP, int KB>
 struct AttnWave {
     using Rows = KvRows<DP>;
     static constexpr int kSteps = DP / 16, kOut = DP / 32;
-    v4u q[RB][kSteps];
-    v16f o[RB][kOut];
-    float m[RB], l[RB];      // of query lane % 32; l: this lane's keys only
+    v4u q[kSteps];
+    v16f o[kOut];
+    float m, l;              // of query lane % 32; l: this lane's keys only
     int lane, k_at, v_at;    // byte addresses in a tile, before the chunk permutation
     int k_x, v_x;            // the permutations, as byte masks
 
@@ -77,23 +77,20 @@ struct AttnWave {
         k_x = (half ^ Rows::swz_k(r)) * 16;
         v_at = vr * Rows::kBytes + (i & 1) * 8;
         v_x = ((2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ Rows::swz_v(vr)) * 16;
+        m = kNoScore;
+        l = 0.0f;
 #pragma unroll
-        for (int b = 0; b < RB; b++) {
-            m[b] = kNoScore;
-            l[b] = 0.0f;
+        for (int j = 0; j < kOut; j++)
 #pragma unroll
-            for (int j = 0; j < kOut; j++)
-#pragma unroll
-                for (int e = 0; e < 16; e++) o[b][j][e] = 0.0f;
-        }
+            for (int e = 0; e < 16; e++) o[j][e] = 0.0f;
     }
 
-    // Query row of set b; D values at p, or zeros.
-    __device__ __forceinline__ void load_q(int b, const uint16_t* p, bool live, int D) {
+    // D values of the query row at p, or zeros.
+    __device__ __forceinline__ void load_q(const uint16_t* p, bool live, int D) {
 #pragma unroll
         for (int s = 0; s < kSteps; s++) {
             const int d = 16 * s + 8 * (lane >> 5);
-            q[b][s] = live && d < D ? *reinterpret_cast<const v4u*>(p + d) : v4u{0u, 0u, 0u, 0u};
+            q[s] = live && d < D ? *reinterpret_cast<const v4u*>(p + d) : v4u{0u, 0u, 0u, 0u};
         }
     }
 
@@ -111,8 +108,8 @@ struct AttnWave {
         }
     }
 
-    using Scores = v16f[RB][KB];
-    using Weights = v4u[RB][KB][2];
+    using Scores = v16f[KB];
+    using Weights = v4u[KB][2];
 
     // Scores of a tile of 32 KB keys; products in a row go to different sums.
     __device__ __forceinline__ void scores(const int8_t* ks, Scores& s) const {
@@ -121,45 +118,40 @@ struct AttnWave {
 #pragma unroll
             for (int kb = 0; kb < KB; kb++) {
                 const v4u k = *reinterpret_cast<const v4u*>(ks + 32 * kb * Rows::kBytes + k_at + ((32 * st) ^ k_x));
-#pragma unroll
-                for (int b = 0; b < RB; b++) {
-                    const v16f zero = {};
-                    s[b][kb] = T::mfma32(k, q[b][st], st == 0 ? zero : s[b][kb]);
-                }
+                const v16f zero = {};
+                s[kb] = T::mfma32(k, q[st], st == 0 ? zero : s[kb]);
             }
-        if constexpr (RB == 1) interleave<KB * kSteps, 1, kAhead>();
+        interleave<KB * kSteps, 1, kAhead>();
     }
 
-    // seen(b, kb) has a bit for each key of block kb that this lane's row of set b sees.
+    // seen(kb) has a bit for each key of block kb that this lane's row sees.
     template <class Seen>
     __device__ __forceinline__ void mask(Scores& s, const Seen& seen) const {
 #pragma unroll
-        for (int b = 0; b < RB; b++)
+        for (int kb = 0; kb < KB; kb++) {
+            const uint32_t bits = seen(kb) >> (4 * (lane >> 5));
 #pragma unroll
-            for (int kb = 0; kb < KB; kb++) {
-                const uint32_t bits = seen(b, kb) >> (4 * (lane >> 5));
-#pragma unroll
-                for (int e = 0; e < 16; e++)
-                    if (!(bits & (1u << (8 * (e / 4) + e % 4)))) s[b][kb][e] = -INFINITY;
-            }
+            for (int e = 0; e < 16; e++)
+                if (!(bits & (1u << (8 * (e / 4) + e % 4)))) s[kb][e] = -INFINITY;
+        }
     }
 
-    // The largest score of set b's row, in the exponent's units.
-    __device__ __forceinline__ float largest(const Scores& s, int b, float scale2) const {
+    // The row's largest score, in the exponent's units.
+    __device__ __forceinline__ float largest(const Scores& s, float scale2) const {
         float mx[4];
 #pragma unroll
         for (int c = 0; c < 4; c++) {                                // four chains of maxima of three
-            mx[c] = s[b][0][4 * c];
+            mx[c] = s[0][4 * c];
 #pragma unroll
             for (int kb = 0; kb < KB; kb++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) mx[c] = fmaxf(mx[c], s[b][kb][4 * c + e]);
+                for (int e = 0; e < 4; e++) mx[c] = fmaxf(mx[c], s[kb][4 * c + e]);
         }
         return half_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))) * scale2;
     }
 
-    // The weights of set b against its maximum as it stands; returns their sum.
-    __device__ __forceinline__ float weights(const Scores& s, int b, float scale2, Weights& p) const {
+    // The weights against the maximum as it stands; returns their sum.
+    __device__ __forceinline__ float weights(const Scores& s, float scale2, Weights& p) const {
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
@@ -167,10 +159,10 @@ struct AttnWave {
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int d = 0; d < 4; d++) {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][kb][8 * h + 2 * d], scale2, -m[b]));
-                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[b][kb][8 * h + 2 * d + 1], scale2, -m[b]));
-                    p[b][kb][h][d] = T::pack(x, y);
-                    sum[h] = T::add_pair(p[b][kb][h][d], sum[h]);
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * h + 2 * d], scale2, -m));
+                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * h + 2 * d + 1], scale2, -m));
+                    p[kb][h][d] = T::pack(x, y);
+                    sum[h] = T::add_pair(p[kb][h][d], sum[h]);
                 }
         return sum[0] + sum[1];
     }
@@ -186,45 +178,31 @@ struct AttnWave {
                     const int8_t* at = vs + (32 * kb + 16 * h) * Rows::kBytes + v_at + ((64 * j) ^ v_x);
                     const v2u lo = lds_read_tr(at), hi = lds_read_tr(at + 8 * Rows::kBytes);
                     const v4u v = {lo[0], lo[1], hi[0], hi[1]};
-#pragma unroll
-                    for (int b = 0; b < RB; b++) o[b][j] = T::mfma32(v, p[b][kb][h], o[b][j]);
+                    o[j] = T::mfma32(v, p[kb][h], o[j]);
                 }
-        if constexpr (RB == 1) interleave<2 * KB * kOut, 2, kAhead>();
+        interleave<2 * KB * kOut, 2, kAhead>();
     }
 
     // A tile from its scores on; masked if `masked`. `first`: nothing has been summed yet. (Both uniform.)
     template <class Seen>
     __device__ __forceinline__ void finish(Scores& s, const int8_t* vs, float scale2, bool first, bool masked, const Seen& seen) {
         if (masked) mask(s, seen);
-        if (first) {
-#pragma unroll
-            for (int b = 0; b < RB; b++) m[b] = fmaxf(m[b], largest(s, b, scale2));
-        }
+        if (first) m = fmaxf(m, largest(s, scale2));
         Weights p;
-        float sum[RB], mx[RB];
-        bool grown = false;
-#pragma unroll
-        for (int b = 0; b < RB; b++) {
-            sum[b] = weights(s, b, scale2, p);
-            mx[b] = largest(s, b, scale2);
-            grown |= mx[b] > m[b] + kRescale;
-        }
+        float sum = weights(s, scale2, p);
+        const float mx = largest(s, scale2);
         // A maximum that has grown is met seldom, and so the weights do not wait for it: they are taken again.
-        if (__any(grown)) {
+        if (__any(mx > m + kRescale)) {
+            const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= f;
 #pragma unroll
-            for (int b = 0; b < RB; b++) {
-                const float mn = fmaxf(m[b], mx[b]), f = __builtin_amdgcn_exp2f(m[b] - mn);
-                m[b] = mn;
-                l[b] *= f;
+            for (int j = 0; j < kOut; j++)
 #pragma unroll
-                for (int j = 0; j < kOut; j++)
-#pragma unroll
-                    for (int e = 0; e < 16; e++) o[b][j][e] *= f;
-                sum[b] = weights(s, b, scale2, p);
-            }
+                for (int e = 0; e < 16; e++) o[j][e] *= f;
+            sum = weights(s, scale2, p);
         }
-#pragma unroll
-        for (int b = 0; b < RB; b++) l[b] += sum[b];
+        l += sum;
         values(vs, p);
     }
 
@@ -238,14 +216,14 @@ struct AttnWave {
     };
     template <int W>
     __device__ __forceinline__ void leave(Shared<W>* sh, int wave, bool live) const {
-        const float sum = half_sum(l[0]);
-        if (lane < 32) sh->stat[wave][lane] = v2f{m[0], sum};
+        const float sum = half_sum(l);
+        if (lane < 32) sh->stat[wave][lane] = v2f{m, sum};
         if (!live) return;                                           // a row that nobody asks for
 #pragma unroll
         for (int j = 0; j < kOut; j++)
 #pragma unroll
             for (int e = 0; e < 4; e++)
-                sh->sums[wave][4 * j + e][lane] = v4f{o[0][j][4 * e], o[0][j][4 * e + 1], o[0][j][4 * e + 2], o[0][j][4 * e + 3]};
+                sh->sums[wave][4 * j + e][lane] = v4f{o[j][4 * e], o[j][4 * e + 1], o[j][4 * e + 2], o[j][4 * e + 3]};
     }
     template <int KS, int W, class Put>
     __device__ __forceinline__ void join(const Shared<W>* sh, int wave, const Put& put) const {
@@ -279,13 +257,13 @@ struct AttnWave {
     }
 
     // Whether some value of the rows `live` is no finite number.
-    __device__ __forceinline__ bool odd(int b, bool live) const {
+    __device__ __forceinline__ bool odd(bool live) const {
         float z = 0.0f;
 #pragma unroll
         for (int j = 0; j < kOut; j++)
 #pragma unroll
-            for (int e = 0; e < 16; e++) z = __builtin_fmaf(o[b][j][e], 0.0f, z);
-        z = __builtin_fmaf(l[b], 0.0f, z);
+            for (int e = 0; e < 16; e++) z = __builtin_fmaf(o[j][e], 0.0f, z);
+        z = __builtin_fmaf(l, 0.0f, z);
         return __any(live && z != 0.0f);
     }
 };

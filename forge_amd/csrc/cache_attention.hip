@@ -50,7 +50,7 @@ __device__ __forceinline__ int cache_keys(const CacheArgs& a, int b) {
 // LDS of the tiles, in which the waves' sums are left afterwards; the chunk's page numbers follow.
 template <class T, int DP, int RS, int KS, int KB>
 constexpr int kCacheLds = std::max<int>(4 * 32 * KS * KB * KvRows<DP>::kBytes,
-                                        sizeof(typename AttnWave<T, DP, 1, KB>::template Shared<RS * KS>));
+                                        sizeof(typename AttnWave<T, DP, KB>::template Shared<RS * KS>));
 
 template <class T, int DP, int RS, int KS, int KB>
 __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attention_kernel(CacheArgs a)
@@ -94,11 +94,11 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
         return a.tree ? static_cast<unsigned long long>(a.tree[static_cast<size_t>(b) * a.T + t]) : ~0ull >> (63 - t);
     };
 
-    AttnWave<T, DP, 1, KB> w;
+    AttnWave<T, DP, KB> w;
     w.init();
     const int row = (set * RS + rs) * 32 + (lane & 31);
     const bool live = row < rows;
-    w.load_q(0, row_of(a.q, row), live, a.D);
+    w.load_q(row_of(a.q, row), live, a.D);
     const unsigned long long drafts = live ? drafts_of(row) : 0ull;
     const int keys = cache_keys(a, b), len = max(a.lens[b], 0), n = min(keys - key0, a.chunk);
     if (n <= 0) return;
@@ -135,9 +135,9 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
         if (t + 1 < tiles) load(t + 1);
         const int k0 = t * kKeys + 32 * KB * ks;                     // this wave's keys of the tile
         const int8_t* at = lds + (t & 1) * 2 * kTile + 32 * KB * ks * Rows::kBytes;
-        v16f s[1][KB];
+        v16f s[KB];
         w.scores(at, s);
-        w.finish(s, at + kTile, scale2, t == 0, k0 + 32 * KB > min(open, n), [&](int, int kb) {
+        w.finish(s, at + kTile, scale2, t == 0, k0 + 32 * KB > min(open, n), [&](int kb) {
             const int d = open - (k0 + 32 * kb);                     // bits below d: the cache; from d on: drafts
             uint32_t bits = bits_to(d - 1);
             if (d < 32) bits |= d >= 0 ? static_cast<uint32_t>(drafts << d) : d > -64 ? static_cast<uint32_t>(drafts >> -d) : 0u;
@@ -147,8 +147,8 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
 
     wait_vm_lgkm<0>();
     __syncthreads();
-    auto* sh = reinterpret_cast<typename AttnWave<T, DP, 1, KB>::template Shared<W>*>(lds);
-    if (w.odd(0, live) && lane == 0) atomicOr(&odd_rows, 1);
+    auto* sh = reinterpret_cast<typename AttnWave<T, DP, KB>::template Shared<W>*>(lds);
+    if (w.odd(live) && lane == 0) atomicOr(&odd_rows, 1);
     w.leave(sh, wave, live);
     __syncthreads();
     const bool whole = keys <= a.chunk;                              // the only chunk: the result itself

@@ -74,9 +74,9 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void prompt_attenti
         return;
     }
 
-    AttnWave<T, DP, 1, kPromptKeys / 32> w;
+    AttnWave<T, DP, kPromptKeys / 32> w;
     w.init();
-    w.load_q(0, a.q + static_cast<size_t>(start + row) * a.q_token + hq * a.q_head, row < len, a.D);
+    w.load_q(a.q + static_cast<size_t>(start + row) * a.q_token + hq * a.q_head, row < len, a.D);
 
     const uint16_t* kbase = a.k + static_cast<size_t>(start) * a.k_token + hk * a.k_head;
     const uint16_t* vbase = a.v + static_cast<size_t>(start) * a.v_token + hk * a.v_head;
@@ -126,10 +126,10 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void prompt_attenti
         next(t);
         const int8_t* at = lds + (t % NS) * 2 * kTile + kPromptKeys * ks * Rows::kBytes;
         const int k0 = t * kKeys + kPromptKeys * ks;
-        v16f s[1][kPromptKeys / 32];
+        v16f s[kPromptKeys / 32];
         w.scores(at, s);
         w.finish(s, at + kTile, scale2, t == 0, (CAUSAL && k0 + kPromptKeys - 1 > first) || k0 + kPromptKeys > len,
-                 [&](int, int kb) { return bits_to((CAUSAL ? min(row, len - 1) : len - 1) - k0 - 32 * kb); });
+                 [&](int kb) { return bits_to((CAUSAL ? min(row, len - 1) : len - 1) - k0 - 32 * kb); });
     }
     for (; t < tiles; t++) next(t);
     const bool live = row < len;
@@ -149,11 +149,11 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void prompt_attenti
         }
     };
     if constexpr (KS == 1) {
-        if (w.odd(0, live)) {
+        if (w.odd(live)) {
             again(32 * rs, 32 * rs + 32, 1);
             return;
         }
-        const float l = half_sum(w.l[0]);
+        const float l = half_sum(w.l);
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
         if (!live) return;
 #pragma unroll
@@ -162,16 +162,16 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void prompt_attenti
             for (int e = 0; e < 16; e += 4) {
                 const int d = 32 * j + 2 * e + 4 * (lane >> 5);
                 if (d < a.D)
-                    *reinterpret_cast<v2u*>(out + d) = v2u{T::pack(w.o[0][j][e] * inv, w.o[0][j][e + 1] * inv),
-                                                           T::pack(w.o[0][j][e + 2] * inv, w.o[0][j][e + 3] * inv)};
+                    *reinterpret_cast<v2u*>(out + d) = v2u{T::pack(w.o[j][e] * inv, w.o[j][e + 1] * inv),
+                                                           T::pack(w.o[j][e + 2] * inv, w.o[j][e + 3] * inv)};
             }
     } else {
         __shared__ int odd_rows;
-        auto* sh = reinterpret_cast<typename AttnWave<T, DP, 1, kPromptKeys / 32>::template Shared<W>*>(lds);
+        auto* sh = reinterpret_cast<typename AttnWave<T, DP, kPromptKeys / 32>::template Shared<W>*>(lds);
         if (threadIdx.x == 0) odd_rows = 0;
         wait_vm_lgkm<0>();
         __syncthreads();
-        if (w.odd(0, live) && lane == 0) atomicOr(&odd_rows, 1);
+        if (w.odd(live) && lane == 0) atomicOr(&odd_rows, 1);
         w.leave(sh, wave, live);
         __syncthreads();
         if (odd_rows) {
@@ -190,7 +190,7 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void prompt_attenti
 
 template <class T, int DP, int RS, int KS, int NS, bool CAUSAL>
 int launch_prompt(PromptArgs a, hipStream_t s) {
-    constexpr int kTiles = NS * 2 * kPromptKeys * KS * KvRows<DP>::kBytes, kSums = KS > 1 ? sizeof(typename AttnWave<T, DP, 1, 2>::template Shared<RS * KS>) : 0;
+    constexpr int kTiles = NS * 2 * kPromptKeys * KS * KvRows<DP>::kBytes, kSums = KS > 1 ? sizeof(typename AttnWave<T, DP, 2>::template Shared<RS * KS>) : 0;
     constexpr int kLds = kTiles > kSums ? kTiles : kSums;
     const long long tiles = a.tokens / (32 * RS) + static_cast<long long>(a.sequences) + 1;
     const long long units = tiles * a.Hkv, wgs = divupll(units, 8) * 8 * (a.Hq / a.Hkv);
