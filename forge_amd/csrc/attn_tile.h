@@ -18,10 +18,13 @@
 #include "float16_types.h"
 #include "lds_dma.h"
 
+#include <cfloat>
+
 namespace forge_amd {
 
-constexpr float kNoScore = -1e30f;   // running maximum of a row that has seen nothing
+constexpr float kNoScore = -FLT_MAX;   // running maximum of a row that has seen nothing: no score is below it
 constexpr float kRescale = 8.0f;
+constexpr float kFar = 1048576.0f;
 
 typedef short v4s __attribute__((ext_vector_type(4)));
 
@@ -67,6 +70,7 @@ struct AttnWave {
     v4u q[kSteps];
     v16f o[kOut];
     float m, l;              // of query lane % 32; l: this lane's keys only
+    float limit;             // a larger score has the weights taken again
     int lane, k_at, v_at;    // byte addresses in a tile, before the chunk permutation
     int k_x, v_x;            // the permutations, as byte masks
 
@@ -78,6 +82,7 @@ struct AttnWave {
         v_at = vr * Rows::kBytes + (i & 1) * 8;
         v_x = ((2 * ((lane >> 4) & 1) + ((i & 3) >> 1)) ^ Rows::swz_v(vr)) * 16;
         m = kNoScore;
+        limit = kNoScore;
         l = 0.0f;
 #pragma unroll
         for (int j = 0; j < kOut; j++)
@@ -150,8 +155,8 @@ struct AttnWave {
         return half_max(fmaxf(fmaxf(mx[0], mx[1]), fmaxf(mx[2], mx[3]))) * scale2;
     }
 
-    // The weights against the maximum as it stands; returns their sum.
-    __device__ __forceinline__ float weights(const Scores& s, float scale2, Weights& p) const {
+    // The weights 2^(unit s + shift); returns their sum.
+    __device__ __forceinline__ float weights(const Scores& s, float unit, float shift, Weights& p) const {
         float sum[2] = {0.0f, 0.0f};
 #pragma unroll
         for (int kb = 0; kb < KB; kb++)
@@ -159,12 +164,32 @@ struct AttnWave {
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int d = 0; d < 4; d++) {
-                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * h + 2 * d], scale2, -m));
-                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * h + 2 * d + 1], scale2, -m));
+                    const float x = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * h + 2 * d], unit, shift));
+                    const float y = __builtin_amdgcn_exp2f(__builtin_fmaf(s[kb][8 * h + 2 * d + 1], unit, shift));
                     p[kb][h][d] = T::pack(x, y);
                     sum[h] = T::add_pair(p[kb][h][d], sum[h]);
                 }
         return sum[0] + sum[1];
+    }
+
+    // The maximum takes x in. Rows whose scores lie far from zero have their weights always taken again: a fused multiply-add does
+    // not round scale2 s, as the maximum was, and that difference (2^-4 of an exponent at kFar) would at last move
+    // all weights of a row out of their type.
+    __device__ __forceinline__ void raise(float x) {
+        m = fmaxf(m, x);
+        limit = fabsf(m) > kFar && m != kNoScore ? -INFINITY : m + kRescale;
+    }
+
+    // The exponents in place of the scores, each product rounded as the maximum's was.
+    __device__ __forceinline__ void exponents(Scores& s, float scale2) const {
+#pragma clang fp contract(off)
+#pragma unroll
+        for (int kb = 0; kb < KB; kb++)
+#pragma unroll
+            for (int e = 0; e < 16; e++) {
+                const float x = s[kb][e] * scale2;
+                s[kb][e] = x - m;
+            }
     }
 
     // O += P V of a tile.
@@ -187,20 +212,22 @@ struct AttnWave {
     template <class Seen>
     __device__ __forceinline__ void finish(Scores& s, const int8_t* vs, float scale2, bool first, bool masked, const Seen& seen) {
         if (masked) mask(s, seen);
-        if (first) m = fmaxf(m, largest(s, scale2));
+        if (first) raise(largest(s, scale2));
         Weights p;
-        float sum = weights(s, scale2, p);
+        float sum = weights(s, scale2, -m, p);
         const float mx = largest(s, scale2);
-        // A maximum that has grown is met seldom, and so the weights do not wait for it: they are taken again.
-        if (__any(mx > m + kRescale)) {
-            const float mn = fmaxf(m, mx), f = __builtin_amdgcn_exp2f(m - mn);
-            m = mn;
+        // A maximum that has grown is met seldom: the weights are taken again.
+        if (__any(mx > limit)) {
+            const float was = m;
+            raise(mx);
+            const float f = __builtin_amdgcn_exp2f(was - m);
             l *= f;
 #pragma unroll
             for (int j = 0; j < kOut; j++)
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[j][e] *= f;
-            sum = weights(s, scale2, p);
+            exponents(s, scale2);
+            sum = weights(s, 1.0f, 0.0f, p);
         }
         l += sum;
         values(vs, p);

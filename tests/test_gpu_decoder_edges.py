@@ -133,10 +133,63 @@ def test_heads_of_no_values_are_refused(dev):
 
 # ---- attention -----------------------------------------------------------------------------------
 
+def prompt(q, k, v, **kw):
+    """prompt_attention of one sequence: q (n, Hq, D), k and v (n, Hkv, D)."""
+    import torch
+    from forge_amd import ops
+    return ops.prompt_attention(q, k, v, torch.tensor([0, q.shape[0]], dtype=torch.int32, device=q.device), **kw)
+
+
+def cached(q, k, v, T, page=16, tree=None):
+    """cache_attention of the last T tokens of one sequence over the others' keys and values: (T, Hq, D)."""
+    import torch
+    from forge_amd import ops
+    n, Hkv, D = k.shape
+    pages = (n + page - 1) // page
+    kc, vc = (torch.zeros((pages * page, Hkv, D), dtype=k.dtype, device=k.device) for _ in range(2))
+    kc[:n], vc[:n] = k, v
+    table = torch.arange(pages, dtype=torch.int32, device=k.device)[None]
+    lens = torch.tensor([n - T], dtype=torch.int32, device=k.device)
+    return ops.cache_attention(q[None, n - T:].contiguous(), kc.view(pages, page, Hkv, D), vc.view(pages, page, Hkv, D), table, lens,
+                               tree=tree)[0]
+
+
+# (tokens, Hq, Hkv, D): every way in which a prompt's rows and keys are split
+PROMPTS = [(200, 4, 2, 64), (300, 2, 1, 64), (300, 2, 1, 80), (300, 2, 2, 128), (700, 64, 8, 128), (300, 3, 1, 256)]
+# (keys, T, Hq, Hkv, D): one, two and four sets of rows, one chunk of keys and several
+CACHES = [(40, 1, 4, 1, 64), (900, 1, 8, 2, 128), (900, 5, 16, 2, 64), (700, 61, 4, 1, 128), (900, 3, 2, 1, 256), (500, 40, 4, 1, 256),
+          (2500, 16, 4, 2, 80)]
+
+
 def normals(shape, dt, dev, seed):
     import torch
     g = torch.Generator().manual_seed(seed)
     return torch.randn(shape, generator=g).to(getattr(torch, dt)).to(dev)
+
+
+@pytest.mark.parametrize("dt,top,step", [("bfloat16", -1.0, -1.0), ("bfloat16", -512.0, -512.0), ("bfloat16", 64.0, -1.0),
+                                         ("float16", 3.0, -0.25), ("float16", -0.5, -0.25)])
+def test_scores_far_from_zero(dev, dt, top, step):
+    """Scores of any size that FP32 holds, far apart from key to key: a row's result is the value of its best key. In units of the largest
+    scores tried, q k is top + step * (the key's rank)."""
+    import torch
+    q_one = 1e16 if dt == "bfloat16" else 3e4
+    k_one = 1e16 if dt == "bfloat16" else 5e3
+    for i, (n, T, Hq, Hkv, D) in enumerate([(n, 0, *rest) for n, *rest in PROMPTS] + CACHES):
+        say(f"scores far from zero {dt} top={top} n={n} T={T} Hq={Hq} D={D}")
+        v = normals((n, Hkv, D), dt, dev, i)
+        q = torch.full((n, Hq, D), q_one, dtype=v.dtype, device=dev)
+        rank = torch.randperm(n, generator=torch.Generator().manual_seed(i)) % 8      # 8 different scores, the first keys not the best
+        best = torch.tensor([int(rank[:r + 1].min()) for r in range(n)])
+        k = ((top + step * rank.float()) * k_one).to(v.dtype).to(dev)[:, None, None].expand(n, Hkv, D).contiguous()
+        out = prompt(q, k, v) if T == 0 else cached(q, k, v, T)
+        for r in range(n - T if T else 0, n, 1 if T else 7):
+            ties = (rank[:r + 1] == best[r]).to(dev)
+            mean = v[:r + 1][ties].double().mean(0).repeat_interleave(Hq // Hkv, 0)
+            size = v[:r + 1][ties].double().abs().mean(0).repeat_interleave(Hq // Hkv, 0)
+            u = 2.0 ** -8 if dt == "bfloat16" else 2.0 ** -11
+            got = out[r - (n - T) if T else r].double()
+            assert ((got - mean).abs() <= u * mean.abs() + n * 2.0 ** -23 * size + 2.0 ** -25).all(), (r, best[r])
 
 
 def test_longest_table(dev):
