@@ -71,6 +71,7 @@ struct AttnWave {
     v16f o[kOut];
     float m, l;              // of query lane % 32; l: this lane's keys only
     float limit;             // a larger score has the weights taken again
+    float low, shift;        // all weights are 2^-low of themselves; -(m + low)
     int lane, k_at, v_at;    // byte addresses in a tile, before the chunk permutation
     int k_x, v_x;            // the permutations, as byte masks
 
@@ -89,6 +90,11 @@ struct AttnWave {
 #pragma unroll
             for (int e = 0; e < 16; e++) o[j][e] = 0.0f;
     }
+
+    // The keys of the sequence. BF16 values may be as large as FP32 holds, and a sum of them must not pass that: the weights, each
+    // up to 2^kRescale, are taken so low that all of them add up to less than one. BF16 has the range for it; FP16 has not,
+    // and its values do not need it.
+    __device__ __forceinline__ void keys(int n) { low = T::kWide ? kRescale + 33 - __builtin_clz(n) : 0.0f; }
 
     // D values of the query row at p, or zeros.
     __device__ __forceinline__ void load_q(const uint16_t* p, bool live, int D) {
@@ -178,6 +184,7 @@ struct AttnWave {
     __device__ __forceinline__ void raise(float x) {
         m = fmaxf(m, x);
         limit = fabsf(m) > kFar && m != kNoScore ? -INFINITY : m + kRescale;
+        shift = -(m + low);
     }
 
     // The exponents in place of the scores, each product rounded as the maximum's was.
@@ -214,7 +221,7 @@ struct AttnWave {
         if (masked) mask(s, seen);
         if (first) raise(largest(s, scale2));
         Weights p;
-        float sum = weights(s, scale2, -m, p);
+        float sum = weights(s, scale2, shift, p);
         const float mx = largest(s, scale2);
         // A maximum that has grown is met seldom: the weights are taken again.
         if (__any(mx > limit)) {
@@ -227,7 +234,7 @@ struct AttnWave {
 #pragma unroll
                 for (int e = 0; e < 16; e++) o[j][e] *= f;
             exponents(s, scale2);
-            sum = weights(s, 1.0f, 0.0f, p);
+            sum = weights(s, 1.0f, -low, p);
         }
         l += sum;
         values(vs, p);

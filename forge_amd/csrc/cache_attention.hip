@@ -102,6 +102,7 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
     const unsigned long long drafts = live ? drafts_of(row) : 0ull;
     const int keys = cache_keys(a, b), len = max(a.lens[b], 0), n = min(keys - key0, a.chunk);
     if (n <= 0) return;
+    w.keys(keys);
     __syncthreads();
     const int open = len - key0;                                     // keys of this chunk that every row sees
 

@@ -76,6 +76,7 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void prompt_attenti
 
     AttnWave<T, DP, kPromptKeys / 32> w;
     w.init();
+    w.keys(len);
     w.load_q(a.q + static_cast<size_t>(start + row) * a.q_token + hq * a.q_head, row < len, a.D);
 
     const uint16_t* kbase = a.k + static_cast<size_t>(start) * a.k_token + hk * a.k_head;

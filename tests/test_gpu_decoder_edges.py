@@ -192,6 +192,57 @@ def test_scores_far_from_zero(dev, dt, top, step):
             assert ((got - mean).abs() <= u * mean.abs() + n * 2.0 ** -23 * size + 2.0 ** -25).all(), (r, best[r])
 
 
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("n,Hq,Hkv,D", PROMPTS)
+def test_largest_values_prompt(dev, n, Hq, Hkv, D, causal):
+    """Means of BF16 values whose sum FP32 does not hold."""
+    import torch
+    from attention_plain import check
+    say(f"largest values, prompt n={n} Hq={Hq} D={D} causal={causal}")
+    q, k, v = normals((n, Hq, D), "bfloat16", dev, 1), normals((n, Hkv, D), "bfloat16", dev, 2), normals((n, Hkv, D), "bfloat16", dev, 3)
+    big = torch.finfo(torch.bfloat16).max
+    v = (v.sign().float() * big * (1.0 - 0.6 * torch.rand(v.shape, device=dev))).to(torch.bfloat16)
+    v[:, :, 0] = big
+    v[:, :, 1] = -big
+    out = prompt(q, k, v, causal=causal)
+    i = torch.arange(n, device=dev)
+    seen = i[None] <= i[:, None] if causal else torch.ones((n, n), dtype=torch.bool, device=dev)
+    for h in range(0, Hq, max(1, Hq // 4)):
+        g = h // (Hq // Hkv)
+        check(out[:, h], q[:, h], k[:, g], v[:, g], seen, D ** -0.5)
+    assert (out[:, :, 0] == big).all() and (out[:, :, 1] == -big).all()
+
+
+@pytest.mark.parametrize("n,T,Hq,Hkv,D", CACHES)
+def test_largest_values_cache(dev, n, T, Hq, Hkv, D):
+    import torch
+    from attention_plain import check
+    say(f"largest values, cache n={n} T={T} Hq={Hq} D={D}")
+    q, k, v = normals((n, Hq, D), "bfloat16", dev, 4), normals((n, Hkv, D), "bfloat16", dev, 5), normals((n, Hkv, D), "bfloat16", dev, 6)
+    big = torch.finfo(torch.bfloat16).max
+    v = (v.sign().float() * big * (1.0 - 0.6 * torch.rand(v.shape, device=dev))).to(torch.bfloat16)
+    v[:, :, 0] = big
+    out = cached(q, k, v, T)
+    i = torch.arange(n, device=dev)
+    seen = i[None] <= i[n - T:, None]
+    for h in range(Hq):
+        g = h // (Hq // Hkv)
+        check(out[:, h], q[n - T:, h], k[:, g], v[:, g], seen, D ** -0.5)
+    assert (out[:, :, 0] == big).all()
+
+
+@pytest.mark.parametrize("e", [-60, -100, -110])
+def test_smallest_values(dev, e):
+    """Means of BF16 values near the lower end of its range keep their bits."""
+    import torch
+    for i, (n, T, Hq, Hkv, D) in enumerate([(n, 0, *rest) for n, *rest in PROMPTS] + CACHES):
+        say(f"smallest values 2^{e} n={n} T={T} Hq={Hq} D={D}")
+        q, k = normals((n, Hq, D), "bfloat16", dev, i), normals((n, Hkv, D), "bfloat16", dev, i + 1)
+        v = torch.full((n, Hkv, D), 2.0 ** e, dtype=torch.bfloat16, device=dev)
+        out = prompt(q, k, v) if T == 0 else cached(q, k, v, T)
+        assert (out == 2.0 ** e).all()
+
+
 def test_longest_table(dev):
     """A table of 2^27 positions, the most that there may be."""
     import torch
