@@ -58,6 +58,14 @@ struct KvRows {
     }
 };
 
+// Two 16-bit values, those that are no finite numbers as zeros.
+template <class T>
+__device__ __forceinline__ uint32_t finite_or_zero(uint32_t w) {
+    const uint32_t lo = (w & T::kInfinity) == T::kInfinity ? 0u : 0x0000FFFFu;
+    const uint32_t hi = (w >> 16 & T::kInfinity) == T::kInfinity ? 0u : 0xFFFF0000u;
+    return w & (lo | hi);
+}
+
 // Bits 0 to last.
 __device__ __forceinline__ uint32_t bits_to(int last) {
     return last >= 31 ? ~0u : last < 0 ? 0u : (2u << last) - 1u;
@@ -215,6 +223,66 @@ struct AttnWave {
         interleave<2 * KB * kOut, 2, kAhead>();
     }
 
+    // A tile of V (32 KB KS rows at v, one wave's at vs) that some rows of the workgroup see in part, before its products: these would
+    // take a value times the zero weight of a row that does not see it, which is NaN where that value is infinite or
+    // NaN. Such values are added to the sums of the rows that see them (their weights are positive) and are zeros then. All waves
+    // call it, between the barrier that makes the tile whole and the products; `odd`, in LDS, holds no number of this tile yet.
+    // us of a prompt of 9001, 32 / 8 heads of 128, and of one of 1024, 8 heads: finite values 709 and 17.4, a NaN in the first
+    // 703 and 17.4, infinities in one of a hundred values 1161 and 78, NaN only 1296 and 92.
+    template <int W, int KS, class Seen>
+    __device__ __forceinline__ void take_odd_values(int8_t* v, const int8_t* vs, int wave, int number, int* odd, const Seen& seen) {
+        constexpr int kShare = 32 * KB * KS * Rows::kBytes / W;      // each wave looks through a part
+        static_assert(kShare % 1024 == 0, "whole instructions");
+        v4u* at = reinterpret_cast<v4u*>(v + wave * kShare + 16 * lane);
+        float z = 0.0f;
+#pragma unroll
+        for (int i = 0; i < kShare / 1024; i++) {
+            const v4u x = at[kWave * i];
+#pragma unroll
+            for (int d = 0; d < 4; d++) z = T::times_zero(x[d], z);
+        }
+        if (z != 0.0f) *odd = number;
+        wait_lgkm0();
+        lds_barrier();
+        if (__builtin_amdgcn_readfirstlane(*odd) != number) return;
+        add_odd_values(vs, seen);
+        wait_lgkm0();
+        lds_barrier();
+#pragma unroll 1
+        for (int i = 0; i < kShare / 1024; i++) {
+            const v4u x = at[kWave * i];
+            at[kWave * i] = v4u{finite_or_zero<T>(x[0]), finite_or_zero<T>(x[1]), finite_or_zero<T>(x[2]), finite_or_zero<T>(x[3])};
+        }
+        wait_lgkm0();
+        lds_barrier();
+    }
+    template <class Seen>
+    __device__ __forceinline__ void add_odd_values(const int8_t* vs, const Seen& seen) {
+#pragma unroll 1
+        for (int k = 0; k < 32 * KB; k++) {
+            const int8_t* row = vs + k * Rows::kBytes;
+            float z = 0.0f;
+            if (lane < Rows::kChunks) {
+                const v4u x = *reinterpret_cast<const v4u*>(row + 16 * lane);
+#pragma unroll
+                for (int d = 0; d < 4; d++) z = T::times_zero(x[d], z);
+            }
+            if (!__any(z != 0.0f)) continue;
+            const bool on = seen(k >> 5) >> (k & 31) & 1u;
+#pragma unroll
+            for (int j = 0; j < kOut; j++)
+#pragma unroll
+                for (int c = 0; c < 4; c++) {
+                    const v2u x = *reinterpret_cast<const v2u*>(row + ((4 * j + c) ^ Rows::swz_v(k)) * 16 + 8 * (lane >> 5));
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const float y = T::widen(static_cast<uint16_t>(x[e / 2] >> (16 * (e & 1))));
+                        o[j][4 * c + e] += on && !(fabsf(y) < INFINITY) ? y : 0.0f;
+                    }
+                }
+        }
+    }
+
     // A tile from its scores on; masked if `masked`. `first`: nothing has been summed yet. (Both uniform.)
     template <class Seen>
     __device__ __forceinline__ void finish(Scores& s, const int8_t* vs, float scale2, bool first, bool masked, const Seen& seen) {
@@ -289,61 +357,6 @@ struct AttnWave {
             }
         }
     }
-
-    // Whether some value of the rows `live` is no finite number.
-    __device__ __forceinline__ bool odd(bool live) const {
-        float z = 0.0f;
-#pragma unroll
-        for (int j = 0; j < kOut; j++)
-#pragma unroll
-            for (int e = 0; e < 16; e++) z = __builtin_fmaf(o[j][e], 0.0f, z);
-        z = __builtin_fmaf(l, 0.0f, z);
-        return __any(live && z != 0.0f);
-    }
 };
-
-// One query row over keys [0, n) by a whole wave, key by key, reading nothing that the row does not
-// see: for rows whose tile result is not finite, as a product takes a masked key's value times zero,
-// which is NaN where that value is infinite or NaN. key(j) / value(j): the rows of key j; seen(j).
-// Returns m and l, and in acc the columns lane + 64 i.
-template <class T, int DP, class Key, class Value, class Seen>
-__device__ __forceinline__ void attn_row(const uint16_t* q, int D, int n, float scale2, const Key& key, const Value& value,
-                                         const Seen& seen, float& m, float& l, float (&acc)[(DP + 63) / 64]) {
-    const int lane = threadIdx.x & (kWave - 1);
-    auto score = [&](int j) {
-        const uint16_t* k = key(j);
-        float s = 0.0f;
-#pragma unroll 1
-        for (int d = 0; d < D; d++) s = __builtin_fmaf(T::widen(q[d]), T::widen(k[d]), s);
-        return s * scale2;
-    };
-    m = kNoScore;
-    l = 0.0f;
-#pragma unroll
-    for (int i = 0; i < (DP + 63) / 64; i++) acc[i] = 0.0f;
-#pragma unroll 1
-    for (int j0 = 0; j0 < n; j0 += kWave) {
-        const int j = j0 + lane;
-        if (j < n && seen(j)) m = fmaxf(m, score(j));
-    }
-    m = wave_max(m);
-#pragma unroll 1
-    for (int j0 = 0; j0 < n; j0 += kWave) {
-        const int j = j0 + lane;
-        const bool on = j < n && seen(j);
-        const float p = on ? __builtin_amdgcn_exp2f(score(j) - m) : 0.0f;
-        unsigned long long left = __ballot(on);
-        while (left) {
-            const int i = __builtin_ctzll(left);
-            left &= left - 1;
-            const float pj = __shfl(p, i, kWave);
-            l += pj;
-            const uint16_t* v = value(j0 + i);
-#pragma unroll
-            for (int c = 0; c < (DP + 63) / 64; c++)
-                if (lane + 64 * c < D) acc[c] = __builtin_fmaf(pj, T::widen(v[lane + 64 * c]), acc[c]);
-        }
-    }
-}
 
 }  // namespace forge_amd

@@ -60,7 +60,7 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
     constexpr int kIns = kKeys * Rows::kChunks / kWave / W;
     static_assert(kKeys * Rows::kChunks % (kWave * W) == 0, "a tile splits evenly over the waves");
     extern __shared__ __align__(1024) int8_t lds[];
-    __shared__ int odd_rows;
+    __shared__ int odd;
     int* page_of = reinterpret_cast<int*>(lds + kCacheLds<T, DP, RS, KS, KB>);
 
     const int group = a.group, rows = a.T * group;
@@ -75,7 +75,6 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
         const int pg = a.table[static_cast<size_t>(b) * a.width + p];
         page_of[p - page0] = pg >= 0 && pg < a.pages ? pg : -1;
     }
-    if (threadIdx.x == 0) odd_rows = 0;
 
     const size_t token = static_cast<size_t>(a.Hkv) * a.D;
     // element offset of key j's row (of both tensors), or -1
@@ -95,6 +94,7 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
     };
 
     AttnWave<T, DP, KB> w;
+    if (threadIdx.x == 0) odd = -1;
     w.init();
     const int row = (set * RS + rs) * 32 + (lane & 31);
     const bool live = row < rows;
@@ -129,6 +129,7 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
     };
     const float scale2 = a.scale * 1.44269504f;
     const int tiles = (n + kKeys - 1) / kKeys;
+    const bool some = a.T > 1 || a.tree;                             // drafts that not every row sees
     load(0);
     for (int t = 0; t < tiles; t++) {
         wait_vm_lgkm<0>();
@@ -136,57 +137,26 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void cache_attentio
         if (t + 1 < tiles) load(t + 1);
         const int k0 = t * kKeys + 32 * KB * ks;                     // this wave's keys of the tile
         const int8_t* at = lds + (t & 1) * 2 * kTile + 32 * KB * ks * Rows::kBytes;
-        v16f s[KB];
-        w.scores(at, s);
-        w.finish(s, at + kTile, scale2, t == 0, k0 + 32 * KB > min(open, n), [&](int kb) {
+        auto seen = [&](int kb) {
             const int d = open - (k0 + 32 * kb);                     // bits below d: the cache; from d on: drafts
             uint32_t bits = bits_to(d - 1);
             if (d < 32) bits |= d >= 0 ? static_cast<uint32_t>(drafts << d) : d > -64 ? static_cast<uint32_t>(drafts >> -d) : 0u;
             return bits & bits_to(n - 1 - (k0 + 32 * kb));
-        });
+        };
+        if (some && (t + 1) * kKeys > open)                          // (what lies past the last key is zeros)
+            w.template take_odd_values<W, KS>(lds + (t & 1) * 2 * kTile + kTile, at + kTile, wave, t, &odd, seen);
+        v16f s[KB];
+        w.scores(at, s);
+        w.finish(s, at + kTile, scale2, t == 0, k0 + 32 * KB > min(open, n), seen);
     }
 
     wait_vm_lgkm<0>();
     __syncthreads();
     auto* sh = reinterpret_cast<typename AttnWave<T, DP, KB>::template Shared<W>*>(lds);
-    if (w.odd(live) && lane == 0) atomicOr(&odd_rows, 1);
     w.leave(sh, wave, live);
     __syncthreads();
     const bool whole = keys <= a.chunk;                              // the only chunk: the result itself
     const size_t part0 = ((static_cast<size_t>(b) * a.Hkv + hk) * a.chunks + chunk) * rows;
-    if (odd_rows) {
-        // some row's sum is not finite: every row again, key by key
-        for (int i = wave; i < 32 * RS; i += W) {
-            const int r = set * RS * 32 + i;
-            if (r >= rows) break;
-            const unsigned long long rb = drafts_of(r);
-            float m, l, acc[(DP + 63) / 64];
-            auto at = [&](const uint16_t* base, int j) {
-                const long long o = row_at(j);
-                return o < 0 ? reinterpret_cast<const uint16_t*>(kZeroRow) : base + o;
-            };
-            attn_row<T, DP>(
-                row_of(a.q, r), a.D, n, scale2, [&](int j) { return at(a.k, j); }, [&](int j) { return at(a.v, j); },
-                [&](int j) {
-                    const int d = j - open;
-                    return d < 0 || ((rb >> (d & 63)) & 1ull);
-                },
-                m, l, acc);
-            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-            for (int c = 0; c < (DP + 63) / 64; c++) {
-                const int d = lane + 64 * c;
-                if (d >= a.D) break;
-                if (whole) row_of(a.out, r)[d] = narrow<T>(acc[c] * inv);
-                else a.part[(part0 + r) * a.D + d] = acc[c];
-            }
-            if (!whole && lane == 0) {
-                a.stat[(part0 + r) * 2] = m;
-                a.stat[(part0 + r) * 2 + 1] = l;
-            }
-        }
-        return;
-    }
     if (!live) return;
     float* part = a.part + (part0 + row) * a.D;
     uint16_t* out = row_of(a.out, row);

@@ -17,6 +17,7 @@ struct Fp16 {
     typedef _Float16 v2 __attribute__((ext_vector_type(2)));
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     static constexpr uint32_t kOnes = 0x3C003C00u;
+    static constexpr uint32_t kInfinity = 0x7C00u;
     static constexpr bool kWide = false;   // FP32's range
     static __device__ __forceinline__ float widen(uint16_t b) { return h2f(b); }
     // Two values rounded to nearest even, the first in the low half. (No inline asm: the wait state between an
@@ -27,6 +28,10 @@ struct Fp16 {
     // c + both values of the pair
     static __device__ __forceinline__ float add_pair(uint32_t p, float c) {
         return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, p), __builtin_bit_cast(v2, kOnes), c, false);
+    }
+    // c, or NaN if one of the pair is no finite number
+    static __device__ __forceinline__ float times_zero(uint32_t p, float c) {
+        return __builtin_amdgcn_fdot2(__builtin_bit_cast(v2, p), __builtin_bit_cast(v2, 0u), c, false);
     }
     static __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);
@@ -40,6 +45,7 @@ struct Bf16 {
     typedef __bf16 v2 __attribute__((ext_vector_type(2)));
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     static constexpr uint32_t kOnes = 0x3F803F80u;
+    static constexpr uint32_t kInfinity = 0x7F80u;
     static constexpr bool kWide = true;
     static __device__ __forceinline__ float widen(uint16_t b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {
@@ -47,6 +53,9 @@ struct Bf16 {
     }
     static __device__ __forceinline__ float add_pair(uint32_t p, float c) {
         return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, p), __builtin_bit_cast(v2, kOnes), c, false);
+    }
+    static __device__ __forceinline__ float times_zero(uint32_t p, float c) {
+        return __builtin_amdgcn_fdot2_f32_bf16(__builtin_bit_cast(v2, p), __builtin_bit_cast(v2, 0u), c, false);
     }
     static __device__ __forceinline__ v4f mfma16(v4u a, v4u b, v4f c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(v8, a), __builtin_bit_cast(v8, b), c, 0, 0, 0);

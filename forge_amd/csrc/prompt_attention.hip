@@ -113,11 +113,20 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void prompt_attenti
     const int first = row0 + 32 * rs, ahead = first - kPromptKeys * ks;
     // tiles that reach this wave's rows
     const int mine = !CAUSAL ? tiles : ahead < 0 ? 0 : min(tiles, ahead / kKeys + 1);
+    __shared__ int odd;
+    if (threadIdx.x == 0) odd = -1;
+    auto seen = [&](int t) {
+        return [&, k0 = t * kKeys + kPromptKeys * ks](int kb) { return bits_to((CAUSAL ? min(row, len - 1) : len - 1) - k0 - 32 * kb); };
+    };
     auto next = [&](int t) {
         if (t + NS - 1 <= tiles) wait_vm_lgkm<2 * kIns*(NS - 2)>();
         else wait_vm_lgkm<0>();
         lds_barrier();                                               // tile t is whole, tile t - 1 is read
         if (t + NS - 1 < tiles) load(t + NS - 1);
+        if (CAUSAL && (t + 1) * kKeys - 1 > row0) {                  // rows see it in part (what lies past the end is zeros)
+            int8_t* v = lds + (t % NS) * 2 * kTile + kTile;
+            w.template take_odd_values<W, KS>(v, v + kPromptKeys * ks * Rows::kBytes, wave, t, &odd, seen(t));
+        }
     };
 #pragma unroll
     for (int t = 0; t < NS - 1; t++)
@@ -129,31 +138,11 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void prompt_attenti
         const int k0 = t * kKeys + kPromptKeys * ks;
         v16f s[kPromptKeys / 32];
         w.scores(at, s);
-        w.finish(s, at + kTile, scale2, t == 0, (CAUSAL && k0 + kPromptKeys - 1 > first) || k0 + kPromptKeys > len,
-                 [&](int kb) { return bits_to((CAUSAL ? min(row, len - 1) : len - 1) - k0 - 32 * kb); });
+        w.finish(s, at + kTile, scale2, t == 0, (CAUSAL && k0 + kPromptKeys - 1 > first) || k0 + kPromptKeys > len, seen(t));
     }
     for (; t < tiles; t++) next(t);
     const bool live = row < len;
-    auto out_row = [&](int r) { return a.out + (static_cast<size_t>(start + r) * a.Hq + hq) * a.D; };
-    // some row's sum is not finite: rows r0, r0 + step, ... of the workgroup again, key by key
-    auto again = [&](int r0, int end, int step) {
-        for (int r = row0 + r0; r < min(row0 + end, len); r += step) {
-            float m, l, acc[(DP + 63) / 64];
-            attn_row<T, DP>(
-                a.q + static_cast<size_t>(start + r) * a.q_token + hq * a.q_head, a.D, CAUSAL ? r + 1 : len, scale2,
-                [&](int j) { return kbase + static_cast<size_t>(j) * a.k_token; },
-                [&](int j) { return vbase + static_cast<size_t>(j) * a.v_token; }, [](int) { return true; }, m, l, acc);
-            const float inv = l != 0.0f ? 1.0f / l : 0.0f;
-#pragma unroll
-            for (int c = 0; c < (DP + 63) / 64; c++)
-                if (lane + 64 * c < a.D) out_row(r)[lane + 64 * c] = narrow<T>(acc[c] * inv);
-        }
-    };
     if constexpr (KS == 1) {
-        if (w.odd(live)) {
-            again(32 * rs, 32 * rs + 32, 1);
-            return;
-        }
         const float l = half_sum(w.l);
         const float inv = l > 0.0f ? 1.0f / l : 0.0f;
         if (!live) return;
@@ -167,18 +156,11 @@ __global__ __launch_bounds__(64 * RS * KS, DP > 128 ? 1 : 2) void prompt_attenti
                                                            T::pack(w.o[j][e + 2] * inv, w.o[j][e + 3] * inv)};
             }
     } else {
-        __shared__ int odd_rows;
         auto* sh = reinterpret_cast<typename AttnWave<T, DP, kPromptKeys / 32>::template Shared<W>*>(lds);
-        if (threadIdx.x == 0) odd_rows = 0;
         wait_vm_lgkm<0>();
         __syncthreads();
-        if (w.odd(live) && lane == 0) atomicOr(&odd_rows, 1);
         w.leave(sh, wave, live);
         __syncthreads();
-        if (odd_rows) {
-            again(wave, kRows, W);
-            return;
-        }
         if (!live) return;
         w.template join<KS>(sh, wave, [&](int j, int e, v4f s, float, float sum) {
             const int d = 32 * j + 8 * e + 4 * (lane >> 5);

@@ -309,7 +309,8 @@ int forge_int8_depthwise_conv2d_forward(const uint16_t* input, const int8_t* wei
  * No counterparts in the reference's INT8 path: what a decoder runs between and beside its linear
  * layers. Activations, queries, keys, values and caches are FP16 or BF16 (dtype); sums and softmax
  * statistics are FP32 and results are rounded once, except for the softmax weights, which are rounded to the
- * 16-bit type for their product with V. 16-bit tensors are 16-byte aligned, strides are in elements, not negative and
+ * 16-bit type for their product with V. Attention scores past FP32's range count as infinite, and an infinite value
+ * whose weight is rounded to zero gives NaN; keys and values that a row does not see may hold anything. 16-bit tensors are 16-byte aligned, strides are in elements, not negative and
  * multiples of 8, head sizes D are multiples of 8 up to 256. */
 #define FORGE_FP16 0
 #define FORGE_BF16 1

@@ -243,6 +243,53 @@ def test_smallest_values(dev, e):
         assert (out == 2.0 ** e).all()
 
 
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("n,Hq,Hkv,D", PROMPTS)
+def test_neighbours_keep_their_bits_prompt(dev, n, Hq, Hkv, D, dt):
+    """Infinities and NaN change the bits of nothing but the rows that see them, and of these, where only values are not
+    finite, only those columns."""
+    import torch
+    say(f"neighbours, prompt {dt} n={n} Hq={Hq} D={D}")
+    q, k, v = normals((n, Hq, D), dt, dev, 7), normals((n, Hkv, D), dt, dev, 8), normals((n, Hkv, D), dt, dev, 9)
+    clean = prompt(q, k, v)
+    for p, bad in ((n - 1, float("nan")), (n // 2 + 5, float("inf")), (97, float("-inf")), (0, float("nan"))):
+        v2 = v.clone()
+        v2[p, :, D - 3] = bad
+        out = prompt(q, k, v2)
+        rest = [d for d in range(D) if d != D - 3]
+        assert torch.equal(out[:p], clean[:p]) and torch.equal(out[p:, :, rest], clean[p:, :, rest])
+        assert not torch.isfinite(out[p:, :, D - 3]).any()
+        k2 = k.clone()
+        k2[p] = float("nan")
+        out = prompt(q, k2, v2)
+        assert torch.equal(out[:p], clean[:p]) and torch.isnan(out[p:]).all()
+
+
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("n,T,Hq,Hkv,D", [c for c in CACHES if c[1] > 1])
+def test_neighbours_keep_their_bits_cache(dev, n, T, Hq, Hkv, D, dt):
+    import torch
+    say(f"neighbours, cache {dt} n={n} T={T} Hq={Hq} D={D}")
+    q, k, v = normals((n, Hq, D), dt, dev, 10), normals((n, Hkv, D), dt, dev, 11), normals((n, Hkv, D), dt, dev, 12)
+    tree = torch.tensor([[1 << t for t in range(T)]], dtype=torch.int64, device=dev)      # every draft on its own
+    tree[0, 0] |= 1 << (T - 1)
+    clean = cached(q, k, v, T, tree=tree)
+    for t, bad in ((T - 1, float("inf")), (1, float("nan"))):
+        v2, k2 = v.clone(), k.clone()
+        v2[n - T + t, :, 2] = bad
+        sees = [r for r in range(T) if r == t or (r == 0 and t == T - 1)]
+        others = [r for r in range(T) if r not in sees]
+        rest = [d for d in range(D) if d != 2]
+        out = cached(q, k, v2, T, tree=tree)
+        assert torch.equal(out[others], clean[others]) and torch.equal(out[:, :, rest], clean[:, :, rest])
+        assert not torch.isfinite(out[sees][:, :, 2]).any()
+        if bad == float("inf"):
+            assert (out[sees][:, :, 2] == bad).all()
+        k2[n - T + t] = float("nan")
+        out = cached(q, k2, v2, T, tree=tree)
+        assert torch.equal(out[others], clean[others]) and torch.isnan(out[sees]).all()
+
+
 def test_longest_table(dev):
     """A table of 2^27 positions, the most that there may be."""
     import torch
