@@ -78,6 +78,38 @@ def test_int4_large_tokens(dev, M, K, N):
     assert ((y - want).abs() <= 2.0 ** -8 * want.abs() + (K + 32) * 2.0 ** -23 * mag).all()
 
 
+def int4_bound(x, q, s):
+    """The result in 64 bits, and what a kernel with FP32 sums of these products may be off by."""
+    ws = q.double() * s.double().repeat_interleave(32, 1)
+    want, mag = x.double() @ ws.T.contiguous(), x.double().abs() @ ws.abs().T.contiguous()
+    u = 2.0 ** -11 if str(x.dtype) == "torch.float16" else 2.0 ** -8
+    return want, u * want.abs() + (x.shape[1] + 32) * 2.0 ** -23 * mag
+
+
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("M,K,N", [(257, 384, 40), (1025, 256, 60), (4099, 128, 17), (300, 512, 8200), (700, 544, 2881)])
+def test_int4_prompts(dev, M, K, N, dt):
+    """Tokens of whole prompts: many tiles of 64, and rows of fewer values than a unit."""
+    from forge_amd import ops
+    x, q, s, w = int4_case(M, K, N, dt, dev, M)
+    say(f"int4_linear prompt {dt} M={M} K={K} N={N}")
+    want, bound = int4_bound(x, q, s)
+    assert ((ops.int4_linear(x, w, s).double() - want).abs() <= bound).all()
+
+
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+def test_int4_one_token_among_others(dev, dt):
+    """A token's sums are taken in another order alone than with 15, 31 or 63 others: within the bound, not bit for bit."""
+    import torch
+    from forge_amd import ops
+    x, q, s, w = int4_case(64, 4096, 3000, dt, dev, 5)
+    want, bound = int4_bound(x, q, s)
+    for M in (1, 4, 5, 16, 17, 32, 33, 64):
+        y = ops.int4_linear(x[:M].contiguous(), w, s)
+        assert ((y.double() - want[:M]).abs() <= bound[:M]).all()
+        assert torch.equal(ops.int4_linear(x[:M].contiguous(), w, s), y)
+
+
 # ---- arguments -----------------------------------------------------------------------------------
 
 class NoBool:
@@ -290,6 +322,28 @@ def test_neighbours_keep_their_bits_cache(dev, n, T, Hq, Hkv, D, dt):
         assert torch.equal(out[others], clean[others]) and torch.isnan(out[sees]).all()
 
 
+def test_alone_and_in_a_batch(dev):
+    """Chunks depend on the number of sequences: a sequence alone agrees with itself in a batch within the bound."""
+    import torch
+    from attention_plain import check
+    from forge_amd import ops
+    B, n, T, Hq, Hkv, D, page = 5, 1500, 3, 8, 2, 128, 16
+    pages = (n + page - 1) // page
+    q = normals((B, T, Hq, D), "float16", dev, 20)
+    kc, vc = normals((B * pages, page, Hkv, D), "float16", dev, 21), normals((B * pages, page, Hkv, D), "float16", dev, 22)
+    table = torch.arange(B * pages, dtype=torch.int32, device=dev).view(B, pages)
+    lens = torch.tensor([n - T, 700, 0, 64, 1111], dtype=torch.int32, device=dev)
+    out = ops.cache_attention(q, kc, vc, table, lens)
+    for b in range(B):
+        alone = ops.cache_attention(q[b:b + 1], kc, vc, table[b:b + 1], lens[b:b + 1])
+        m = int(lens[b]) + T
+        seen = torch.arange(m, device=dev)[None] <= torch.arange(m - T, m, device=dev)[:, None]
+        k, v = (c.view(B, -1, Hkv, D)[b, :m] for c in (kc, vc))
+        for h in range(Hq):
+            for got in (out[b, :, h], alone[0, :, h]):
+                check(got, q[b, :, h], k[:, h // 4], v[:, h // 4], seen, D ** -0.5)
+
+
 def test_longest_table(dev):
     """A table of 2^27 positions, the most that there may be."""
     import torch
@@ -323,3 +377,78 @@ def test_many_sequences(dev, keys):
         rows = torch.arange(r, B, 3, device=dev)
         kk, vv = k.view(-1, D)[:n], v.view(-1, D)[:n]
         check(out[rows, 0, 0], q[rows, 0, 0], kk, vv, torch.ones((len(rows), n), dtype=torch.bool, device=dev), D ** -0.5)
+
+
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("D", [64, 80, 128, 200])
+def test_rows_past_the_end_are_zeros(dev, D, causal, dt):
+    """Whatever the call before has left in LDS (NaN in every key and value here), the rows of a last tile that lie past the
+    sequence count as zeros."""
+    import torch
+    say(f"rows past the end {dt} D={D} causal={causal}")
+    for n, Hq, Hkv in ((300, 2, 1), (65, 64, 8), (1, 300, 300), (129, 200, 8), (700, 64, 8)):
+        q, k, v = normals((n, Hq, D), dt, dev, n), normals((n, Hkv, D), dt, dev, n + 1), normals((n, Hkv, D), dt, dev, n + 2)
+        nq, nk = normals((2048, 32, D), dt, dev, 1), torch.full((2048, 32, D), float("nan"), dtype=q.dtype, device=dev)
+        want = prompt(q, k, v, causal=causal)
+        assert torch.isfinite(want).all()
+        for _ in range(3):
+            left = prompt(nq, nk, nk, causal=causal)
+            assert torch.equal(prompt(q, k, v, causal=causal), want)
+        assert torch.isnan(left).all()
+    for n, T, Hq, Hkv in ((100, 1, 4, 1), (900, 1, 8, 8), (333, 5, 16, 2), (1000, 61, 4, 1)):
+        q, k, v = normals((n, Hq, D), dt, dev, n), normals((n, Hkv, D), dt, dev, n + 1), normals((n, Hkv, D), dt, dev, n + 2)
+        want = cached(q, k, v, T)
+        assert torch.isfinite(want).all()
+        for _ in range(3):
+            prompt(nq, nk, nk, causal=causal)
+            assert torch.equal(cached(q, k, v, T), want)
+
+
+# ---- compiled calls ------------------------------------------------------------------------------
+
+def test_both_call_paths_agree(dev, monkeypatch):
+    """The compiled call and the checks with the foreign call behind them hand over the same arguments."""
+    import torch
+    from forge_amd import ops
+    calls = []
+
+    def both(name, f):
+        fast = f()
+        with monkeypatch.context() as m:
+            m.setattr(ops, "_fast", lambda called, *a: calls.append(called))
+            slow = f()
+        for a, b in zip(fast, slow):
+            assert torch.equal(a, b), name
+
+    x, q4, s, w = int4_case(7, 384, 50, "bfloat16", dev, 1)
+    bias = torch.randn((50,), device=dev).to(torch.bfloat16)
+    both("int4_linear", lambda: [ops.int4_linear(x, w, s, bias)])
+    T, Hq, Hkv, D = 40, 6, 2, 80
+    qkv = normals((T, Hq + 2 * Hkv, D), "float16", dev, 2)
+    q, k, v = qkv.split((Hq, Hkv, Hkv), 1)
+    cos, sin = torch.rand((64, 24), device=dev), torch.rand((64, 24), device=dev)
+    pos = torch.randint(0, 64, (T,), device=dev, dtype=torch.int32)
+    slots = torch.randperm(48, device=dev)[:T].to(torch.int32)
+    nw = torch.rand((D,), device=dev).half()
+    for inter in (False, True):
+        both("qk_norm_rope", lambda: ops.qk_norm_rope(q, k, nw, None, cos, sin, pos, eps=1e-5, interleaved=inter))
+
+        def into_cache():
+            kc, vc = (torch.zeros((3, 16, Hkv, D), dtype=torch.float16, device=dev) for _ in range(2))
+            ko = torch.empty((T, Hkv, D), dtype=torch.float16, device=dev)
+            return ops.qk_norm_rope_cache(q, k, v, None, nw, cos, sin, pos, kc, vc, slots, interleaved=inter, k_out=ko), ko, kc, vc
+        both("qk_norm_rope_cache", into_cache)
+    cu = torch.tensor([0, 13, 40], dtype=torch.int32, device=dev)
+    for causal in (False, True):
+        both("prompt_attention", lambda: [ops.prompt_attention(q, k, v, cu, 0.3, causal)])
+    B, T = 2, 3
+    q = normals((B, T, Hq, D), "float16", dev, 3)
+    kc, vc = normals((5, 16, Hkv, D), "float16", dev, 4), normals((5, 16, Hkv, D), "float16", dev, 5)
+    table = torch.tensor([[4, 0, 2], [1, 3, 0]], dtype=torch.int32, device=dev)
+    lens = torch.tensor([40, 17], dtype=torch.int32, device=dev)
+    tree = torch.tensor([[1, 3, 5], [1, 2, 7]], device=dev)
+    ws = torch.empty((max(16, ops.cache_attention_workspace_size(B, T, Hq, Hkv, D, 48)),), dtype=torch.uint8, device=dev)
+    for tr in (None, tree):
+        both("cache_attention", lambda: [ops.cache_attention(q, kc, vc, table, lens, tr, workspace=ws, out=torch.empty_like(q))])
+    assert set(calls) == {"int4_linear", "qk_norm_rope", "prompt_attention", "cache_attention"}
