@@ -93,6 +93,15 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkArgs a)
         for (int e = 0; e < 8; e++) ss = __builtin_fmaf(x[e], x[e], ss);
 #pragma unroll
         for (int d = 1; d < LPH; d <<= 1) ss += __shfl_xor(ss, d, kWave);
+        // BF16 heads whose squares FP32 does not hold (values from about 2^60 on): once more in 64 bits
+        float inv = 1.0f / sqrtf(ss / static_cast<float>(a.D) + a.eps);
+        if (T::kWide && __any(ss == INFINITY)) {
+            double sd = 0.0;
+#pragma unroll
+            for (int e = 0; e < 8; e++) sd += static_cast<double>(x[e]) * x[e];
+            for (int d = 1; d < LPH; d <<= 1) sd += __shfl_xor(sd, d, kWave);
+            if (ss == INFINITY) inv = static_cast<float>(1.0 / sqrt(sd / a.D + a.eps));
+        }
         if (!live) continue;
         if (is_v) {
             if (slot >= 0)
@@ -100,7 +109,6 @@ __global__ __launch_bounds__(256) void qk_norm_rope_kernel(QkArgs a)
             continue;
         }
         if (wgt) {
-            const float inv = 1.0f / sqrtf(ss / static_cast<float>(a.D) + a.eps);
             float w[8];
             widen8<T>(*reinterpret_cast<const v4u*>(wgt + d0), w);
 #pragma unroll

@@ -7,6 +7,12 @@ from helpers import say
 pytestmark = pytest.mark.gpu
 
 
+def normals(shape, dt, dev, seed):
+    import torch
+    g = torch.Generator().manual_seed(seed)
+    return torch.randn(shape, generator=g).to(getattr(torch, dt)).to(dev)
+
+
 # ---- int4_linear ---------------------------------------------------------------------------------
 
 def test_no_values_is_refused(dev):
@@ -110,6 +116,42 @@ def test_int4_one_token_among_others(dev, dt):
         assert torch.equal(ops.int4_linear(x[:M].contiguous(), w, s), y)
 
 
+# ---- qk_norm_rope --------------------------------------------------------------------------------
+
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("D,e", [(64, 61), (128, 64), (256, 100), (80, 126)])
+def test_norm_of_large_heads(dev, D, e, interleaved):
+    """Heads of BF16 values whose squares FP32 does not hold are normed as any others; an infinity gives NaN in its own pair
+    and zeros elsewhere, as x / inf does. Bound: a head's size and its product with the weight, and the turn, each rounded in
+    FP32, then to BF16: 2^-8 of the result and 2^-20 of the pair."""
+    import torch
+    from forge_amd import ops
+    T, Hq, Hkv = 33, 5, 2
+    q, k = (normals((T, h, D), "float32", dev, D + h) for h in (Hq, Hkv))
+    q[::2] *= 2.0 ** e
+    k[1::3] *= 2.0 ** e
+    q, k = q.clamp(-3e38, 3e38).to(torch.bfloat16), k.clamp(-3e38, 3e38).to(torch.bfloat16)
+    w = (normals((D,), "float32", dev, 1).abs() + 0.5).to(torch.bfloat16)
+    R = D // 2 // 16 * 16
+    pos = torch.arange(T, dtype=torch.int32, device=dev)
+    angle = torch.rand((T, R // 2), device=dev) * 6.0
+    cos, sin = angle.cos(), angle.sin()
+    qo, ko = ops.qk_norm_rope(q, k, w, w, cos, sin, pos, interleaved=interleaved)
+    for x, got in ((q, qo), (k, ko)):
+        y = x.double() / (x.double().square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+        first = torch.arange(R // 2, device=dev) * (2 if interleaved else 1)
+        second = first + (1 if interleaved else R // 2)
+        a, b, c, s = y[..., first], y[..., second], cos.double()[:, None], sin.double()[:, None]
+        want, size = y.clone(), y.abs()
+        want[..., first], want[..., second] = a * c - b * s, b * c + a * s
+        size[..., first] = size[..., second] = a.abs() + b.abs()
+        assert ((got.double() - want).abs() <= 2.0 ** -8 * want.abs() + 2.0 ** -20 * size + 1e-37).all()
+    q[3, 1, D - 1] = float("inf")
+    qo = ops.qk_norm_rope(q, k, w, w, cos, sin, pos, interleaved=interleaved)[0]
+    assert torch.isnan(qo[3, 1, D - 1]) and (qo[3, 1, :D - 2 * (R == D) - 1] == 0).all()
+    assert torch.isfinite(qo[3, [0, 2, 3, 4]]).all()
+
+
 # ---- arguments -----------------------------------------------------------------------------------
 
 class NoBool:
@@ -191,12 +233,6 @@ PROMPTS = [(200, 4, 2, 64), (300, 2, 1, 64), (300, 2, 1, 80), (300, 2, 2, 128), 
 # (keys, T, Hq, Hkv, D): one, two and four sets of rows, one chunk of keys and several
 CACHES = [(40, 1, 4, 1, 64), (900, 1, 8, 2, 128), (900, 5, 16, 2, 64), (700, 61, 4, 1, 128), (900, 3, 2, 1, 256), (500, 40, 4, 1, 256),
           (2500, 16, 4, 2, 80)]
-
-
-def normals(shape, dt, dev, seed):
-    import torch
-    g = torch.Generator().manual_seed(seed)
-    return torch.randn(shape, generator=g).to(getattr(torch, dt)).to(dev)
 
 
 @pytest.mark.parametrize("dt,top,step", [("bfloat16", -1.0, -1.0), ("bfloat16", -512.0, -512.0), ("bfloat16", 64.0, -1.0),
