@@ -7,9 +7,11 @@
 // and the probabilities, rounded in pairs, are as they stand the B operand of O^T = V^T P^T: a
 // product's sum over keys may take them in any order, if V^T's operand takes the same one. That operand
 // is 4 + 4 keys of one column of V, which the transposing LDS read gathers from V's rows.
-// The running maximum m, sum l and O follow the usual recurrence, FP32; P is rounded to 16 bits for
-// its product, and l sums the rounded weights, so that they add up to one. O is rescaled only when some row's maximum has grown by more than
-// 2^8 since the last time: until then P stays below 2^8, well inside both types.
+// The running maximum m, sum l and O follow the published recurrence (online softmax), FP32; P is rounded to 16 bits for
+// its product, which the matrix instructions take, and l sums the rounded weights, so that they add up to one (a prompt's errors in the 2-norm 2.6e-4
+// of the result in FP16 and 2.0e-3 in BF16, against 2.0e-4 and 1.6e-3 with FP32 weights: the result's own rounding is
+// most of both). O is rescaled only when some row's maximum has grown by more than 2^8 since the last time: until then P stays
+// below 2^8, well inside both types.
 //
 // K and V tiles are rows of DP values (D padded with zeros) in 16-byte chunks, permuted in each row so that what
 // LDS serves in one clock falls on different banks: one chunk of 16 rows of K, four chunks of 4 rows of V.
@@ -291,7 +293,8 @@ struct AttnWave {
         Weights p;
         float sum = weights(s, scale2, shift, p);
         const float mx = largest(s, scale2);
-        // A maximum that has grown is met seldom: the weights are taken again.
+        // A maximum that has grown is met seldom: the weights are taken again. (The compiler takes the ones above where nothing has
+        // grown, so that they wait for the maximum after all.)
         if (__any(mx > limit)) {
             const float was = m;
             raise(mx);

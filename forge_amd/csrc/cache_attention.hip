@@ -10,7 +10,7 @@
 // over workgroups in chunks of equal length, whatever the sequence's, and a chunk's tiles, which come by
 // LDS DMA into two buffers, over the KS waves of a row set. The waves' results are joined in LDS; the chunks'
 // go as FP32 to the workspace and are joined by a second kernel, in a fixed order. 16 sequences with 16 drafts of
-// 32 / 8 heads of 128 over 278 thousand keys: 253 us, 4.27 TB/s; one token over 1000 keys 9.6 (7.2 and 2.0 in two launches).
+// 32 / 8 heads of 128 over 278 thousand keys: 252 us, 4.28 TB/s; one token over 1000 keys 9.4 (6.9 and 1.9 in two launches).
 #include "attn_tile.h"
 
 #include <algorithm>

@@ -31,7 +31,8 @@ __device__ __forceinline__ size_t int4_word_at(int c) {
     return static_cast<size_t>(c >> 4) * 16 + 4 * (c & 3) + ((c & 15) >> 2);
 }
 
-// One thread per word; the threads of a scale group (4, 8 or 16) are neighbours. Bound: reading w once.
+// One thread per word; the threads of a scale group (4, 8 or 16) are neighbours. Bound: reading w once, value by value: 8192 x 11008
+// 81 to 91 us, 2.8 TB/s from FP16, 4.5 to 4.9 from FP32 (packing 56, 2.4).
 template <bool FP16W>
 __global__ __launch_bounds__(256) void quantize_weight_int4_kernel(const void* __restrict__ w, uint32_t* __restrict__ out,
                                                                    uint16_t* __restrict__ scale, int K, int group,

@@ -6,10 +6,10 @@
 // the next tiles' while this one is multiplied, one barrier a tile. Tiles past the diagonal are not
 // loaded, only those that cross it are masked.
 //
-// Bound: the matrix units at the clock that they leave (1.6 to 1.7 GHz; busy 44 to 52 %), and the softmax's vector
-// instructions that the other wave of a SIMD does not cover. Causal, 32 / 8 heads of 128: a prompt of 4096 155 us
-// (887 TFLOP/s), of 9001 + 5120 + 2263 905 to 940 (980 to 1017). Two workgroups of 4 waves a CU; 8 waves that share
-// their tiles measured the same.
+// Bound: the softmax, whose vector instructions wait for each tile's maximum and which the other wave of a SIMD does not cover (matrix
+// units busy 42 to 53 %), at the clock that the matrix units leave (1.6 to 1.7 GHz). Causal, 32 / 8 heads of 128: a prompt of
+// 4096 150 to 162 us by box (850 to 915 TFLOP/s), of 9001 + 5120 + 2263 859 to 917 (1003 to 1071). Two workgroups of 4 waves a CU;
+// 8 waves that share their tiles measured the same.
 //
 // The grid is laid out without reading cu_seqlens on the host: sequence b's tiles start at
 // cu[b] / rows + b, which leaves room for each sequence's last partial tile.

@@ -524,7 +524,8 @@ def prepare_sparse_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, 
 
 # ---- decoder attention (extension; include/forge_amd.h "decoder attention") -----------
 # A call whose operands are all in order goes through csrc/torch_calls.cpp, which checks them and calls the library in
-# about a microsecond; any other takes the checks below, which say what is wrong.
+# about a microsecond (cache_attention where the caller brings workspace and out); any other takes the checks
+# below, which say what is wrong.
 
 _DTYPE = {torch.float16: 0, torch.bfloat16: 1}   # FORGE_FP16, FORGE_BF16
 _NOT_IN_ORDER = -1000
