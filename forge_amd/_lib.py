@@ -66,6 +66,15 @@ SIGNATURES = {
     "forge_prompt_attention": (_I, [_P] * 5 + [_I] * 5 + [_L] * 6 + [_F, _I, _I, _P]),
     "forge_cache_attention_workspace_size": (ctypes.c_size_t, [_I] * 5 + [_L]),
     "forge_cache_attention": (_I, [_P] * 7 + [_I] * 8 + [_F, _I, _P, ctypes.c_size_t, _P]),
+    "forge_cache4_write": (_I, [_P] * 4 + [_I] * 5 + [_L] * 4 + [_I, _P]),
+    "forge_cache4_read": (_I, [_P] * 4 + [_I] * 6 + [_P]),
+    "forge_cache4_attention_workspace_size": (ctypes.c_size_t, [_I] * 5 + [_L]),
+    "forge_cache4_attention": (_I, [_P] * 6 + [_I] * 8 + [_F, _I, _P, ctypes.c_size_t, _P]),
+    "forge_beam_select_workspace_size": (ctypes.c_size_t, [_I] * 4),
+    "forge_beam_select": (_I, [_P] * 3 + [_I] + [_P] * 3 + [_I] * 4 + [_L] * 2 + [_I, _P, ctypes.c_size_t, _P]),
+    "forge_fork_pages_workspace_size": (ctypes.c_size_t, [_I] * 2),
+    "forge_fork_pages": (_I, [_P] * 10 + [_I] * 5 + [_P, ctypes.c_size_t, _P]),
+    "forge_copy_pages": (_I, [_P, _I, _L, _I, _P, _P, _I, _P]),
 }
 
 _lib = None

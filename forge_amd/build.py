@@ -56,6 +56,10 @@ SOURCES = [
     "qk_norm_rope.hip",
     "prompt_attention.hip",
     "cache_attention.hip",
+    "cache4_store.hip",
+    "cache4_attention.hip",
+    "cache_pages.hip",
+    "beam_select.hip",
     "forge_api.cpp",
 ]
 

@@ -1,0 +1,499 @@
+// Attention of a few new tokens per sequence over the 4-bit paged cache (cache4.h): one token or a tree of up to 64 drafts,
+// as cache_attention.
+//
+// With k = m + s n the score of row r and key j is scale (s_j (q_r . n_j) + m_j sum q_r), and the result is
+// (sum_j p_rj v_j) / sum_j p_rj with v_j = m'_j + s'_j n'_j, so the products are of 16-bit numbers with the integers themselves, which FP16 holds
+// exactly, and steps and lowest values enter in FP32: no key or value is rounded to 16 bits, and what a row does not see (its
+// integers are always finite) is left out by a select of its weight.
+//
+// A wave owns 16 RT rows and takes blocks of 16 keys, two at a time, on 16 x 16 x 32 products, S^T = K Q^T and O^T = V^T P^T as in attn_tile.h. All of
+// its operands come straight from memory: a lane's 8 values of one key are a word, and its word of four keys lies together (cache4.h).
+// Nibbles are masked in place as FP16 subnormals, n 2^-24 at bits 0 and 16 and n 2^-20 at bits 4 and 20; the powers of two go
+// into the queries, which are scaled by one of their own per row (BF16 queries fit FP16 then), and into the result.
+// Weights w = p s' are rounded to FP16, in either type, the row's largest at 2^4 or above; sums are FP32. v is taken as (m' + 8 s') + s' (n' - 8):
+// sum w n' less 8 times the sum of the same rounded w, so that a rounding weighs with n' - 8.
+#include "cache4.h"
+#include "cache_split.h"
+
+namespace forge_amd {
+
+struct Cache4Args : CacheArgs {
+    const uint8_t* cache;
+};
+
+// Four values of the same word position as half pairs, in the order of the word: (0, 1), (2, 3) x 16, (4, 5), (6, 7) x 16.
+__device__ __forceinline__ v4u nibble_pairs(uint32_t w) {
+    const uint32_t u = w >> 8;
+    return v4u{w & 0x000F000Fu, w & 0x00F000F0u, u & 0x000F000Fu, u & 0x00F000F0u};
+}
+
+__device__ __forceinline__ float swap16_max(float x) {
+    const v2u r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return fmaxf(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
+__device__ __forceinline__ float swap16_sum(float x) {
+    const v2u r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return __uint_as_float(r[0]) + __uint_as_float(r[1]);
+}
+// Over the four lanes of a column.
+__device__ __forceinline__ float column_max(float x) { return half_max(swap16_max(x)); }
+__device__ __forceinline__ float column_sum(float x) { return half_sum(swap16_sum(x)); }
+
+template <int U>
+struct Words4 {
+    // Operands of 16 words for all 8 values of each (full sets), of 8 words for the first and second half of the lanes (a half set).
+    static constexpr int kFull = U == 2 ? 0 : U == 8 ? 2 : 1, kHalf = U == 2 || U == 6, kSets = kFull + kHalf;
+    static constexpr int kOut = 8 * kFull + 4 * kHalf;   // products of 16 columns of the result
+    static constexpr int kRow = 32 * U + 4;              // floats of a row in LDS
+    static __device__ __forceinline__ int word(int s, int n) {
+        return s < kFull ? min(16 * s + n, 4 * U - 1) : 16 * kFull + (n & 7);
+    }
+};
+
+template <int U>
+struct Block4 {   // a lane's part of 16 keys
+    uint32_t k[U];
+    v4u v[Words4<U>::kSets];
+    v4u num[2];           // numbers of keys 4 g to 4 g + 3
+};
+
+// One row tile's softmax state (the lane's column).
+template <int U>
+struct Rows4 {
+    v4u q[U];
+    v4f o[Words4<U>::kOut];
+    float unit, qsum;        // of a score; the sum of the row's queries
+    float m, limit, shift;   // running maximum of the exponents; above limit it is raised; -(m + low)
+    float l, c, u;           // this lane's sums of p, of p (m' + 8 s') and of the rounded weights
+    float f, top;            // weights are f p s'; the largest p s' when f was chosen
+    int e;                   // f = 2^e
+};
+
+template <class T, int U, int RT, int RS, int KS>
+__global__ __launch_bounds__(64 * RS * KS) void cache4_attention_kernel(Cache4Args a)
+{
+#pragma clang fp contract(off)
+    using Words = Words4<U>;
+    constexpr int W = RS * KS, kRowTiles = RT * RS;
+    extern __shared__ __align__(1024) int8_t lds[];
+    float* sums = reinterpret_cast<float*>(lds);                     // W x 16 x kRow, one row tile of each wave at a time
+    v2f* stat = reinterpret_cast<v2f*>(sums + W * 16 * Words::kRow);  // W x 16
+    int* page_of = reinterpret_cast<int*>(stat + W * 16);
+
+    const int group = a.group, rows = a.T * group;
+    const int hk = blockIdx.x, chunk = blockIdx.y, b = udiv_magic(blockIdx.z, a.mg_sets), set = blockIdx.z - b * a.sets;
+    const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
+    const int lane = threadIdx.x & (kWave - 1), col = lane & 15, g = lane >> 4;
+    const int rs = wave / KS, ks = wave % KS;
+    const int key0 = chunk * a.chunk, page_mask = (1 << a.page_shift) - 1, page0 = key0 >> a.page_shift;
+    const int last_page = min((key0 + a.chunk - 1) >> a.page_shift, a.width - 1);
+    for (int p = page0 + threadIdx.x; p <= last_page; p += 64 * W) {
+        const int pg = a.table[static_cast<size_t>(b) * a.width + p];
+        page_of[p - page0] = pg >= 0 && pg < a.pages ? pg : -1;
+    }
+    auto row_of = [&](auto* base, int r) {                           // of q and out
+        const int t = udiv_magic(r, a.mg_group);
+        return base + ((static_cast<size_t>(b) * a.T + t) * a.Hq + hk * group + (r - t * group)) * a.D;
+    };
+    const int row0 = (set * kRowTiles + rs * RT) * 16;               // this wave's rows
+
+    Rows4<U> st[RT];
+    unsigned long long drafts[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const int row = row0 + 16 * rt + col;
+        const bool live = row < rows;
+        v4u raw[U];
+        const uint16_t* src = row_of(a.q, live ? row : 0);
+#pragma unroll
+        for (int c = 0; c < U; c++) {
+            const int d = 8 * (g * U + c);
+            raw[c] = live && d < a.D ? *reinterpret_cast<const v4u*>(src + d) : v4u{0u, 0u, 0u, 0u};
+        }
+        float x[U][8], most = 0.0f, odd = 0.0f;
+#pragma unroll
+        for (int c = 0; c < U; c++) {
+            widen8<T>(raw[c], x[c]);
+#pragma unroll
+            for (int i = 0; i < 8; i++) most = fmaxf(most, fabsf(x[c][i]));
+#pragma unroll
+            for (int i = 0; i < 4; i++) odd = T::times_zero(raw[c][i], odd);
+        }
+        most = column_max(most);
+        // the row's largest query becomes 2^14 to 2^15; rows that are not finite become NaN
+        const int up = most > 0.0f && most < INFINITY ? 15 - __builtin_amdgcn_frexp_expf(most) : 0;
+        float sum = odd;
+#pragma unroll
+        for (int c = 0; c < U; c++) {
+            float y[8];
+#pragma unroll
+            for (int i = 0; i < 8; i++) {
+                const float z = ldexpf(x[c][i], up);
+                sum += z;
+                y[i] = i & 2 ? z * 0.0625f : z;
+            }
+            st[rt].q[c] = narrow8<Fp16>(y);
+        }
+        st[rt].qsum = column_sum(sum) * 0x1p-24f;
+        // (a unit past FP32 belongs to scores that only differ by more than any exponent)
+        st[rt].unit = fminf(ldexpf(a.scale * 1.44269504f, 24 - up), 0x1p126f);
+        st[rt].m = kNoScore;
+        st[rt].limit = kNoScore;
+        st[rt].shift = 0.0f;
+        st[rt].l = st[rt].c = st[rt].u = st[rt].top = 0.0f;
+        st[rt].e = 120;
+        st[rt].f = 0x1p120f;
+#pragma unroll
+        for (int j = 0; j < Words::kOut; j++) st[rt].o[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+        drafts[rt] = 0ull;
+        if (live) {
+            const int t = udiv_magic(row, a.mg_group);
+            drafts[rt] = a.tree ? static_cast<unsigned long long>(a.tree[static_cast<size_t>(b) * a.T + t]) : ~0ull >> (63 - t);
+        }
+    }
+    const int keys = cache_keys(a, b), len = max(a.lens[b], 0), n = min(keys - key0, a.chunk);
+    if (n <= 0) return;
+    // all weights are 2^-low of themselves, so that no sum of values passes FP32 (those of a head span twice BF16's range)
+    const float low = kRescale + 35 - __builtin_clz(keys);
+    __syncthreads();
+    const int open = len - key0;                                     // keys of this chunk that every row sees
+
+    const size_t piece = static_cast<size_t>(32 * U + 8) << a.page_shift;
+    const uint32_t at_v = 16u * U << a.page_shift, at_num = 32u * U << a.page_shift;
+    const uint32_t lane_k = 16 * U * col + 4 * U * g;
+    auto load = [&](Block4<U>& t, int j) -> bool {                   // 16 keys from j on; false: a page that is not there
+        const int pg = __builtin_amdgcn_readfirstlane(j < n ? page_of[((key0 + j) >> a.page_shift) - page0] : -1);
+        const uint8_t* p = a.cache + (static_cast<size_t>(max(pg, 0)) * a.Hkv + hk) * piece;
+        const uint32_t r = (key0 + j) & page_mask;
+        const uint8_t* pk = p + r * (16 * U) + lane_k;
+        if constexpr (U % 4 == 0) {
+#pragma unroll
+            for (int c = 0; c < U; c += 4) *reinterpret_cast<v4u*>(t.k + c) = *reinterpret_cast<const v4u*>(pk + 4 * c);
+        } else if constexpr (U % 2 == 0) {
+#pragma unroll
+            for (int c = 0; c < U; c += 2) *reinterpret_cast<v2u*>(t.k + c) = *reinterpret_cast<const v2u*>(pk + 4 * c);
+        } else {
+#pragma unroll
+            for (int c = 0; c < U; c++) t.k[c] = *reinterpret_cast<const uint32_t*>(pk + 4 * c);
+        }
+#pragma unroll
+        for (int s = 0; s < Words::kSets; s++)
+            t.v[s] = *reinterpret_cast<const v4u*>(p + at_v + r * (16 * U) + 64 * U * g + 16 * Words::word(s, col));
+        const v4u* num = reinterpret_cast<const v4u*>(p + at_num + r * 8 + 32 * g);
+        t.num[0] = num[0];
+        t.num[1] = num[1];
+        return pg >= 0;
+    };
+
+    auto take = [&](const Block4<U> (&t)[2], bool there0, bool there1, int k0) {
+        v4u num[2][2] = {{t[0].num[0], t[0].num[1]}, {t[1].num[0], t[1].num[1]}};
+        const bool masked = k0 + 32 > min(open, n);
+        if (!there0) num[0][0] = num[0][1] = v4u{0u, 0u, 0u, 0u};    // pages that are not there are zeros
+        if (!there1) num[1][0] = num[1][1] = v4u{0u, 0u, 0u, 0u};
+        float vs[2][4], vm[2][4];
+        v4f x[RT][2];
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+            v4f s[RT];
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) s[rt] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int c = 0; c < U; c++) {
+                const v4u k = nibble_pairs(t[h].k[c]);
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++) s[rt] = Fp16::mfma16(k, st[rt].q[c], s[rt]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) {
+                const uint32_t kn = num[h][e >> 1][2 * (e & 1)], vn = num[h][e >> 1][2 * (e & 1) + 1];
+                const float step = T::widen(static_cast<uint16_t>(kn & 0xFFFFu)), least = T::widen(static_cast<uint16_t>(kn >> 16));
+                vs[h][e] = T::widen(static_cast<uint16_t>(vn & 0xFFFFu));
+                vm[h][e] = __builtin_fmaf(8.0f, vs[h][e], T::widen(static_cast<uint16_t>(vn >> 16)));
+#pragma unroll
+                for (int rt = 0; rt < RT; rt++)
+                    x[rt][h][e] = __builtin_fmaf(s[rt][e], step, least * st[rt].qsum) * st[rt].unit;
+            }
+        }
+        uint32_t bits[RT];
+        if (masked) {
+#pragma unroll
+            for (int rt = 0; rt < RT; rt++) {
+                const int d = open - k0;                             // bits below d: the cache; from d on: drafts
+                uint32_t all = bits_to(d - 1);
+                if (d < 32) all |= d >= 0 ? static_cast<uint32_t>(drafts[rt] << d) : d > -64 ? static_cast<uint32_t>(drafts[rt] >> -d) : 0u;
+                bits[rt] = (all & bits_to(n - 1 - k0)) >> (4 * g);
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++)
+                        if (!(bits[rt] >> (16 * h + e) & 1u)) x[rt][h][e] = -INFINITY;
+            }
+        }
+        v4u weights[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; rt++) {
+            Rows4<U>& r = st[rt];
+            float mx = x[rt][0][0];
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) mx = fmaxf(mx, x[rt][h][e]);
+            if (__any(mx > r.limit)) {                               // a maximum that has grown
+                const float was = r.m;
+                r.m = fmaxf(was, column_max(mx));
+                r.limit = r.m + kRescale;
+                r.shift = -(r.m + low);
+                const float down = __builtin_amdgcn_exp2f(was - r.m);
+                r.l *= down;
+                r.c *= down;
+                r.top *= down;
+                const int to = r.top > 0.0f ? max(-120, min(120, 5 - __builtin_amdgcn_frexp_expf(r.top))) : 120;
+                const float by = ldexpf(down, to - r.e);
+                r.e = to;
+                r.f = ldexpf(1.0f, to);
+#pragma unroll
+                for (int j = 0; j < Words::kOut; j++) r.o[j] *= by;
+                r.u *= by;
+            }
+            float w[2][4], wx = 0.0f;
+#pragma unroll
+            for (int h = 0; h < 2; h++)
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const float p = __builtin_amdgcn_exp2f(x[rt][h][e] + r.shift);
+                    r.l += p;
+                    if (masked) {
+                        const bool on = bits[rt] >> (16 * h + e) & 1u;
+                        r.c = __builtin_fmaf(p, on ? vm[h][e] : 0.0f, r.c);
+                        w[h][e] = p * (on ? vs[h][e] : 0.0f);
+                    } else {
+                        r.c = __builtin_fmaf(p, vm[h][e], r.c);
+                        w[h][e] = p * vs[h][e];
+                    }
+                    wx = fmaxf(wx, w[h][e]);
+                }
+            if (__any(wx * r.f > 32768.0f)) {                        // weights that FP16 would not hold
+                r.top = fmaxf(r.top, column_max(wx));
+                const int to = max(-120, min(r.e, 5 - __builtin_amdgcn_frexp_expf(r.top)));
+                const float by = ldexpf(1.0f, to - r.e);
+                r.e = to;
+                r.f = ldexpf(1.0f, to);
+#pragma unroll
+                for (int j = 0; j < Words::kOut; j++) r.o[j] *= by;
+                r.u *= by;
+            }
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                weights[rt][2 * h] = Fp16::pack(w[h][0] * r.f, w[h][1] * r.f);
+                weights[rt][2 * h + 1] = Fp16::pack(w[h][2] * r.f, w[h][3] * r.f);
+                r.u = Fp16::add_pair(weights[rt][2 * h], Fp16::add_pair(weights[rt][2 * h + 1], r.u));
+            }
+        }
+#pragma unroll
+        for (int s = 0; s < Words::kSets; s++) {
+            constexpr uint32_t kLow = 0x05040100u, kHigh = 0x07060302u;
+            const bool full = s < Words::kFull;
+#pragma unroll
+            for (int half = 0; half < (full ? 2 : 1); half++) {
+                const uint32_t sel = full ? (half ? kHigh : kLow) : (col < 8 ? kLow : kHigh);
+                v4u w = {__builtin_amdgcn_perm(t[0].v[s][1], t[0].v[s][0], sel), __builtin_amdgcn_perm(t[0].v[s][3], t[0].v[s][2], sel),
+                         __builtin_amdgcn_perm(t[1].v[s][1], t[1].v[s][0], sel), __builtin_amdgcn_perm(t[1].v[s][3], t[1].v[s][2], sel)};
+#pragma unroll
+                for (int i = 0; i < 4; i++) {
+                    if (i == 2) w = w >> 8;
+                    const v4u v = w & (i & 1 ? 0x00F000F0u : 0x000F000Fu);
+#pragma unroll
+                    for (int rt = 0; rt < RT; rt++) {
+                        v4f& o = st[rt].o[8 * s + 4 * half + i];
+                        o = Fp16::mfma16(v, weights[rt], o);
+                    }
+                }
+            }
+        }
+    };
+
+    const int tiles = (n + 31) / 32;
+    Block4<U> t[2][2];
+    bool there[2][2];
+    auto fetch = [&](int i, int tile) {
+        there[i][0] = load(t[i][0], 32 * tile);
+        there[i][1] = load(t[i][1], 32 * tile + 16);
+    };
+    if (ks < tiles) fetch(0, ks);
+    for (int tile = ks; tile < tiles; tile += 2 * KS) {              // one tile ahead
+        if (tile + KS < tiles) fetch(1, tile + KS);
+        take(t[0], there[0][0], there[0][1], 32 * tile);
+        if (tile + KS >= tiles) break;
+        if (tile + 2 * KS < tiles) fetch(0, tile + 2 * KS);
+        take(t[1], there[1][0], there[1][1], 32 * (tile + KS));
+    }
+
+    // The KS waves of the same rows are joined in LDS, a row tile at a time.
+    const bool whole = keys <= a.chunk;                              // the only chunk: the result itself
+    const size_t part0 = ((static_cast<size_t>(b) * a.Hkv + hk) * a.chunks + chunk) * rows;
+#pragma unroll
+    for (int rt = 0; rt < RT; rt++) {
+        const Rows4<U>& r = st[rt];
+        __syncthreads();                                             // the page list, the tile before
+        const float l = column_sum(r.l), c = column_sum(r.c), u = 8.0f * column_sum(r.u);
+        float* mine = sums + (wave * 16 + col) * Words::kRow;
+        auto value = [&](int j, int e, int i) { return ldexpf(r.o[j][e] * (i & 1 ? 0x1p20f : 0x1p24f) - u, -r.e) + c; };
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+#pragma unroll
+            for (int s = 0; s < Words::kFull; s++) {
+                const int w = 16 * s + 4 * g + e;                    // value 2 i + half of the word is product 4 half + i
+                if (w >= 4 * U) continue;
+                *reinterpret_cast<v4f*>(mine + 8 * w) = v4f{value(8 * s, e, 0), value(8 * s + 4, e, 0), value(8 * s + 1, e, 1), value(8 * s + 5, e, 1)};
+                *reinterpret_cast<v4f*>(mine + 8 * w + 4) = v4f{value(8 * s + 2, e, 2), value(8 * s + 6, e, 2), value(8 * s + 3, e, 3), value(8 * s + 7, e, 3)};
+            }
+            if constexpr (Words::kHalf != 0) {
+                const int at = 4 * g + e, w = 16 * Words::kFull + (at & 7);
+#pragma unroll
+                for (int i = 0; i < 4; i++) mine[8 * w + 2 * i + (at >> 3)] = value(8 * Words::kFull + i, e, i);
+            }
+        }
+        if (g == 0) stat[wave * 16 + col] = v2f{r.m, l};
+        __syncthreads();
+        const int quads = a.D / 4;
+        for (int i = threadIdx.x; i < RS * 16 * quads; i += 64 * W) {
+            const int rr = i / quads, d = 4 * (i - rr * quads), set_row = rr >> 4, cc = rr & 15;
+            const int row = (set * kRowTiles + set_row * RT + rt) * 16 + cc;
+            if (row >= rows) continue;
+            float top = kNoScore, sum = 0.0f;
+#pragma unroll
+            for (int v = 0; v < KS; v++) top = fmaxf(top, stat[(set_row * KS + v) * 16 + cc][0]);
+            v4f y = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+            for (int v = 0; v < KS; v++) {
+                const v2f ml = stat[(set_row * KS + v) * 16 + cc];
+                const float f = __builtin_amdgcn_exp2f(ml[0] - top);
+                sum = __builtin_fmaf(f, ml[1], sum);
+                const v4f z = *reinterpret_cast<const v4f*>(sums + ((set_row * KS + v) * 16 + cc) * Words::kRow + d);
+#pragma unroll
+                for (int e = 0; e < 4; e++) y[e] = __builtin_fmaf(f, z[e], y[e]);
+            }
+            if (whole) {
+                const float inv = sum != 0.0f ? 1.0f / sum : 0.0f;
+                *reinterpret_cast<v2u*>(row_of(a.out, row) + d) = v2u{T::pack(y[0] * inv, y[1] * inv), T::pack(y[2] * inv, y[3] * inv)};
+            } else {
+                *reinterpret_cast<v4f*>(a.part + (part0 + row) * a.D + d) = y;
+                if (d == 0) *reinterpret_cast<v2f*>(a.stat + (part0 + row) * 2) = v2f{top, sum};
+            }
+        }
+    }
+}
+
+template <int U, int RS, int KS>
+constexpr int kCache4Lds = RS * KS * 16 * (Words4<U>::kRow * 4 + 8);
+
+// Rows of a workgroup: 16, 32, 64 or 128.
+CachePlan cache4_plan(int B, int T, int Hq, int Hkv, long long max_keys) {
+    CachePlan p;
+    const int rows = T * (Hq / Hkv);
+    for (p.sets = 1; 16 * p.sets < rows && p.sets < 8;) p.sets *= 2;
+    const long long heads = static_cast<long long>(B) * Hkv * divup(rows, 16 * p.sets);
+    const long long want = std::max<long long>(1, divupll(2 * default_cu_count(), heads));
+    const long long chunk = divupll(std::max<long long>(divupll(max_keys, want), rows), 128) * 128;
+    const long long most = std::max<long long>(kCacheMaxChunk, divupll(divupll(max_keys, kGridRows), 128) * 128);
+    p.chunk = static_cast<int>(std::min(chunk, most));
+    p.chunks = static_cast<int>(std::max<long long>(1, divupll(max_keys, p.chunk)));
+    return p;
+}
+
+template <class T, int U, int RT, int RS, int KS>
+int launch_cache4(Cache4Args a, hipStream_t s) {
+    constexpr int LPR = U <= 2 ? 16 : U <= 4 ? 32 : 64;
+    constexpr int kMost = kCache4Lds<U, RS, KS> + 4 * ((kCacheMaxChunk + 128) / kCache4MinPage + 2);
+    static_assert(kMost <= 159 * 1024, "sums and page numbers fit");
+    static_assert(divupll(kCacheMaxKeys, kGridRows) <= kCacheMaxChunk + 128, "the longest table's chunks are a grid's rows");
+    const int lds = kCache4Lds<U, RS, KS> + 4 * ((a.chunk >> a.page_shift) + 2);
+    const int rows = a.T * (a.Hq / a.Hkv);
+    a.sets = divup(rows, 16 * RT * RS);
+    a.mg_sets = udiv_multiplier(a.sets);
+    static const hipError_t attr = hipFuncSetAttribute(reinterpret_cast<const void*>(&cache4_attention_kernel<T, U, RT, RS, KS>),
+                                                       hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
+    if (attr != hipSuccess) return static_cast<int>(attr);
+    // as many sequences at a time as a grid has rows
+    const long long total = a.B, most = kGridRows / a.sets;
+    const size_t parts = static_cast<size_t>(a.T) * a.Hq * a.chunks;     // of a sequence
+    for (long long b = 0; b < total; b += most) {
+        a.B = static_cast<int>(std::min(most, total - b));
+        const dim3 grid(static_cast<unsigned>(a.Hkv), static_cast<unsigned>(a.chunks), static_cast<unsigned>(a.B * a.sets));
+        cache4_attention_kernel<T, U, RT, RS, KS><<<grid, 64 * RS * KS, lds, s>>>(a);
+        int st = launch_status();
+        if (st == FORGE_OK && a.chunks > 1) {
+            const dim3 rows_grid(static_cast<unsigned>(divup(a.Hq, 4)), static_cast<unsigned>(a.T), static_cast<unsigned>(a.B));
+            cache_join_kernel<T, LPR><<<rows_grid, 256, 0, s>>>(a);
+            st = launch_status();
+        }
+        if (st != FORGE_OK) return st;
+        const size_t q = static_cast<size_t>(a.B) * a.T * a.Hq * a.D;
+        a.q += q;
+        a.out += q;
+        a.table += static_cast<size_t>(a.B) * a.width;
+        a.lens += a.B;
+        if (a.tree) a.tree += static_cast<size_t>(a.B) * a.T;
+        if (a.part) {
+            a.part += a.B * parts * a.D;
+            a.stat += a.B * parts * 2;
+        }
+    }
+    return FORGE_OK;
+}
+
+template <class T, int U>
+int launch_cache4(const Cache4Args& a, int sets, hipStream_t s) {
+    switch (sets) {
+    case 1: return launch_cache4<T, U, 1, 1, 4>(a, s);
+    case 2: return launch_cache4<T, U, 2, 1, 4>(a, s);
+    case 4: return launch_cache4<T, U, 2, 2, 2>(a, s);
+    default: return launch_cache4<T, U, 2, 4, 1>(a, s);
+    }
+}
+
+template <class T>
+int launch_cache4(const Cache4Args& a, int sets, hipStream_t s) {
+    switch (cache4_units(a.D)) {
+    case 2: return launch_cache4<T, 2>(a, sets, s);
+    case 3: return launch_cache4<T, 3>(a, sets, s);
+    case 4: return launch_cache4<T, 4>(a, sets, s);
+    case 6: return launch_cache4<T, 6>(a, sets, s);
+    default: return launch_cache4<T, 8>(a, sets, s);
+    }
+}
+
+}  // namespace forge_amd
+
+using namespace forge_amd;
+
+extern "C" size_t forge_cache4_attention_workspace_size(int B, int T, int Hq, int Hkv, int D, long long max_keys) {
+    if (!cache_shape_ok(B, T, Hq, Hkv, D) || max_keys <= 0 || max_keys > kCacheMaxKeys) return 0;
+    return 4 * cache_floats(B, T, Hq, D, cache4_plan(B, T, Hq, Hkv, max_keys));
+}
+
+extern "C" int forge_cache4_attention(const uint16_t* q, const uint8_t* cache, const int32_t* page_table, const int32_t* cache_lens,
+                                      const int64_t* tree, uint16_t* out, int B, int T, int Hq, int Hkv, int D, int pages,
+                                      int page_size, int table_width, float scale, int dtype, void* workspace,
+                                      size_t workspace_bytes, void* stream)
+{
+    if (B <= 0 || T <= 0 || Hq <= 0 || D <= 0) return FORGE_OK;
+    if (!cache_shape_ok(B, T, Hq, Hkv, D) || !cache4_shape_ok(Hkv, D, pages, page_size) || !q || !cache || !page_table ||
+        !cache_lens || !out || table_width <= 0 || !(scale > 0.0f && scale < INFINITY) || (dtype != FORGE_FP16 && dtype != FORGE_BF16))
+        return FORGE_EINVAL;
+    for (const void* p : {static_cast<const void*>(q), static_cast<const void*>(cache), static_cast<const void*>(out),
+                          static_cast<const void*>(workspace)})
+        if (!aligned(p, 16)) return FORGE_EINVAL;
+    const long long max_keys = static_cast<long long>(table_width) * page_size;
+    if (max_keys > kCacheMaxKeys) return FORGE_EINVAL;
+    const CachePlan p = cache4_plan(B, T, Hq, Hkv, max_keys);
+    const size_t floats = cache_floats(B, T, Hq, D, p);
+    if (floats && (!workspace || workspace_bytes < 4 * floats)) return FORGE_EINVAL;
+    float* part = static_cast<float*>(workspace);
+    const size_t parts = static_cast<size_t>(B) * T * Hq * p.chunks;
+    const Cache4Args a{{q, nullptr, nullptr, page_table, cache_lens, tree, out, part, part ? part + parts * D : nullptr,
+                        B, T, Hq, Hkv, D, pages, __builtin_ctz(static_cast<unsigned>(page_size)), table_width,
+                        p.chunk, p.chunks, Hq / Hkv, 1, udiv_multiplier(Hq / Hkv), 0u, scale}, cache};
+    hipStream_t s = as_stream(stream);
+    return dtype == FORGE_FP16 ? launch_cache4<Fp16>(a, p.sets, s) : launch_cache4<Bf16>(a, p.sets, s);
+}

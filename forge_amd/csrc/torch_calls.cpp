@@ -198,8 +198,154 @@ PyObject* cache_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// (pages, heads, page size, bytes of a position) of a 4-bit cache for heads of D values.
+bool cache4(const at::Tensor* t, long device, int64_t heads, int64_t D) {
+    if (!t || t->dim() != 4 || D < 1 || D > 256) return false;
+    const int64_t units = D <= 64 ? 2 : D <= 96 ? 3 : D <= 128 ? 4 : D <= 192 ? 6 : 8;
+    return dense(t, at::kByte, device, {t->size(0), heads, t->size(2), 32 * units + 8}) && t->size(0) <= INT32_MAX && t->size(2) <= INT32_MAX;
+}
+
+// cache4_write(k, v, cache, slots, device, stream)
+PyObject* cache4_write(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return call<6>(args, n, [](const Call& c) -> long {
+        const at::Tensor *k0 = tensor(c.a[0]), *cache = tensor(c.a[2]), *slots = tensor(c.a[3]);
+        if (!k0) return kNotInOrder;
+        const at::ScalarType type = k0->scalar_type();
+        Heads k, v;
+        if (code(type) < 0 || !k.take(c.a[0], type, c.device) || !v.take(c.a[1], type, c.device) || v.tokens != k.tokens ||
+            v.heads != k.heads || v.D != k.D || k.heads == 0 || k.heads > INT32_MAX || k.tokens > INT32_MAX || !cache4(cache, c.device, k.heads, k.D) ||
+            !dense(slots, at::kInt, c.device, {k.tokens}))
+            return kNotInOrder;
+        return forge_cache4_write(at_<uint16_t>(k.t), at_<uint16_t>(v.t), at_<uint8_t>(cache), at_<int32_t>(slots),
+                                  static_cast<int>(k.tokens), static_cast<int>(k.heads), static_cast<int>(k.D),
+                                  static_cast<int>(cache->size(0)), static_cast<int>(cache->size(2)), k.token, k.head, v.token, v.head,
+                                  code(type), c.stream);
+    });
+}
+
+// cache4_read(cache, slots, k_out, v_out, device, stream)
+PyObject* cache4_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return call<6>(args, n, [](const Call& c) -> long {
+        const at::Tensor *cache = tensor(c.a[0]), *slots = tensor(c.a[1]), *k = tensor(c.a[2]), *v = tensor(c.a[3]);
+        if (!k || k->dim() != 3) return kNotInOrder;
+        const at::ScalarType type = k->scalar_type();
+        const int64_t T = k->size(0), heads = k->size(1), D = k->size(2);
+        if (code(type) < 0 || heads == 0 || heads > INT32_MAX || T > INT32_MAX || !cache4(cache, c.device, heads, D) ||
+            !dense(slots, at::kInt, c.device, {T}) || !dense(k, type, c.device, {T, heads, D}) || !dense(v, type, c.device, {T, heads, D}))
+            return kNotInOrder;
+        return forge_cache4_read(at_<uint8_t>(cache), at_<int32_t>(slots), at_<uint16_t>(k), at_<uint16_t>(v), static_cast<int>(T),
+                                 static_cast<int>(heads), static_cast<int>(D), static_cast<int>(cache->size(0)),
+                                 static_cast<int>(cache->size(2)), code(type), c.stream);
+    });
+}
+
+// cache4_attention(q, cache, page_table, cache_lens, tree, workspace, out, scale, device, stream)
+PyObject* cache4_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return call<10>(args, n, [](const Call& c) -> long {
+        const at::Tensor *q = tensor(c.a[0]), *cache = tensor(c.a[1]), *table = tensor(c.a[2]), *lens = tensor(c.a[3]);
+        const at::Tensor *tree = nullptr, *ws = nullptr, *out = tensor(c.a[6]);
+        if (!q || q->dim() != 4 || !cache || cache->dim() != 4 || !table || table->dim() != 2) return kNotInOrder;
+        const at::ScalarType type = q->scalar_type();
+        const int64_t B = q->size(0), T = q->size(1), Hq = q->size(2), D = q->size(3), Hkv = cache->size(1), width = table->size(1);
+        float scale;
+        if (!c.number(7, &scale)) return kNotInOrder;
+        if (code(type) < 0 || T < 1 || T > 64 || D < 1 || Hkv < 1 || !dense(q, type, c.device, {B, T, Hq, D}) || !cache4(cache, c.device, Hkv, D) ||
+            !dense(table, at::kInt, c.device, {B, width}) || !dense(lens, at::kInt, c.device, {B}) || !dense(out, type, c.device, {B, T, Hq, D}) ||
+            B > INT32_MAX || Hq > INT32_MAX || Hkv > INT32_MAX || width > INT32_MAX)
+            return kNotInOrder;
+        if (!c.none(4) && !dense(tree = tensor(c.a[4]), at::kLong, c.device, {B, T})) return kNotInOrder;
+        if (!c.none(5) && (!on(ws = tensor(c.a[5]), at::kByte, c.device) || !ws->is_contiguous())) return kNotInOrder;
+        return forge_cache4_attention(at_<uint16_t>(q), at_<uint8_t>(cache), at_<int32_t>(table), at_<int32_t>(lens), at_<int64_t>(tree),
+                                      at_<uint16_t>(out), static_cast<int>(B), static_cast<int>(T), static_cast<int>(Hq),
+                                      static_cast<int>(Hkv), static_cast<int>(D), static_cast<int>(cache->size(0)),
+                                      static_cast<int>(cache->size(2)), static_cast<int>(width), scale, code(type), at_<void>(ws),
+                                      ws ? static_cast<size_t>(ws->numel()) : 0, c.stream);
+    });
+}
+
+// beam_select(logits, scores, ended, out_scores, out_beams, out_tokens, workspace, count, end_token, device, stream)
+PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return call<11>(args, n, [](const Call& c) -> long {
+        const at::Tensor *x = tensor(c.a[0]), *scores = tensor(c.a[1]), *ended = nullptr, *os = tensor(c.a[3]), *ob = tensor(c.a[4]);
+        const at::Tensor *ot = tensor(c.a[5]), *ws = tensor(c.a[6]);
+        if (!x || x->dim() != 3 || !PyLong_CheckExact(c.a[7]) || !PyLong_CheckExact(c.a[8])) return kNotInOrder;
+        const at::ScalarType type = x->scalar_type();
+        const int kind = type == at::kFloat ? FORGE_FP32 : code(type);
+        const int64_t B = x->size(0), W = x->size(1), V = x->size(2);
+        const long count = PyLong_AsLong(c.a[7]), end = PyLong_AsLong(c.a[8]);
+        if (PyErr_Occurred() || kind < 0 || !on(x, type, c.device) || B < 1 || W < 1 || V < 1 || B > INT32_MAX || W > INT32_MAX || V > INT32_MAX ||
+            (V > 1 && x->stride(2) != 1) || count < 1 || count > 64 || end < INT32_MIN || end > INT32_MAX ||
+            !dense(scores, at::kFloat, c.device, {B, W}) || !dense(os, at::kFloat, c.device, {B, count}) ||
+            !dense(ob, at::kInt, c.device, {B, count}) || !dense(ot, at::kInt, c.device, {B, count}) ||
+            !on(ws, at::kByte, c.device) || !ws->is_contiguous())
+            return kNotInOrder;
+        if (!c.none(2) && !dense(ended = tensor(c.a[2]), at::kBool, c.device, {B, W})) return kNotInOrder;
+        return forge_beam_select(at_<void>(x), at_<float>(scores), at_<uint8_t>(ended), static_cast<int>(end), at_<float>(os),
+                                 at_<int32_t>(ob), at_<int32_t>(ot), static_cast<int>(B), static_cast<int>(W), static_cast<int>(V),
+                                 static_cast<int>(count), x->stride(0), x->stride(1), kind, at_<void>(ws),
+                                 static_cast<size_t>(ws->numel()), c.stream);
+    });
+}
+
+// fork_pages(page_table, cache_lens, parents, refs, table, lens, refs, slots, src, dst, workspace, page_size, device, stream)
+PyObject* fork_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return call<14>(args, n, [](const Call& c) -> long {
+        const at::Tensor* t[11];
+        for (int i = 0; i < 11; i++)
+            if (!(t[i] = tensor(c.a[i]))) return kNotInOrder;
+        if (t[0]->dim() != 2 || t[2]->dim() != 2 || t[3]->dim() != 1 || !PyLong_CheckExact(c.a[11])) return kNotInOrder;
+        const int64_t rows = t[0]->size(0), width = t[0]->size(1), group = t[2]->size(1), pages = t[3]->size(0);
+        const long page = PyLong_AsLong(c.a[11]);
+        if (PyErr_Occurred() || page < 1 || page > INT32_MAX || rows < 1 || rows > INT32_MAX || width > INT32_MAX || pages > INT32_MAX || group < 1 ||
+            t[2]->size(0) * group != rows || !on(t[10], at::kByte, c.device) || !t[10]->is_contiguous())
+            return kNotInOrder;
+        for (int i : {0, 4})
+            if (!dense(t[i], at::kInt, c.device, {rows, width})) return kNotInOrder;
+        for (int i : {1, 5, 7, 8, 9})
+            if (!dense(t[i], at::kInt, c.device, {rows})) return kNotInOrder;
+        for (int i : {3, 6})
+            if (!dense(t[i], at::kInt, c.device, {pages})) return kNotInOrder;
+        if (!dense(t[2], at::kInt, c.device, {t[2]->size(0), group})) return kNotInOrder;
+        auto p = [&](int i) { return at_<int32_t>(t[i]); };
+        return forge_fork_pages(p(0), p(1), p(2), p(3), p(4), p(5), p(6), p(7), p(8), p(9), static_cast<int>(rows),
+                                static_cast<int>(group), static_cast<int>(width), static_cast<int>(pages), static_cast<int>(page),
+                                at_<void>(t[10]), static_cast<size_t>(t[10]->numel()), c.stream);
+    });
+}
+
+// copy_pages(caches, src, dst, device, stream)
+PyObject* copy_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return call<5>(args, n, [](const Call& c) -> long {
+        constexpr int kMost = 256;
+        const at::Tensor *src = tensor(c.a[1]), *dst = tensor(c.a[2]);
+        const bool list = PyList_CheckExact(c.a[0]);
+        if (!src || !dst || (!list && !PyTuple_CheckExact(c.a[0]))) return kNotInOrder;
+        const Py_ssize_t count = list ? PyList_GET_SIZE(c.a[0]) : PyTuple_GET_SIZE(c.a[0]);
+        if (count < 1 || count > kMost || !on(src, at::kInt, c.device) || !on(dst, at::kInt, c.device) || !src->is_contiguous() ||
+            !dst->is_contiguous() || !src->sizes().equals(dst->sizes()) || src->numel() > INT32_MAX)
+            return kNotInOrder;
+        void* at[kMost];
+        int64_t pages = 0, bytes = 0;
+        for (Py_ssize_t i = 0; i < count; i++) {
+            const at::Tensor* t = tensor(list ? PyList_GET_ITEM(c.a[0], i) : PyTuple_GET_ITEM(c.a[0], i));
+            if (!t || !on(t, t->scalar_type(), c.device) || !t->is_contiguous() || t->dim() < 1 || t->size(0) < 1) return kNotInOrder;
+            if (i == 0) {
+                pages = t->size(0);
+                bytes = static_cast<int64_t>(t->nbytes());
+            }
+            if (t->size(0) != pages || static_cast<int64_t>(t->nbytes()) != bytes) return kNotInOrder;
+            at[i] = t->data_ptr();
+        }
+        if (pages > INT32_MAX || bytes == 0) return kNotInOrder;
+        return forge_copy_pages(at, static_cast<int>(count), bytes / pages, static_cast<int>(pages), at_<int32_t>(src), at_<int32_t>(dst),
+                                static_cast<int>(src->numel()), c.stream);
+    });
+}
+
 #define FASTCALL(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FASTCALL(int4_linear), FASTCALL(qk_norm_rope), FASTCALL(prompt_attention), FASTCALL(cache_attention),
+                         FASTCALL(cache4_write), FASTCALL(cache4_read), FASTCALL(cache4_attention), FASTCALL(beam_select),
+                         FASTCALL(fork_pages), FASTCALL(copy_pages),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "forge_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

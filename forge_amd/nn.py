@@ -274,8 +274,8 @@ class DecoderAttention(nn.Module):
     """The attention block of a decoder: one 4-bit projection to queries, keys and values, RMS norm and rotation of
     the query and key heads, attention, and the 4-bit output projection.
 
-    Keys and values live in a paged cache of the caller's, (pages, page size, kv_heads, head_dim) each; `slots` says
-    where each token's go (page * page size + offset)."""
+    Keys and values live in a paged cache of the caller's, (pages, page size, kv_heads, head_dim) each, or in one 4-bit cache
+    (ops.cache4_shape) as k_cache, with None as v_cache; `slots` says where each token's go (page * page size + offset)."""
 
     def __init__(self, hidden: int, heads: int, kv_heads: int, head_dim: int, positions: int, group_size: int = 128,
                  theta: float = 10000.0, eps: float = 1e-6, dtype: torch.dtype = torch.float16):
@@ -298,27 +298,98 @@ class DecoderAttention(nn.Module):
 
     @torch.no_grad()
     def prompt(self, x: torch.Tensor, cu_seqlens: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tensor,
-               v_cache: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
+               v_cache: Optional[torch.Tensor], slots: torch.Tensor) -> torch.Tensor:
         """Whole prompts packed into x (tokens, hidden), sequence b being tokens cu_seqlens[b] to cu_seqlens[b + 1] - 1; their
         keys and values go into the cache too."""
         q, k, v = self._heads(x)
+        if v_cache is None:
+            q, keys = ops.qk_norm_rope(q, k, self.q_norm, self.k_norm, self.cos, self.sin, positions, eps=self.eps)
+            ops.cache4_write(keys, v, k_cache, slots)
+            return self.out(ops.prompt_attention(q, keys, v, cu_seqlens).view(x.shape[0], -1))
         keys = torch.empty(k.shape, dtype=k.dtype, device=k.device)
         q = ops.qk_norm_rope_cache(q, k, v, self.q_norm, self.k_norm, self.cos, self.sin, positions, k_cache, v_cache, slots,
                                    eps=self.eps, k_out=keys)
         return self.out(ops.prompt_attention(q, keys, v, cu_seqlens).view(x.shape[0], -1))
 
     @torch.no_grad()
-    def cached(self, x: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tensor,
+    def cached(self, x: torch.Tensor, positions: torch.Tensor, k_cache: torch.Tensor, v_cache: Optional[torch.Tensor],
                slots: torch.Tensor, page_table: torch.Tensor, cache_lens: torch.Tensor,
                tree: Optional[torch.Tensor] = None) -> torch.Tensor:
         """The newest T tokens of each sequence, x (B, T, hidden), over the cache: one token, or a tree of drafts
         (tree_masks). positions and slots are (B * T,); token t of sequence b is at cache position cache_lens[b] + t."""
         B, T, hidden = x.shape
         q, k, v = self._heads(x.reshape(B * T, hidden))
+        if v_cache is None:
+            q, k = ops.qk_norm_rope(q, k, self.q_norm, self.k_norm, self.cos, self.sin, positions, eps=self.eps)
+            ops.cache4_write(k, v, k_cache, slots)
+            o = ops.cache4_attention(q.view(B, T, self.heads, self.head_dim), k_cache, page_table, cache_lens, tree)
+            return self.out(o.view(B, T, -1))
         q = ops.qk_norm_rope_cache(q, k, v, self.q_norm, self.k_norm, self.cos, self.sin, positions, k_cache, v_cache, slots,
                                    eps=self.eps)
         o = ops.cache_attention(q.view(B, T, self.heads, self.head_dim), k_cache, v_cache, page_table, cache_lens, tree)
         return self.out(o.view(B, T, -1))
+
+
+class PagedBeams:
+    """The rows of a beam search, `beams` to a request, over paged caches of `pages` pages (any number of caches, of one page
+    count each: every layer's): which pages each row names, how long it is, its score and whether it has ended.
+
+    After start(), prompts go into the cache at the slots that it returns. Then, again and again, step() takes the logits of each row's newest
+    token and the caches, and what it leaves is for the rows' next tokens: `slots` (-1: no page is free), `lens` (their
+    positions, and cache_attention's cache_lens) and `table`. Row w of request b is row b * beams + w. All of it stays on the device."""
+
+    def __init__(self, requests: int, beams: int, pages: int, page_size: int, max_len: int, device):
+        if page_size < 1 or page_size & (page_size - 1):
+            raise ValueError(f"page_size must be a power of two, got {page_size}")
+        self.requests, self.beams, self.page_size = requests, beams, page_size
+        rows, width = requests * beams, max_len // page_size + 1
+        self.table = torch.full((rows, width), -1, dtype=torch.int32, device=device)
+        self.lens = torch.zeros(rows, dtype=torch.int32, device=device)
+        self.refs = torch.zeros(pages, dtype=torch.int32, device=device)
+        self.slots = torch.full((rows,), -1, dtype=torch.int32, device=device)
+        self.scores = torch.full((requests, beams), float("-inf"), dtype=torch.float32, device=device)
+        self.ended = torch.zeros((requests, beams), dtype=torch.bool, device=device)
+        self._written = False                       # whether the slots' tokens are in the caches
+
+    def start(self, prompt_lens) -> torch.Tensor:
+        """Empties all rows and gives each request's first row the pages of a prompt of prompt_lens[b] tokens (integers on the
+        host). Returns the packed prompts' slots."""
+        P, device = self.page_size, self.table.device
+        need = [(n + P - 1) // P for n in prompt_lens]
+        if len(prompt_lens) != self.requests or min(prompt_lens, default=0) < 0 or max(need, default=0) > self.table.shape[1]:
+            raise ValueError(f"prompts of {self.requests} requests, of up to {self.table.shape[1] * P} tokens, got {prompt_lens}")
+        if sum(need) > self.refs.shape[0]:
+            raise ValueError(f"the prompts take {sum(need)} pages, the cache has {self.refs.shape[0]}")
+        table = torch.full(self.table.shape, -1, dtype=torch.int32)
+        lens = torch.zeros(self.lens.shape, dtype=torch.int32)
+        slots, page = [], 0
+        for b, n in enumerate(prompt_lens):
+            table[b * self.beams, :need[b]] = torch.arange(page, page + need[b])
+            lens[b * self.beams] = n
+            slots.append(torch.arange(page * P, page * P + n, dtype=torch.int32))
+            page += need[b]
+        self.table, self.lens = table.to(device), lens.to(device)
+        self.refs = (torch.arange(self.refs.shape[0], device=device) < page).to(torch.int32)
+        self.scores.fill_(float("-inf"))
+        self.scores[:, 0] = 0.0
+        self.ended.zero_()
+        self._written = False
+        return torch.cat(slots).to(device) if slots else torch.zeros(0, dtype=torch.int32, device=device)
+
+    def step(self, logits: torch.Tensor, caches, end_token: Optional[int] = None):
+        """The rows' next tokens from logits (requests, beams, tokens) of their newest ones, and the rows behind them: returns
+        tokens and beams (requests, beams) int32, -1 where a request has fewer continuations. caches: the tensors whose pages the rows share."""
+        if self._written:
+            self.lens = self.lens + (self.slots >= 0).to(torch.int32)
+        ended = None if end_token is None else self.ended
+        self.scores, beams, tokens = ops.beam_select(logits, self.scores, self.beams, ended, 0 if end_token is None else end_token)
+        forked = ops.fork_pages(self.table, self.lens, beams, self.refs, self.page_size)
+        ops.copy_pages(caches, forked.src, forked.dst)
+        self.table, self.lens, self.refs, self.slots = forked.table, forked.lens, forked.refs, forked.slots
+        if end_token is not None:
+            self.ended = self.ended.gather(1, beams.clamp_min(0).long()) | (tokens == end_token)
+        self._written = True
+        return tokens, beams
 
 
 def _gfx950_word_positions(N: int, W: int, device) -> torch.Tensor:

@@ -9,7 +9,7 @@ libforge_amd.so.
 """
 from __future__ import annotations
 
-from typing import Optional, Tuple
+from typing import NamedTuple, Optional, Sequence, Tuple
 
 import torch
 
@@ -855,3 +855,277 @@ def cache_attention(q: torch.Tensor, k_cache: torch.Tensor, v_cache: torch.Tenso
     _call("forge_cache_attention", _p(q), _p(k_cache), _p(v_cache), _p(page_table), _p(cache_lens), _p(tree), _p(out), B, T,
           Hq, Hkv, D, pages, page, width, scale, code, _p(workspace) if size else None, size, _stream())
     return out
+
+
+# ---- beams over a 4-bit cache (extension; include/forge_amd.h "beams over a 4-bit cache") ------
+
+def cache4_shape(pages: int, page_size: int, kv_heads: int, D: int) -> Tuple[int, int, int, int]:
+    """Shape of the uint8 tensor that is a 4-bit cache (its bytes' order is forge_cache4_write's)."""
+    if D % 8 or not 0 < D <= 256:
+        raise ValueError(f"a head must have a multiple of 8 values up to 256, got {D}")
+    units = next(u for u in (2, 3, 4, 6, 8) if D <= 32 * u)
+    return pages, kv_heads, page_size, 32 * units + 8
+
+
+def _need_cache4(cache: torch.Tensor, heads: int, D: int) -> Tuple[int, int]:
+    """The pages and page size of a 4-bit cache of these heads."""
+    if not isinstance(cache, torch.Tensor) or cache.dim() != 4:
+        raise ValueError("cache must be a 4-bit cache: uint8 of cache4_shape(pages, page size, KV heads, D)")
+    pages, _, page, _ = cache.shape
+    _need_shape(cache, torch.uint8, "cache", cache4_shape(pages, page, heads, D))
+    if pages == 0 or page & (page - 1) or not 16 <= page <= 1 << 20 or pages * page > 1 << 31:
+        raise ValueError(f"the cache must hold pages of a power of two of positions from 16 on, got {tuple(cache.shape)}")
+    return pages, page
+
+
+def cache4_write(k: torch.Tensor, v: torch.Tensor, cache: torch.Tensor, slots: torch.Tensor) -> torch.Tensor:
+    """forge_cache4_write: keys and values (T, Hkv, D), float16 or bfloat16 and possibly strided views, into rows slots[t] (int32,
+    page * page size + offset, each once; a slot outside the cache writes nothing) of a 4-bit cache. A cache holds
+    one type: it is read and attended to with the type that wrote it. Returns the cache."""
+    if _fast("cache4_write", k, v, cache, slots):
+        return cache
+    code = _act_type(k, "k")
+    T = k.shape[0] if k.dim() else 0
+    ks, vs = _need_heads(k, k.dtype, "k", T), _need_heads(v, k.dtype, "v", T)
+    if k.shape != v.shape:
+        raise ValueError(f"v must have k's shape {tuple(k.shape)}, got {tuple(v.shape)}")
+    Hkv, D = k.shape[1], k.shape[2]
+    pages, page = _need_cache4(cache, Hkv, D)
+    _need(slots, torch.int32, "slots")
+    if slots.shape != (T,):
+        raise ValueError(f"slots must have shape ({T},), got {tuple(slots.shape)}")
+    _same_device(k, v, cache, slots)
+    _call("forge_cache4_write", _p(k), _p(v), _p(cache), _p(slots), T, Hkv, D, pages, page, *ks, *vs, code, _stream())
+    return cache
+
+
+def cache4_read(cache: torch.Tensor, slots: torch.Tensor, D: int, dtype: torch.dtype = torch.float16,
+                k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """forge_cache4_read: what rows `slots` (int32) of a 4-bit cache stand for, keys and values (T, Hkv, D) of the cache's type;
+    zeros for slots outside it. k_out and v_out may be passed to reuse buffers."""
+    if isinstance(slots, torch.Tensor) and isinstance(cache, torch.Tensor) and slots.dim() == 1 and cache.dim() == 4:
+        shape = (slots.shape[0], cache.shape[1], D)
+        if k_out is None:
+            k_out = torch.empty(shape, dtype=dtype, device=cache.device)
+        if v_out is None:
+            v_out = torch.empty(shape, dtype=dtype, device=cache.device)
+        if k_out.dtype is dtype and _fast("cache4_read", cache, slots, k_out, v_out):
+            return k_out, v_out
+    code = _DTYPE.get(dtype)
+    if code is None:
+        raise TypeError(f"dtype must be torch.float16 or torch.bfloat16, got {dtype}")
+    _need(slots, torch.int32, "slots")
+    if slots.dim() != 1:
+        raise ValueError(f"slots must have one dimension, got shape {tuple(slots.shape)}")
+    heads = cache.shape[1] if isinstance(cache, torch.Tensor) and cache.dim() == 4 else 0
+    pages, page = _need_cache4(cache, heads, D)
+    T = slots.shape[0]
+    _need_shape(k_out, dtype, "k_out", (T, heads, D))
+    _need_shape(v_out, dtype, "v_out", (T, heads, D))
+    _same_device(cache, slots, k_out, v_out)
+    _call("forge_cache4_read", _p(cache), _p(slots), _p(k_out), _p(v_out), T, heads, D, pages, page, code, _stream())
+    return k_out, v_out
+
+
+def cache4_attention_workspace_size(B: int, T: int, Hq: int, Hkv: int, D: int, max_keys: int) -> int:
+    """Bytes of cache4_attention's workspace; max_keys = page_table.shape[1] * page size."""
+    return _lib.load().forge_cache4_attention_workspace_size(B, T, Hq, Hkv, D, max_keys)
+
+
+def cache4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Tensor, cache_lens: torch.Tensor,
+                     tree: Optional[torch.Tensor] = None, scale: Optional[float] = None,
+                     workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """forge_cache4_attention: cache_attention over a 4-bit cache (cache4_shape(pages, page size, Hkv, D)), with the same queries
+    (B, T, Hq, D), tables, lengths and trees. The new tokens' keys and values are in the cache already (cache4_write)."""
+    if workspace is not None and out is not None and isinstance(q, torch.Tensor):
+        if _fast("cache4_attention", q, cache, page_table, cache_lens, tree, workspace, out, _scale_of(scale, q)):
+            return out
+    code = _act_type(q, "q")
+    dt = q.dtype
+    if q.dim() != 4:
+        raise ValueError(f"q must be (B, T, Hq, D), got {tuple(q.shape)}")
+    B, T, Hq, D = q.shape
+    if not 1 <= T <= 64:
+        raise ValueError(f"1 to 64 new tokens per sequence, got {T}")
+    if D % 8 or D > 256 or D == 0:
+        raise ValueError(f"a head must have a multiple of 8 values up to 256, got {D}")
+    _need_shape(q, dt, "q", (B, T, Hq, D))
+    Hkv = cache.shape[1] if isinstance(cache, torch.Tensor) and cache.dim() == 4 else 0
+    pages, page = _need_cache4(cache, Hkv, D)
+    if Hkv == 0 or Hq % Hkv:
+        raise ValueError(f"query heads must be a multiple of the KV heads, got {Hq} and {Hkv}")
+    _need(page_table, torch.int32, "page_table")
+    if page_table.dim() != 2 or page_table.shape[0] != B or page_table.shape[1] == 0:
+        raise ValueError(f"page_table must be ({B}, pages of the longest sequence), got {tuple(page_table.shape)}")
+    _need(cache_lens, torch.int32, "cache_lens")
+    if cache_lens.shape != (B,):
+        raise ValueError(f"cache_lens must have shape ({B},), got {tuple(cache_lens.shape)}")
+    if tree is not None:
+        _need(tree, torch.int64, "tree")
+        if tree.shape != (B, T):
+            raise ValueError(f"tree must have shape ({B}, {T}), got {tuple(tree.shape)}")
+    scale = _softmax_scale(scale, D)
+    width = page_table.shape[1]
+    size = cache4_attention_workspace_size(B, T, Hq, Hkv, D, width * page)
+    if workspace is None and size:
+        workspace = torch.empty((size,), dtype=torch.uint8, device=q.device)
+    elif workspace is not None:
+        _need(workspace, torch.uint8, "workspace", size)
+        if workspace.data_ptr() % 16:
+            raise ValueError("workspace must be 16-byte aligned")
+    if out is None:
+        out = torch.empty((B, T, Hq, D), dtype=dt, device=q.device)
+    else:
+        _need_shape(out, dt, "out", (B, T, Hq, D))
+    _same_device(q, cache, page_table, cache_lens, tree, workspace, out)
+    _call("forge_cache4_attention", _p(q), _p(cache), _p(page_table), _p(cache_lens), _p(tree), _p(out), B, T, Hq, Hkv, D,
+          pages, page, width, scale, code, _p(workspace) if size else None, size, _stream())
+    return out
+
+
+_LOGITS = {torch.float16: 0, torch.bfloat16: 1, torch.float32: 2}   # FORGE_FP16, FORGE_BF16, FORGE_FP32
+
+
+def beam_select_workspace_size(B: int, W: int, V: int, count: int) -> int:
+    """Bytes of beam_select's workspace, for logits of any type."""
+    return _lib.load().forge_beam_select_workspace_size(B, W, V, count)
+
+
+def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int, ended: Optional[torch.Tensor] = None,
+                end_token: int = 0, workspace: Optional[torch.Tensor] = None,
+                out: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None
+                ) -> Tuple[torch.Tensor, torch.Tensor, torch.Tensor]:
+    """forge_beam_select: the `count` (1 to 64) best continuations of each request's beams by log softmax(logits) + scores, for logits
+    (B, W, V) float16, bfloat16 or float32 (rows of V contiguous values, any strides otherwise) and the beams' scores (B, W) float32. Returns scores
+    (float32), beams and tokens (int32), (B, count) each, in descending order, equal ones by (beam, token); places that nothing is left for
+    hold -inf, -1, -1. ended (B, W) bool: beams with end_token, at their score, as their one candidate."""
+    if workspace is not None and out is not None and isinstance(out, tuple) and len(out) == 3:
+        if _fast("beam_select", logits, scores, ended, *out, workspace, count, end_token):
+            return out
+    if not isinstance(logits, torch.Tensor) or logits.dtype not in _LOGITS:
+        raise TypeError("logits must be a float16, bfloat16 or float32 torch.Tensor")
+    if not logits.is_cuda:
+        raise ValueError("logits must be a device tensor")
+    if logits.dim() != 3 or 0 in logits.shape[1:]:
+        raise ValueError(f"logits must be (requests, beams, tokens), got {tuple(logits.shape)}")
+    B, W, V = logits.shape
+    batch, beam, one = logits.stride()
+    if one != 1 and V > 1:
+        raise ValueError(f"logits must have contiguous rows, got strides {logits.stride()}")
+    _need_shape(scores, torch.float32, "scores", (B, W), align=4)
+    if ended is not None:
+        _need_shape(ended, torch.bool, "ended", (B, W), align=1)
+    if isinstance(count, bool) or not isinstance(count, int) or not 1 <= count <= 64:
+        raise ValueError(f"count must be 1 to 64, got {count!r}")
+    if isinstance(end_token, bool) or not isinstance(end_token, int) or (ended is not None and not 0 <= end_token < V):
+        raise ValueError(f"end_token must be one of {V} tokens, got {end_token!r}")
+    if W > 1024:
+        raise ValueError(f"a request has up to 1024 beams, got {W}")
+    size = beam_select_workspace_size(B, W, V, count) if B else 0
+    if B and not size:
+        raise ValueError(f"logits of {tuple(logits.shape)} and {count} places are more than one call takes")
+    if workspace is None:
+        workspace = torch.empty((size,), dtype=torch.uint8, device=logits.device)
+    else:
+        _need(workspace, torch.uint8, "workspace", size)
+        if workspace.data_ptr() % 16:
+            raise ValueError("workspace must be 16-byte aligned")
+    if out is None:
+        out = (torch.empty((B, count), dtype=torch.float32, device=logits.device),
+               torch.empty((B, count), dtype=torch.int32, device=logits.device),
+               torch.empty((B, count), dtype=torch.int32, device=logits.device))
+    else:
+        for t, dt, name in zip(out, (torch.float32, torch.int32, torch.int32), ("scores", "beams", "tokens")):
+            _need_shape(t, dt, f"out: {name}", (B, count), align=4)
+    _same_device(logits, scores, ended, workspace, *out)
+    _call("forge_beam_select", _p(logits), _p(scores), _p(ended), end_token, *(_p(t) for t in out), B, W, V, count, batch, beam,
+          _LOGITS[logits.dtype], _p(workspace), size, _stream())
+    return out
+
+
+class Forked(NamedTuple):
+    """What fork_pages returns, int32: the new rows' page table (rows, width), lengths, page counts (pages,), slots of the next
+    tokens, and the pages to be copied (copy_pages)."""
+    table: torch.Tensor
+    lens: torch.Tensor
+    refs: torch.Tensor
+    slots: torch.Tensor
+    src: torch.Tensor
+    dst: torch.Tensor
+
+
+def fork_pages_workspace_size(rows: int, pages: int) -> int:
+    """Bytes of fork_pages's workspace."""
+    return _lib.load().forge_fork_pages_workspace_size(rows, pages)
+
+
+def fork_pages(page_table: torch.Tensor, cache_lens: torch.Tensor, parents: torch.Tensor, refs: torch.Tensor, page_size: int,
+               workspace: Optional[torch.Tensor] = None, out: Optional[Forked] = None) -> Forked:
+    """forge_fork_pages: the page table (rows, width) after each row went on from another row of its request: parents
+    (requests, rows of each) holds their numbers within the request (anything else ends the row), as beam_select returns them. Full
+    pages are shared (refs (pages,) counts their names), a page in use is the first child's and copied for the others, and every row has a page for
+    its next token. All int32; the outputs are not the inputs."""
+    if out is not None and workspace is not None and isinstance(out, tuple) and len(out) == 6:
+        if _fast("fork_pages", page_table, cache_lens, parents, refs, *out, workspace, page_size):
+            return out
+    for t, name, dims in ((page_table, "page_table", 2), (cache_lens, "cache_lens", 1), (parents, "parents", 2), (refs, "refs", 1)):
+        _need(t, torch.int32, name)
+        if t.dim() != dims:
+            raise ValueError(f"{name} must have {dims} dimension{'s' if dims > 1 else ''}, got shape {tuple(t.shape)}")
+    rows, width = page_table.shape
+    group, pages = parents.shape[1], refs.shape[0]
+    if cache_lens.shape != (rows,) or parents.numel() != rows:
+        raise ValueError(f"cache_lens and parents must hold a number for each of {rows} rows, got {tuple(cache_lens.shape)} and "
+                         f"{tuple(parents.shape)}")
+    if isinstance(page_size, bool) or not isinstance(page_size, int) or page_size < 1 or page_size & (page_size - 1):
+        raise ValueError(f"page_size must be a power of two, got {page_size!r}")
+    if rows > 8192:
+        raise ValueError(f"up to 8192 rows, got {rows}")
+    if width == 0 or pages == 0 or pages * page_size > 1 << 31 or width * page_size >= 1 << 31:
+        raise ValueError(f"a table of {width} and a cache of {pages} pages of {page_size} positions cannot be addressed")
+    size = fork_pages_workspace_size(rows, pages) if rows else 0
+    if workspace is None:
+        workspace = torch.empty((size,), dtype=torch.uint8, device=page_table.device)
+    else:
+        _need(workspace, torch.uint8, "workspace", size)
+        if workspace.data_ptr() % 4:
+            raise ValueError("workspace must be 4-byte aligned")
+    shapes = ((rows, width), (rows,), (pages,), (rows,), (rows,), (rows,))
+    if out is None:
+        out = Forked(*(torch.empty(s, dtype=torch.int32, device=page_table.device) for s in shapes))
+    else:
+        for t, s, name in zip(out, shapes, Forked._fields):
+            _need_shape(t, torch.int32, f"out.{name}", s, align=4)
+    _same_device(page_table, cache_lens, parents, refs, workspace, *out)
+    _call("forge_fork_pages", _p(page_table), _p(cache_lens), _p(parents), _p(refs), *(_p(t) for t in out), rows, group, width,
+          pages, page_size, _p(workspace), size, _stream())
+    return out
+
+
+def copy_pages(caches: Sequence[torch.Tensor], src: torch.Tensor, dst: torch.Tensor) -> None:
+    """forge_copy_pages: page dst[i] of each of the caches (contiguous tensors of any type whose first dimension is the pages, all of the same number and
+    size) becomes a copy of page src[i] (int32, of any shape, the same for both); pairs with an index that is no page copy nothing. No page of dst may
+    be in another pair."""
+    if _fast("copy_pages", caches, src, dst):
+        return
+    _need(src, torch.int32, "src")
+    _need(dst, torch.int32, "dst")
+    if src.shape != dst.shape:
+        raise ValueError(f"src and dst must have one shape, got {tuple(src.shape)} and {tuple(dst.shape)}")
+    caches = list(caches)
+    if not caches:
+        return
+    for t in caches:
+        if not isinstance(t, torch.Tensor):
+            raise TypeError("caches must be torch.Tensors")
+        _need(t, t.dtype, "caches")
+        if t.dim() < 1 or t.shape[0] == 0 or t.shape[0] != caches[0].shape[0] or t.nbytes != caches[0].nbytes:
+            raise ValueError("caches must have pages of one number and size in their first dimension")
+        if t.nbytes // t.shape[0] % 16 or t.data_ptr() % 16:
+            raise ValueError("caches must be 16-byte aligned, with pages of a multiple of 16 bytes")
+    _same_device(src, dst, *caches)
+    import ctypes
+    pointers = (ctypes.c_void_p * len(caches))(*(t.data_ptr() for t in caches))
+    pages = caches[0].shape[0]
+    _call("forge_copy_pages", ctypes.addressof(pointers), len(caches), caches[0].nbytes // pages, pages, _p(src), _p(dst),
+          src.numel(), _stream())

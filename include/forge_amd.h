@@ -370,6 +370,65 @@ int forge_cache_attention(const uint16_t* q, const uint16_t* k_cache, const uint
                           int B, int T, int Hq, int Hkv, int D, int pages, int page_size, int table_width,
                           float scale, int dtype, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- beams over a 4-bit cache -----------------------------------------------------------
+ *
+ * The paged cache with 4 bits a value: per position and KV head, keys and values are m + s n with integers n in 0..15
+ * and a step s and a lowest value m of the 16-bit type, s = (max / 15 - min / 15) rounded toward zero (both quotients in FP32), m = min,
+ * n = min(round_half_even((x - m) / s), 15), 0 where s is 0; a head with an infinity or NaN has s = m = NaN. cache:
+ * (pages, Hkv, page_size, 32 U + 8) bytes, U = 2, 3, 4, 6 or 8, the smallest with D <= 32 U, 16-byte aligned; page_size a power of two
+ * from 16 to 2^20, pages * page_size <= 2^31. The piece of a page and head holds page_size rows of a key's 4 U words of 32 bits (word w: values
+ * 8 w to 8 w + 7, of these value 2 i at bits 4 i and value 2 i + 1 at bits 16 + 4 i; words past D are zeros), then the values' words as
+ * (position / 4, word, position % 4), then per position four 16-bit numbers: step and lowest value of its key, and of its value. */
+/* Row slots[t] (page * page_size + offset) of the cache takes k and v (T,Hkv,D) of token t, strided as above; a slot outside it writes
+ * nothing. The slots of a call differ. */
+int forge_cache4_write(const uint16_t* k, const uint16_t* v, uint8_t* cache, const int32_t* slots, int T, int Hkv, int D,
+                       int pages, int page_size, long long k_token, long long k_head, long long v_token,
+                       long long v_head, int dtype, void* stream);
+/* The other way: k and v (T,Hkv,D), contiguous, m + s n in FP32 rounded once; zeros for a slot outside the cache. */
+int forge_cache4_read(const uint8_t* cache, const int32_t* slots, uint16_t* k, uint16_t* v, int T, int Hkv, int D,
+                      int pages, int page_size, int dtype, void* stream);
+
+/* forge_cache_attention over the 4-bit cache, with the same arguments and limits. Keys and values enter as m + s n, not
+ * rounded to 16 bits; the softmax weights times the values' steps are rounded to FP16, scaled by a power of two of the row's, in both types. */
+size_t forge_cache4_attention_workspace_size(int B, int T, int Hq, int Hkv, int D, long long max_keys);
+int forge_cache4_attention(const uint16_t* q, const uint8_t* cache, const int32_t* page_table, const int32_t* cache_lens,
+                           const int64_t* tree, uint16_t* out, int B, int T, int Hq, int Hkv, int D, int pages,
+                           int page_size, int table_width, float scale, int dtype, void* workspace,
+                           size_t workspace_bytes, void* stream);
+
+/* A beam search's selection. For each of B requests, score[w,v] = logits[w,v] - log(sum over v of exp(logits[w,v])) + scores[w] of its
+ * W (up to 1024) beams and V tokens; the `count` (1 to 64) largest go to out_scores (FP32), out_beams (w) and out_tokens (v), (B,count) each,
+ * in descending order, equal ones by (w, v). Sums, scores and their order are taken in 64 bits from FP32 exponentials. -inf
+ * logits are no candidates; neither is a beam whose score is not finite or whose logits hold an infinity or NaN, or -inf only. A beam that has
+ * ended (ended[b,w] != 0; NULL: none has) has one candidate, end_token with the beam's score, and its logits are not read. Places
+ * that no candidate is left for are -inf, -1, -1. logits: dtype FORGE_FP16, FORGE_BF16 or FORGE_FP32, rows of V contiguous values at
+ * b * batch_stride + w * beam_stride elements, at any alignment. workspace: scratch of the size below, 16-byte aligned. */
+#define FORGE_FP32 2
+size_t forge_beam_select_workspace_size(int B, int W, int V, int count);
+int forge_beam_select(const void* logits, const float* scores, const uint8_t* ended, int end_token, float* out_scores,
+                      int32_t* out_beams, int32_t* out_tokens, int B, int W, int V, int count, long long batch_stride,
+                      long long beam_stride, int dtype, void* workspace, size_t workspace_bytes, void* stream);
+
+/* The pages of a paged cache's rows (up to 8192, `group` to a request) that go on from one another. New row r goes on from row parents[r] of its
+ * own group (0..group-1; any other value: row r ends and its pages are released). It names that row's full pages, those before cache_lens / page_size;
+ * the page of its next token (position cache_lens) is the parent's where r is the parent's first child and
+ * refs, the number of names of each page, is 1 there; else the lowest page with refs 0 that no row before r takes. Where the parent's
+ * page holds tokens, src[r], dst[r] say what is to be copied (-1, -1: nothing). Pages that this call releases
+ * are not taken by it. Without room in the table or a free page the row has no page (-1) and no slot. table_out
+ * (rows,table_width), -1 past the row's pages; lens_out: cache_lens of the parents, 0 for rows that end; refs_out (pages): refs less page_table's names
+ * and plus table_out's; slots: the next tokens' cache rows, or -1. Entries outside 0..pages-1 name no page.
+ * The outputs are not the inputs. workspace: scratch of the size below. */
+size_t forge_fork_pages_workspace_size(int rows, int pages);
+int forge_fork_pages(const int32_t* page_table, const int32_t* cache_lens, const int32_t* parents, const int32_t* refs,
+                     int32_t* table_out, int32_t* lens_out, int32_t* refs_out, int32_t* slots, int32_t* src, int32_t* dst,
+                     int rows, int group, int table_width, int pages, int page_size, void* workspace,
+                     size_t workspace_bytes, void* stream);
+/* In each of the caches (a host array of `tensors` device pointers, 16-byte aligned, pages of page_bytes, a multiple of 16), page dst[i] becomes a copy
+ * of page src[i], for `pairs` pairs on the device; a pair with an index outside 0..pages-1 copies nothing. No dst may be
+ * another pair's src or dst. */
+int forge_copy_pages(void* const* caches, int tensors, long long page_bytes, int pages, const int32_t* src,
+                     const int32_t* dst, int pairs, void* stream);
+
 #ifdef __cplusplus
 }
 #endif
