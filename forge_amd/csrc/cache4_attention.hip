@@ -15,6 +15,8 @@
 #include "cache4.h"
 #include "cache_split.h"
 
+#include <type_traits>
+
 namespace forge_amd {
 
 struct Cache4Args : CacheArgs {
@@ -62,15 +64,25 @@ template <int U>
 struct Rows4 {
     v4u q[U];
     v4f o[Words4<U>::kOut];
-    float unit, qsum;        // of a score; the sum of the row's queries
-    float m, limit, shift;   // running maximum of the exponents; above limit it is raised; -(m + low)
+    float unit, qsum;        // of a score; the sum of the row's queries, in exponents
+    float shift, limit;      // exponents are scores + shift; above limit the shift is lowered (-FLT_MAX: none yet)
     float l, c, u;           // this lane's sums of p, of p (m' + 8 s') and of the rounded weights
     float f, top;            // weights are f p s'; the largest p s' when f was chosen
     int e;                   // f = 2^e
+    __device__ __forceinline__ void scale(float by) {
+#pragma unroll
+        for (int j = 0; j < Words4<U>::kOut; j++) o[j] *= by;
+        u *= by;
+    }
 };
 
+__device__ const uint4 kNoNumbers[8] = {};   // those of a page that is not there
+
+// Waves of a SIMD that the registers are to leave room for.
+constexpr int cache4_waves(int U, int RT) { return U <= 4 ? (RT == 1 ? 3 : 2) : RT == 1 ? 2 : 1; }
+
 template <class T, int U, int RT, int RS, int KS>
-__global__ __launch_bounds__(64 * RS * KS) void cache4_attention_kernel(Cache4Args a)
+__global__ __launch_bounds__(64 * RS * KS, cache4_waves(U, RT)) void cache4_attention_kernel(Cache4Args a)
 {
 #pragma clang fp contract(off)
     using Words = Words4<U>;
@@ -98,7 +110,6 @@ __global__ __launch_bounds__(64 * RS * KS) void cache4_attention_kernel(Cache4Ar
     const int row0 = (set * kRowTiles + rs * RT) * 16;               // this wave's rows
 
     Rows4<U> st[RT];
-    unsigned long long drafts[RT];
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const int row = row0 + 16 * rt + col;
@@ -134,22 +145,16 @@ __global__ __launch_bounds__(64 * RS * KS) void cache4_attention_kernel(Cache4Ar
             }
             st[rt].q[c] = narrow8<Fp16>(y);
         }
-        st[rt].qsum = column_sum(sum) * 0x1p-24f;
         // (a unit past FP32 belongs to scores that only differ by more than any exponent)
         st[rt].unit = fminf(ldexpf(a.scale * 1.44269504f, 24 - up), 0x1p126f);
-        st[rt].m = kNoScore;
-        st[rt].limit = kNoScore;
+        st[rt].qsum = column_sum(sum) * 0x1p-24f * st[rt].unit;
         st[rt].shift = 0.0f;
+        st[rt].limit = -FLT_MAX;
         st[rt].l = st[rt].c = st[rt].u = st[rt].top = 0.0f;
         st[rt].e = 120;
         st[rt].f = 0x1p120f;
 #pragma unroll
         for (int j = 0; j < Words::kOut; j++) st[rt].o[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
-        drafts[rt] = 0ull;
-        if (live) {
-            const int t = udiv_magic(row, a.mg_group);
-            drafts[rt] = a.tree ? static_cast<unsigned long long>(a.tree[static_cast<size_t>(b) * a.T + t]) : ~0ull >> (63 - t);
-        }
     }
     const int keys = cache_keys(a, b), len = max(a.lens[b], 0), n = min(keys - key0, a.chunk);
     if (n <= 0) return;
@@ -161,35 +166,42 @@ __global__ __launch_bounds__(64 * RS * KS) void cache4_attention_kernel(Cache4Ar
     const size_t piece = static_cast<size_t>(32 * U + 8) << a.page_shift;
     const uint32_t at_v = 16u * U << a.page_shift, at_num = 32u * U << a.page_shift;
     const uint32_t lane_k = 16 * U * col + 4 * U * g;
-    auto load = [&](Block4<U>& t, int j) -> bool {                   // 16 keys from j on; false: a page that is not there
-        const int pg = __builtin_amdgcn_readfirstlane(j < n ? page_of[((key0 + j) >> a.page_shift) - page0] : -1);
-        const uint8_t* p = a.cache + (static_cast<size_t>(max(pg, 0)) * a.Hkv + hk) * piece;
-        const uint32_t r = (key0 + j) & page_mask;
-        const uint8_t* pk = p + r * (16 * U) + lane_k;
-        if constexpr (U % 4 == 0) {
+    struct Pages { int pg[2]; };
+    auto look = [&](int tile) {                                      // the pages of a tile (past the last one: any)
+        Pages p;
 #pragma unroll
-            for (int c = 0; c < U; c += 4) *reinterpret_cast<v4u*>(t.k + c) = *reinterpret_cast<const v4u*>(pk + 4 * c);
-        } else if constexpr (U % 2 == 0) {
+        for (int h = 0; h < 2; h++) p.pg[h] = page_of[((key0 + min(32 * tile + 16 * h, n - 1)) >> a.page_shift) - page0];
+        return p;
+    };
+    auto load = [&](Block4<U> (&t)[2], int tile, const Pages& pages) {
 #pragma unroll
-            for (int c = 0; c < U; c += 2) *reinterpret_cast<v2u*>(t.k + c) = *reinterpret_cast<const v2u*>(pk + 4 * c);
-        } else {
+        for (int h = 0; h < 2; h++) {
+            const int pg = __builtin_amdgcn_readfirstlane(pages.pg[h]);
+            const uint8_t* p = a.cache + (static_cast<size_t>(max(pg, 0)) * a.Hkv + hk) * piece;
+            const uint32_t r = (key0 + 32 * tile + 16 * h) & page_mask;
+            const uint8_t* pk = p + r * (16 * U) + lane_k;
+            if constexpr (U % 4 == 0) {
 #pragma unroll
-            for (int c = 0; c < U; c++) t.k[c] = *reinterpret_cast<const uint32_t*>(pk + 4 * c);
+                for (int c = 0; c < U; c += 4) *reinterpret_cast<v4u*>(t[h].k + c) = *reinterpret_cast<const v4u*>(pk + 4 * c);
+            } else if constexpr (U % 2 == 0) {
+#pragma unroll
+                for (int c = 0; c < U; c += 2) *reinterpret_cast<v2u*>(t[h].k + c) = *reinterpret_cast<const v2u*>(pk + 4 * c);
+            } else {
+#pragma unroll
+                for (int c = 0; c < U; c++) t[h].k[c] = *reinterpret_cast<const uint32_t*>(pk + 4 * c);
+            }
+#pragma unroll
+            for (int s = 0; s < Words::kSets; s++)
+                t[h].v[s] = *reinterpret_cast<const v4u*>(p + at_v + r * (16 * U) + 64 * U * g + 16 * Words::word(s, col));
+            const uint8_t* pn = pg >= 0 ? p + at_num + r * 8 : reinterpret_cast<const uint8_t*>(kNoNumbers);
+            t[h].num[0] = *reinterpret_cast<const v4u*>(pn + 32 * g);
+            t[h].num[1] = *reinterpret_cast<const v4u*>(pn + 32 * g + 16);
         }
-#pragma unroll
-        for (int s = 0; s < Words::kSets; s++)
-            t.v[s] = *reinterpret_cast<const v4u*>(p + at_v + r * (16 * U) + 64 * U * g + 16 * Words::word(s, col));
-        const v4u* num = reinterpret_cast<const v4u*>(p + at_num + r * 8 + 32 * g);
-        t.num[0] = num[0];
-        t.num[1] = num[1];
-        return pg >= 0;
     };
 
-    auto take = [&](const Block4<U> (&t)[2], bool there0, bool there1, int k0) {
-        v4u num[2][2] = {{t[0].num[0], t[0].num[1]}, {t[1].num[0], t[1].num[1]}};
-        const bool masked = k0 + 32 > min(open, n);
-        if (!there0) num[0][0] = num[0][1] = v4u{0u, 0u, 0u, 0u};    // pages that are not there are zeros
-        if (!there1) num[1][0] = num[1][1] = v4u{0u, 0u, 0u, 0u};
+    // 32 keys from k0 on; masked: some rows do not see all of them.
+    auto take = [&](const Block4<U> (&t)[2], int k0, auto masked) {
+        constexpr bool kMasked = decltype(masked)::value;
         float vs[2][4], vm[2][4];
         v4f x[RT][2];
 #pragma unroll
@@ -205,82 +217,74 @@ __global__ __launch_bounds__(64 * RS * KS) void cache4_attention_kernel(Cache4Ar
             }
 #pragma unroll
             for (int e = 0; e < 4; e++) {
-                const uint32_t kn = num[h][e >> 1][2 * (e & 1)], vn = num[h][e >> 1][2 * (e & 1) + 1];
+                const uint32_t kn = t[h].num[e >> 1][2 * (e & 1)], vn = t[h].num[e >> 1][2 * (e & 1) + 1];
                 const float step = T::widen(static_cast<uint16_t>(kn & 0xFFFFu)), least = T::widen(static_cast<uint16_t>(kn >> 16));
                 vs[h][e] = T::widen(static_cast<uint16_t>(vn & 0xFFFFu));
                 vm[h][e] = __builtin_fmaf(8.0f, vs[h][e], T::widen(static_cast<uint16_t>(vn >> 16)));
 #pragma unroll
                 for (int rt = 0; rt < RT; rt++)
-                    x[rt][h][e] = __builtin_fmaf(s[rt][e], step, least * st[rt].qsum) * st[rt].unit;
-            }
-        }
-        uint32_t bits[RT];
-        if (masked) {
-#pragma unroll
-            for (int rt = 0; rt < RT; rt++) {
-                const int d = open - k0;                             // bits below d: the cache; from d on: drafts
-                uint32_t all = bits_to(d - 1);
-                if (d < 32) all |= d >= 0 ? static_cast<uint32_t>(drafts[rt] << d) : d > -64 ? static_cast<uint32_t>(drafts[rt] >> -d) : 0u;
-                bits[rt] = (all & bits_to(n - 1 - k0)) >> (4 * g);
-#pragma unroll
-                for (int h = 0; h < 2; h++)
-#pragma unroll
-                    for (int e = 0; e < 4; e++)
-                        if (!(bits[rt] >> (16 * h + e) & 1u)) x[rt][h][e] = -INFINITY;
+                    x[rt][h][e] = __builtin_fmaf(s[rt][e] * step, st[rt].unit, __builtin_fmaf(least, st[rt].qsum, st[rt].shift));
             }
         }
         v4u weights[RT];
 #pragma unroll
         for (int rt = 0; rt < RT; rt++) {
             Rows4<U>& r = st[rt];
-            float mx = x[rt][0][0];
+            uint32_t bits = ~0u;
+            if constexpr (kMasked) {
+                const int row = row0 + 16 * rt + col, token = udiv_magic(min(row, rows - 1), a.mg_group);
+                const unsigned long long drafts =
+                    a.tree ? static_cast<unsigned long long>(a.tree[static_cast<size_t>(b) * a.T + token]) : ~0ull >> (63 - token);
+                const int d = open - k0;                             // bits below d: the cache; from d on: drafts
+                bits = bits_to(d - 1);
+                if (d < 32) bits |= d >= 0 ? static_cast<uint32_t>(drafts << d) : d > -64 ? static_cast<uint32_t>(drafts >> -d) : 0u;
+                bits = (bits & bits_to(n - 1 - k0)) >> (4 * g);
+            }
+            auto on = [&](int h, int e) { return (bits >> (16 * h + e) & 1u) != 0u; };
+            float mx = -INFINITY;
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
-                for (int e = 0; e < 4; e++) mx = fmaxf(mx, x[rt][h][e]);
+                for (int e = 0; e < 4; e++) {
+                    if (kMasked && !on(h, e)) x[rt][h][e] = -INFINITY;
+                    mx = fmaxf(mx, x[rt][h][e]);
+                }
             if (__any(mx > r.limit)) {                               // a maximum that has grown
-                const float was = r.m;
-                r.m = fmaxf(was, column_max(mx));
-                r.limit = r.m + kRescale;
-                r.shift = -(r.m + low);
-                const float down = __builtin_amdgcn_exp2f(was - r.m);
+                const float most = column_max(mx);
+                const bool grown = most > r.limit, none = r.limit == -FLT_MAX;
+                const float to = grown ? r.shift - (most + low) : r.shift, d = to - r.shift;
+                const float down = none ? 1.0f : __builtin_amdgcn_exp2f(d);
+                if (grown) r.limit = kRescale - low;
+                r.shift = to;
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) x[rt][h][e] += d;
                 r.l *= down;
                 r.c *= down;
                 r.top *= down;
-                const int to = r.top > 0.0f ? max(-120, min(120, 5 - __builtin_amdgcn_frexp_expf(r.top))) : 120;
-                const float by = ldexpf(down, to - r.e);
-                r.e = to;
-                r.f = ldexpf(1.0f, to);
-#pragma unroll
-                for (int j = 0; j < Words::kOut; j++) r.o[j] *= by;
-                r.u *= by;
+                const int e = r.top > 0.0f ? max(-120, min(120, 5 - __builtin_amdgcn_frexp_expf(r.top))) : 120;
+                r.scale(ldexpf(down, e - r.e));
+                r.e = e;
+                r.f = ldexpf(1.0f, e);
             }
             float w[2][4], wx = 0.0f;
 #pragma unroll
             for (int h = 0; h < 2; h++)
 #pragma unroll
                 for (int e = 0; e < 4; e++) {
-                    const float p = __builtin_amdgcn_exp2f(x[rt][h][e] + r.shift);
+                    const float p = __builtin_amdgcn_exp2f(x[rt][h][e]);
                     r.l += p;
-                    if (masked) {
-                        const bool on = bits[rt] >> (16 * h + e) & 1u;
-                        r.c = __builtin_fmaf(p, on ? vm[h][e] : 0.0f, r.c);
-                        w[h][e] = p * (on ? vs[h][e] : 0.0f);
-                    } else {
-                        r.c = __builtin_fmaf(p, vm[h][e], r.c);
-                        w[h][e] = p * vs[h][e];
-                    }
+                    r.c = __builtin_fmaf(p, kMasked && !on(h, e) ? 0.0f : vm[h][e], r.c);
+                    w[h][e] = p * (kMasked && !on(h, e) ? 0.0f : vs[h][e]);
                     wx = fmaxf(wx, w[h][e]);
                 }
             if (__any(wx * r.f > 32768.0f)) {                        // weights that FP16 would not hold
                 r.top = fmaxf(r.top, column_max(wx));
-                const int to = max(-120, min(r.e, 5 - __builtin_amdgcn_frexp_expf(r.top)));
-                const float by = ldexpf(1.0f, to - r.e);
-                r.e = to;
-                r.f = ldexpf(1.0f, to);
-#pragma unroll
-                for (int j = 0; j < Words::kOut; j++) r.o[j] *= by;
-                r.u *= by;
+                const int e = max(-120, min(r.e, 5 - __builtin_amdgcn_frexp_expf(r.top)));
+                r.scale(ldexpf(1.0f, e - r.e));
+                r.e = e;
+                r.f = ldexpf(1.0f, e);
             }
 #pragma unroll
             for (int h = 0; h < 2; h++) {
@@ -312,20 +316,36 @@ __global__ __launch_bounds__(64 * RS * KS) void cache4_attention_kernel(Cache4Ar
         }
     };
 
-    const int tiles = (n + 31) / 32;
+    // The wave's tiles, every KS-th, loaded one ahead and their pages looked up two ahead: those that all rows see whole, then the others.
+    const int tiles = (n + 31) / 32, whole_tiles = max(min(open, n), 0) / 32;
+    int tile = ks;
     Block4<U> t[2][2];
-    bool there[2][2];
-    auto fetch = [&](int i, int tile) {
-        there[i][0] = load(t[i][0], 32 * tile);
-        there[i][1] = load(t[i][1], 32 * tile + 16);
-    };
-    if (ks < tiles) fetch(0, ks);
-    for (int tile = ks; tile < tiles; tile += 2 * KS) {              // one tile ahead
-        if (tile + KS < tiles) fetch(1, tile + KS);
-        take(t[0], there[0][0], there[0][1], 32 * tile);
-        if (tile + KS >= tiles) break;
-        if (tile + 2 * KS < tiles) fetch(0, tile + 2 * KS);
-        take(t[1], there[1][0], there[1][1], 32 * (tile + KS));
+    Pages next = look(tile);
+    load(t[0], tile, next);
+    next = look(tile + KS);
+    bool second = false;
+    while (tile < whole_tiles) {
+        load(t[1], tile + KS, next);
+        next = look(tile + 2 * KS);
+        take(t[0], 32 * tile, std::false_type{});
+        tile += KS;
+        second = tile >= whole_tiles;
+        if (second) break;
+        load(t[0], tile + KS, next);
+        next = look(tile + 2 * KS);
+        take(t[1], 32 * tile, std::false_type{});
+        tile += KS;
+    }
+    if (second) {
+#pragma unroll
+        for (int h = 0; h < 2; h++) t[0][h] = t[1][h];
+    }
+    for (; tile < tiles; tile += KS) {
+        load(t[1], tile + KS, next);
+        next = look(tile + 2 * KS);
+        take(t[0], 32 * tile, std::true_type{});
+#pragma unroll
+        for (int h = 0; h < 2; h++) t[0][h] = t[1][h];
     }
 
     // The KS waves of the same rows are joined in LDS, a row tile at a time.
@@ -353,7 +373,7 @@ __global__ __launch_bounds__(64 * RS * KS) void cache4_attention_kernel(Cache4Ar
                 for (int i = 0; i < 4; i++) mine[8 * w + 2 * i + (at >> 3)] = value(8 * Words::kFull + i, e, i);
             }
         }
-        if (g == 0) stat[wave * 16 + col] = v2f{r.m, l};
+        if (g == 0) stat[wave * 16 + col] = v2f{r.limit == -FLT_MAX ? kNoScore : -(r.shift + low), l};
         __syncthreads();
         const int quads = a.D / 4;
         for (int i = threadIdx.x; i < RS * 16 * quads; i += 64 * W) {
@@ -444,11 +464,13 @@ int launch_cache4(Cache4Args a, hipStream_t s) {
 
 template <class T, int U>
 int launch_cache4(const Cache4Args& a, int sets, hipStream_t s) {
-    switch (sets) {
-    case 1: return launch_cache4<T, U, 1, 1, 4>(a, s);
-    case 2: return launch_cache4<T, U, 2, 1, 4>(a, s);
-    case 4: return launch_cache4<T, U, 2, 2, 2>(a, s);
-    default: return launch_cache4<T, U, 2, 4, 1>(a, s);
+    if (sets == 1) return launch_cache4<T, U, 1, 1, 4>(a, s);
+    if constexpr (U <= 4) {
+        if (sets == 2) return launch_cache4<T, U, 2, 1, 4>(a, s);
+        return sets == 4 ? launch_cache4<T, U, 2, 2, 2>(a, s) : launch_cache4<T, U, 2, 4, 1>(a, s);
+    } else {                                                         // (two row tiles a wave do not fit the registers)
+        if (sets == 2) return launch_cache4<T, U, 1, 2, 2>(a, s);
+        return sets == 4 ? launch_cache4<T, U, 1, 4, 1>(a, s) : launch_cache4<T, U, 1, 8, 1>(a, s);
     }
 }
 
