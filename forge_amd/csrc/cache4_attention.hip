@@ -193,9 +193,11 @@ __global__ __launch_bounds__(64 * RS * KS, cache4_waves(U, RT)) void cache4_atte
 #pragma unroll
             for (int s = 0; s < Words::kSets; s++)
                 t[h].v[s] = *reinterpret_cast<const v4u*>(p + at_v + r * (16 * U) + 64 * U * g + 16 * Words::word(s, col));
-            const uint8_t* pn = pg >= 0 ? p + at_num + r * 8 : reinterpret_cast<const uint8_t*>(kNoNumbers);
-            t[h].num[0] = *reinterpret_cast<const v4u*>(pn + 32 * g);
-            t[h].num[1] = *reinterpret_cast<const v4u*>(pn + 32 * g + 16);
+            // (global addresses, or the choice makes flat loads, which LDS reads wait for)
+            typedef __attribute__((address_space(1))) const v4u* Numbers;
+            const Numbers pn = pg >= 0 ? (Numbers)(p + at_num + r * 8) : (Numbers)kNoNumbers;
+            t[h].num[0] = pn[2 * g];
+            t[h].num[1] = pn[2 * g + 1];
         }
     };
 
