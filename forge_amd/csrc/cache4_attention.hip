@@ -409,14 +409,17 @@ __global__ __launch_bounds__(64 * RS * KS, cache4_waves(U, RT)) void cache4_atte
 template <int U, int RS, int KS>
 constexpr int kCache4Lds = RS * KS * 16 * (Words4<U>::kRow * 4 + 8);
 
-// Rows of a workgroup: 16, 32, 64 or 128.
+// Rows of a workgroup: 16, 32, 64 or 128. Chunks such that sequences of the table's length make two workgroups per CU, or three of 64 and
+// 128 rows, which lengths that differ leave to few CUs, of as many keys as there are rows at least (a chunk's sums are as large as its keys
+// and values in 16 bits then) and of 256. us: 6 trees of 16 drafts, 32 / 4 heads of 128, over 32768, 28001, 16384, 9999, 31000 and 517, with chunks of 512 91, 1024
+// 77, 1536 96, 2048 118; one token over 16 sequences of up to 32768, 1024 67, 2048 62; one over 1000, 128 10.9, 256 9.3.
 CachePlan cache4_plan(int B, int T, int Hq, int Hkv, long long max_keys) {
     CachePlan p;
     const int rows = T * (Hq / Hkv);
     for (p.sets = 1; 16 * p.sets < rows && p.sets < 8;) p.sets *= 2;
     const long long heads = static_cast<long long>(B) * Hkv * divup(rows, 16 * p.sets);
-    const long long want = std::max<long long>(1, divupll(2 * default_cu_count(), heads));
-    const long long chunk = divupll(std::max<long long>(divupll(max_keys, want), rows), 128) * 128;
+    const long long want = std::max<long long>(1, divupll((p.sets >= 4 ? 3 : 2) * default_cu_count(), heads));
+    const long long chunk = divupll(std::max<long long>({divupll(max_keys, want), rows, 256}), 128) * 128;
     const long long most = std::max<long long>(kCacheMaxChunk, divupll(divupll(max_keys, kGridRows), 128) * 128);
     p.chunk = static_cast<int>(std::min(chunk, most));
     p.chunks = static_cast<int>(std::max<long long>(1, divupll(max_keys, p.chunk)));

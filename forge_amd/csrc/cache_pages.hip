@@ -7,7 +7,7 @@
 // whose order does not matter; everything else is in the rows' order.
 //
 // Bound: latency at few rows; two launches. First, a workgroup looks at the rows (first children, places among the takers) while others
-// copy the counts and count free pages, a thousand each; then a workgroup per row finds its page and writes its table. copy_pages: memory.
+// copy the counts and list the free pages of 1024 pages each; then a workgroup per row finds its page and writes its table. copy_pages: memory.
 #include "common.h"
 
 #include <algorithm>
@@ -16,18 +16,24 @@
 namespace forge_amd {
 
 constexpr int kForkRows = 8192;      // rows that one workgroup looks at (first children in LDS)
-constexpr int kForkThreads = 256;
-constexpr int kForkPart = 1024;      // pages whose free ones are counted together
+constexpr int kForkThreads = 1024, kTableThreads = 256;
+constexpr int kForkPart = 1024;      // pages whose free ones are listed together
 
+struct ForkRow {
+    int parent, len, last;   // parent: -1 none; last: its page of the next token, or -1
+    int rank;                // the row's place among those that take a page, or -1
+};
 struct ForkArgs {
     const int32_t *table, *lens, *parents, *refs;
     int32_t *table_out, *lens_out, *refs_out, *slots, *src, *dst;
-    int32_t *rank, *free;   // a row's place among those that take a page, or -1; free pages of a part
+    ForkRow* row;
+    int32_t *counts, *free;  // free pages of each part, and their numbers (kForkPart places a part)
     int rows, group, width, pages, page_shift;
 };
 
-// Sum over the threads before this one, and over all (in *all), of a workgroup of 256.
-__device__ __forceinline__ int sum_before(int x, int* all, int (&part)[4]) {
+// Sum over the threads before this one, and over all (in *all), of a workgroup of N.
+template <int N>
+__device__ __forceinline__ int sum_before(int x, int* all, int (&part)[N / kWave]) {
     const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
     int s = x;
 #pragma unroll
@@ -39,134 +45,105 @@ __device__ __forceinline__ int sum_before(int x, int* all, int (&part)[4]) {
     if (lane == kWave - 1) part[wave] = s;
     __syncthreads();
     int before = s - x;
+    *all = 0;
 #pragma unroll
-    for (int w = 0; w < 4; w++) before += w < wave ? part[w] : 0;
-    *all = part[0] + part[1] + part[2] + part[3];
+    for (int w = 0; w < N / kWave; w++) {
+        before += w < wave ? part[w] : 0;
+        *all += part[w];
+    }
     return before;
-}
-
-__device__ __forceinline__ int fork_parent(const ForkArgs& a, int r) {
-    const int p = a.parents[r];
-    return p >= 0 && p < a.group ? r - r % a.group + p : -1;
-}
-__device__ __forceinline__ int fork_len(const ForkArgs& a, int p) {
-    const long long cap = static_cast<long long>(a.width) << a.page_shift;
-    return p < 0 ? 0 : static_cast<int>(min(static_cast<long long>(max(a.lens[p], 0)), cap));
-}
-// The parent's page of the next token, or -1.
-__device__ __forceinline__ int fork_last(const ForkArgs& a, int p, int at) {
-    const int pg = at < a.width ? a.table[static_cast<size_t>(p) * a.width + at] : -1;
-    return pg >= 0 && pg < a.pages ? pg : -1;
 }
 
 __global__ __launch_bounds__(kForkThreads) void fork_rows_kernel(ForkArgs a)
 {
-    __shared__ int part[4];
+    __shared__ int part[kForkThreads / kWave];
+    const int tid = threadIdx.x;
+    int all;
     if (blockIdx.x > 0) {                                            // a part of the counts
-        const int at = (blockIdx.x - 1) * kForkPart + threadIdx.x;
-        int n = 0, all;
-#pragma unroll
-        for (int i = 0; i < kForkPart / kForkThreads; i++) {
-            const int pg = at + i * kForkThreads;
-            if (pg >= a.pages) continue;
-            const int x = a.refs[pg];
-            a.refs_out[pg] = x;
-            n += x == 0;
-        }
-        sum_before(n, &all, part);
-        if (threadIdx.x == 0) a.free[blockIdx.x - 1] = all;
+        const int which = blockIdx.x - 1, pg = which * kForkPart + tid;
+        const int x = pg < a.pages ? a.refs[pg] : 1;
+        if (pg < a.pages) a.refs_out[pg] = x;
+        const int before = sum_before<kForkThreads>(x == 0, &all, part);
+        if (x == 0) a.free[which * kForkPart + before] = pg;
+        if (tid == 0) a.counts[which] = all;
         return;
     }
     extern __shared__ int first[];                                   // a row's first child
-    for (int r = threadIdx.x; r < a.rows; r += kForkThreads) first[r] = a.rows;
+    for (int r = tid; r < a.rows; r += kForkThreads) first[r] = a.rows;
     __syncthreads();
-    for (int r = threadIdx.x; r < a.rows; r += kForkThreads) {
-        const int p = fork_parent(a, r);
+    auto parent_of = [&](int r) {
+        const int p = a.parents[r];
+        return p >= 0 && p < a.group ? r - r % a.group + p : -1;
+    };
+    for (int r = tid; r < a.rows; r += kForkThreads) {
+        const int p = parent_of(r);
         if (p >= 0) atomicMin(&first[p], r);
     }
     __syncthreads();
+    const int cap = a.width << a.page_shift;
     int base = 0;
     for (int r0 = 0; r0 < a.rows; r0 += kForkThreads) {
-        const int r = r0 + threadIdx.x;
+        const int r = r0 + tid;
+        ForkRow row = {-1, 0, -1, -1};
         bool take = false;
-        if (r < a.rows) {
-            const int p = fork_parent(a, r), at = fork_len(a, p) >> a.page_shift;
-            if (p >= 0 && at < a.width) {
-                const int last = fork_last(a, p, at);
-                take = !(last >= 0 && first[p] == r && a.refs[last] == 1);
+        if (r < a.rows && (row.parent = parent_of(r)) >= 0) {
+            row.len = min(max(a.lens[row.parent], 0), cap);
+            const int at = row.len >> a.page_shift;
+            if (at < a.width) {
+                const int pg = a.table[static_cast<size_t>(row.parent) * a.width + at];
+                row.last = pg >= 0 && pg < a.pages ? pg : -1;
+                take = !(row.last >= 0 && first[row.parent] == r && a.refs[row.last] == 1);
             }
         }
-        int all;
-        const int before = sum_before(take ? 1 : 0, &all, part);
-        if (r < a.rows) a.rank[r] = take ? base + before : -1;
+        const int before = sum_before<kForkThreads>(take, &all, part);
+        if (take) row.rank = base + before;
+        if (r < a.rows) a.row[r] = row;
         base += all;
     }
 }
 
-__global__ __launch_bounds__(kForkThreads) void fork_table_kernel(ForkArgs a)
+__global__ __launch_bounds__(kTableThreads) void fork_table_kernel(ForkArgs a)
 {
-    __shared__ int part[4], mine;
+    __shared__ int part[kTableThreads / kWave], mine;
     const int r = blockIdx.x, tid = threadIdx.x;
-    const int p = fork_parent(a, r), len = fork_len(a, p), at = len >> a.page_shift;
-    const int rank = a.rank[r];
-    const bool room = p >= 0 && at < a.width;
-    const int last = room ? fork_last(a, p, at) : -1;
-    if (tid == 0) mine = rank < 0 ? last : -1;
-    __syncthreads();
-    if (rank >= 0) {
-        // the part of the counts, then the page in it, that has the rank-th free one
+    const ForkRow row = a.row[r];
+    const int at = row.len >> a.page_shift, p = row.parent;
+    const int32_t* from = a.table + static_cast<size_t>(max(p, 0)) * a.width;
+    const int32_t* was = a.table + static_cast<size_t>(r) * a.width;
+    int32_t* to = a.table_out + static_cast<size_t>(r) * a.width;
+    // (loaded before the search for a page)
+    const int i0 = min(tid, a.width - 1), from0 = from[i0], was0 = was[i0];
+    int page = row.rank < 0 ? row.last : -1;
+    if (row.rank >= 0) {
+        // the part that has the rank-th free page
+        if (tid == 0) mine = -1;
         const int parts = (a.pages + kForkPart - 1) / kForkPart;
-        int left = rank, which = -1;
-        for (int i0 = 0; i0 < parts && which < 0; i0 += kForkThreads) {
-            const int i = i0 + tid, x = i < parts ? a.free[i] : 0;
+        int left = row.rank;
+        for (int j = 0; j < parts; j += kTableThreads) {
+            const int x = j + tid < parts ? a.counts[j + tid] : 0;
             int all;
-            const int before = sum_before(x, &all, part);
-            if (left < all) {
-                __shared__ int found[2];
-                if (before <= left && left < before + x) {
-                    found[0] = i;
-                    found[1] = left - before;
-                }
-                __syncthreads();
-                which = found[0];
-                left = found[1];
-            } else {
-                left -= all;
-            }
-        }
-        if (which >= 0) {
-            constexpr int kPer = kForkPart / kForkThreads;
-            int n = 0, all;
-            bool is[kPer];
-#pragma unroll
-            for (int i = 0; i < kPer; i++) {
-                const int pg = which * kForkPart + tid * kPer + i;
-                is[i] = pg < a.pages && a.refs[pg] == 0;
-                n += is[i];
-            }
-            int before = sum_before(n, &all, part);
-#pragma unroll
-            for (int i = 0; i < kPer; i++) {
-                if (is[i] && before == left) mine = which * kForkPart + tid * kPer + i;
-                before += is[i];
-            }
+            const int before = sum_before<kTableThreads>(x, &all, part);
+            if (before <= left && left < before + x) mine = a.free[(j + tid) * kForkPart + left - before];
+            if (left < all) break;
+            left -= all;
         }
         __syncthreads();
+        page = mine;
     }
-    const int page = mine, in_page = len & ((1 << a.page_shift) - 1);
+    const int in_page = row.len & ((1 << a.page_shift) - 1);
     if (tid == 0) {
-        const bool copied = rank >= 0 && page >= 0 && last >= 0 && in_page > 0;
-        a.lens_out[r] = len;
+        const bool copied = row.rank >= 0 && page >= 0 && row.last >= 0 && in_page > 0;
+        a.lens_out[r] = row.len;
         a.slots[r] = page >= 0 ? (page << a.page_shift) + in_page : -1;
-        a.src[r] = copied ? last : -1;
+        a.src[r] = copied ? row.last : -1;
         a.dst[r] = copied ? page : -1;
     }
     // the old row's names go, the new row's come
-    for (int i = tid; i < a.width; i += kForkThreads) {
-        const int old = a.table[static_cast<size_t>(r) * a.width + i];
-        int pg = p >= 0 && i < at ? a.table[static_cast<size_t>(p) * a.width + i] : room && i == at ? page : -1;
+    for (int i = tid; i < a.width; i += kTableThreads) {
+        const int old = i == tid ? was0 : was[i];
+        int pg = p >= 0 && i < at ? (i == tid ? from0 : from[i]) : i == at ? page : -1;
         if (pg < 0 || pg >= a.pages) pg = -1;
-        a.table_out[static_cast<size_t>(r) * a.width + i] = pg;
+        to[i] = pg;
         if (old != pg) {
             if (old >= 0 && old < a.pages) atomicAdd(&a.refs_out[old], -1);
             if (pg >= 0) atomicAdd(&a.refs_out[pg], 1);
@@ -204,7 +181,8 @@ using namespace forge_amd;
 
 extern "C" size_t forge_fork_pages_workspace_size(int rows, int pages) {
     if (rows <= 0 || rows > kForkRows || pages <= 0) return 0;
-    return 4 * (static_cast<size_t>(rows) + divup(pages, kForkPart));
+    const size_t parts = divup(pages, kForkPart);
+    return sizeof(ForkRow) * rows + 4 * parts * (1 + kForkPart);
 }
 
 extern "C" int forge_fork_pages(const int32_t* page_table, const int32_t* cache_lens, const int32_t* parents, const int32_t* refs,
@@ -216,21 +194,23 @@ extern "C" int forge_fork_pages(const int32_t* page_table, const int32_t* cache_
     if (rows > kForkRows || group <= 0 || rows % group != 0 || table_width <= 0 || pages <= 0 || page_size <= 0 ||
         (page_size & (page_size - 1)) != 0 || static_cast<long long>(pages) * page_size > INT_MAX + 1LL ||
         static_cast<long long>(table_width) * page_size > INT_MAX || !page_table || !cache_lens || !parents || !refs || !table_out ||
-        !lens_out || !refs_out || !slots || !src || !dst || !workspace || !aligned(workspace, 4) ||
+        !lens_out || !refs_out || !slots || !src || !dst || !workspace || !aligned(workspace, 16) ||
         workspace_bytes < forge_fork_pages_workspace_size(rows, pages))
         return FORGE_EINVAL;
     // the second launch reads what the outputs would overwrite
     const size_t table = static_cast<size_t>(rows) * table_width;
     if (overlap(page_table, table, table_out, table) || overlap(refs, pages, refs_out, pages) || overlap(cache_lens, rows, lens_out, rows))
         return FORGE_EINVAL;
-    int32_t* rank = static_cast<int32_t*>(workspace);
-    const ForkArgs a{page_table, cache_lens, parents, refs, table_out, lens_out, refs_out, slots, src, dst, rank, rank + rows,
+    const int parts = divup(pages, kForkPart);
+    ForkRow* row = static_cast<ForkRow*>(workspace);
+    int32_t* counts = reinterpret_cast<int32_t*>(row + rows);
+    const ForkArgs a{page_table, cache_lens, parents, refs, table_out, lens_out, refs_out, slots, src, dst, row, counts, counts + parts,
                      rows, group, table_width, pages, __builtin_ctz(static_cast<unsigned>(page_size))};
     hipStream_t s = as_stream(stream);
-    fork_rows_kernel<<<static_cast<unsigned>(1 + divup(pages, kForkPart)), kForkThreads, 4 * rows, s>>>(a);
+    fork_rows_kernel<<<static_cast<unsigned>(1 + parts), kForkThreads, 4 * rows, s>>>(a);
     const int st = launch_status();
     if (st != FORGE_OK) return st;
-    fork_table_kernel<<<static_cast<unsigned>(rows), kForkThreads, 0, s>>>(a);
+    fork_table_kernel<<<static_cast<unsigned>(rows), kTableThreads, 0, s>>>(a);
     return launch_status();
 }
 

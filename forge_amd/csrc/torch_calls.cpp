@@ -8,6 +8,7 @@
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
+#include <ATen/ops/empty.h>
 #include <torch/csrc/autograd/python_variable.h>
 
 #include "forge_amd.h"
@@ -287,30 +288,66 @@ PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// A call of fork_pages: its inputs in a[0..3] and the page size, checked.
+struct Fork {
+    const at::Tensor *table, *lens, *parents, *refs;
+    int64_t rows, width, group, pages;
+    long page;
+    bool take(const Call& c, PyObject* page_size) {
+        table = tensor(c.a[0]); lens = tensor(c.a[1]); parents = tensor(c.a[2]); refs = tensor(c.a[3]);
+        if (!table || table->dim() != 2 || !parents || parents->dim() != 2 || !refs || refs->dim() != 1 || !PyLong_CheckExact(page_size)) return false;
+        rows = table->size(0); width = table->size(1); group = parents->size(1); pages = refs->size(0);
+        page = PyLong_AsLong(page_size);
+        return !PyErr_Occurred() && page >= 1 && page <= INT32_MAX && rows >= 1 && rows <= INT32_MAX && width >= 1 && width <= INT32_MAX &&
+               pages >= 1 && pages <= INT32_MAX && group >= 1 && parents->size(0) * group == rows && dense(table, at::kInt, c.device, {rows, width}) &&
+               dense(lens, at::kInt, c.device, {rows}) && dense(refs, at::kInt, c.device, {pages}) &&
+               dense(parents, at::kInt, c.device, {parents->size(0), group});
+    }
+    long run(const Call& c, const at::Tensor* const (&o)[6], const at::Tensor& ws) const {
+        auto p = [](const at::Tensor* t) { return at_<int32_t>(t); };
+        return forge_fork_pages(p(table), p(lens), p(parents), p(refs), p(o[0]), p(o[1]), p(o[2]), p(o[3]), p(o[4]), p(o[5]),
+                                static_cast<int>(rows), static_cast<int>(group), static_cast<int>(width), static_cast<int>(pages),
+                                static_cast<int>(page), at_<void>(ws), static_cast<size_t>(ws.numel()), c.stream);
+    }
+};
+
 // fork_pages(page_table, cache_lens, parents, refs, table, lens, refs, slots, src, dst, workspace, page_size, device, stream)
 PyObject* fork_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return call<14>(args, n, [](const Call& c) -> long {
-        const at::Tensor* t[11];
-        for (int i = 0; i < 11; i++)
-            if (!(t[i] = tensor(c.a[i]))) return kNotInOrder;
-        if (t[0]->dim() != 2 || t[2]->dim() != 2 || t[3]->dim() != 1 || !PyLong_CheckExact(c.a[11])) return kNotInOrder;
-        const int64_t rows = t[0]->size(0), width = t[0]->size(1), group = t[2]->size(1), pages = t[3]->size(0);
-        const long page = PyLong_AsLong(c.a[11]);
-        if (PyErr_Occurred() || page < 1 || page > INT32_MAX || rows < 1 || rows > INT32_MAX || width > INT32_MAX || pages > INT32_MAX || group < 1 ||
-            t[2]->size(0) * group != rows || !on(t[10], at::kByte, c.device) || !t[10]->is_contiguous())
-            return kNotInOrder;
-        for (int i : {0, 4})
-            if (!dense(t[i], at::kInt, c.device, {rows, width})) return kNotInOrder;
-        for (int i : {1, 5, 7, 8, 9})
-            if (!dense(t[i], at::kInt, c.device, {rows})) return kNotInOrder;
-        for (int i : {3, 6})
-            if (!dense(t[i], at::kInt, c.device, {pages})) return kNotInOrder;
-        if (!dense(t[2], at::kInt, c.device, {t[2]->size(0), group})) return kNotInOrder;
-        auto p = [&](int i) { return at_<int32_t>(t[i]); };
-        return forge_fork_pages(p(0), p(1), p(2), p(3), p(4), p(5), p(6), p(7), p(8), p(9), static_cast<int>(rows),
-                                static_cast<int>(group), static_cast<int>(width), static_cast<int>(pages), static_cast<int>(page),
-                                at_<void>(t[10]), static_cast<size_t>(t[10]->numel()), c.stream);
+        Fork f;
+        const at::Tensor *o[6], *ws = tensor(c.a[10]);
+        if (!f.take(c, c.a[11]) || !on(ws, at::kByte, c.device) || !ws->is_contiguous()) return kNotInOrder;
+        for (int i = 0; i < 6; i++) o[i] = tensor(c.a[4 + i]);
+        if (!dense(o[0], at::kInt, c.device, {f.rows, f.width}) || !dense(o[2], at::kInt, c.device, {f.pages})) return kNotInOrder;
+        for (int i : {1, 3, 4, 5})
+            if (!dense(o[i], at::kInt, c.device, {f.rows})) return kNotInOrder;
+        return f.run(c, o, *ws);
     });
+}
+
+// fork_pages_new(page_table, cache_lens, parents, refs, page_size, device, stream): the outputs, or a status
+PyObject* fork_pages_new(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    at::Tensor made[6];
+    PyObject* status = call<7>(args, n, [&](const Call& c) -> long {
+        Fork f;
+        if (!f.take(c, c.a[4]) || f.rows > INT32_MAX || f.pages > INT32_MAX) return kNotInOrder;
+        const size_t size = forge_fork_pages_workspace_size(static_cast<int>(f.rows), static_cast<int>(f.pages));
+        if (size == 0) return kNotInOrder;
+        const auto ints = f.table->options();
+        made[0] = at::empty({f.rows, f.width}, ints);
+        made[2] = at::empty({f.pages}, ints);
+        for (int i : {1, 3, 4, 5}) made[i] = at::empty({f.rows}, ints);
+        const at::Tensor ws = at::empty({static_cast<int64_t>(size)}, ints.dtype(at::kByte));
+        const at::Tensor* o[6];
+        for (int i = 0; i < 6; i++) o[i] = &made[i];
+        return f.run(c, o, ws);
+    });
+    if (!status || PyLong_AsLong(status) != 0) return status;
+    PyObject* tuple = PyTuple_New(6);
+    if (!tuple) return nullptr;
+    Py_DECREF(status);
+    for (int i = 0; i < 6; i++) PyTuple_SET_ITEM(tuple, i, THPVariable_Wrap(std::move(made[i])));
+    return tuple;
 }
 
 // copy_pages(caches, src, dst, device, stream)
@@ -345,7 +382,7 @@ PyObject* copy_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
 #define FASTCALL(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FASTCALL(int4_linear), FASTCALL(qk_norm_rope), FASTCALL(prompt_attention), FASTCALL(cache_attention),
                          FASTCALL(cache4_write), FASTCALL(cache4_read), FASTCALL(cache4_attention), FASTCALL(beam_select),
-                         FASTCALL(fork_pages), FASTCALL(copy_pages),
+                         FASTCALL(fork_pages), FASTCALL(fork_pages_new), FASTCALL(copy_pages),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "forge_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -551,6 +551,23 @@ def _fast(name: str, *args) -> bool:
     return False
 
 
+def _fast_new(name: str, *args) -> Optional[tuple]:
+    """The tensors that a compiled call made and filled, or None if it was not made; raises as _fast does."""
+    global _calls
+    if _calls is None:
+        _calls = _lib.calls()
+    try:
+        dev = _device()
+    except RuntimeError:
+        return None
+    made = getattr(_calls, name)(*args, dev, _raw_stream(dev))
+    if isinstance(made, tuple):
+        return made
+    if made > 0:
+        _lib_check(made, name)
+    return None
+
+
 def _act_type(t: torch.Tensor, name: str) -> int:
     if not isinstance(t, torch.Tensor):
         raise TypeError(f"{name} must be a torch.Tensor")
@@ -1065,7 +1082,11 @@ def fork_pages(page_table: torch.Tensor, cache_lens: torch.Tensor, parents: torc
     (requests, rows of each) holds their numbers within the request (anything else ends the row), as beam_select returns them. Full
     pages are shared (refs (pages,) counts their names), a page in use is the first child's and copied for the others, and every row has a page for
     its next token. All int32; the outputs are not the inputs."""
-    if out is not None and workspace is not None and isinstance(out, tuple) and len(out) == 6:
+    if out is None and workspace is None:
+        made = _fast_new("fork_pages_new", page_table, cache_lens, parents, refs, page_size)
+        if made is not None:
+            return Forked._make(made)
+    elif out is not None and workspace is not None and isinstance(out, tuple) and len(out) == 6:
         if _fast("fork_pages", page_table, cache_lens, parents, refs, *out, workspace, page_size):
             return out
     for t, name, dims in ((page_table, "page_table", 2), (cache_lens, "cache_lens", 1), (parents, "parents", 2), (refs, "refs", 1)):
@@ -1088,8 +1109,8 @@ def fork_pages(page_table: torch.Tensor, cache_lens: torch.Tensor, parents: torc
         workspace = torch.empty((size,), dtype=torch.uint8, device=page_table.device)
     else:
         _need(workspace, torch.uint8, "workspace", size)
-        if workspace.data_ptr() % 4:
-            raise ValueError("workspace must be 4-byte aligned")
+        if workspace.data_ptr() % 16:
+            raise ValueError("workspace must be 16-byte aligned")
     shapes = ((rows, width), (rows,), (pages,), (rows,), (rows,), (rows,))
     if out is None:
         out = Forked(*(torch.empty(s, dtype=torch.int32, device=page_table.device) for s in shapes))

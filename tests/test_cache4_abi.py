@@ -80,7 +80,7 @@ def test_beam_select(lib):
 def test_fork_and_copy(lib):
     import torch
     size = lib.forge_fork_pages_workspace_size(6, 5000)
-    assert size == 4 * (6 + 5) and lib.forge_fork_pages_workspace_size(8193, 10) == 0
+    assert size == 16 * 6 + 4 * 5 * 1025 and lib.forge_fork_pages_workspace_size(8193, 10) == 0
     at = [ctypes.c_void_p(1 << 20 | i << 16) for i in range(10)]
     a = dict(table=at[0], lens=at[1], parents=at[2], refs=at[3], table_out=at[4], lens_out=at[5], refs_out=at[6], slots=at[7], src=at[8],
              dst=at[9], rows=6, group=3, width=40, pages=5000, page=16, ws=FAKE, bytes=size, stream=None)

@@ -265,7 +265,7 @@ def test_refusals(dev):
         ops.fork_pages(t[0].cpu(), *t[1:], 4)
     out = ops.fork_pages(*t, 4)
     from forge_amd import _lib
-    ws = torch.empty(64, dtype=torch.uint8, device=dev)
+    ws = torch.empty(ops.fork_pages_workspace_size(2, 4), dtype=torch.uint8, device=dev)
     for same in (out._replace(table=t[0]), out._replace(refs=t[3])):
         with pytest.raises(_lib.ForgeError):
             ops.fork_pages(*t, 4, workspace=ws, out=same)
