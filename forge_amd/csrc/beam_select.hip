@@ -241,11 +241,15 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a)
     __shared__ double group[kWaves][kWave];
     __shared__ BeamCandidate found[kBeamRoom];
     __shared__ BeamCandidate part[kWaves];
+    __shared__ int queue[kBeamRoom];
     __shared__ double bound_of;
-    __shared__ int total;
+    __shared__ int total, waiting;
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
     const size_t row0 = static_cast<size_t>(blockIdx.x) * a.W;
-    const int lists = a.W * a.splits;
+    const int lists = a.W * a.splits, deep = max(1, min(a.count, kMergeThreads / lists));
+    const BeamEntry* entries = a.entries + row0 * a.splits * a.count;
+    BeamEntry mine = {0.0f, -1};                                     // (loaded before the sums)
+    if (tid < lists * deep) mine = entries[static_cast<size_t>(tid / deep) * a.count + tid % deep];
     for (int w = wave; w < a.W; w += kWaves) {
         const size_t row = row0 + w;
         const bool ended = a.ended && a.ended[row];
@@ -263,27 +267,28 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a)
         const bool live = ended || (sum > 0.0 && sum < INFINITY && top < INFINITY);
         if (lane == 0) shift[w] = live && fabs(score) < INFINITY ? (ended ? score : score - (top + log(sum))) : -INFINITY;
     }
-    if (tid == 0) total = 0;
+    if (tid == 0) total = waiting = 0;
     __syncthreads();
     auto beam_of = [&](int list) { return static_cast<int>(static_cast<unsigned>(list) / static_cast<unsigned>(a.splits)); };
     auto place_of = [](int w, int token) { return static_cast<unsigned long long>(w) << 32 | static_cast<uint32_t>(token); };
     auto ended = [&](int w) { return a.ended && a.ended[row0 + w]; };
-    const BeamEntry* entries = a.entries + row0 * a.splits * a.count;
-    auto candidate = [&](int list, int depth) -> BeamCandidate {
+    // (the lists of a beam that has ended or has no candidates hold anything)
+    auto score_of = [&](int list, const BeamEntry& e) -> double {
         const int w = beam_of(list);
-        if (shift[w] == -INFINITY || ended(w)) return {-INFINITY, ~0ull};
+        return shift[w] == -INFINITY || ended(w) || e.token < 0 ? -INFINITY : e.logit + shift[w];
+    };
+    auto candidate = [&](int list, int depth) -> BeamCandidate {
         const BeamEntry e = entries[static_cast<size_t>(list) * a.count + depth];
-        return e.token < 0 ? BeamCandidate{-INFINITY, ~0ull} : BeamCandidate{e.logit + shift[w], place_of(w, e.token)};
+        return {score_of(list, e), place_of(beam_of(list), e.token)};
     };
     auto own = [&](int w) -> BeamCandidate {                         // of a beam that has ended
         return ended(w) ? BeamCandidate{shift[w], place_of(w, a.end_token)} : BeamCandidate{-INFINITY, ~0ull};
     };
-    // The bound: from all lists' first entries, or from 64 of the first ones of fewer lists.
-    const int heads = lists >= kWave ? lists : min(kWave, lists * a.count);
+    // The bound: from each list's first entries, as many as threads allow, neighbours in different groups.
     double best = -INFINITY;
-    for (int i = tid; i < heads; i += kMergeThreads) {
-        const int depth = i / lists;
-        best = fmax(best, candidate(i - depth * lists, depth).score);
+    for (int i = tid; i < lists * deep; i += kMergeThreads) {
+        const int list = i / deep;
+        best = fmax(best, score_of(list, i == tid ? mine : entries[static_cast<size_t>(list) * a.count + i - list * deep]));
     }
     group[wave][lane] = best;
     __syncthreads();
@@ -299,12 +304,27 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a)
         const int at = atomicAdd(&total, 1);
         if (at < kBeamRoom) found[at] = c;
     };
-    for (int list = tid; list < lists; list += kMergeThreads)
+    // lists whose first entry reaches the bound (few), then all their entries at once: entry by entry, one list's 16 took 9 us
+    for (int list = tid; list < lists; list += kMergeThreads) {
+        if (!(candidate(list, 0).score >= bound)) continue;
+        const int at = atomicAdd(&waiting, 1);
+        if (at < kBeamRoom) {
+            queue[at] = list;
+            continue;
+        }
         for (int depth = 0; depth < a.count; depth++) {
             const BeamCandidate c = candidate(list, depth);
             if (!(c.score >= bound)) break;
             gather(c);
         }
+    }
+    __syncthreads();
+    const int queued = min(waiting, kBeamRoom) * a.count;
+    for (int i = tid; i < queued; i += kMergeThreads) {
+        const int q = i / a.count;
+        const BeamCandidate c = candidate(queue[q], i - q * a.count);
+        if (c.score >= bound) gather(c);
+    }
     if (a.ended)
         for (int w = tid; w < a.W; w += kMergeThreads) {
             const BeamCandidate c = own(w);
