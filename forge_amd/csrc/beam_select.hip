@@ -85,12 +85,15 @@ __device__ __forceinline__ double lane_value(double x, int lane) {
     return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
 }
 
-// The nth largest (from 0) of a wave's 64 numbers: the smallest of those that n or fewer are above.
+// The nth largest (from 0) of a wave's 64 numbers: the one that n are above, or, among equal ones, the smallest of those that n or fewer
+// are above.
 template <class F>
 __device__ __forceinline__ F wave_nth(F x, int n) {
     int above = 0;
 #pragma unroll
     for (int l = 0; l < kWave; l++) above += lane_value(x, l) > x;
+    const unsigned long long at = __ballot(above == n);
+    if (at) return lane_value(x, __builtin_ctzll(at));
     F least = above <= n ? x : static_cast<F>(INFINITY);
 #pragma unroll
     for (int o = 1; o < kWave; o <<= 1) {

@@ -3,11 +3,9 @@
 // Per head: m = min x, s = (max / 15 - min / 15 in FP32) rounded toward zero to the 16-bit type, so that no m + s n
 // passes its largest value, and n = round_half_even((x - m) / s), at most 15 (0 where s is 0). A head that holds an infinity or NaN has none of
 // that: its s and m are NaN, and so is what reads it. Read: m + s n in FP32, rounded once.
-// Bound: memory; a lane has a word of 8 values, a wave one head of some neighbouring tokens, whose words of the values
-// (4 bytes every 16) then make whole cache lines.
+// Bound: memory; a lane has a word of 8 values of a key and its value, a workgroup one head of 8, 16 or 32 neighbouring tokens, whose words and
+// numbers then make whole cache lines.
 #include "cache4.h"
-
-#include <algorithm>
 
 namespace forge_amd {
 
@@ -34,88 +32,129 @@ __device__ __forceinline__ long long store4_slot(const Store4Args& a, int t) {
     return s < a.rows ? s : -1;
 }
 
+// A reduction over the LPH lanes of a head, in registers: neighbours, pairs, then mirrored halves of 8 and 16 lanes.
+template <int CTRL>
+__device__ __forceinline__ float lane_move(float x) {
+    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, false));
+}
+template <int LPH, class F>
+__device__ __forceinline__ float head_reduce(float x, const F& f) {
+    x = f(x, lane_move<0xB1>(x));
+    x = f(x, lane_move<0x4E>(x));
+    x = f(x, lane_move<0x141>(x));
+    if (LPH >= 16) x = f(x, lane_move<0x140>(x));
+    if (LPH >= 32) {
+        const v2u r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+        x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    }
+    return x;
+}
+
+// A head's 8 values of this lane: its word, and (on all lanes) step and lowest value.
 template <class T, int LPH>
-__global__ __launch_bounds__(256) void cache4_write_kernel(Store4Args a)
-{
-    const int lane = threadIdx.x & (kWave - 1), lh = lane & (LPH - 1), d0 = 8 * lh;
-    const int t = blockIdx.x * (kWave / LPH) + lane / LPH;
-    const int h = blockIdx.y * 4 + threadIdx.x / kWave;              // keys' heads, then values'
-    if (h >= 2 * a.at.Hkv) return;
-    const bool is_v = h >= a.at.Hkv;
-    const int hk = is_v ? h - a.at.Hkv : h;
-    const long long slot = store4_slot(a, t);
-    const bool in = slot >= 0 && d0 < a.D;
-    v4u own = {0u, 0u, 0u, 0u};
-    if (in) own = *reinterpret_cast<const v4u*>((is_v ? a.v + t * a.v_token + hk * a.v_head : a.k + t * a.k_token + hk * a.k_head) + d0);
+__device__ __forceinline__ uint32_t quantize_head(v4u own, bool in, uint32_t* numbers) {
     float x[8];
     widen8<T>(own, x);
-    float low = INFINITY, top = -INFINITY, odd = 0.0f;
+    float low = INFINITY, top = -INFINITY;
     if (in) {
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             low = fminf(low, x[e]);
             top = fmaxf(top, x[e]);
         }
+        float odd = 0.0f;
 #pragma unroll
         for (int d = 0; d < 4; d++) odd = T::times_zero(own[d], odd);
+        if (odd != 0.0f) top = INFINITY;                             // an infinity or NaN
     }
-#pragma unroll
-    for (int o = 1; o < LPH; o <<= 1) {
-        low = fminf(low, __shfl_xor(low, o, kWave));
-        top = fmaxf(top, __shfl_xor(top, o, kWave));
-        odd += __shfl_xor(odd, o, kWave);
-    }
-    if (slot < 0 || lh >= 4 * a.at.U) return;
+    low = head_reduce<LPH>(low, [](float p, float q) { return fminf(p, q); });
+    top = head_reduce<LPH>(top, [](float p, float q) { return fmaxf(p, q); });
+    constexpr uint32_t kNaN = T::kInfinity | T::kInfinity >> 1;
+    *numbers = kNaN | kNaN << 16;
+    if (!(top < INFINITY)) return 0u;
     const uint16_t step = toward_zero<T>(top / 15.0f - low / 15.0f);
+    *numbers = step | static_cast<uint32_t>(narrow<T>(low)) << 16;
     const float s = T::widen(step) * 0.5f, m = low * 0.5f;           // halves: x - m stays in range
-    uint32_t word = 0u;
-    if (d0 < a.D && odd == 0.0f && s > 0.0f) {
+    if (!in || !(s > 0.0f)) return 0u;
+    // A product with the reciprocal is the quotient but for 2^-21 of it; only next to a half (or without a reciprocal) does it take
+    // the division to know where that rounds.
+    const float inv = __builtin_amdgcn_rcpf(s);
+    float n[8], off = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            const float n = fminf(__builtin_rintf((x[e] * 0.5f - m) / s), 15.0f);
-            word |= static_cast<uint32_t>(n) << (4 * (e >> 1) + 16 * (e & 1));
-        }
+    for (int e = 0; e < 8; e++) {
+        const float q = (x[e] * 0.5f - m) * inv;
+        n[e] = __builtin_rintf(q);
+        off = fabsf(q - n[e]) < 0.4999f ? off : 1.0f;
     }
+    if (off != 0.0f) {
+#pragma unroll
+        for (int e = 0; e < 8; e++) n[e] = __builtin_rintf((x[e] * 0.5f - m) / s);
+    }
+    uint32_t word = 0u;
+#pragma unroll
+    for (int e = 0; e < 8; e++) word |= static_cast<uint32_t>(fminf(n[e], 15.0f)) << (4 * (e >> 1) + 16 * (e & 1));
+    return word;
+}
+
+template <class T, int LPH>
+__global__ __launch_bounds__(256) void cache4_write_kernel(Store4Args a)
+{
+    const int lane = threadIdx.x & (kWave - 1), lh = lane & (LPH - 1), d0 = 8 * lh, hk = blockIdx.y;
+    const int t = (blockIdx.x * 4 + threadIdx.x / kWave) * (kWave / LPH) + lane / LPH;
+    const long long slot = store4_slot(a, t);
+    const bool in = slot >= 0 && d0 < a.D;
+    v4u k = {0u, 0u, 0u, 0u}, v = k;
+    if (in) {
+        k = *reinterpret_cast<const v4u*>(a.k + t * a.k_token + hk * a.k_head + d0);
+        v = *reinterpret_cast<const v4u*>(a.v + t * a.v_token + hk * a.v_head + d0);
+    }
+    v2u numbers;
+    uint32_t kn, vn;
+    const uint32_t kw = quantize_head<T, LPH>(k, in, &kn), vw = quantize_head<T, LPH>(v, in, &vn);
+    numbers = v2u{kn, vn};
+    if (slot < 0 || lh >= 4 * a.at.U) return;
     const int r = static_cast<int>(slot) & ((1 << a.at.page_shift) - 1);
     uint8_t* piece = a.cache + a.at.at(slot >> a.at.page_shift, hk);
-    *reinterpret_cast<uint32_t*>(piece + (is_v ? a.at.value_word(r, lh) : a.at.key_row(r) + 4 * lh)) = word;
-    if (lh == 0) {
-        const uint32_t nan = T::kInfinity | T::kInfinity >> 1;       // a quiet NaN
-        const uint32_t numbers = odd == 0.0f ? step | static_cast<uint32_t>(narrow<T>(low)) << 16 : nan | nan << 16;
-        *reinterpret_cast<uint32_t*>(piece + a.at.numbers(r) + (is_v ? 4 : 0)) = numbers;
-    }
+    *reinterpret_cast<uint32_t*>(piece + a.at.key_row(r) + 4 * lh) = kw;
+    *reinterpret_cast<uint32_t*>(piece + a.at.value_word(r, lh)) = vw;
+    if (lh == 0) *reinterpret_cast<v2u*>(piece + a.at.numbers(r)) = numbers;
+}
+
+template <class T>
+__device__ __forceinline__ v4u values_of(uint32_t word, uint32_t numbers) {
+    const float s = T::widen(static_cast<uint16_t>(numbers & 0xFFFFu)), m = T::widen(static_cast<uint16_t>(numbers >> 16));
+    float x[8];
+#pragma unroll
+    for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(static_cast<float>(word >> (4 * (e >> 1) + 16 * (e & 1)) & 15u), s, m);
+    return narrow8<T>(x);
 }
 
 template <class T, int LPH>
 __global__ __launch_bounds__(256) void cache4_read_kernel(Store4Args a)
 {
-    const int lane = threadIdx.x & (kWave - 1), lh = lane & (LPH - 1), d0 = 8 * lh;
-    const int t = blockIdx.x * (kWave / LPH) + lane / LPH;
-    const int h = blockIdx.y * 4 + threadIdx.x / kWave;
-    if (h >= 2 * a.at.Hkv || t >= a.T || d0 >= a.D) return;
-    const bool is_v = h >= a.at.Hkv;
-    const int hk = is_v ? h - a.at.Hkv : h;
+    const int lane = threadIdx.x & (kWave - 1), lh = lane & (LPH - 1), d0 = 8 * lh, hk = blockIdx.y;
+    const int t = (blockIdx.x * 4 + threadIdx.x / kWave) * (kWave / LPH) + lane / LPH;
+    if (t >= a.T || d0 >= a.D) return;
     const long long slot = store4_slot(a, t);
-    uint32_t word = 0u, numbers = 0u;                                // a slot outside the cache: zeros
+    uint32_t kw = 0u, vw = 0u;                                       // a slot outside the cache: zeros
+    v2u numbers = {0u, 0u};
     if (slot >= 0) {
         const int r = static_cast<int>(slot) & ((1 << a.at.page_shift) - 1);
         const uint8_t* piece = a.cache + a.at.at(slot >> a.at.page_shift, hk);
-        word = *reinterpret_cast<const uint32_t*>(piece + (is_v ? a.at.value_word(r, lh) : a.at.key_row(r) + 4 * lh));
-        numbers = *reinterpret_cast<const uint32_t*>(piece + a.at.numbers(r) + (is_v ? 4 : 0));
+        kw = *reinterpret_cast<const uint32_t*>(piece + a.at.key_row(r) + 4 * lh);
+        vw = *reinterpret_cast<const uint32_t*>(piece + a.at.value_word(r, lh));
+        numbers = *reinterpret_cast<const v2u*>(piece + a.at.numbers(r));
     }
-    const float s = T::widen(static_cast<uint16_t>(numbers & 0xFFFFu)), m = T::widen(static_cast<uint16_t>(numbers >> 16));
-    float x[8];
-#pragma unroll
-    for (int e = 0; e < 8; e++) x[e] = __builtin_fmaf(static_cast<float>(word >> (4 * (e >> 1) + 16 * (e & 1)) & 15u), s, m);
-    uint16_t* out = (is_v ? a.v_out : a.k_out) + (static_cast<size_t>(t) * a.at.Hkv + hk) * a.D + d0;
-    *reinterpret_cast<v4u*>(out) = narrow8<T>(x);
+    const size_t out = (static_cast<size_t>(t) * a.at.Hkv + hk) * a.D + d0;
+    *reinterpret_cast<v4u*>(a.k_out + out) = values_of<T>(kw, numbers[0]);
+    *reinterpret_cast<v4u*>(a.v_out + out) = values_of<T>(vw, numbers[1]);
 }
 
 template <class T, int LPH>
 int launch_store4(const Store4Args& a, bool write, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(divup(a.T, kWave / LPH)), static_cast<unsigned>(divup(2 * a.at.Hkv, 4)));
-    if (write) cache4_write_kernel<T, LPH><<<grid, 64 * std::min(4, 2 * a.at.Hkv), 0, s>>>(a);
-    else cache4_read_kernel<T, LPH><<<grid, 64 * std::min(4, 2 * a.at.Hkv), 0, s>>>(a);
+    const dim3 grid(static_cast<unsigned>(divup(a.T, 4 * kWave / LPH)), static_cast<unsigned>(a.at.Hkv));
+    if (write) cache4_write_kernel<T, LPH><<<grid, 256, 0, s>>>(a);
+    else cache4_read_kernel<T, LPH><<<grid, 256, 0, s>>>(a);
     return launch_status();
 }
 
