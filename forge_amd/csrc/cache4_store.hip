@@ -7,6 +7,8 @@
 // numbers then make whole cache lines.
 #include "cache4.h"
 
+#include <climits>
+
 namespace forge_amd {
 
 struct Store4Args {
@@ -50,6 +52,15 @@ __device__ __forceinline__ float head_reduce(float x, const F& f) {
     return x;
 }
 
+// x / 15, correctly rounded: the product with the rounded reciprocal, corrected by its exact remainder, which FP32 holds for FP16's values.
+template <class T>
+__device__ __forceinline__ float fifteenth(float x) {
+    if constexpr (T::kWide) return x / 15.0f;
+    constexpr float kInv = 1.0f / 15.0f;
+    const float q = x * kInv;
+    return __builtin_fmaf(__builtin_fmaf(-15.0f, q, x), kInv, q);
+}
+
 // A head's 8 values of this lane: its word, and (on all lanes) step and lowest value.
 template <class T, int LPH>
 __device__ __forceinline__ uint32_t quantize_head(v4u own, bool in, uint32_t* numbers) {
@@ -72,37 +83,46 @@ __device__ __forceinline__ uint32_t quantize_head(v4u own, bool in, uint32_t* nu
     constexpr uint32_t kNaN = T::kInfinity | T::kInfinity >> 1;
     *numbers = kNaN | kNaN << 16;
     if (!(top < INFINITY)) return 0u;
-    const uint16_t step = toward_zero<T>(top / 15.0f - low / 15.0f);
+    const uint16_t step = toward_zero<T>(fifteenth<T>(top) - fifteenth<T>(low));
     *numbers = step | static_cast<uint32_t>(narrow<T>(low)) << 16;
     const float s = T::widen(step) * 0.5f, m = low * 0.5f;           // halves: x - m stays in range
     if (!in || !(s > 0.0f)) return 0u;
     // A product with the reciprocal is the quotient but for 2^-21 of it; only next to a half (or without a reciprocal) does it take
-    // the division to know where that rounds.
+    // the division to know where that rounds. kWhole's sum with a small number rounds it to an integer in its last bits. 16384 tokens of
+    // 8 heads of 128: eight divisions a lane 29 us, this 25.
+    constexpr float kWhole = 12582912.0f;
+    constexpr uint32_t kBits = 0x4B400000u;
     const float inv = __builtin_amdgcn_rcpf(s);
-    float n[8], off = 0.0f;
+    float n[8], off = inv < INFINITY ? 0.0f : 1.0f;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        const float q = (x[e] * 0.5f - m) * inv;
-        n[e] = __builtin_rintf(q);
-        off = fabsf(q - n[e]) < 0.4999f ? off : 1.0f;
+        const float q = fminf((x[e] * 0.5f - m) * inv, 15.0f);
+        n[e] = q + kWhole;
+        off = fmaxf(off, fabsf(q - (n[e] - kWhole)));
     }
-    if (off != 0.0f) {
+    if (__any(!(off < 0.4999f))) {
+        asm volatile("" : "+v"(n[0]));                               // (the compiler would divide in any case)
 #pragma unroll
-        for (int e = 0; e < 8; e++) n[e] = __builtin_rintf((x[e] * 0.5f - m) / s);
+        for (int e = 0; e < 8; e++) n[e] = fminf((x[e] * 0.5f - m) / s, 15.0f) + kWhole;
     }
-    uint32_t word = 0u;
+    uint32_t word = 0u, all = 0u;
 #pragma unroll
-    for (int e = 0; e < 8; e++) word |= static_cast<uint32_t>(fminf(n[e], 15.0f)) << (4 * (e >> 1) + 16 * (e & 1));
-    return word;
+    for (int e = 0; e < 8; e++) {
+        const int shift = 4 * (e >> 1) + 16 * (e & 1);
+        word += __float_as_uint(n[e]) << shift;
+        all += kBits << shift;
+    }
+    return word - all;
 }
 
 template <class T, int LPH>
 __global__ __launch_bounds__(256) void cache4_write_kernel(Store4Args a)
 {
-    const int lane = threadIdx.x & (kWave - 1), lh = lane & (LPH - 1), d0 = 8 * lh, hk = blockIdx.y;
-    const int t = (blockIdx.x * 4 + threadIdx.x / kWave) * (kWave / LPH) + lane / LPH;
+    const int lane = threadIdx.x & (kWave - 1), lh = lane & (LPH - 1), d0 = 8 * lh;
+    const unsigned part = blockIdx.x / static_cast<unsigned>(a.at.Hkv);
+    const int hk = blockIdx.x - part * a.at.Hkv, t = (part * 4 + threadIdx.x / kWave) * (kWave / LPH) + lane / LPH;
+    const bool in = t < a.T && d0 < a.D;                             // (without waiting for the slot)
     const long long slot = store4_slot(a, t);
-    const bool in = slot >= 0 && d0 < a.D;
     v4u k = {0u, 0u, 0u, 0u}, v = k;
     if (in) {
         k = *reinterpret_cast<const v4u*>(a.k + t * a.k_token + hk * a.k_head + d0);
@@ -132,8 +152,9 @@ __device__ __forceinline__ v4u values_of(uint32_t word, uint32_t numbers) {
 template <class T, int LPH>
 __global__ __launch_bounds__(256) void cache4_read_kernel(Store4Args a)
 {
-    const int lane = threadIdx.x & (kWave - 1), lh = lane & (LPH - 1), d0 = 8 * lh, hk = blockIdx.y;
-    const int t = (blockIdx.x * 4 + threadIdx.x / kWave) * (kWave / LPH) + lane / LPH;
+    const int lane = threadIdx.x & (kWave - 1), lh = lane & (LPH - 1), d0 = 8 * lh;
+    const unsigned part = blockIdx.x / static_cast<unsigned>(a.at.Hkv);
+    const int hk = blockIdx.x - part * a.at.Hkv, t = (part * 4 + threadIdx.x / kWave) * (kWave / LPH) + lane / LPH;
     if (t >= a.T || d0 >= a.D) return;
     const long long slot = store4_slot(a, t);
     uint32_t kw = 0u, vw = 0u;                                       // a slot outside the cache: zeros
@@ -152,9 +173,10 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(Store4Args a)
 
 template <class T, int LPH>
 int launch_store4(const Store4Args& a, bool write, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(divup(a.T, 4 * kWave / LPH)), static_cast<unsigned>(a.at.Hkv));
-    if (write) cache4_write_kernel<T, LPH><<<grid, 256, 0, s>>>(a);
-    else cache4_read_kernel<T, LPH><<<grid, 256, 0, s>>>(a);
+    const long long grid = static_cast<long long>(divup(a.T, 4 * kWave / LPH)) * a.at.Hkv;
+    if (grid > INT_MAX) return FORGE_EINVAL;
+    if (write) cache4_write_kernel<T, LPH><<<static_cast<unsigned>(grid), 256, 0, s>>>(a);
+    else cache4_read_kernel<T, LPH><<<static_cast<unsigned>(grid), 256, 0, s>>>(a);
     return launch_status();
 }
 
