@@ -411,7 +411,9 @@ constexpr int kCache4Lds = RS * KS * 16 * (Words4<U>::kRow * 4 + 8);
 
 // Rows of a workgroup: 16, 32, 64 or 128. Chunks such that sequences of the table's length make two workgroups per CU, or three of 64 and
 // 128 rows, which lengths that differ leave to few CUs, of as many keys as there are rows at least (a chunk's sums are as large as its keys
-// and values in 16 bits then) and of 256. us: 6 trees of 16 drafts, 32 / 4 heads of 128, over 32768, 28001, 16384, 9999, 31000 and 517, with chunks of 512 91, 1024
+// and values in 16 bits then) and of 256; and one chunk, without a join, where up to 16 rows have 512 keys, or 1024 and heads for half the CUs.
+// us, 32 / 8 heads of 128: one token over 500 keys, in one chunk and in chunks of 256, 7.2 and 8.2 (32 sequences 8.0 and 10.6); 32 over 1000, in
+// one and in two, 10.5 and 12.9 (1 over 1000 9.9 and 8.2); 6 trees of 16 drafts, 32 / 4 heads of 128, over 32768, 28001, 16384, 9999, 31000 and 517, with chunks of 512 91, 1024
 // 77, 1536 96, 2048 118; one token over 16 sequences of up to 32768, 1024 67, 2048 62; one over 1000, 128 10.9, 256 9.3.
 CachePlan cache4_plan(int B, int T, int Hq, int Hkv, long long max_keys) {
     CachePlan p;
@@ -419,7 +421,9 @@ CachePlan cache4_plan(int B, int T, int Hq, int Hkv, long long max_keys) {
     for (p.sets = 1; 16 * p.sets < rows && p.sets < 8;) p.sets *= 2;
     const long long heads = static_cast<long long>(B) * Hkv * divup(rows, 16 * p.sets);
     const long long want = std::max<long long>(1, divupll((p.sets >= 4 ? 3 : 2) * default_cu_count(), heads));
-    const long long chunk = divupll(std::max<long long>({divupll(max_keys, want), rows, 256}), 128) * 128;
+    long long least = std::max(rows, 256);
+    if (p.sets == 1) least = 2 * heads >= default_cu_count() ? 1024 : 512;
+    const long long chunk = divupll(max_keys <= least ? max_keys : std::max(divupll(max_keys, want), std::max<long long>(rows, 256)), 128) * 128;
     const long long most = std::max<long long>(kCacheMaxChunk, divupll(divupll(max_keys, kGridRows), 128) * 128);
     p.chunk = static_cast<int>(std::min(chunk, most));
     p.chunks = static_cast<int>(std::max<long long>(1, divupll(max_keys, p.chunk)));
@@ -472,7 +476,11 @@ int launch_cache4(const Cache4Args& a, int sets, hipStream_t s) {
     if (sets == 1) return launch_cache4<T, U, 1, 1, 4>(a, s);
     if constexpr (U <= 4) {
         if (sets == 2) return launch_cache4<T, U, 2, 1, 4>(a, s);
-        return sets == 4 ? launch_cache4<T, U, 2, 2, 2>(a, s) : launch_cache4<T, U, 2, 4, 1>(a, s);
+        if (sets == 4) return launch_cache4<T, U, 2, 2, 2>(a, s);
+        // twice the waves while there is a workgroup per CU at most: 4 trees of 29 drafts over 3001, 17, 0 and 2048, 14 / 2 heads of 64, 19.4 -> 16.8 us;
+        // with more of them it takes from the others: 6 trees of 16 over 119 thousand keys 77 -> 88
+        const long long groups = static_cast<long long>(a.B) * a.Hkv * divup(a.T * a.group, 128) * a.chunks;
+        return groups <= default_cu_count() ? launch_cache4<T, U, 2, 4, 2>(a, s) : launch_cache4<T, U, 2, 4, 1>(a, s);
     } else {                                                         // (two row tiles a wave do not fit the registers)
         if (sets == 2) return launch_cache4<T, U, 1, 2, 2>(a, s);
         return sets == 4 ? launch_cache4<T, U, 1, 4, 1>(a, s) : launch_cache4<T, U, 1, 8, 1>(a, s);

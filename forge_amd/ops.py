@@ -920,14 +920,12 @@ def cache4_read(cache: torch.Tensor, slots: torch.Tensor, D: int, dtype: torch.d
                 k_out: Optional[torch.Tensor] = None, v_out: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
     """forge_cache4_read: what rows `slots` (int32) of a 4-bit cache stand for, keys and values (T, Hkv, D) of the cache's type;
     zeros for slots outside it. k_out and v_out may be passed to reuse buffers."""
-    if isinstance(slots, torch.Tensor) and isinstance(cache, torch.Tensor) and slots.dim() == 1 and cache.dim() == 4:
-        shape = (slots.shape[0], cache.shape[1], D)
-        if k_out is None:
-            k_out = torch.empty(shape, dtype=dtype, device=cache.device)
-        if v_out is None:
-            v_out = torch.empty(shape, dtype=dtype, device=cache.device)
-        if k_out.dtype is dtype and _fast("cache4_read", cache, slots, k_out, v_out):
-            return k_out, v_out
+    if (k_out is None or v_out is None) and isinstance(slots, torch.Tensor) and isinstance(cache, torch.Tensor) and cache.dim() == 4:
+        shape = (slots.numel(), cache.shape[1], D)
+        k_out = torch.empty(shape, dtype=dtype, device=cache.device) if k_out is None else k_out
+        v_out = torch.empty(shape, dtype=dtype, device=cache.device) if v_out is None else v_out
+    if _fast("cache4_read", cache, slots, k_out, v_out, D, dtype):
+        return k_out, v_out
     code = _DTYPE.get(dtype)
     if code is None:
         raise TypeError(f"dtype must be torch.float16 or torch.bfloat16, got {dtype}")
