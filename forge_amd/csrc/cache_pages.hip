@@ -6,7 +6,7 @@
 // this call frees are not taken by it, so no copied page is written. Counts are added to with integer atomics,
 // whose order does not matter; everything else is in the rows' order.
 //
-// Bound: latency at few rows; two launches. First, a workgroup looks at the rows (first children, places among the takers) while others
+// Bound: latency at few rows. Small tables and pools take one workgroup that holds all counts in LDS, others two launches. First, a workgroup looks at the rows (first children, places among the takers) while others
 // copy the counts and list the free pages of 1024 pages each; then a workgroup per row finds its page and writes its table. copy_pages: memory.
 #include "common.h"
 
@@ -54,6 +54,88 @@ __device__ __forceinline__ int sum_before(int x, int* all, int (&part)[N / kWave
     return before;
 }
 
+// Row r as its parent leaves it, but for its rank.
+__device__ __forceinline__ ForkRow fork_row(const ForkArgs& a, int parent) {
+    ForkRow row = {parent, 0, -1, -1};
+    if (parent < 0) return row;
+    row.len = min(max(a.lens[parent], 0), a.width << a.page_shift);
+    const int at = row.len >> a.page_shift;
+    const int pg = at < a.width ? a.table[static_cast<size_t>(parent) * a.width + at] : -1;
+    row.last = pg >= 0 && pg < a.pages ? pg : -1;
+    return row;
+}
+__device__ __forceinline__ int fork_parent(const ForkArgs& a, int r) {
+    const int p = a.parents[r];
+    return p >= 0 && p < a.group ? r - r % a.group + p : -1;
+}
+__device__ __forceinline__ void fork_put(const ForkArgs& a, int r, const ForkRow& row, int page) {
+    const int in_page = row.len & ((1 << a.page_shift) - 1);
+    const bool copied = row.rank >= 0 && page >= 0 && row.last >= 0 && in_page > 0;
+    a.lens_out[r] = row.len;
+    a.slots[r] = page >= 0 ? (page << a.page_shift) + in_page : -1;
+    a.src[r] = copied ? row.last : -1;
+    a.dst[r] = copied ? page : -1;
+}
+
+// All of it in one workgroup. us in a graph, this and the two launches: 4 rows of 40 entries and 59 pages 4.1 and 5.3, 128 of 32 and 1061
+// 5.6 and 6.1, 128 of 128 9.8 and 6.1, 512 of 16 and 3461 8.0 and 6.5.
+constexpr int kSmallRows = 1024, kSmallPages = 2048, kSmallTable = 4096;
+__global__ __launch_bounds__(kForkThreads) void fork_small_kernel(ForkArgs a)
+{
+    __shared__ int counts[kSmallPages], first[kSmallRows], free[kSmallRows], mine[kSmallRows], up[kSmallRows], from[kSmallRows];
+    __shared__ int part[kForkThreads / kWave];
+    const int tid = threadIdx.x;
+    int p = -1, x[kSmallPages / kForkThreads], all;
+#pragma unroll
+    for (int i = 0; i < kSmallPages / kForkThreads; i++) {
+        const int pg = tid + i * kForkThreads;
+        x[i] = pg < a.pages ? a.refs[pg] : 1;
+    }
+    if (tid < a.rows) {
+        first[tid] = a.rows;
+        p = fork_parent(a, tid);
+    }
+    __syncthreads();
+    if (p >= 0) atomicMin(&first[p], tid);
+    ForkRow row = fork_row(a, p);
+    int base = 0;                                                    // the lowest free pages, one a row at most
+#pragma unroll
+    for (int i = 0; i < kSmallPages / kForkThreads; i++) {
+        const int pg = tid + i * kForkThreads;
+        counts[pg] = x[i];
+        if (i * kForkThreads >= a.pages || base >= a.rows) continue;
+        const int before = base + sum_before<kForkThreads>(x[i] == 0, &all, part);
+        if (x[i] == 0 && before < a.rows) free[before] = pg;
+        base += all;
+    }
+    __syncthreads();
+    const int at = row.len >> a.page_shift;
+    const bool take = p >= 0 && at < a.width && !(row.last >= 0 && first[p] == tid && counts[row.last] == 1);
+    const int rank = sum_before<kForkThreads>(take, &all, part);
+    if (tid < a.rows) {
+        if (take) row.rank = rank;
+        const int page = !take ? row.last : rank < base ? free[rank] : -1;
+        mine[tid] = page;
+        up[tid] = p;
+        from[tid] = at;
+        fork_put(a, tid, row, page);
+    }
+    __syncthreads();
+    for (int i = tid; i < a.rows * a.width; i += kForkThreads) {
+        const int r = static_cast<unsigned>(i) / static_cast<unsigned>(a.width), c = i - r * a.width, q = up[r];
+        const int old = a.table[i];
+        int pg = q >= 0 && c < from[r] ? a.table[q * a.width + c] : c == from[r] ? mine[r] : -1;
+        if (pg < 0 || pg >= a.pages) pg = -1;
+        a.table_out[i] = pg;
+        if (old != pg) {
+            if (old >= 0 && old < a.pages) atomicAdd(&counts[old], -1);
+            if (pg >= 0) atomicAdd(&counts[pg], 1);
+        }
+    }
+    __syncthreads();
+    for (int pg = tid; pg < a.pages; pg += kForkThreads) a.refs_out[pg] = counts[pg];
+}
+
 __global__ __launch_bounds__(kForkThreads) void fork_rows_kernel(ForkArgs a)
 {
     __shared__ int part[kForkThreads / kWave];
@@ -71,29 +153,20 @@ __global__ __launch_bounds__(kForkThreads) void fork_rows_kernel(ForkArgs a)
     extern __shared__ int first[];                                   // a row's first child
     for (int r = tid; r < a.rows; r += kForkThreads) first[r] = a.rows;
     __syncthreads();
-    auto parent_of = [&](int r) {
-        const int p = a.parents[r];
-        return p >= 0 && p < a.group ? r - r % a.group + p : -1;
-    };
     for (int r = tid; r < a.rows; r += kForkThreads) {
-        const int p = parent_of(r);
+        const int p = fork_parent(a, r);
         if (p >= 0) atomicMin(&first[p], r);
     }
     __syncthreads();
-    const int cap = a.width << a.page_shift;
     int base = 0;
     for (int r0 = 0; r0 < a.rows; r0 += kForkThreads) {
         const int r = r0 + tid;
         ForkRow row = {-1, 0, -1, -1};
         bool take = false;
-        if (r < a.rows && (row.parent = parent_of(r)) >= 0) {
-            row.len = min(max(a.lens[row.parent], 0), cap);
-            const int at = row.len >> a.page_shift;
-            if (at < a.width) {
-                const int pg = a.table[static_cast<size_t>(row.parent) * a.width + at];
-                row.last = pg >= 0 && pg < a.pages ? pg : -1;
-                take = !(row.last >= 0 && first[row.parent] == r && a.refs[row.last] == 1);
-            }
+        if (r < a.rows) {
+            row = fork_row(a, fork_parent(a, r));
+            take = row.parent >= 0 && row.len >> a.page_shift < a.width &&
+                   !(row.last >= 0 && first[row.parent] == r && a.refs[row.last] == 1);
         }
         const int before = sum_before<kForkThreads>(take, &all, part);
         if (take) row.rank = base + before;
@@ -130,14 +203,7 @@ __global__ __launch_bounds__(kTableThreads) void fork_table_kernel(ForkArgs a)
         __syncthreads();
         page = mine;
     }
-    const int in_page = row.len & ((1 << a.page_shift) - 1);
-    if (tid == 0) {
-        const bool copied = row.rank >= 0 && page >= 0 && row.last >= 0 && in_page > 0;
-        a.lens_out[r] = row.len;
-        a.slots[r] = page >= 0 ? (page << a.page_shift) + in_page : -1;
-        a.src[r] = copied ? row.last : -1;
-        a.dst[r] = copied ? page : -1;
-    }
+    if (tid == 0) fork_put(a, r, row, page);
     // the old row's names go, the new row's come
     for (int i = tid; i < a.width; i += kTableThreads) {
         const int old = i == tid ? was0 : was[i];
@@ -207,6 +273,10 @@ extern "C" int forge_fork_pages(const int32_t* page_table, const int32_t* cache_
     const ForkArgs a{page_table, cache_lens, parents, refs, table_out, lens_out, refs_out, slots, src, dst, row, counts, counts + parts,
                      rows, group, table_width, pages, __builtin_ctz(static_cast<unsigned>(page_size))};
     hipStream_t s = as_stream(stream);
+    if (rows <= kSmallRows && pages <= kSmallPages && table <= kSmallTable) {
+        fork_small_kernel<<<1, kForkThreads, 0, s>>>(a);
+        return launch_status();
+    }
     fork_rows_kernel<<<static_cast<unsigned>(1 + parts), kForkThreads, 4 * rows, s>>>(a);
     const int st = launch_status();
     if (st != FORGE_OK) return st;

@@ -87,7 +87,8 @@ def check(dev, table, lens, parents, refs, page, **more):
 
 
 @pytest.mark.parametrize("requests,group,width,page,pages", [(1, 1, 1, 1, 3), (1, 4, 5, 16, 40), (3, 5, 30, 4, 700), (64, 8, 9, 16, 6000), (2, 300, 3, 8, 2500),
-                                                            (1000, 8, 2, 32, 20000), (7, 3, 260, 2, 9001), (8192, 1, 1, 16, 9000)])
+                                                            (1000, 8, 2, 32, 20000), (7, 3, 260, 2, 9001), (8192, 1, 1, 16, 9000), (512, 2, 4, 256, 2048), (513, 2, 4, 256, 2048),
+                                                            (8, 4, 128, 1, 2048), (8, 4, 128, 1, 2049)])
 def test_sizes(dev, requests, group, width, page, pages):
     for seed in range(3):
         say(f"fork_pages {requests} x {group} width={width} page={page} pages={pages} seed={seed}")
