@@ -76,32 +76,43 @@ __device__ __forceinline__ float key_value(BeamKey k) {
     return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
 
-__device__ __forceinline__ float lane_value(float x, int lane) {
-    return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(x), lane));
-}
-__device__ __forceinline__ double lane_value(double x, int lane) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, x);
-    const uint32_t lo = __builtin_amdgcn_readlane(static_cast<int>(u), lane), hi = __builtin_amdgcn_readlane(static_cast<int>(u >> 32), lane);
-    return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo);
-}
-
-// The nth largest (from 0) of a wave's 64 numbers: the one that n are above, or, among equal ones, the smallest of those that n or fewer
-// are above.
-template <class F>
-__device__ __forceinline__ F wave_nth(F x, int n) {
-    int above = 0;
+// The nth largest (from 0) of the 64 groups' largest numbers: each thread compares one of them with some others, the first wave picks the one
+// that n are above (the smallest of those that n or fewer are above, where some are equal). All of N threads call it; part[w][l] is
+// wave w's largest of group l; the result is wave 0's.
+template <class F, int N>
+struct NthGroup {
+    F part[N / kWave][kWave], group[kWave];
+    int above[kWave];
+    __device__ __forceinline__ F nth(int n) {
+        constexpr int kWaves = N / kWave, kEach = kWave / kWaves;
+        const int lane = threadIdx.x & (kWave - 1), wave = threadIdx.x / kWave;
+        __syncthreads();
+        F x = part[0][lane];
 #pragma unroll
-    for (int l = 0; l < kWave; l++) above += lane_value(x, l) > x;
-    const unsigned long long at = __ballot(above == n);
-    if (at) return lane_value(x, __builtin_ctzll(at));
-    F least = above <= n ? x : static_cast<F>(INFINITY);
+        for (int w = 1; w < kWaves; w++) x = x > part[w][lane] ? x : part[w][lane];
+        if (wave == 0) {
+            group[lane] = x;
+            above[lane] = 0;
+        }
+        __syncthreads();
+        int count = 0;
 #pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) {
-        const F y = __shfl_xor(least, o, kWave);
-        least = y < least ? y : least;
+        for (int e = 0; e < kEach; e++) count += group[wave * kEach + e] > x;
+        atomicAdd(&above[lane], count);
+        __syncthreads();
+        if (wave != 0) return x;
+        const int all = above[lane];
+        const unsigned long long at = __ballot(all == n);
+        F least = all <= n ? x : static_cast<F>(INFINITY);
+        if (at) return __shfl(x, __builtin_ctzll(at), kWave);
+#pragma unroll
+        for (int o = 1; o < kWave; o <<= 1) {
+            const F y = __shfl_xor(least, o, kWave);
+            least = y < least ? y : least;
+        }
+        return least;
     }
-    return least;
-}
+};
 
 __device__ __forceinline__ double wave_sum(double x) {
 #pragma unroll
@@ -115,7 +126,7 @@ template <class L, int VEC>
 __global__ __launch_bounds__(kBeamThreads) void beam_piece_kernel(BeamArgs a)
 {
     constexpr int kPiece = kBeamThreads * VEC * L::kPer;
-    __shared__ float group[4][kWave];
+    __shared__ NthGroup<float, kBeamThreads> groups;
     __shared__ BeamKey found[kBeamRoom];
     __shared__ double part_sum[4];
     __shared__ float part_top[4], bound_of;
@@ -149,7 +160,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_piece_kernel(BeamArgs a)
     for (int i = 0; i < VEC; i++)
 #pragma unroll
         for (int e = 0; e < L::kPer; e++) most = fmaxf(most, L::value(v[i], e));
-    group[wave][lane] = most;
+    groups.part[wave][lane] = most;
     const float top = fmaxf(wave_max(most), -FLT_MAX);
     float sum = 0.0f;
 #pragma unroll
@@ -162,11 +173,9 @@ __global__ __launch_bounds__(kBeamThreads) void beam_piece_kernel(BeamArgs a)
         part_sum[wave] = wsum;
     }
     if (tid == 0) total = 0;
-    __syncthreads();
-    if (wave == 0) {
-        const float x = fmaxf(fmaxf(group[0][lane], group[1][lane]), fmaxf(group[2][lane], group[3][lane]));
-        const float nth = wave_nth(x, a.count - 1);
-        if (lane == 0) bound_of = fmaxf(nth, -FLT_MAX);              // -inf is no candidate
+    const float nth = groups.nth(a.count - 1);
+    if (tid == 0) {
+        bound_of = fmaxf(nth, -FLT_MAX);                             // -inf is no candidate
     } else if (tid == kWave) {
         const float m = fmaxf(fmaxf(part_top[0], part_top[1]), fmaxf(part_top[2], part_top[3]));
         double s = 0.0;
@@ -241,7 +250,7 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a)
 {
     constexpr int kWaves = kMergeThreads / kWave;
     __shared__ double shift[kBeamWidth];     // score - logsumexp, -inf for a beam without candidates
-    __shared__ double group[kWaves][kWave];
+    __shared__ NthGroup<double, kMergeThreads> groups;
     __shared__ BeamCandidate found[kBeamRoom];
     __shared__ BeamCandidate part[kWaves];
     __shared__ int queue[kBeamRoom];
@@ -287,45 +296,52 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a)
     auto own = [&](int w) -> BeamCandidate {                         // of a beam that has ended
         return ended(w) ? BeamCandidate{shift[w], place_of(w, a.end_token)} : BeamCandidate{-INFINITY, ~0ull};
     };
-    // The bound: from each list's first entries, as many as threads allow, neighbours in different groups.
-    double best = -INFINITY;
-    for (int i = tid; i < lists * deep; i += kMergeThreads) {
-        const int list = i / deep;
-        best = fmax(best, score_of(list, i == tid ? mine : entries[static_cast<size_t>(list) * a.count + i - list * deep]));
-    }
-    group[wave][lane] = best;
-    __syncthreads();
-    if (wave == 0) {
-#pragma unroll
-        for (int w = 1; w < kWaves; w++) best = fmax(best, group[w][lane]);
-        const double nth = wave_nth(best, a.count - 1);
-        if (lane == 0) bound_of = fmax(nth, -DBL_MAX);
-    }
+    // The bound: from each list's first entries, as many as there are threads for, neighbours in different groups.
+    const int list0 = tid / deep, depth0 = tid - list0 * deep;
+    const bool has = tid < lists * deep;
+    const double score0 = has ? score_of(list0, mine) : -INFINITY;
+    double best = score0;
+    for (int list = tid + kMergeThreads; list < lists; list += kMergeThreads)     // (deep is 1)
+        best = fmax(best, score_of(list, entries[static_cast<size_t>(list) * a.count]));
+    groups.part[wave][lane] = best;
+    const double nth = groups.nth(a.count - 1);
+    if (tid == 0) bound_of = fmax(nth, -DBL_MAX);
     __syncthreads();
     const double bound = bound_of;
     auto gather = [&](const BeamCandidate& c) {
         const int at = atomicAdd(&total, 1);
         if (at < kBeamRoom) found[at] = c;
     };
-    // lists whose first entry reaches the bound (few), then all their entries at once: entry by entry, one list's 16 took 9 us
-    for (int list = tid; list < lists; list += kMergeThreads) {
-        if (!(candidate(list, 0).score >= bound)) continue;
+    // What reaches the bound of those entries, and the rest of the lists (few) whose last one of them does: all their entries at once. (Entry by
+    // entry, one list's 16 took 9 us.)
+    auto rest = [&](int list) {
+        if (deep == a.count) return;
         const int at = atomicAdd(&waiting, 1);
         if (at < kBeamRoom) {
             queue[at] = list;
-            continue;
+            return;
         }
-        for (int depth = 0; depth < a.count; depth++) {
+        for (int depth = deep; depth < a.count; depth++) {
             const BeamCandidate c = candidate(list, depth);
             if (!(c.score >= bound)) break;
             gather(c);
         }
+    };
+    if (score0 >= bound) {
+        gather({score0, place_of(beam_of(list0), mine.token)});
+        if (depth0 == deep - 1) rest(list0);
+    }
+    for (int list = tid + kMergeThreads; list < lists; list += kMergeThreads) {
+        const BeamCandidate c = candidate(list, 0);
+        if (!(c.score >= bound)) continue;
+        gather(c);
+        rest(list);
     }
     __syncthreads();
-    const int queued = min(waiting, kBeamRoom) * a.count;
+    const int left = a.count - deep, queued = min(waiting, kBeamRoom) * left;
     for (int i = tid; i < queued; i += kMergeThreads) {
-        const int q = i / a.count;
-        const BeamCandidate c = candidate(queue[q], i - q * a.count);
+        const int q = i / left;
+        const BeamCandidate c = candidate(queue[q], deep + i - q * left);
         if (c.score >= bound) gather(c);
     }
     if (a.ended)
