@@ -242,52 +242,116 @@ PyObject* cache4_read(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// A call of cache4_attention: q, cache, page_table, cache_lens and tree in a[0..4], checked.
+struct Attend4 {
+    const at::Tensor *q, *cache, *table, *lens, *tree;
+    bool take(const Call& c) {
+        q = tensor(c.a[0]); cache = tensor(c.a[1]); table = tensor(c.a[2]); lens = tensor(c.a[3]); tree = nullptr;
+        if (!q || q->dim() != 4 || !cache || cache->dim() != 4 || !table || table->dim() != 2) return false;
+        const at::ScalarType type = q->scalar_type();
+        const int64_t B = q->size(0), T = q->size(1), Hq = q->size(2), D = q->size(3), Hkv = cache->size(1), width = table->size(1);
+        return code(type) >= 0 && T >= 1 && T <= 64 && D >= 1 && Hkv >= 1 && dense(q, type, c.device, {B, T, Hq, D}) && cache4(cache, c.device, Hkv, D) &&
+               dense(table, at::kInt, c.device, {B, width}) && dense(lens, at::kInt, c.device, {B}) && B <= INT32_MAX && Hq <= INT32_MAX &&
+               Hkv <= INT32_MAX && width <= INT32_MAX && (c.none(4) || dense(tree = tensor(c.a[4]), at::kLong, c.device, {B, T}));
+    }
+    long run(const Call& c, const at::Tensor& out, const at::Tensor* ws, float scale) const {
+        return forge_cache4_attention(at_<uint16_t>(q), at_<uint8_t>(cache), at_<int32_t>(table), at_<int32_t>(lens), at_<int64_t>(tree),
+                                      at_<uint16_t>(out), static_cast<int>(q->size(0)), static_cast<int>(q->size(1)), static_cast<int>(q->size(2)),
+                                      static_cast<int>(cache->size(1)), static_cast<int>(q->size(3)), static_cast<int>(cache->size(0)),
+                                      static_cast<int>(cache->size(2)), static_cast<int>(table->size(1)), scale, code(q->scalar_type()),
+                                      at_<void>(ws), ws ? ws->nbytes() : 0, c.stream);
+    }
+};
+
 // cache4_attention(q, cache, page_table, cache_lens, tree, workspace, out, scale, device, stream)
 PyObject* cache4_attention(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return call<10>(args, n, [](const Call& c) -> long {
-        const at::Tensor *q = tensor(c.a[0]), *cache = tensor(c.a[1]), *table = tensor(c.a[2]), *lens = tensor(c.a[3]);
-        const at::Tensor *tree = nullptr, *ws = nullptr, *out = tensor(c.a[6]);
-        if (!q || q->dim() != 4 || !cache || cache->dim() != 4 || !table || table->dim() != 2) return kNotInOrder;
-        const at::ScalarType type = q->scalar_type();
-        const int64_t B = q->size(0), T = q->size(1), Hq = q->size(2), D = q->size(3), Hkv = cache->size(1), width = table->size(1);
+        Attend4 f;
+        const at::Tensor *ws = nullptr, *out = tensor(c.a[6]);
         float scale;
-        if (!c.number(7, &scale)) return kNotInOrder;
-        if (code(type) < 0 || T < 1 || T > 64 || D < 1 || Hkv < 1 || !dense(q, type, c.device, {B, T, Hq, D}) || !cache4(cache, c.device, Hkv, D) ||
-            !dense(table, at::kInt, c.device, {B, width}) || !dense(lens, at::kInt, c.device, {B}) || !dense(out, type, c.device, {B, T, Hq, D}) ||
-            B > INT32_MAX || Hq > INT32_MAX || Hkv > INT32_MAX || width > INT32_MAX)
+        if (!c.number(7, &scale) || !f.take(c) || !out || !dense(out, f.q->scalar_type(), c.device, {f.q->size(0), f.q->size(1), f.q->size(2), f.q->size(3)}))
             return kNotInOrder;
-        if (!c.none(4) && !dense(tree = tensor(c.a[4]), at::kLong, c.device, {B, T})) return kNotInOrder;
         if (!c.none(5) && (!on(ws = tensor(c.a[5]), at::kByte, c.device) || !ws->is_contiguous())) return kNotInOrder;
-        return forge_cache4_attention(at_<uint16_t>(q), at_<uint8_t>(cache), at_<int32_t>(table), at_<int32_t>(lens), at_<int64_t>(tree),
-                                      at_<uint16_t>(out), static_cast<int>(B), static_cast<int>(T), static_cast<int>(Hq),
-                                      static_cast<int>(Hkv), static_cast<int>(D), static_cast<int>(cache->size(0)),
-                                      static_cast<int>(cache->size(2)), static_cast<int>(width), scale, code(type), at_<void>(ws),
-                                      ws ? static_cast<size_t>(ws->numel()) : 0, c.stream);
+        return f.run(c, *out, ws, scale);
     });
 }
+
+// The tensors that a call has made, if its status is 0.
+template <size_t N>
+PyObject* made_or(PyObject* status, at::Tensor (&made)[N]) {
+    if (!status || PyLong_AsLong(status) != 0) return status;
+    PyObject* tuple = PyTuple_New(N);
+    if (!tuple) return nullptr;
+    Py_DECREF(status);
+    for (size_t i = 0; i < N; i++) PyTuple_SET_ITEM(tuple, i, THPVariable_Wrap(std::move(made[i])));
+    return tuple;
+}
+
+// cache4_attention_new(q, cache, page_table, cache_lens, tree, scale, device, stream): the output, or a status
+PyObject* cache4_attention_new(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    at::Tensor made[1];
+    return made_or(call<8>(args, n, [&](const Call& c) -> long {
+        Attend4 f;
+        float scale;
+        if (!c.number(5, &scale) || !f.take(c) || f.q->numel() == 0) return kNotInOrder;
+        const size_t size = forge_cache4_attention_workspace_size(static_cast<int>(f.q->size(0)), static_cast<int>(f.q->size(1)),
+                                                                  static_cast<int>(f.q->size(2)), static_cast<int>(f.cache->size(1)),
+                                                                  static_cast<int>(f.q->size(3)), f.table->size(1) * f.cache->size(2));
+        made[0] = at::empty(f.q->sizes(), f.q->options());
+        at::Tensor ws;
+        if (size) ws = at::empty({static_cast<int64_t>(size)}, f.cache->options());
+        return f.run(c, made[0], size ? &ws : nullptr, scale);
+    }), made);
+}
+
+// A call of beam_select: logits, scores and ended in a[0..2], the count and the end token, checked.
+struct Beams {
+    const at::Tensor *x, *scores, *ended;
+    int64_t B, W, V;
+    long count, end;
+    int kind;
+    bool take(const Call& c, PyObject* count_of, PyObject* end_of) {
+        x = tensor(c.a[0]); scores = tensor(c.a[1]); ended = nullptr;
+        if (!x || x->dim() != 3 || !PyLong_CheckExact(count_of) || !PyLong_CheckExact(end_of)) return false;
+        const at::ScalarType type = x->scalar_type();
+        kind = type == at::kFloat ? FORGE_FP32 : code(type);
+        B = x->size(0); W = x->size(1); V = x->size(2);
+        count = PyLong_AsLong(count_of); end = PyLong_AsLong(end_of);
+        return !PyErr_Occurred() && kind >= 0 && on(x, type, c.device) && B >= 1 && W >= 1 && V >= 1 && B <= INT32_MAX && W <= INT32_MAX &&
+               V <= INT32_MAX && (V == 1 || x->stride(2) == 1) && count >= 1 && count <= 64 && end >= INT32_MIN && end <= INT32_MAX &&
+               dense(scores, at::kFloat, c.device, {B, W}) && (c.none(2) || dense(ended = tensor(c.a[2]), at::kBool, c.device, {B, W}));
+    }
+    long run(const Call& c, const at::Tensor& os, const at::Tensor& ob, const at::Tensor& ot, const at::Tensor& ws) const {
+        return forge_beam_select(at_<void>(x), at_<float>(scores), at_<uint8_t>(ended), static_cast<int>(end), at_<float>(os),
+                                 at_<int32_t>(ob), at_<int32_t>(ot), static_cast<int>(B), static_cast<int>(W), static_cast<int>(V),
+                                 static_cast<int>(count), x->stride(0), x->stride(1), kind, at_<void>(ws), ws.nbytes(), c.stream);
+    }
+};
 
 // beam_select(logits, scores, ended, out_scores, out_beams, out_tokens, workspace, count, end_token, device, stream)
 PyObject* beam_select(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return call<11>(args, n, [](const Call& c) -> long {
-        const at::Tensor *x = tensor(c.a[0]), *scores = tensor(c.a[1]), *ended = nullptr, *os = tensor(c.a[3]), *ob = tensor(c.a[4]);
-        const at::Tensor *ot = tensor(c.a[5]), *ws = tensor(c.a[6]);
-        if (!x || x->dim() != 3 || !PyLong_CheckExact(c.a[7]) || !PyLong_CheckExact(c.a[8])) return kNotInOrder;
-        const at::ScalarType type = x->scalar_type();
-        const int kind = type == at::kFloat ? FORGE_FP32 : code(type);
-        const int64_t B = x->size(0), W = x->size(1), V = x->size(2);
-        const long count = PyLong_AsLong(c.a[7]), end = PyLong_AsLong(c.a[8]);
-        if (PyErr_Occurred() || kind < 0 || !on(x, type, c.device) || B < 1 || W < 1 || V < 1 || B > INT32_MAX || W > INT32_MAX || V > INT32_MAX ||
-            (V > 1 && x->stride(2) != 1) || count < 1 || count > 64 || end < INT32_MIN || end > INT32_MAX ||
-            !dense(scores, at::kFloat, c.device, {B, W}) || !dense(os, at::kFloat, c.device, {B, count}) ||
-            !dense(ob, at::kInt, c.device, {B, count}) || !dense(ot, at::kInt, c.device, {B, count}) ||
-            !on(ws, at::kByte, c.device) || !ws->is_contiguous())
+        Beams f;
+        const at::Tensor *os = tensor(c.a[3]), *ob = tensor(c.a[4]), *ot = tensor(c.a[5]), *ws = tensor(c.a[6]);
+        if (!f.take(c, c.a[7], c.a[8]) || !dense(os, at::kFloat, c.device, {f.B, f.count}) || !dense(ob, at::kInt, c.device, {f.B, f.count}) ||
+            !dense(ot, at::kInt, c.device, {f.B, f.count}) || !on(ws, at::kByte, c.device) || !ws->is_contiguous())
             return kNotInOrder;
-        if (!c.none(2) && !dense(ended = tensor(c.a[2]), at::kBool, c.device, {B, W})) return kNotInOrder;
-        return forge_beam_select(at_<void>(x), at_<float>(scores), at_<uint8_t>(ended), static_cast<int>(end), at_<float>(os),
-                                 at_<int32_t>(ob), at_<int32_t>(ot), static_cast<int>(B), static_cast<int>(W), static_cast<int>(V),
-                                 static_cast<int>(count), x->stride(0), x->stride(1), kind, at_<void>(ws),
-                                 static_cast<size_t>(ws->numel()), c.stream);
+        return f.run(c, *os, *ob, *ot, *ws);
     });
+}
+
+// beam_select_new(logits, scores, ended, count, end_token, device, stream): the outputs, or a status
+PyObject* beam_select_new(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    at::Tensor made[3];
+    return made_or(call<7>(args, n, [&](const Call& c) -> long {
+        Beams f;
+        if (!f.take(c, c.a[3], c.a[4])) return kNotInOrder;
+        const size_t size = forge_beam_select_workspace_size(static_cast<int>(f.B), static_cast<int>(f.W), static_cast<int>(f.V), static_cast<int>(f.count));
+        if (size == 0) return kNotInOrder;
+        made[0] = at::empty({f.B, f.count}, f.scores->options());
+        for (int i : {1, 2}) made[i] = at::empty({f.B, f.count}, f.scores->options().dtype(at::kInt));
+        return f.run(c, made[0], made[1], made[2], at::empty({static_cast<int64_t>(size)}, f.scores->options().dtype(at::kByte)));
+    }), made);
 }
 
 // A call of fork_pages: its inputs in a[0..3] and the page size, checked.
@@ -338,7 +402,7 @@ at::Tensor part_of(const at::Tensor& all, int64_t first, c10::IntArrayRef sizes)
 // fork_pages_new(page_table, cache_lens, parents, refs, page_size, device, stream): the outputs, or a status
 PyObject* fork_pages_new(PyObject*, PyObject* const* args, Py_ssize_t n) {
     at::Tensor made[6];
-    PyObject* status = call<7>(args, n, [&](const Call& c) -> long {
+    return made_or(call<7>(args, n, [&](const Call& c) -> long {
         Fork f;
         if (!f.take(c, c.a[4]) || f.rows > INT32_MAX || f.pages > INT32_MAX) return kNotInOrder;
         const size_t size = forge_fork_pages_workspace_size(static_cast<int>(f.rows), static_cast<int>(f.pages));
@@ -361,13 +425,7 @@ PyObject* fork_pages_new(PyObject*, PyObject* const* args, Py_ssize_t n) {
         const at::Tensor* o[6];
         for (int i = 0; i < 6; i++) o[i] = &made[i];
         return f.run(c, o, ws);
-    });
-    if (!status || PyLong_AsLong(status) != 0) return status;
-    PyObject* tuple = PyTuple_New(6);
-    if (!tuple) return nullptr;
-    Py_DECREF(status);
-    for (int i = 0; i < 6; i++) PyTuple_SET_ITEM(tuple, i, THPVariable_Wrap(std::move(made[i])));
-    return tuple;
+    }), made);
 }
 
 // copy_pages(caches, src, dst, device, stream)
@@ -401,8 +459,8 @@ PyObject* copy_pages(PyObject*, PyObject* const* args, Py_ssize_t n) {
 
 #define FASTCALL(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)()>(name)), METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {FASTCALL(int4_linear), FASTCALL(qk_norm_rope), FASTCALL(prompt_attention), FASTCALL(cache_attention),
-                         FASTCALL(cache4_write), FASTCALL(cache4_read), FASTCALL(cache4_attention), FASTCALL(beam_select),
-                         FASTCALL(fork_pages), FASTCALL(fork_pages_new), FASTCALL(copy_pages),
+                         FASTCALL(cache4_write), FASTCALL(cache4_read), FASTCALL(cache4_attention), FASTCALL(cache4_attention_new),
+                         FASTCALL(beam_select), FASTCALL(beam_select_new),                         FASTCALL(fork_pages), FASTCALL(fork_pages_new), FASTCALL(copy_pages),
                          {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "forge_torch", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

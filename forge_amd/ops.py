@@ -524,7 +524,7 @@ def prepare_sparse_weight(w: torch.Tensor) -> Tuple[torch.Tensor, torch.Tensor, 
 
 # ---- decoder attention (extension; include/forge_amd.h "decoder attention") -----------
 # A call whose operands are all in order goes through csrc/torch_calls.cpp, which checks them and calls the library in
-# about a microsecond (cache_attention where the caller brings workspace and out); any other takes the checks
+# about a microsecond (cache_attention where the caller brings workspace and out; the operators of a 4-bit cache and of beams make theirs as well); any other takes the checks
 # below, which say what is wrong.
 
 _DTYPE = {torch.float16: 0, torch.bfloat16: 1}   # FORGE_FP16, FORGE_BF16
@@ -952,7 +952,11 @@ def cache4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Ten
                      workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """forge_cache4_attention: cache_attention over a 4-bit cache (cache4_shape(pages, page size, Hkv, D)), with the same queries
     (B, T, Hq, D), tables, lengths and trees. The new tokens' keys and values are in the cache already (cache4_write)."""
-    if workspace is not None and out is not None and isinstance(q, torch.Tensor):
+    if workspace is None and out is None and isinstance(q, torch.Tensor):
+        made = _fast_new("cache4_attention_new", q, cache, page_table, cache_lens, tree, _scale_of(scale, q))
+        if made is not None:
+            return made[0]
+    elif out is not None and isinstance(q, torch.Tensor):
         if _fast("cache4_attention", q, cache, page_table, cache_lens, tree, workspace, out, _scale_of(scale, q)):
             return out
     code = _act_type(q, "q")
@@ -1014,7 +1018,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, count: int, ended: O
     (B, W, V) float16, bfloat16 or float32 (rows of V contiguous values, any strides otherwise) and the beams' scores (B, W) float32. Returns scores
     (float32), beams and tokens (int32), (B, count) each, in descending order, equal ones by (beam, token); places that nothing is left for
     hold -inf, -1, -1. ended (B, W) bool: beams with end_token, at their score, as their one candidate."""
-    if workspace is not None and out is not None and isinstance(out, tuple) and len(out) == 3:
+    if workspace is None and out is None:
+        made = _fast_new("beam_select_new", logits, scores, ended, count, end_token)
+        if made is not None:
+            return made
+    elif workspace is not None and out is not None and isinstance(out, tuple) and len(out) == 3:
         if _fast("beam_select", logits, scores, ended, *out, workspace, count, end_token):
             return out
     if not isinstance(logits, torch.Tensor) or logits.dtype not in _LOGITS:
