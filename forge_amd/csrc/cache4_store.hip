@@ -196,7 +196,7 @@ extern "C" int forge_cache4_write(const uint16_t* k, const uint16_t* v, uint8_t*
                                   long long v_head, int dtype, void* stream)
 {
     if (T <= 0 || Hkv <= 0 || D <= 0) return FORGE_OK;
-    if (!cache4_shape_ok(Hkv, D, pages, page_size) || !k || !v || !cache || !slots || (dtype != FORGE_FP16 && dtype != FORGE_BF16))
+    if (!cache4_shape_ok(Hkv, D, pages, page_size) || T > INT_MAX - 64 || !k || !v || !cache || !slots || (dtype != FORGE_FP16 && dtype != FORGE_BF16))
         return FORGE_EINVAL;
     for (const void* p : {static_cast<const void*>(k), static_cast<const void*>(v), static_cast<const void*>(cache)})
         if (!aligned(p, 16)) return FORGE_EINVAL;
@@ -213,7 +213,7 @@ extern "C" int forge_cache4_read(const uint8_t* cache, const int32_t* slots, uin
                                  int pages, int page_size, int dtype, void* stream)
 {
     if (T <= 0 || Hkv <= 0 || D <= 0) return FORGE_OK;
-    if (!cache4_shape_ok(Hkv, D, pages, page_size) || !k || !v || !cache || !slots || (dtype != FORGE_FP16 && dtype != FORGE_BF16))
+    if (!cache4_shape_ok(Hkv, D, pages, page_size) || T > INT_MAX - 64 || !k || !v || !cache || !slots || (dtype != FORGE_FP16 && dtype != FORGE_BF16))
         return FORGE_EINVAL;
     for (const void* p : {static_cast<const void*>(k), static_cast<const void*>(v), static_cast<const void*>(cache)})
         if (!aligned(p, 16)) return FORGE_EINVAL;

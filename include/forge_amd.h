@@ -398,7 +398,8 @@ int forge_cache4_attention(const uint16_t* q, const uint8_t* cache, const int32_
 
 /* A beam search's selection. For each of B requests, score[w,v] = logits[w,v] - log(sum over v of exp(logits[w,v])) + scores[w] of its
  * W (up to 1024) beams and V tokens; the `count` (1 to 64) largest go to out_scores (FP32), out_beams (w) and out_tokens (v), (B,count) each,
- * in descending order, equal ones by (w, v). Sums, scores and their order are taken in 64 bits from FP32 exponentials. -inf
+ * in descending order, equal ones by (w, v). Sums, scores and their order are taken in 64 bits from FP32 exponentials (scores
+ * nearer to each other than about 10^-6 may come in either order; equal rows have equal scores). -inf
  * logits are no candidates; neither is a beam whose score is not finite or whose logits hold an infinity or NaN, or -inf only. A beam that has
  * ended (ended[b,w] != 0; NULL: none has) has one candidate, end_token with the beam's score, and its logits are not read. Places
  * that no candidate is left for are -inf, -1, -1. logits: dtype FORGE_FP16, FORGE_BF16 or FORGE_FP32, rows of V contiguous values at

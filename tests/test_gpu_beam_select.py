@@ -104,6 +104,20 @@ def test_equal_logits(dev, dt, V):
     assert got[1][1].tolist() == [1] * 40
 
 
+@pytest.mark.parametrize("dt,B,W,V", [("float16", 2, 64, 300), ("float32", 40, 8, 16500), ("bfloat16", 40, 8, 16500)])
+def test_more_equal_than_there_is_room_for(dev, dt, B, W, V):
+    """Thousands of candidates with the very same score, in one piece or in one request; with ended beams among them."""
+    import torch
+    x = torch.full((B, W, V), 1.25, dtype=getattr(torch, dt), device=dev)
+    s = torch.full((B, W), -4.0, device=dev)
+    _, _, got = run(dev, dt, B, W, V, 64, logits=x, scores=s)
+    assert (got[1] == 0).all() and torch.equal(got[2], torch.arange(64, device=dev, dtype=torch.int32).expand(B, 64))
+    ended = torch.zeros((B, W), dtype=torch.bool, device=dev)
+    ended[:, 1], ended[::2, 3] = True, True
+    s[:, 3] = -4.5
+    run(dev, dt, B, W, V, 64, logits=x, scores=s, ended=ended, end_token=2)
+
+
 @pytest.mark.parametrize("V", [501, 4099])
 def test_equal_beams(dev, V):
     """Two beams with the same logits, at addresses of different alignment, tie exactly."""

@@ -283,6 +283,24 @@ def test_ranges(dev, dt):
     run(dev, dt, [200], 1, 4, 2, 64, 16, scale=40.0)
 
 
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("far", [9.0, 13.0, 15.0])
+def test_many_small_weights(dev, dt, far):
+    """One key far above thousands of others, whose weights are subnormal in FP16 next to its own and still add up."""
+    import torch
+    from forge_amd import ops
+    say(f"cache4_attention small weights {dt} far={far}")
+    n, D = 30000, 64
+    q = queries(1, 1, 1, D, dt, dev, 40)
+
+    def one(b, k, v):
+        k.zero_()
+        k[n // 2, 0] = (q[0, 0, 0].float() * (far * 8.0 / q.float().square().sum())).to(k.dtype)
+    c = Cache4([n], 1, 1, D, 16, dt, dev, 41, change=one)
+    out = ops.cache4_attention(q, c.cache, c.table, c.lens)
+    check_all(out, q, c, [n], None)
+
+
 def test_rising_scores(dev):
     """Maxima that grow from tile to tile by far, with steps that fall."""
     def rising(b, k, v):
