@@ -11,13 +11,17 @@
 
 namespace forge_amd {
 
+constexpr long long kMaxStride = 1 << 25;   // elements; 32 tokens of them stay in 32 bits
+
 struct Store4Args {
     const uint16_t *k, *v;
     uint16_t *k_out, *v_out;
     uint8_t* cache;
     const int32_t* slots;
-    long long k_token, k_head, v_token, v_head, rows;
+    long long k_head, v_head, rows;
+    size_t page_bytes;
     Cache4Layout at;
+    int k_token, v_token;
     int T, D;
 };
 
@@ -28,28 +32,43 @@ __device__ __forceinline__ uint16_t toward_zero(float x) {
     return T::widen(h) > x ? static_cast<uint16_t>(h - 1) : h;
 }
 
-// The cache's row of token t, or -1.
-__device__ __forceinline__ long long store4_slot(const Store4Args& a, int t) {
-    const long long s = t < a.T ? a.slots[t] : -1;
-    return s < a.rows ? s : -1;
+// The cache's row of token t, or -1. (Loaded for any t, so that no branch waits for it.)
+__device__ __forceinline__ int store4_slot(const Store4Args& a, int t) {
+    const int s = a.slots[min(t, a.T - 1)];
+    return t < a.T && s < a.rows ? s : -1;
+}
+// The piece of a slot's page and head hk (of the whole workgroup).
+__device__ __forceinline__ uint8_t* store4_piece(const Store4Args& a, int slot, int hk) {
+    return a.cache + hk * a.at.piece() + static_cast<uint32_t>(slot >> a.at.page_shift) * a.page_bytes;
 }
 
-// A reduction over the LPH lanes of a head, in registers: neighbours, pairs, then mirrored halves of 8 and 16 lanes.
+// Pairs of 16-bit numbers as integers of the same order, and back.
+typedef short v2s __attribute__((ext_vector_type(2)));
+__device__ __forceinline__ v2s ordered(v2s x) { return x ^ ((x >> 15) & static_cast<short>(0x7FFF)); }
+
+// Least and largest value over the LPH lanes of a head, both of which are numbers of the type: as a pair, the least one negated, in registers
+// (neighbours, pairs, then mirrored halves of 8 and 16 lanes).
 template <int CTRL>
-__device__ __forceinline__ float lane_move(float x) {
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(x), CTRL, 0xF, 0xF, false));
+__device__ __forceinline__ v2s with_lane(v2s x) {
+    const int y = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, x), CTRL, 0xF, 0xF, false);
+    return __builtin_elementwise_max(x, __builtin_bit_cast(v2s, y));
 }
-template <int LPH, class F>
-__device__ __forceinline__ float head_reduce(float x, const F& f) {
-    x = f(x, lane_move<0xB1>(x));
-    x = f(x, lane_move<0x4E>(x));
-    x = f(x, lane_move<0x141>(x));
-    if (LPH >= 16) x = f(x, lane_move<0x140>(x));
+template <class T, int LPH>
+__device__ __forceinline__ void head_range(float* low, float* top) {
+    v2s x = ordered(__builtin_bit_cast(v2s, T::pack(*top, -*low)));
+    x = with_lane<0xB1>(x);
+    x = with_lane<0x4E>(x);
+    x = with_lane<0x141>(x);
+    if (LPH >= 16) x = with_lane<0x140>(x);
     if (LPH >= 32) {
-        const v2u r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
-        x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+        const uint32_t u = __builtin_bit_cast(uint32_t, x);
+        const v2u r = __builtin_amdgcn_permlane16_swap(u, u, false, false);
+        const uint32_t r0 = r[0], r1 = r[1];                         // (a bit cast of r[1] itself takes r[0])
+        x = __builtin_elementwise_max(__builtin_bit_cast(v2s, r0), __builtin_bit_cast(v2s, r1));
     }
-    return x;
+    x = ordered(x);
+    *top = T::widen(static_cast<uint16_t>(x[0]));
+    *low = -T::widen(static_cast<uint16_t>(x[1]));
 }
 
 // x / 15, correctly rounded: the product with the rounded reciprocal, corrected by its exact remainder, which FP32 holds for FP16's values.
@@ -67,19 +86,18 @@ __device__ __forceinline__ uint32_t quantize_head(v4u own, bool in, uint32_t* nu
     float x[8];
     widen8<T>(own, x);
     float low = INFINITY, top = -INFINITY;
-    if (in) {
+    float odd = 0.0f;
 #pragma unroll
-        for (int e = 0; e < 8; e++) {
-            low = fminf(low, x[e]);
-            top = fmaxf(top, x[e]);
-        }
-        float odd = 0.0f;
-#pragma unroll
-        for (int d = 0; d < 4; d++) odd = T::times_zero(own[d], odd);
-        if (odd != 0.0f) top = INFINITY;                             // an infinity or NaN
+    for (int e = 0; e < 8; e++) {
+        low = fminf(low, x[e]);
+        top = fmaxf(top, x[e]);
     }
-    low = head_reduce<LPH>(low, [](float p, float q) { return fminf(p, q); });
-    top = head_reduce<LPH>(top, [](float p, float q) { return fmaxf(p, q); });
+#pragma unroll
+    for (int d = 0; d < 4; d++) odd = T::times_zero(own[d], odd);
+    top = odd != 0.0f ? INFINITY : top;                              // an infinity or NaN
+    low = in ? low : INFINITY;
+    top = in ? top : -INFINITY;
+    head_range<T, LPH>(&low, &top);
     constexpr uint32_t kNaN = T::kInfinity | T::kInfinity >> 1;
     *numbers = kNaN | kNaN << 16;
     if (!(top < INFINITY)) return 0u;
@@ -87,20 +105,21 @@ __device__ __forceinline__ uint32_t quantize_head(v4u own, bool in, uint32_t* nu
     *numbers = step | static_cast<uint32_t>(narrow<T>(low)) << 16;
     const float s = T::widen(step) * 0.5f, m = low * 0.5f;           // halves: x - m stays in range
     if (!in || !(s > 0.0f)) return 0u;
-    // A product with the reciprocal is the quotient but for 2^-21 of it; only next to a half (or without a reciprocal) does it take
+    // A product with the reciprocal is the quotient but for 2^-21 of it; only next to a half (or with a subnormal step) does it take
     // the division to know where that rounds. kWhole's sum with a small number rounds it to an integer in its last bits. 16384 tokens of
-    // 8 heads of 128: eight divisions a lane 29 us, this 25.
+    // 8 heads of 128: eight divisions a lane 29 us, this 22.
     constexpr float kWhole = 12582912.0f;
     constexpr uint32_t kBits = 0x4B400000u;
     const float inv = __builtin_amdgcn_rcpf(s);
-    float n[8], off = inv < INFINITY ? 0.0f : 1.0f;
+    // (A step of all its bits takes no quotient to 15.5.)
+    float n[8], off = s < T::kNormal ? 1.0f : 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        const float q = fminf((x[e] * 0.5f - m) * inv, 15.0f);
+        const float q = (x[e] * 0.5f - m) * inv;
         n[e] = q + kWhole;
         off = fmaxf(off, fabsf(q - (n[e] - kWhole)));
     }
-    if (__any(!(off < 0.4999f))) {
+    if (__any(!(off < 0.49999f))) {
         asm volatile("" : "+v"(n[0]));                               // (the compiler would divide in any case)
 #pragma unroll
         for (int e = 0; e < 8; e++) n[e] = fminf((x[e] * 0.5f - m) / s, 15.0f) + kWhole;
@@ -121,20 +140,19 @@ __global__ __launch_bounds__(256) void cache4_write_kernel(Store4Args a)
     const int lane = threadIdx.x & (kWave - 1), lh = lane & (LPH - 1), d0 = 8 * lh;
     const unsigned part = blockIdx.x / static_cast<unsigned>(a.at.Hkv);
     const int hk = blockIdx.x - part * a.at.Hkv, t = (part * 4 + threadIdx.x / kWave) * (kWave / LPH) + lane / LPH;
-    const bool in = t < a.T && d0 < a.D;                             // (without waiting for the slot)
-    const long long slot = store4_slot(a, t);
-    v4u k = {0u, 0u, 0u, 0u}, v = k;
-    if (in) {
-        k = *reinterpret_cast<const v4u*>(a.k + t * a.k_token + hk * a.k_head + d0);
-        v = *reinterpret_cast<const v4u*>(a.v + t * a.v_token + hk * a.v_head + d0);
-    }
+    const bool in = t < a.T && d0 < a.D;
+    // (from the wave's first token on in 32 bits)
+    const int t0 = __builtin_amdgcn_readfirstlane(t - lane / LPH), tt = min(lane / LPH, a.T - 1 - t0), dd = min(d0, a.D - 8);
+    const v4u k = *reinterpret_cast<const v4u*>(a.k + static_cast<long long>(t0) * a.k_token + hk * a.k_head + (tt * a.k_token + dd));
+    const v4u v = *reinterpret_cast<const v4u*>(a.v + static_cast<long long>(t0) * a.v_token + hk * a.v_head + (tt * a.v_token + dd));
+    const int slot = store4_slot(a, t);
     v2u numbers;
     uint32_t kn, vn;
     const uint32_t kw = quantize_head<T, LPH>(k, in, &kn), vw = quantize_head<T, LPH>(v, in, &vn);
     numbers = v2u{kn, vn};
     if (slot < 0 || lh >= 4 * a.at.U) return;
-    const int r = static_cast<int>(slot) & ((1 << a.at.page_shift) - 1);
-    uint8_t* piece = a.cache + a.at.at(slot >> a.at.page_shift, hk);
+    const int r = slot & ((1 << a.at.page_shift) - 1);
+    uint8_t* piece = store4_piece(a, slot, hk);
     *reinterpret_cast<uint32_t*>(piece + a.at.key_row(r) + 4 * lh) = kw;
     *reinterpret_cast<uint32_t*>(piece + a.at.value_word(r, lh)) = vw;
     if (lh == 0) *reinterpret_cast<v2u*>(piece + a.at.numbers(r)) = numbers;
@@ -156,12 +174,12 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(Store4Args a)
     const unsigned part = blockIdx.x / static_cast<unsigned>(a.at.Hkv);
     const int hk = blockIdx.x - part * a.at.Hkv, t = (part * 4 + threadIdx.x / kWave) * (kWave / LPH) + lane / LPH;
     if (t >= a.T || d0 >= a.D) return;
-    const long long slot = store4_slot(a, t);
+    const int slot = store4_slot(a, t);
     uint32_t kw = 0u, vw = 0u;                                       // a slot outside the cache: zeros
     v2u numbers = {0u, 0u};
     if (slot >= 0) {
-        const int r = static_cast<int>(slot) & ((1 << a.at.page_shift) - 1);
-        const uint8_t* piece = a.cache + a.at.at(slot >> a.at.page_shift, hk);
+        const int r = slot & ((1 << a.at.page_shift) - 1);
+        const uint8_t* piece = store4_piece(a, slot, hk);
         kw = *reinterpret_cast<const uint32_t*>(piece + a.at.key_row(r) + 4 * lh);
         vw = *reinterpret_cast<const uint32_t*>(piece + a.at.value_word(r, lh));
         numbers = *reinterpret_cast<const v2u*>(piece + a.at.numbers(r));
@@ -201,10 +219,10 @@ extern "C" int forge_cache4_write(const uint16_t* k, const uint16_t* v, uint8_t*
     for (const void* p : {static_cast<const void*>(k), static_cast<const void*>(v), static_cast<const void*>(cache)})
         if (!aligned(p, 16)) return FORGE_EINVAL;
     for (long long st : {k_token, k_head, v_token, v_head})
-        if (st < 0 || st % 8 != 0) return FORGE_EINVAL;
-    const Store4Args a{k, v, nullptr, nullptr, cache, slots, k_token, k_head, v_token, v_head,
-                       static_cast<long long>(pages) * page_size,
-                       {cache4_units(D), __builtin_ctz(static_cast<unsigned>(page_size)), Hkv}, T, D};
+        if (st < 0 || st % 8 != 0 || st > kMaxStride) return FORGE_EINVAL;
+    const Cache4Layout at{cache4_units(D), __builtin_ctz(static_cast<unsigned>(page_size)), Hkv};
+    const Store4Args a{k, v, nullptr, nullptr, cache, slots, k_head, v_head, static_cast<long long>(pages) * page_size, at.at(1, 0), at,
+                       static_cast<int>(k_token), static_cast<int>(v_token), T, D};
     hipStream_t s = as_stream(stream);
     return dtype == FORGE_FP16 ? launch_store4<Fp16>(a, true, s) : launch_store4<Bf16>(a, true, s);
 }
@@ -217,9 +235,9 @@ extern "C" int forge_cache4_read(const uint8_t* cache, const int32_t* slots, uin
         return FORGE_EINVAL;
     for (const void* p : {static_cast<const void*>(k), static_cast<const void*>(v), static_cast<const void*>(cache)})
         if (!aligned(p, 16)) return FORGE_EINVAL;
-    const Store4Args a{nullptr, nullptr, k, v, const_cast<uint8_t*>(cache), slots, 0, 0, 0, 0,
-                       static_cast<long long>(pages) * page_size,
-                       {cache4_units(D), __builtin_ctz(static_cast<unsigned>(page_size)), Hkv}, T, D};
+    const Cache4Layout at{cache4_units(D), __builtin_ctz(static_cast<unsigned>(page_size)), Hkv};
+    const Store4Args a{nullptr, nullptr, k, v, const_cast<uint8_t*>(cache), slots, 0, 0, static_cast<long long>(pages) * page_size,
+                       at.at(1, 0), at, 0, 0, T, D};
     hipStream_t s = as_stream(stream);
     return dtype == FORGE_FP16 ? launch_store4<Fp16>(a, false, s) : launch_store4<Bf16>(a, false, s);
 }

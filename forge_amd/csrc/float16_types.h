@@ -18,6 +18,7 @@ struct Fp16 {
     typedef _Float16 v8 __attribute__((ext_vector_type(8)));
     static constexpr uint32_t kOnes = 0x3C003C00u;
     static constexpr uint32_t kInfinity = 0x7C00u;
+    static constexpr float kNormal = 0x1p-14f;   // the smallest number of all its bits
     static constexpr bool kWide = false;   // FP32's range
     static __device__ __forceinline__ float widen(uint16_t b) { return h2f(b); }
     // Two values rounded to nearest even, the first in the low half. (No inline asm: the wait state between an
@@ -46,6 +47,7 @@ struct Bf16 {
     typedef __bf16 v8 __attribute__((ext_vector_type(8)));
     static constexpr uint32_t kOnes = 0x3F803F80u;
     static constexpr uint32_t kInfinity = 0x7F80u;
+    static constexpr float kNormal = 0x1p-126f;
     static constexpr bool kWide = true;
     static __device__ __forceinline__ float widen(uint16_t b) { return __uint_as_float(static_cast<uint32_t>(b) << 16); }
     static __device__ __forceinline__ uint32_t pack(float a, float b) {

@@ -380,7 +380,7 @@ int forge_cache_attention(const uint16_t* q, const uint16_t* k_cache, const uint
  * 8 w to 8 w + 7, of these value 2 i at bits 4 i and value 2 i + 1 at bits 16 + 4 i; words past D are zeros), then the values' words as
  * (position / 4, word, position % 4), then per position four 16-bit numbers: step and lowest value of its key, and of its value. */
 /* Row slots[t] (page * page_size + offset) of the cache takes k and v (T,Hkv,D) of token t, strided as above; a slot outside it writes
- * nothing. The slots of a call differ. */
+ * nothing. The slots of a call differ, and strides are up to 2^25. */
 int forge_cache4_write(const uint16_t* k, const uint16_t* v, uint8_t* cache, const int32_t* slots, int T, int Hkv, int D,
                        int pages, int page_size, long long k_token, long long k_head, long long v_token,
                        long long v_head, int dtype, void* stream);

@@ -25,7 +25,7 @@ def test_write_and_read(lib):
     w = dict(k=FAKE, v=FAKE, cache=FAKE, slots=FAKE, T=3, Hkv=2, D=64, pages=10, page=16, kt=128, kh=64, vt=128, vh=64, dtype=0,
              stream=None)
     for bad in (dict(k=None), dict(v=None), dict(cache=None), dict(slots=None), dict(D=60), dict(D=264), dict(pages=0), dict(page=8),
-                dict(page=24), dict(page=1 << 21), dict(pages=1 << 28), dict(Hkv=65536), dict(kt=12), dict(vh=-8), dict(dtype=2),
+                dict(page=24), dict(page=1 << 21), dict(pages=1 << 28), dict(Hkv=65536), dict(kt=12), dict(vh=-8), dict(kt=(1 << 25) + 8), dict(vh=1 << 40), dict(dtype=2),
                 dict(dtype=-1), dict(k=ODD), dict(v=ODD), dict(cache=ODD), dict(T=(1 << 31) - 1)):
         assert call(lib.forge_cache4_write, w, **bad) == -1, bad
     for none in (dict(T=0), dict(Hkv=0), dict(D=-8)):
