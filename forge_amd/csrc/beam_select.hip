@@ -8,6 +8,9 @@
 // The largest of many: of 64 groups' maxima the count-th largest is a bound that at least `count` numbers reach, and what reaches it, few
 // more as a rule, is gathered in LDS and ranked by counting, with ties by place. Where LDS has no room for that, the places are filled one
 // after the other.
+//
+// us, pieces + merge: 32 x 8 beams of 131072 FP32 logits, three in ten ended, 20.4 (94 MB at 4.6 TB/s) + 8.2; 4 beams of 32000 FP16 4.9 + 5.8, two chains
+// of dependent steps.
 #include "float16_types.h"
 
 #include <algorithm>
