@@ -79,6 +79,56 @@ __device__ __forceinline__ float key_value(BeamKey k) {
     return __uint_as_float(o & 0x80000000u ? o ^ 0x80000000u : ~o);
 }
 
+// Reductions over a wave in registers, the same on all lanes: neighbours, pairs, mirrored halves of 8 and 16 lanes, then rows of 16. (Through LDS
+// the same took half a microsecond a kernel.)
+template <int STEP>
+__device__ __forceinline__ uint32_t other_lane(uint32_t x) {
+    constexpr int kCtrl = STEP == 0 ? 0xB1 : STEP == 1 ? 0x4E : STEP == 2 ? 0x141 : 0x140;
+    return static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(x), kCtrl, 0xF, 0xF, false));
+}
+template <class F>
+__device__ __forceinline__ float wave_reduce(float x, const F& f) {
+    auto step = [&](uint32_t y) { x = f(x, __uint_as_float(y)); };
+    step(other_lane<0>(__float_as_uint(x)));
+    step(other_lane<1>(__float_as_uint(x)));
+    step(other_lane<2>(__float_as_uint(x)));
+    step(other_lane<3>(__float_as_uint(x)));
+    const v2u r = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    x = f(__uint_as_float(r[0]), __uint_as_float(r[1]));
+    const v2u q = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+    return f(__uint_as_float(q[0]), __uint_as_float(q[1]));
+}
+template <class F>
+__device__ __forceinline__ double wave_reduce(double x, const F& f) {
+    auto words = [&](uint32_t* lo, uint32_t* hi) {
+        const uint64_t u = __builtin_bit_cast(uint64_t, x);
+        *lo = static_cast<uint32_t>(u);
+        *hi = static_cast<uint32_t>(u >> 32);
+    };
+    auto number = [](uint32_t lo, uint32_t hi) { return __builtin_bit_cast(double, static_cast<uint64_t>(hi) << 32 | lo); };
+    uint32_t lo, hi;
+    words(&lo, &hi);
+    x = f(x, number(other_lane<0>(lo), other_lane<0>(hi)));
+    words(&lo, &hi);
+    x = f(x, number(other_lane<1>(lo), other_lane<1>(hi)));
+    words(&lo, &hi);
+    x = f(x, number(other_lane<2>(lo), other_lane<2>(hi)));
+    words(&lo, &hi);
+    x = f(x, number(other_lane<3>(lo), other_lane<3>(hi)));
+    words(&lo, &hi);
+    const v2u l16 = __builtin_amdgcn_permlane16_swap(lo, lo, false, false), h16 = __builtin_amdgcn_permlane16_swap(hi, hi, false, false);
+    x = f(number(l16[0], h16[0]), number(l16[1], h16[1]));
+    words(&lo, &hi);
+    const v2u l32 = __builtin_amdgcn_permlane32_swap(lo, lo, false, false), h32 = __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+    return f(number(l32[0], h32[0]), number(l32[1], h32[1]));
+}
+__device__ __forceinline__ double wave_sum(double x) {
+    return wave_reduce(x, [](double a, double b) { return a + b; });
+}
+__device__ __forceinline__ float wave_most(float x) {
+    return wave_reduce(x, [](float a, float b) { return fmaxf(a, b); });
+}
+
 // The nth largest (from 0) of the 64 groups' largest numbers: each thread compares one of them with some others, the first wave picks the one
 // that n are above (the smallest of those that n or fewer are above, where some are equal). All of N threads call it; part[w][l] is
 // wave w's largest of group l; the result is wave 0's.
@@ -108,20 +158,9 @@ struct NthGroup {
         const unsigned long long at = __ballot(all == n);
         F least = all <= n ? x : static_cast<F>(INFINITY);
         if (at) return __shfl(x, __builtin_ctzll(at), kWave);
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const F y = __shfl_xor(least, o, kWave);
-            least = y < least ? y : least;
-        }
-        return least;
+        return wave_reduce(least, [](F a, F b) { return b < a ? b : a; });
     }
 };
-
-__device__ __forceinline__ double wave_sum(double x) {
-#pragma unroll
-    for (int o = 1; o < kWave; o <<= 1) x += __shfl_xor(x, o, kWave);
-    return x;
-}
 
 // A row's piece of 256 x VEC vectors. Places are counted from the piece's start, whatever its address, so that equal rows
 // have equal sums.
@@ -164,7 +203,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_piece_kernel(BeamArgs a)
 #pragma unroll
         for (int e = 0; e < L::kPer; e++) most = fmaxf(most, L::value(v[i], e));
     groups.part[wave][lane] = most;
-    const float top = fmaxf(wave_max(most), -FLT_MAX);
+    const float top = fmaxf(wave_most(most), -FLT_MAX);
     float sum = 0.0f;
 #pragma unroll
     for (int i = 0; i < VEC; i++)
@@ -274,7 +313,7 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a)
         double sum = 0.0;
         if (!ended) {
             for (int i = lane; i < a.splits; i += kWave) top = fmaxf(top, p[i].top);
-            top = wave_max(top);
+            top = wave_most(top);
             for (int i = lane; i < a.splits; i += kWave) sum += p[i].sum * exp(static_cast<double>(p[i].top) - top);
             sum = wave_sum(sum);
         }
