@@ -52,20 +52,25 @@ def words(cache, page, D):
 def attention(q, k, v, seen, scale, dtype):
     """(result, bound) of cache4_attention for rows q (R, D) over held k and v (held()'s tuples, (n, D)), seen (R, n).
 
-    With u half a unit in the last place of `dtype`, w = p s' and N the additions of a lane (keys / 4 of them, and a tile's):
+    With u half a unit in the last place of `dtype` and w = p s':
       the result's rounding u |o|; the weights' 2^-11 w |n' - 8| each, or 2^-29 of the row's largest w (half of FP16's
       smallest step, the largest being at 2^4 or above);
-      scores: ds = (D + 8) 2^-23 scale (s sum |q| n + |m| sum |q|), which moves a weight by 2 ds of itself; and the FP32
-      sums, N 2^-23 of what they sum, 2^-18 for the exponentials and factors."""
+      the matrix unit: of the 8 products of a group 7 may lose 2^-18 of the group's largest factor beside the integers (those
+      are FP16 subnormals n 2^-20, whose exponent counts as 2^-14, and 24 bits are kept), and a group's products next to each
+      other 2^-21 of themselves. Scores, of D / 8 groups, then miss
+      ds = 7 2^-18 scale s sum over groups of max |q| + (D / 8 + 12) 2^-23 scale (s sum |q| n + |m| sum |q|) (2^-23 for each
+      group's addition, or half of it for the D / 4 of a lane's sum of q, and the few of steps and lowest values), which moves a weight by 2 ds of itself; the sum of w n'
+      misses 7 2^-18 of the sum of w, and (keys / 8 + 16) 2^-23 of itself and of 8 times the sum of w, which is taken off;
+      the other FP32 sums: (keys / 4 + 64) 2^-23 of what they sum, 2^-18 for the exponentials and factors."""
     q = q.double()
-    val_k, _, _, _, up_k, low_k = k
-    val_v, mid_v, off_v, step_v, _, _ = v
+    val_k, _, _, step_k, up_k, low_k = k
+    val_v, mid_v, off_v, step_v, up_v, _ = v
     R, n = q.shape[0], val_k.shape[0]
     if n == 0:
         return torch.zeros((R, val_v.shape[1]), dtype=torch.float64, device=q.device), 0.0
     fix = lambda t: torch.nan_to_num(t, nan=0.0)                     # noqa: E731  (unseen ones; a seen NaN is the caller's)
     val_k, up_k, low_k = fix(val_k), fix(up_k), fix(low_k)
-    val_v, mid_v, off_v, step_v = fix(val_v), fix(mid_v), fix(off_v), fix(step_v)
+    val_v, mid_v, off_v, step_v, up_v = fix(val_v), fix(mid_v), fix(off_v), fix(step_v), fix(up_v)
     s = ((q @ val_k.T) * scale).masked_fill(~seen, float("-inf"))
     mag = ((q.abs() @ up_k.T + q.abs().sum(-1, keepdim=True) * low_k.abs()) * scale).masked_fill(~seen, 0.0).amax(-1, keepdim=True)
     p = torch.exp(s - s.amax(-1, keepdim=True).clamp_min(-1e300))
@@ -76,9 +81,12 @@ def attention(q, k, v, seen, scale, dtype):
     A = (p @ (mid_v.abs() + off_v)) / l
     most = (p * step_v).amax(-1, keepdim=True) / l
     u = HALF_ULP[dtype]
-    N = n / 4 + 64
-    ds = (q.shape[1] + 8) * 2.0 ** -23 * mag
-    bound = u * o.abs() + 2.0 ** -11 * w + 2.0 ** -29 * 8 * n * most + (2 * ds + 2.0 ** -18 + N * 2.0 ** -23) * A
+    D = q.shape[1]
+    group = q.abs().view(R, D // 8, 8).amax(-1).sum(-1, keepdim=True)
+    ds = 7 * 2.0 ** -18 * scale * group * fix(step_k).max() + (D / 8 + 12) * 2.0 ** -23 * mag
+    W, S = (p @ up_v) / l + 8 * (p @ step_v)[:, None] / l, (p @ step_v)[:, None] / l
+    bound = u * o.abs() + 2.0 ** -11 * w + 2.0 ** -29 * 8 * n * most + (2 * ds + 2.0 ** -18 + (n / 4 + 64) * 2.0 ** -23) * A
+    bound = bound + 7 * 2.0 ** -18 * S + (n / 8 + 16) * 2.0 ** -23 * W
     bound = bound + (2.0 ** -25 if dtype == torch.float16 else 1e-38)
     return o, torch.where(any_seen, bound * (1 + u), 0.0)
 

@@ -301,6 +301,45 @@ def test_many_small_weights(dev, dt, far):
     check_all(out, q, c, [n], None)
 
 
+@pytest.mark.parametrize("dt", ["float16", "bfloat16"])
+@pytest.mark.parametrize("T,D,channel", [(1, 128, 0), (1, 128, 3), (29, 64, 60), (2, 256, 129), (64, 72, 5)])
+def test_large_channels(dev, dt, T, D, channel):
+    """A channel of queries and keys far above the others, whose products lie next to theirs in the matrix unit."""
+    import torch
+    from forge_amd import ops
+    say(f"large channels {dt} T={T} D={D} channel={channel}")
+
+    def change(b, k, v):
+        k[:, :, channel] = 20.0 + k[:, :, channel]
+    lens = [700, 0, 33]
+    c = Cache4(lens, T, 2, D, 16, dt, dev, 41 + D, change=change, spread=0.5)
+    q = queries(3, T, 4, D, dt, dev, 42 + D)
+    q[..., channel] = 48.0
+    out = ops.cache4_attention(q, c.cache, c.table, c.lens)
+    check_all(out, q, c, lens, None)
+
+
+def test_a_key_between_its_integers(dev):
+    """One key with nearly all of the weight, whose values are the middle of its range: the sum of its products, 8 w, is taken off."""
+    import torch
+    from forge_amd import ops
+    D = 64
+    k = torch.zeros((16, 1, D), dtype=torch.float16, device=dev)
+    v = heads(16, 1, D, "float16", dev, 51, 0.5)
+    k[:, 0, 0] = torch.arange(16, device=dev) * -0.5               # weights e^-0.5j
+    k[:, 0, 1] = 1.0
+    v[0] = 0.0
+    v[0, 0, 0], v[0, 0, 1] = -8.0, 7.0                             # step 1, the others 0 = -8 + 8
+    cache = torch.zeros(ops.cache4_shape(1, 16, 1, D), dtype=torch.uint8, device=dev)
+    ops.cache4_write(k, v, cache, torch.arange(16, dtype=torch.int32, device=dev))
+    q = torch.zeros((1, 1, 1, D), dtype=torch.float16, device=dev)
+    q[..., 0] = 8.0
+    out = ops.cache4_attention(q, cache, torch.zeros((1, 1), dtype=torch.int32, device=dev), torch.full((1,), 15, dtype=torch.int32, device=dev),
+                               scale=0.5)
+    hk, hv = plain.held(k), plain.held(v)
+    plain.check(out[0, 0], q[0, 0], [t[:, 0] for t in hk], [t[:, 0] for t in hv], torch.ones((1, 16), dtype=torch.bool, device=dev), 0.5)
+
+
 def test_rising_scores(dev):
     """Maxima that grow from tile to tile by far, with steps that fall."""
     def rising(b, k, v):
