@@ -18,8 +18,8 @@
 // with n' 5.4e-4; rounding the exact result alone 2.1e-4).
 //
 // Bound: reading the cache for up to 16 rows: one token over 16 sequences of 278 thousand keys, 32 / 8 heads of 128, 55 us, 5.5 TB/s of 303 MB (and
-// 4.9 for the join of the chunks, cache_split.h; 16-bit caches read 3.8 times as much). Many rows: the vector units. 6 trees of 16 drafts, 32 / 4 heads of
-// 128, over 119 thousand keys take 75 us (420 TFLOP/s): 400 vector and 32 matrix instructions for 32 rows and 32 keys, of them 88 for the operands, 40 for
+// 4.8 for the join of the chunks; 16-bit caches read 3.8 times as much). Many rows: the vector units. 6 trees of 16 drafts, 32 / 4 heads of
+// 128, over 119 thousand keys take 68 us (460 TFLOP/s): 430 vector and 32 matrix instructions for 32 rows and 32 keys, of them 120 for the operands, 40 for
 // steps and lowest values and 13 (16 with the exponential's rate) per score. Sharing the operands of four waves in LDS took 16 % of the
 // instructions away, but 83 us: the waves wait for each other at every tile.
 #include "cache4.h"
@@ -31,7 +31,63 @@ namespace forge_amd {
 
 struct Cache4Args : CacheArgs {
     const uint8_t* cache;
+    int2* info;          // by sequence: its first slot and its chunks
+    int slots, target, least, grain, fit;   // find_chunk; slots 0: chunks of `chunk` keys, `chunks` of them for each sequence
 };
+
+// Chunks by what the sequences hold: a length, in whole `grain` keys and of `least` at least, that makes `target` of all keys together;
+// with `fit` (64 sequences at most) up to a quarter more, while the sequences' last ones make them more than `target`. Each sequence then has its
+// chunks of equal length. A grid row takes a chunk; target + B of them are always enough, and go to the sequences in order (one may be left
+// empty by the rounding). All of it follows from the lengths, which every wave looks through.
+struct Cache4Chunk {
+    int b, index, length;        // sequence, chunk of it, keys of its chunks
+    int first;                   // of them
+};
+// Sum over the lanes up to this one.
+__device__ __forceinline__ int lanes_before(int x) {
+    x += __builtin_amdgcn_update_dpp(0, x, 0x111, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x112, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x114, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x118, 0xF, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x142, 0xA, 0xF, false);
+    x += __builtin_amdgcn_update_dpp(0, x, 0x143, 0xC, 0xF, false);
+    return x;
+}
+__device__ __forceinline__ bool find_chunk(const Cache4Args& a, int slot, int lane, Cache4Chunk* c) {
+    auto keys_of = [&](int b) { return b < a.B ? cache_keys(a, b) : 0; };
+    const int mine = keys_of(lane);
+    int total = __builtin_amdgcn_readlane(lanes_before(mine), 63);   // (2^30 at most: the launcher's check)
+    for (int b = kWave; b < a.B; b += kWave) total += __builtin_amdgcn_readlane(lanes_before(keys_of(b + lane)), 63);
+    auto grains = [&](unsigned keys) { return static_cast<int>((keys + a.grain - 1u) & -a.grain); };
+    auto share = [&](unsigned keys) { return (keys + a.target - 1u) / static_cast<unsigned>(a.target); };   // of `target` chunks
+    auto chunks_of = [&](int k) { return static_cast<int>((static_cast<unsigned>(k) + c->length - 1u) / static_cast<unsigned>(c->length)); };
+    c->length = __builtin_amdgcn_readfirstlane(max(grains(share(total)), a.least));
+    if (a.fit) {
+        const int most = c->length + c->length / 4;
+        for (int i = 0; i < 3; i++) {
+            const int all = __builtin_amdgcn_readlane(lanes_before(chunks_of(mine)), 63);
+            if (all <= a.target) break;
+            c->length = __builtin_amdgcn_readfirstlane(grains(min(share(static_cast<unsigned>(c->length) * all), static_cast<unsigned>(most))));
+        }
+    }
+    int base = 0;
+    for (int b = 0; b < a.B; b += kWave) {
+        const int n = chunks_of(b == 0 ? mine : keys_of(b + lane));
+        const int upto = base + lanes_before(n);
+        const unsigned long long past = __ballot(upto > slot);
+        if (past) {
+            const int l = __builtin_ctzll(past);
+            const unsigned k = cache_keys(a, b + l), mine_n = __builtin_amdgcn_readlane(n, l);
+            c->b = b + l;
+            c->first = __builtin_amdgcn_readlane(upto, l) - mine_n;
+            c->index = slot - c->first;
+            c->length = grains((k + mine_n - 1u) / mine_n);
+            return true;
+        }
+        base = __builtin_amdgcn_readlane(upto, 63);
+    }
+    return false;
+}
 
 // Values 2 i and 2 i + 1 of a word as half pairs, n 2^-20 each.
 constexpr uint32_t kNibble = 0x00F000F0u;
@@ -103,12 +159,30 @@ __global__ __launch_bounds__(64 * RS * KS, cache4_waves(U, RT)) void cache4_atte
     int* page_of = reinterpret_cast<int*>(stat + W * 16);
 
     const int group = a.group, rows = a.T * group;
-    const int hk = blockIdx.x, chunk = blockIdx.y, b = udiv_magic(blockIdx.z, a.mg_sets), set = blockIdx.z - b * a.sets;
     const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave);
     const int lane = threadIdx.x & (kWave - 1), col = lane & 15, g = lane >> 4;
+    const int hk = blockIdx.x;
+    int b, chunk = blockIdx.y, set, chunk_keys;
+    if (a.slots) {
+        Cache4Chunk c;
+        if (!find_chunk(a, blockIdx.y, lane, &c)) return;
+        b = c.b;
+        chunk = c.index;
+        set = blockIdx.z;
+        chunk_keys = c.length;
+        if (hk == 0 && set == 0 && chunk == 0 && threadIdx.x == 0) a.info[b] = int2{c.first, (cache_keys(a, b) + chunk_keys - 1) / chunk_keys};
+    } else {
+        b = udiv_magic(blockIdx.z, a.mg_sets);
+        set = blockIdx.z - b * a.sets;
+        chunk_keys = a.chunk;
+    }
+    b = __builtin_amdgcn_readfirstlane(b);                           // (the same in all lanes, which the compiler does not see)
+    chunk = __builtin_amdgcn_readfirstlane(chunk);
+    set = __builtin_amdgcn_readfirstlane(set);
+    chunk_keys = __builtin_amdgcn_readfirstlane(chunk_keys);
     const int rs = wave / KS, ks = wave % KS;
-    const int key0 = chunk * a.chunk, page_mask = (1 << a.page_shift) - 1, page0 = key0 >> a.page_shift;
-    const int last_page = min((key0 + a.chunk - 1) >> a.page_shift, a.width - 1);
+    const int key0 = chunk * chunk_keys, page_mask = (1 << a.page_shift) - 1, page0 = key0 >> a.page_shift;
+    const int last_page = min((key0 + chunk_keys - 1) >> a.page_shift, a.width - 1);
     for (int p = page0 + threadIdx.x; p <= last_page; p += 64 * W) {
         const int pg = a.table[static_cast<size_t>(b) * a.width + p];
         page_of[p - page0] = pg >= 0 && pg < a.pages ? pg : -1;
@@ -165,7 +239,7 @@ __global__ __launch_bounds__(64 * RS * KS, cache4_waves(U, RT)) void cache4_atte
 #pragma unroll
         for (int j = 0; j < Words::kOut; j++) st[rt].o[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     }
-    const int keys = cache_keys(a, b), len = max(a.lens[b], 0), n = min(keys - key0, a.chunk);
+    const int keys = cache_keys(a, b), len = max(a.lens[b], 0), n = min(keys - key0, chunk_keys);
     if (n <= 0) return;
     // all weights are 2^-low of themselves, so that no sum of values passes FP32 (those of a head span twice BF16's range)
     const float low = kRescale + 35 - __builtin_clz(keys);
@@ -359,8 +433,8 @@ __global__ __launch_bounds__(64 * RS * KS, cache4_waves(U, RT)) void cache4_atte
     }
 
     // The KS waves of the same rows are joined in LDS, a row tile at a time.
-    const bool whole = keys <= a.chunk;                              // the only chunk: the result itself
-    const size_t part0 = ((static_cast<size_t>(b) * a.Hkv + hk) * a.chunks + chunk) * rows;
+    const bool whole = keys <= chunk_keys;                           // the only chunk: the result itself
+    const size_t part0 = (a.slots ? static_cast<size_t>(hk) * a.slots + blockIdx.y : (static_cast<size_t>(b) * a.Hkv + hk) * a.chunks + chunk) * rows;
 #pragma unroll
     for (int rt = 0; rt < RT; rt++) {
         const Rows4<U>& r = st[rt];
@@ -414,37 +488,145 @@ __global__ __launch_bounds__(64 * RS * KS, cache4_waves(U, RT)) void cache4_atte
     }
 }
 
+// W waves join the chunks of one row: their parts of LPR lanes of 4 values take every kSets-th chunk, four in flight, with the running
+// maximum of a softmax; the parts are joined in a fixed order.
+template <class T, int LPR, int W>
+__global__ __launch_bounds__(256) void cache4_join_kernel(Cache4Args a)
+{
+    static_assert(W == 1 || W == 4, "a wave's row, or a workgroup's");
+    constexpr int kParts = kWave / LPR, kSets = W * kParts;
+    const int own = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wave = W == 1 ? 0 : own;
+    const int lane = threadIdx.x & (kWave - 1), d = 4 * (lane % LPR);
+    const int h = W == 1 ? 4 * blockIdx.x + own : blockIdx.x, t = blockIdx.y, b = blockIdx.z, rows = a.T * a.group;
+    if (h >= a.Hq) return;
+    const int hk = udiv_magic(h, a.mg_group), r = t * a.group + h - hk * a.group;
+    int used;
+    size_t first;
+    if (a.slots) {
+        const int2 i = a.info[b];
+        used = i.y;
+        first = static_cast<size_t>(hk) * a.slots + i.x;
+    } else {
+        used = (cache_keys(a, b) + a.chunk - 1) / a.chunk;
+        first = (static_cast<size_t>(b) * a.Hkv + hk) * a.chunks;
+    }
+    if (used <= 1) return;                                           // the only chunk has written the result
+    const bool in = d < a.D;
+    float m = kNoScore, l = 0.0f;
+    v4f s = {0.0f, 0.0f, 0.0f, 0.0f};
+    for (int c0 = wave * kParts; c0 < used; c0 += 4 * kSets) {
+        v4f x[4];
+        v2f st[4];
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            x[u] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
+            st[u] = v2f{kNoScore, 0.0f};
+            if (c0 + u * kSets >= used) continue;
+            const size_t at = (first + min(c0 + u * kSets + lane / LPR, used - 1)) * rows + r;
+            st[u] = *reinterpret_cast<const v2f*>(a.stat + at * 2);
+            x[u] = *reinterpret_cast<const v4f*>(a.part + at * a.D + (in ? d : 0));
+        }
+#pragma unroll
+        for (int u = 0; u < 4; u++) {
+            if (c0 + u * kSets + lane / LPR >= used) continue;
+            const float mn = fmaxf(m, st[u][0]);
+            const float f = __builtin_amdgcn_exp2f(m - mn), g = __builtin_amdgcn_exp2f(st[u][0] - mn);
+            m = mn;
+            l = __builtin_fmaf(l, f, st[u][1] * g);
+#pragma unroll
+            for (int e = 0; e < 4; e++) s[e] = __builtin_fmaf(s[e], f, x[u][e] * g);
+        }
+    }
+    auto add = [&](float om, float ol, v4f os) {
+        const float mn = fmaxf(m, om);
+        const float f = __builtin_amdgcn_exp2f(m - mn), g = __builtin_amdgcn_exp2f(om - mn);
+        m = mn;
+        l = l * f + ol * g;
+#pragma unroll
+        for (int e = 0; e < 4; e++) s[e] = s[e] * f + os[e] * g;
+    };
+#pragma unroll
+    for (int o = LPR; o < kWave; o <<= 1) {
+        const v4f os = {__shfl_xor(s[0], o, kWave), __shfl_xor(s[1], o, kWave), __shfl_xor(s[2], o, kWave), __shfl_xor(s[3], o, kWave)};
+        add(__shfl_xor(m, o, kWave), __shfl_xor(l, o, kWave), os);
+    }
+    if constexpr (W > 1) {
+        __shared__ v4f sums[W][LPR];
+        __shared__ v2f stat[W];
+        if (lane < LPR) sums[wave][lane] = s;
+        if (lane == 0) stat[wave] = v2f{m, l};
+        __syncthreads();
+        if (wave != 0 || lane >= LPR) return;
+#pragma unroll
+        for (int w = 1; w < W; w++) add(stat[w][0], stat[w][1], sums[w][lane]);
+    }
+    const float inv = l != 0.0f ? 1.0f / l : 0.0f;
+    if (in && lane < LPR)
+        *reinterpret_cast<v2u*>(a.out + ((static_cast<size_t>(b) * a.T + t) * a.Hq + h) * a.D + d) =
+            v2u{T::pack(s[0] * inv, s[1] * inv), T::pack(s[2] * inv, s[3] * inv)};
+}
+
 template <int U, int RS, int KS>
 constexpr int kCache4Lds = RS * KS * 16 * (Words4<U>::kRow * 4 + 8);
+constexpr int kCache4MaxChunk = 16384;   // keys of a chunk by lengths; its pages are looked up in LDS
 
-// Rows of a workgroup: 16, 32, 64 or 128. Chunks such that sequences of the table's length make two workgroups per CU, or three of 64 and
-// 128 rows, which lengths that differ leave to few CUs, of as many keys as there are rows at least (a chunk's sums are as large as its keys
-// and values in 16 bits then) and of 256; and one chunk, without a join, where up to 16 rows have 512 keys, or 1024 and heads for half the CUs.
+struct Cache4Plan {
+    int chunk, chunks;             // keys of a chunk; chunks of a sequence of the table's length
+    int sets;                      // 16-row sets of a workgroup
+    int target, least, grain, fit, slots;   // find_chunk's; slots > 0: chunks by lengths
+};
+
+// Rows of a workgroup: 16, 32, 64 or 128. A chunk has as many keys as there are rows at least (its sums are as large as its keys and values in
+// 16 bits then) and 256; up to 16 rows over 512 keys, or over 1024 with heads for half the CUs, take one chunk, without a join. Sequences of the table's
+// length make two workgroups per CU, or three of 64 and 128 rows. Where that makes longer chunks than the shortest (of 16 rows: than twice that),
+// sequences shorter than the table would leave CUs idle: chunks go by the lengths then, for as many workgroups as the card holds at once, or twice as
+// many of 16 rows, which wait for memory.
 // us, 32 / 8 heads of 128: one token over 500 keys, in one chunk and in chunks of 256, 7.2 and 8.2 (32 sequences 8.0 and 10.6); 32 over 1000, in
-// one and in two, 10.5 and 12.9 (1 over 1000 9.9 and 8.2); 6 trees of 16 drafts, 32 / 4 heads of 128, over 32768, 28001, 16384, 9999, 31000 and 517, with chunks of 512 91, 1024
-// 77, 1536 96, 2048 118; one token over 16 sequences of up to 32768, 1024 67, 2048 62; one over 1000, 128 10.9, 256 9.3.
-CachePlan cache4_plan(int B, int T, int Hq, int Hkv, long long max_keys) {
-    CachePlan p;
+// one and in two, 10.5 and 12.9 (1 over 1000 9.9 and 8.2); one over 1000, 128 keys 10.9, 256 9.3. By the table's length and by the sequences':
+// one token over 16 sequences of up to 32768 64 and 60, over 128 of 2000 with tables of 8192 143 and 54, over 16 of 2000 with tables of 2048 13.8 and 15.3; 16 drafts
+// over 8 sequences of 20 to 4000 25 and 17, 29, 32 / 4 heads, over 18191, 17337, 1374 and six short ones 102 and 61, 16, 32 / 4, over 119 thousand keys of 6 84 and 77.
+Cache4Plan cache4_plan(int B, int T, int Hq, int Hkv, int D, long long max_keys) {
+    Cache4Plan p = {};
     const int rows = T * (Hq / Hkv);
     for (p.sets = 1; 16 * p.sets < rows && p.sets < 8;) p.sets *= 2;
-    const long long heads = static_cast<long long>(B) * Hkv * divup(rows, 16 * p.sets);
+    const long long per_keys = static_cast<long long>(Hkv) * divup(rows, 16 * p.sets), heads = B * per_keys;
     const long long want = std::max<long long>(1, divupll((p.sets >= 4 ? 3 : 2) * default_cu_count(), heads));
-    long long least = std::max(rows, 256);
-    if (p.sets == 1) least = 2 * heads >= default_cu_count() ? 1024 : 512;
-    const long long chunk = divupll(max_keys <= least ? max_keys : std::max(divupll(max_keys, want), std::max<long long>(rows, 256)), 128) * 128;
+    const int least = static_cast<int>(divupll(std::max(rows, 256), 128) * 128);
+    const long long one = p.sets > 1 ? least : 2 * heads >= default_cu_count() ? 1024 : 512;
+    const long long chunk = divupll(max_keys <= one ? max_keys : std::max<long long>(divupll(max_keys, want), least), 128) * 128;
     const long long most = std::max<long long>(kCacheMaxChunk, divupll(divupll(max_keys, kGridRows), 128) * 128);
     p.chunk = static_cast<int>(std::min(chunk, most));
     p.chunks = static_cast<int>(std::max<long long>(1, divupll(max_keys, p.chunk)));
+    if (p.chunks == 1 || p.chunk <= (p.sets == 1 ? 2 : 1) * least || B * max_keys > 1LL << 30) return p;
+    // workgroups that a CU holds at once, by their registers (four waves, or eight for 128 rows of the widest heads)
+    const int at_once = cache4_units(D) <= 4 ? (p.sets == 1 ? 3 : 2) : p.sets == 8 ? 1 : 2;
+    const long long groups = static_cast<long long>(at_once) * default_cu_count() * (p.sets == 1 ? 2 : 1) / per_keys;
+    p.fit = p.sets > 1 && B <= kWave;
+    const long long target = std::max<long long>({1, p.fit ? groups : groups - B / 2, groups / 2, divupll(B * max_keys, kCache4MaxChunk / 2)});
+    if (target + B > kGridRows) return p;
+    p.target = static_cast<int>(target);
+    p.least = p.sets == 1 && one == 1024 ? 1024 : least;
+    p.grain = p.sets >= 4 ? 64 : 128;                                // 32 keys of each of a workgroup's waves for the same rows
+    p.slots = static_cast<int>(target + B);
     return p;
+}
+
+// Workspace: with slots, an int2 for each sequence (in whole 16 bytes); then the chunks' sums, then their maxima and sums of weights.
+size_t cache4_parts(int B, int T, int Hq, const Cache4Plan& p) {
+    return p.slots ? static_cast<size_t>(T) * Hq * p.slots : p.chunks == 1 ? 0 : static_cast<size_t>(B) * T * Hq * p.chunks;
+}
+size_t cache4_info_bytes(int B, const Cache4Plan& p) { return p.slots ? (static_cast<size_t>(B) * sizeof(int2) + 15) / 16 * 16 : 0; }
+size_t cache4_bytes(int B, int T, int Hq, int D, const Cache4Plan& p) {
+    return cache4_info_bytes(B, p) + 4 * cache4_parts(B, T, Hq, p) * (D + 2);
 }
 
 template <class T, int U, int RT, int RS, int KS>
 int launch_cache4(Cache4Args a, hipStream_t s) {
     constexpr int LPR = U <= 2 ? 16 : U <= 4 ? 32 : 64;
-    constexpr int kMost = kCache4Lds<U, RS, KS> + 4 * ((kCacheMaxChunk + 128) / kCache4MinPage + 2);
+    constexpr int kMost = kCache4Lds<U, RS, KS> + 4 * (kCache4MaxChunk / kCache4MinPage + 2);
     static_assert(kMost <= 159 * 1024, "sums and page numbers fit");
-    static_assert(divupll(kCacheMaxKeys, kGridRows) <= kCacheMaxChunk + 128, "the longest table's chunks are a grid's rows");
-    const int lds = kCache4Lds<U, RS, KS> + 4 * ((a.chunk >> a.page_shift) + 2);
+    static_assert(std::max<long long>(kCacheMaxChunk, divupll(kCacheMaxKeys, kGridRows) + 128) <= kCache4MaxChunk, "the longest chunks' pages");
+    const int lds = kCache4Lds<U, RS, KS> + 4 * (((a.slots ? kCache4MaxChunk : a.chunk) >> a.page_shift) + 2);
     const int rows = a.T * (a.Hq / a.Hkv);
     a.sets = divup(rows, 16 * RT * RS);
     a.mg_sets = udiv_multiplier(a.sets);
@@ -452,16 +634,20 @@ int launch_cache4(Cache4Args a, hipStream_t s) {
                                                        hipFuncAttributeMaxDynamicSharedMemorySize, kMost);
     if (attr != hipSuccess) return static_cast<int>(attr);
     // as many sequences at a time as a grid has rows
-    const long long total = a.B, most = kGridRows / a.sets;
+    const long long total = a.B, most = a.slots ? total : kGridRows / a.sets;
     const size_t parts = static_cast<size_t>(a.T) * a.Hq * a.chunks;     // of a sequence
     for (long long b = 0; b < total; b += most) {
         a.B = static_cast<int>(std::min(most, total - b));
-        const dim3 grid(static_cast<unsigned>(a.Hkv), static_cast<unsigned>(a.chunks), static_cast<unsigned>(a.B * a.sets));
+        const dim3 grid(static_cast<unsigned>(a.Hkv), static_cast<unsigned>(a.slots ? a.slots : a.chunks),
+                        static_cast<unsigned>(a.slots ? a.sets : a.B * a.sets));
         cache4_attention_kernel<T, U, RT, RS, KS><<<grid, 64 * RS * KS, lds, s>>>(a);
         int st = launch_status();
-        if (st == FORGE_OK && a.chunks > 1) {
-            const dim3 rows_grid(static_cast<unsigned>(divup(a.Hq, 4)), static_cast<unsigned>(a.T), static_cast<unsigned>(a.B));
-            cache_join_kernel<T, LPR><<<rows_grid, 256, 0, s>>>(a);
+        if (st == FORGE_OK && (a.slots || a.chunks > 1)) {
+            // a wave per row where there are few chunks, or rows enough: 4 x 29 rows of 14 heads 4.0 us, and with four 4.9; 6 x 16 of 32 8.6 and 9.5
+            if ((a.slots ? a.slots : a.chunks) > 16 && static_cast<long long>(a.B) * a.T * a.Hq <= 2048)
+                cache4_join_kernel<T, LPR, 4><<<dim3(a.Hq, a.T, a.B), 256, 0, s>>>(a);
+            else
+                cache4_join_kernel<T, LPR, 1><<<dim3(divup(a.Hq, 4), a.T, a.B), 256, 0, s>>>(a);
             st = launch_status();
         }
         if (st != FORGE_OK) return st;
@@ -487,7 +673,7 @@ int launch_cache4(const Cache4Args& a, int sets, hipStream_t s) {
         if (sets == 4) return launch_cache4<T, U, 2, 2, 2>(a, s);
         // twice the waves while there is a workgroup per CU at most: 4 trees of 29 drafts over 3001, 17, 0 and 2048, 14 / 2 heads of 64, 19.4 -> 16.8 us;
         // with more of them it takes from the others: 6 trees of 16 over 119 thousand keys 77 -> 88
-        const long long groups = static_cast<long long>(a.B) * a.Hkv * divup(a.T * a.group, 128) * a.chunks;
+        const long long groups = static_cast<long long>(a.Hkv) * divup(a.T * a.group, 128) * (a.slots ? a.slots : static_cast<long long>(a.B) * a.chunks);
         return groups <= default_cu_count() ? launch_cache4<T, U, 2, 4, 2>(a, s) : launch_cache4<T, U, 2, 4, 1>(a, s);
     } else {                                                         // (two row tiles a wave do not fit the registers)
         if (sets == 2) return launch_cache4<T, U, 1, 2, 2>(a, s);
@@ -512,7 +698,7 @@ using namespace forge_amd;
 
 extern "C" size_t forge_cache4_attention_workspace_size(int B, int T, int Hq, int Hkv, int D, long long max_keys) {
     if (!cache_shape_ok(B, T, Hq, Hkv, D) || max_keys <= 0 || max_keys > kCacheMaxKeys) return 0;
-    return 4 * cache_floats(B, T, Hq, D, cache4_plan(B, T, Hq, Hkv, max_keys));
+    return cache4_bytes(B, T, Hq, D, cache4_plan(B, T, Hq, Hkv, D, max_keys));
 }
 
 extern "C" int forge_cache4_attention(const uint16_t* q, const uint8_t* cache, const int32_t* page_table, const int32_t* cache_lens,
@@ -529,14 +715,14 @@ extern "C" int forge_cache4_attention(const uint16_t* q, const uint8_t* cache, c
         if (!aligned(p, 16)) return FORGE_EINVAL;
     const long long max_keys = static_cast<long long>(table_width) * page_size;
     if (max_keys > kCacheMaxKeys) return FORGE_EINVAL;
-    const CachePlan p = cache4_plan(B, T, Hq, Hkv, max_keys);
-    const size_t floats = cache_floats(B, T, Hq, D, p);
-    if (floats && (!workspace || workspace_bytes < 4 * floats)) return FORGE_EINVAL;
-    float* part = static_cast<float*>(workspace);
-    const size_t parts = static_cast<size_t>(B) * T * Hq * p.chunks;
+    const Cache4Plan p = cache4_plan(B, T, Hq, Hkv, D, max_keys);
+    const size_t bytes = cache4_bytes(B, T, Hq, D, p), parts = cache4_parts(B, T, Hq, p);
+    if (bytes && (!workspace || workspace_bytes < bytes)) return FORGE_EINVAL;
+    float* part = bytes ? reinterpret_cast<float*>(static_cast<char*>(workspace) + cache4_info_bytes(B, p)) : nullptr;
     const Cache4Args a{{q, nullptr, nullptr, page_table, cache_lens, tree, out, part, part ? part + parts * D : nullptr,
                         B, T, Hq, Hkv, D, pages, __builtin_ctz(static_cast<unsigned>(page_size)), table_width,
-                        p.chunk, p.chunks, Hq / Hkv, 1, udiv_multiplier(Hq / Hkv), 0u, scale}, cache};
+                        p.chunk, p.chunks, Hq / Hkv, 1, udiv_multiplier(Hq / Hkv), 0u, scale},
+                       cache, static_cast<int2*>(workspace), p.slots, p.target, p.least, p.grain, p.fit};
     hipStream_t s = as_stream(stream);
     return dtype == FORGE_FP16 ? launch_cache4<Fp16>(a, p.sets, s) : launch_cache4<Bf16>(a, p.sets, s);
 }

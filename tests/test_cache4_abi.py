@@ -52,12 +52,19 @@ def test_attention(lib):
 
 
 @pytest.mark.parametrize("keys", [(1 << 27) - 2048, (1 << 27) - 1, 1 << 27])
-def test_longest_tables(lib, keys):
-    """Up to 2^27 positions, in no more chunks than a grid has rows, of no more keys than a chunk's page table has place for."""
-    row = (64 + 2) * 4
-    size = lib.forge_cache4_attention_workspace_size(1, 1, 1, 1, 64, keys)
-    assert size % row == 0 and 1 < size // row <= 65535
-    assert -(-keys // (size // row)) <= 2048 + 128
+@pytest.mark.parametrize("B", [1, 40])
+def test_longest_tables(lib, keys, B):
+    """Up to 2^27 positions, in no more chunks than a grid has rows, of no more keys than a chunk's page table has place for:
+    16384 where chunks follow the sequences' lengths (an int2 for each comes first then), and 2176 otherwise."""
+    row, size = (64 + 2) * 4, lib.forge_cache4_attention_workspace_size(B, 1, 1, 1, 64, keys)
+    if B == 1:
+        assert (size - 16) % row == 0
+        chunks = (size - 16) // row
+        assert -(-keys // (chunks - 1)) <= 16384 and 1 < chunks <= 65535
+    else:                                                         # 40 2^27 passes what is counted in 32 bits
+        assert size % (B * row) == 0
+        chunks = size // (B * row)
+        assert -(-keys // chunks) <= 2048 + 128 and 1 < chunks <= 65535
     assert lib.forge_cache4_attention_workspace_size(1, 1, 1, 1, 64, (1 << 27) + 1) == 0
     assert lib.forge_cache4_attention_workspace_size(1, 1, 8, 8, 64, 100) == 0     # one chunk
 

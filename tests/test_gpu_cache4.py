@@ -209,6 +209,47 @@ def test_wide_table(dev):
     run(dev, "float16", [70, 0, 300], 1, 4, 2, 64, 16, width=700)
 
 
+@pytest.mark.parametrize("dt,T,Hq,Hkv,D,page,lens,width", [
+    ("float16", 1, 8, 8, 64, 16, [0, 1, 126, 127, 128, 255, 256, 300, 2000] * 7 + [511, 512], 130),        # more than a wave of sequences
+    ("bfloat16", 1, 4, 4, 8, 16, [3] * 64 + [700] + [0] * 70, 130),
+    ("float16", 1, 8, 8, 128, 64, [6000, 0, 17], 300),
+    ("bfloat16", 1, 4, 1, 256, 32, [0, 9000, 2, 4095], 4100),
+    ("bfloat16", 20, 14, 2, 128, 256, [5, 4001], 250),
+    ("float16", 64, 8, 1, 256, 256, [0, 2500], 420),
+    ("float16", 3, 6, 1, 96, 64, [3000, 1, 129], 2100),
+    ("bfloat16", 1, 8, 2, 64, 128, [30000], 1200)])
+def test_chunks_by_lengths(dev, dt, T, Hq, Hkv, D, page, lens, width):
+    """Tables so long that the chunks' length is made from the sequences' own."""
+    from forge_amd import ops
+    size = ops.cache4_attention_workspace_size(len(lens), T, Hq, Hkv, D, width * page)
+    assert (size - -(-len(lens) // 2) * 16) % (4 * T * Hq * (D + 2)) == 0      # what the first line says holds
+    run(dev, dt, lens, T, Hq, Hkv, D, page, width=width)
+
+
+def test_lengths_between_replays(dev):
+    """The lengths change between replays of one graph, and so do the chunks."""
+    import torch
+    from forge_amd import ops
+    full = [6000, 40, 2500]
+    c = Cache4(full, 1, 8, 64, 64, "float16", dev, 31, width=300)
+    q = queries(3, 1, 8, 64, "float16", dev, 32)
+    ws = torch.full((ops.cache4_attention_workspace_size(3, 1, 8, 8, 64, 300 * 64),), 0xFF, dtype=torch.uint8, device=dev)
+    out = torch.zeros_like(q)
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        ops.cache4_attention(q, c.cache, c.table, c.lens, workspace=ws, out=out)
+    for lens in (full, [0, 0, 0], [6000, 0, 0], [255, 40, 256], [100, 1, 2500], full):
+        c.lens.copy_(torch.tensor(lens, dtype=torch.int32))
+        out.fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, ops.cache4_attention(q, c.cache, c.table, c.lens))
+        for b, n in enumerate(lens):
+            for h in range(8):
+                k, v = ([t[:n + 1, h] for t in x] for x in (c.keys[b], c.values[b]))
+                plain.check(out[b, :, h], q[b, :, h], k, v, torch.ones((1, n + 1), dtype=torch.bool, device=dev), 0.125)
+
+
 def test_row_that_sees_nothing(dev):
     import torch
     from forge_amd import ops
@@ -368,7 +409,7 @@ def test_queries_that_are_not_finite(dev):
 
 @pytest.mark.parametrize("T,dt", [(1, "float16"), (20, "bfloat16")])
 def test_same_bits(dev, T, dt):
-    """The same call gives the same bits, alone and among other sequences, with a given workspace and without."""
+    """The same call gives the same bits, with a given workspace and without."""
     import torch
     from forge_amd import ops
     lens = [700, 33, 1200]
