@@ -56,8 +56,9 @@ __device__ __forceinline__ int lanes_before(int x) {
 __device__ __forceinline__ bool find_chunk(const Cache4Args& a, int slot, int lane, Cache4Chunk* c) {
     auto keys_of = [&](int b) { return b < a.B ? cache_keys(a, b) : 0; };
     const int mine = keys_of(lane);
-    int total = __builtin_amdgcn_readlane(lanes_before(mine), 63);   // (2^30 at most: the launcher's check)
-    for (int b = kWave; b < a.B; b += kWave) total += __builtin_amdgcn_readlane(lanes_before(keys_of(b + lane)), 63);
+    int keys = mine;
+    for (int b = kWave; b < a.B; b += kWave) keys += keys_of(b + lane);
+    const int total = __builtin_amdgcn_readlane(lanes_before(keys), 63);   // (2^30 at most: the launcher's check)
     auto grains = [&](unsigned keys) { return static_cast<int>((keys + a.grain - 1u) & -a.grain); };
     auto share = [&](unsigned keys) { return (keys + a.target - 1u) / static_cast<unsigned>(a.target); };   // of `target` chunks
     auto chunks_of = [&](int k) { return static_cast<int>((static_cast<unsigned>(k) + c->length - 1u) / static_cast<unsigned>(c->length)); };
@@ -568,6 +569,7 @@ __global__ __launch_bounds__(256) void cache4_join_kernel(Cache4Args a)
 
 template <int U, int RS, int KS>
 constexpr int kCache4Lds = RS * KS * 16 * (Words4<U>::kRow * 4 + 8);
+constexpr int kCache4MaxFound = 1024;    // sequences that find_chunk looks through (1024 of 50 to 500 keys 291 -> 202 us, 2048 599 -> 704)
 constexpr int kCache4MaxChunk = 16384;   // keys of a chunk by lengths; its pages are looked up in LDS
 
 struct Cache4Plan {
@@ -597,7 +599,7 @@ Cache4Plan cache4_plan(int B, int T, int Hq, int Hkv, int D, long long max_keys)
     const long long most = std::max<long long>(kCacheMaxChunk, divupll(divupll(max_keys, kGridRows), 128) * 128);
     p.chunk = static_cast<int>(std::min(chunk, most));
     p.chunks = static_cast<int>(std::max<long long>(1, divupll(max_keys, p.chunk)));
-    if (p.chunks == 1 || p.chunk <= (p.sets == 1 ? 2 : 1) * least || B * max_keys > 1LL << 30) return p;
+    if (p.chunks == 1 || p.chunk <= (p.sets == 1 ? 2 : 1) * least || B > kCache4MaxFound || B * max_keys > 1LL << 30) return p;
     // workgroups that a CU holds at once, by their registers (four waves, or eight for 128 rows of the widest heads)
     const int at_once = cache4_units(D) <= 4 ? (p.sets == 1 ? 3 : 2) : p.sets == 8 ? 1 : 2;
     const long long groups = static_cast<long long>(at_once) * default_cu_count() * (p.sets == 1 ? 2 : 1) / per_keys;

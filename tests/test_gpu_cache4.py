@@ -212,6 +212,7 @@ def test_wide_table(dev):
 @pytest.mark.parametrize("dt,T,Hq,Hkv,D,page,lens,width", [
     ("float16", 1, 8, 8, 64, 16, [0, 1, 126, 127, 128, 255, 256, 300, 2000] * 7 + [511, 512], 130),        # more than a wave of sequences
     ("bfloat16", 1, 4, 4, 8, 16, [3] * 64 + [700] + [0] * 70, 130),
+    ("float16", 1, 2, 2, 8, 16, [7 * b % 300 for b in range(250)] + [2000, 0, 1000], 700),
     ("float16", 1, 8, 8, 128, 64, [6000, 0, 17], 300),
     ("bfloat16", 1, 4, 1, 256, 32, [0, 9000, 2, 4095], 4100),
     ("bfloat16", 20, 14, 2, 128, 256, [5, 4001], 250),
