@@ -9,7 +9,7 @@
 // more as a rule, is gathered in LDS and ranked by counting, with ties by place. Where LDS has no room for that, the places are filled one
 // after the other.
 //
-// us, pieces + merge: 32 x 8 beams of 131072 FP32 logits, three in ten ended, 20.4 (94 MB at 4.6 TB/s) + 8.2; 4 beams of 32000 FP16 4.9 + 5.8, two chains
+// us, pieces + merge: 32 x 8 beams of 131072 FP32 logits, three in ten ended, 19.8 (94 MB at 4.7 TB/s) + 8.1; 4 beams of 32000 FP16 4.6 + 5.2, two chains
 // of dependent steps.
 #include "float16_types.h"
 
