@@ -6,11 +6,13 @@
 // are merged by a workgroup per request, in 64 bits: the scores of two beams may differ in the last place only.
 //
 // The largest of many: of 64 groups' maxima the count-th largest is a bound that at least `count` numbers reach, and what reaches it, few
-// more as a rule, is gathered in LDS and ranked by counting, with ties by place. Where LDS has no room for that, the places are filled one
-// after the other.
+// more as a rule, is gathered in LDS and ranked by counting, with ties by place. Where more are found, a better bound comes from those (most lists
+// empty, or many places), or they are equal ones (a mask's lowest value): those above the bound are ranked and the first places that equal
+// it follow. Where LDS has no room even so, the places are filled one after the other.
 //
-// us, pieces + merge: 32 x 8 beams of 131072 FP32 logits, three in ten ended, 19.8 (94 MB at 4.7 TB/s) + 8.1; 4 beams of 32000 FP16 4.6 + 5.2, two chains
-// of dependent steps.
+// us, pieces + merge: 32 x 8 beams of 131072 FP32 logits, three in ten ended, 18.4 (94 MB at 5.1 TB/s) + 8.2; 4 beams of 32000 FP16 4.6 + 5.7, two chains
+// of dependent steps. In all, 8 x 4 beams of 128000, 16 places: 15; all but 20 tokens at FP16's lowest value 20 (place after place 65), all logits
+// equal 41 (60); 4 x 8 of 50257, 53 places: 25 (ranking all that the first bound leaves 49), one live beam 25 (137), all equal 33 (433).
 #include "float16_types.h"
 
 #include <algorithm>
@@ -22,6 +24,7 @@ namespace forge_amd {
 constexpr int kBeamCount = 64;      // places
 constexpr int kBeamWidth = 1024;    // beams of a request
 constexpr int kBeamRoom = 1024;     // numbers that are ranked at once
+constexpr int kBeamFew = 256;       // and as many as are ranked without looking for a better bound
 constexpr int kBeamThreads = 256, kMergeThreads = 512;
 
 struct BeamPiece {       // of a row: its largest logit and sum of exp(logit - largest)
@@ -173,7 +176,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_piece_kernel(BeamArgs a)
     __shared__ double part_sum[4];
     __shared__ float part_top[4], bound_of;
     __shared__ BeamKey part_key[4];
-    __shared__ int total;
+    __shared__ int total, part_count[2][4];
 
     const unsigned row = blockIdx.x / static_cast<unsigned>(a.splits), split = blockIdx.x - row * a.splits;
     if (a.ended && a.ended[row]) return;                             // its one candidate needs no logits
@@ -183,19 +186,21 @@ __global__ __launch_bounds__(kBeamThreads) void beam_piece_kernel(BeamArgs a)
     const typename L::Elem* p = static_cast<const typename L::Elem*>(a.logits) + batch * a.batch_stride + beam * a.beam_stride + first;
 
     typedef v4u loose __attribute__((aligned(2)));
-    v4u v[VEC];
-#pragma unroll
-    for (int i = 0; i < VEC; i++) {
+    auto load = [&](int i) {
         const int at = (i * kBeamThreads + tid) * L::kPer;
-        v[i] = v4u{1u, 1u, 1u, 1u} * L::nothing();
+        v4u x = v4u{1u, 1u, 1u, 1u} * L::nothing();
         if (at + L::kPer <= n) {
-            v[i] = *reinterpret_cast<const loose*>(p + at);
+            x = *reinterpret_cast<const loose*>(p + at);
         } else if (at < n) {
 #pragma unroll
             for (int e = 0; e < L::kPer; e++)
-                if (at + e < n) L::set(v[i], e, p[at + e]);
+                if (at + e < n) L::set(x, e, p[at + e]);
         }
-    }
+        return x;
+    };
+    v4u v[VEC];
+#pragma unroll
+    for (int i = 0; i < VEC; i++) v[i] = load(i);
 
     float most = -INFINITY;
 #pragma unroll
@@ -227,32 +232,79 @@ __global__ __launch_bounds__(kBeamThreads) void beam_piece_kernel(BeamArgs a)
     }
     __syncthreads();
     const float bound = bound_of;
-    if (most >= bound) {
+    auto gather = [&](const v4u& x, int i, auto hit) {
+        uint32_t hits = 0u;
 #pragma unroll
-        for (int i = 0; i < VEC; i++) {
-            uint32_t hits = 0u;
+        for (int e = 0; e < L::kPer; e++) hits |= hit(L::value(x, e)) ? 1u << e : 0u;
+        if (!hits) return;
 #pragma unroll
-            for (int e = 0; e < L::kPer; e++) hits |= L::value(v[i], e) >= bound ? 1u << e : 0u;
-            if (!hits) continue;
-#pragma unroll
-            for (int e = 0; e < L::kPer; e++) {
-                if (!(hits >> e & 1u)) continue;
-                const int at = atomicAdd(&total, 1);
-                if (at < kBeamRoom) found[at] = beam_key(L::value(v[i], e), (i * kBeamThreads + tid) * L::kPer + e);
-            }
+        for (int e = 0; e < L::kPer; e++) {
+            if (!(hits >> e & 1u)) continue;
+            const int at = atomicAdd(&total, 1);
+            if (at < kBeamRoom) found[at] = beam_key(L::value(x, e), (i * kBeamThreads + tid) * L::kPer + e);
         }
-    }
-    __syncthreads();
+    };
     BeamEntry* out = a.entries + (static_cast<size_t>(row) * a.splits + split) * a.count;
     auto put = [&](int place, BeamKey k) { out[place] = k ? BeamEntry{key_value(k), first + key_place(k)} : BeamEntry{0.0f, -1}; };
-    const int got = total;
-    if (got <= kBeamRoom) {
+    auto rank = [&](int got) {
         for (int i = tid; i < got; i += kBeamThreads) {
             const BeamKey k = found[i];
-            int rank = 0;
+            int place = 0;
 #pragma unroll 8
-            for (int j = 0; j < got; j++) rank += found[j] > k;
-            if (rank < a.count) put(rank, k);
+            for (int j = 0; j < got; j++) place += found[j] > k;
+            if (place < a.count) put(place, k);
+        }
+    };
+    if (most >= bound) {
+#pragma unroll
+        for (int i = 0; i < VEC; i++) gather(v[i], i, [&](float x) { return x >= bound; });
+    }
+    __syncthreads();
+    int got = total;
+    if (got <= 3 * kBeamFew / 2) {
+        rank(got);
+        for (int i = got + tid; i < a.count; i += kBeamThreads) put(i, 0);
+        return;
+    }
+    // Many, as a rule equal ones (a mask's lowest value): those above the bound, then the first places that equal it. (Loaded again, or the registers
+    // would be kept for it.)
+    __syncthreads();
+    if (tid == 0) total = 0;
+    __syncthreads();
+    if (most > bound) {
+#pragma unroll 1
+        for (int i = 0; i < VEC; i++) gather(load(i), i, [&](float x) { return x > bound; });
+    }
+    __syncthreads();
+    got = total;
+    if (got <= kBeamRoom) {
+        rank(got);
+#pragma unroll 1
+        for (int i = 0; i < VEC; i++) {
+            if (got >= a.count) return;
+            const v4u x = load(i);
+            int mine = 0;
+#pragma unroll
+            for (int e = 0; e < L::kPer; e++) mine += L::value(x, e) == bound;
+            int place = mine;                                        // of the thread's last one, in its wave
+#pragma unroll
+            for (int o = 1; o < kWave; o <<= 1) {
+                const int before = __shfl_up(place, o, kWave);
+                place += lane >= o ? before : 0;
+            }
+            if (lane == kWave - 1) part_count[i & 1][wave] = place;
+            __syncthreads();
+            place += got - mine;
+            for (int w = 0; w < 4; w++) {
+                place += w < wave ? part_count[i & 1][w] : 0;
+                got += part_count[i & 1][w];
+            }
+#pragma unroll
+            for (int e = 0; e < L::kPer; e++) {
+                if (L::value(x, e) != bound) continue;
+                if (place < a.count) put(place, beam_key(bound, (i * kBeamThreads + tid) * L::kPer + e));
+                place++;
+            }
         }
         for (int i = got + tid; i < a.count; i += kBeamThreads) put(i, 0);
         return;
@@ -260,14 +312,16 @@ __global__ __launch_bounds__(kBeamThreads) void beam_piece_kernel(BeamArgs a)
     BeamKey last = ~0ull;
     for (int place = 0; place < a.count; place++) {
         BeamKey next = 0;
-#pragma unroll
-        for (int i = 0; i < VEC; i++)
+#pragma unroll 1
+        for (int i = 0; i < VEC; i++) {
+            const v4u v_i = load(i);
 #pragma unroll
             for (int e = 0; e < L::kPer; e++) {
-                const float x = L::value(v[i], e);
+                const float x = L::value(v_i, e);
                 const BeamKey k = beam_key(x, (i * kBeamThreads + tid) * L::kPer + e);
                 if (x >= -FLT_MAX && k < last && k > next) next = k;
             }
+        }
 #pragma unroll
         for (int o = 1; o < kWave; o <<= 1) next = max(next, static_cast<BeamKey>(__shfl_xor(next, o, kWave)));
         if (lane == 0) part_key[wave] = next;
@@ -291,13 +345,16 @@ __device__ __forceinline__ bool beam_before(const BeamCandidate& x, const BeamCa
 __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a)
 {
     constexpr int kWaves = kMergeThreads / kWave;
-    __shared__ double shift[kBeamWidth];     // score - logsumexp, -inf for a beam without candidates
+    // a beam's largest logit, and its score - log of the sum of exp(logit - largest), -inf for a beam without candidates (apart, or logits near the
+    // type's lowest value would take the score with them)
+    __shared__ double shift[kBeamWidth];
+    __shared__ float largest[kBeamWidth];
     __shared__ NthGroup<double, kMergeThreads> groups;
     __shared__ BeamCandidate found[kBeamRoom];
     __shared__ BeamCandidate part[kWaves];
     __shared__ int queue[kBeamRoom];
     __shared__ double bound_of;
-    __shared__ int total, waiting;
+    __shared__ int total, waiting, part_count[2][kWaves];
     const int tid = threadIdx.x, lane = tid & (kWave - 1), wave = tid / kWave;
     const size_t row0 = static_cast<size_t>(blockIdx.x) * a.W;
     const int lists = a.W * a.splits, deep = max(1, min(a.count, kMergeThreads / lists));
@@ -319,7 +376,10 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a)
         }
         // rows with an infinity or NaN have no sum, and rows of -inf only a sum of zero
         const bool live = ended || (sum > 0.0 && sum < INFINITY && top < INFINITY);
-        if (lane == 0) shift[w] = live && fabs(score) < INFINITY ? (ended ? score : score - (top + log(sum))) : -INFINITY;
+        if (lane == 0) {
+            shift[w] = live && fabs(score) < INFINITY ? (ended ? score : score - log(sum)) : -INFINITY;
+            largest[w] = top;
+        }
     }
     if (tid == 0) total = waiting = 0;
     __syncthreads();
@@ -329,7 +389,7 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a)
     // (the lists of a beam that has ended or has no candidates hold anything)
     auto score_of = [&](int list, const BeamEntry& e) -> double {
         const int w = beam_of(list);
-        return shift[w] == -INFINITY || ended(w) || e.token < 0 ? -INFINITY : e.logit + shift[w];
+        return shift[w] == -INFINITY || ended(w) || e.token < 0 ? -INFINITY : (static_cast<double>(e.logit) - largest[w]) + shift[w];
     };
     auto candidate = [&](int list, int depth) -> BeamCandidate {
         const BeamEntry e = entries[static_cast<size_t>(list) * a.count + depth];
@@ -349,49 +409,66 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a)
     const double nth = groups.nth(a.count - 1);
     if (tid == 0) bound_of = fmax(nth, -DBL_MAX);
     __syncthreads();
-    const double bound = bound_of;
+    double bound = bound_of;
     auto gather = [&](const BeamCandidate& c) {
         const int at = atomicAdd(&total, 1);
         if (at < kBeamRoom) found[at] = c;
     };
     // What reaches the bound of those entries, and the rest of the lists (few) whose last one of them does: all their entries at once. (Entry by
     // entry, one list's 16 took 9 us.)
-    auto rest = [&](int list) {
-        if (deep == a.count) return;
-        const int at = atomicAdd(&waiting, 1);
-        if (at < kBeamRoom) {
-            queue[at] = list;
-            return;
+    auto collect = [&](auto reaches) {
+        auto rest = [&](int list) {
+            if (deep == a.count) return;
+            const int at = atomicAdd(&waiting, 1);
+            if (at < kBeamRoom) {
+                queue[at] = list;
+                return;
+            }
+            for (int depth = deep; depth < a.count; depth++) {
+                const BeamCandidate c = candidate(list, depth);
+                if (!reaches(c.score)) break;
+                gather(c);
+            }
+        };
+        if (reaches(score0)) {
+            gather({score0, place_of(beam_of(list0), mine.token)});
+            if (depth0 == deep - 1) rest(list0);
         }
-        for (int depth = deep; depth < a.count; depth++) {
-            const BeamCandidate c = candidate(list, depth);
-            if (!(c.score >= bound)) break;
+        for (int list = tid + kMergeThreads; list < lists; list += kMergeThreads) {
+            const BeamCandidate c = candidate(list, 0);
+            if (!reaches(c.score)) continue;
             gather(c);
+            rest(list);
         }
+        __syncthreads();
+        const int left = a.count - deep, queued = min(waiting, kBeamRoom) * left;
+        for (int i = tid; i < queued; i += kMergeThreads) {
+            const int q = i / left;
+            const BeamCandidate c = candidate(queue[q], deep + i - q * left);
+            if (reaches(c.score)) gather(c);
+        }
+        if (a.ended)
+            for (int w = tid; w < a.W; w += kMergeThreads) {
+                const BeamCandidate c = own(w);
+                if (reaches(c.score)) gather(c);
+            }
+        __syncthreads();
     };
-    if (score0 >= bound) {
-        gather({score0, place_of(beam_of(list0), mine.token)});
-        if (depth0 == deep - 1) rest(list0);
-    }
-    for (int list = tid + kMergeThreads; list < lists; list += kMergeThreads) {
-        const BeamCandidate c = candidate(list, 0);
-        if (!(c.score >= bound)) continue;
-        gather(c);
-        rest(list);
-    }
-    __syncthreads();
-    const int left = a.count - deep, queued = min(waiting, kBeamRoom) * left;
-    for (int i = tid; i < queued; i += kMergeThreads) {
-        const int q = i / left;
-        const BeamCandidate c = candidate(queue[q], deep + i - q * left);
-        if (c.score >= bound) gather(c);
-    }
-    if (a.ended)
-        for (int w = tid; w < a.W; w += kMergeThreads) {
-            const BeamCandidate c = own(w);
-            if (c.score >= bound) gather(c);
+    // A better bound from what was found, if it is one.
+    auto better = [&]() {
+        best = -INFINITY;
+        for (int i = tid; i < min(total, kBeamRoom); i += kMergeThreads) best = fmax(best, found[i].score);
+        groups.part[wave][lane] = best;
+        const double nth = groups.nth(a.count - 1);
+        if (tid == 0) {
+            bound_of = fmax(nth, bound);
+            total = waiting = 0;
         }
-    __syncthreads();
+        __syncthreads();
+        const bool risen = bound_of > bound;
+        bound = bound_of;
+        return risen;
+    };
     const size_t out = static_cast<size_t>(blockIdx.x) * a.count;
     auto put = [&](int place, const BeamCandidate& c) {
         const bool some = c.score > -INFINITY;
@@ -400,14 +477,49 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a)
         a.out_tokens[out + place] = some ? static_cast<int>(c.place & 0xFFFFFFFFu) : -1;
     };
     const BeamCandidate none = {-INFINITY, ~0ull};
-    const int got = total;
-    if (got <= kBeamRoom) {
+    auto rank = [&](int got) {
         for (int i = tid; i < got; i += kMergeThreads) {
             const BeamCandidate c = found[i];
-            int rank = 0;
+            int place = 0;
 #pragma unroll 4
-            for (int j = 0; j < got; j++) rank += beam_before(found[j], c);
-            if (rank < a.count) put(rank, c);
+            for (int j = 0; j < got; j++) place += beam_before(found[j], c);
+            if (place < a.count) put(place, c);
+        }
+    };
+    for (int round = 0; round < 8; round++) {
+        collect([&](double x) { return x >= bound; });
+        int got = total;
+        if (got <= kBeamFew) {
+            rank(got);
+            for (int i = got + tid; i < a.count; i += kMergeThreads) put(i, none);
+            return;
+        }
+        if (better()) continue;
+        // Many equal ones: those above the bound, then the first that equal it, in the order of beams, pieces and lists.
+        collect([&](double x) { return x > bound; });
+        got = total;
+        if (got > kBeamRoom) {                                       // (all of them are above it)
+            better();
+            continue;
+        }
+        rank(got);
+        const int all = lists * a.count;
+        for (int i0 = 0, turn = 0; i0 < all && got < a.count; i0 += kMergeThreads, turn ^= 1) {
+            const int i = i0 + tid, list = static_cast<unsigned>(i) / static_cast<unsigned>(a.count), w = beam_of(list);
+            BeamCandidate c = none;
+            if (i < all) {
+                if (!ended(w)) c = candidate(list, i - list * a.count);
+                else if (i == w * a.splits * a.count) c = own(w);
+            }
+            const unsigned long long equal = __ballot(c.score == bound);
+            if (lane == 0) part_count[turn][wave] = __popcll(equal);
+            __syncthreads();
+            int place = got + __popcll(equal & ((1ull << lane) - 1ull));
+            for (int v = 0; v < kWaves; v++) {
+                place += v < wave ? part_count[turn][v] : 0;
+                got += part_count[turn][v];
+            }
+            if (c.score == bound && place < a.count) put(place, c);
         }
         for (int i = got + tid; i < a.count; i += kMergeThreads) put(i, none);
         return;

@@ -24,6 +24,7 @@ def plain(logits, scores, count, ended=None, end_token=0):
             row = x[b, w]
             ok = torch.isfinite(prev[b, w]) and not row.isnan().any() and not (row == float("inf")).any() and (row > float("-inf")).any()
             if ok:
+                row = row - row.max()                 # (first: logits near a type's lowest value are all that 64 bits hold)
                 flat[b, w] = row - torch.logsumexp(row, 0) + prev[b, w]
     order = flat.flatten(1).sort(dim=-1, descending=True, stable=True)
     return order.values[:, :count], order.indices[:, :count], flat
@@ -155,6 +156,36 @@ def test_banned_and_odd_rows(dev):
     x[:] = float("-inf")
     _, _, got = run(dev, "float16", 4, 4, 3000, 3, logits=x, scores=scores_of(4, 4, dev, 10))
     assert (got[1] == -1).all()
+
+
+@pytest.mark.parametrize("dt", ["float16", "bfloat16", "float32"])
+@pytest.mark.parametrize("B,W,V,count", [(1, 4, 9001, 8), (1, 2, 20000, 64), (40, 8, 16500, 30)])
+def test_masks_of_the_lowest_value(dev, dt, B, W, V, count):
+    """A few tokens are allowed and the others hold the type's lowest value, which is a candidate still: thousands of equal ones in
+    each piece, of which the first are taken. Then many allowed, and rows of two values."""
+    import torch
+    d = getattr(torch, dt)
+    g = torch.Generator().manual_seed(V)
+    full = logits_of(B, W, V, dt, dev, 21)
+    for allowed in (0, 3, 20, 500):
+        x = torch.full_like(full, torch.finfo(d).min)
+        some = torch.randperm(V, generator=g)[:allowed].to(dev)
+        x[:, :, some] = full[:, :, some]
+        run(dev, dt, B, W, V, count, logits=x)
+    run(dev, dt, B, W, V, count, logits=(full > 2.0).to(d))
+    run(dev, dt, B, W, V, count, logits=(full > -2.0).to(d) * 3)
+
+
+@pytest.mark.parametrize("dt", ["bfloat16", "float32"])
+@pytest.mark.parametrize("W,V", [(9, 100000), (3, 70000), (40, 9000)])
+def test_many_places_of_few_live_beams(dev, dt, W, V):
+    """Most lists are empty, so that far more candidates than there is room for reach the first bound."""
+    import torch
+    ended = torch.ones((2, W), dtype=torch.bool, device=dev)
+    ended[:, W // 2] = False
+    ended[1, -1] = False
+    run(dev, dt, 2, W, V, 60, ended=ended, end_token=11)
+    run(dev, dt, 2, W, V, 60)
 
 
 def test_ended(dev):
