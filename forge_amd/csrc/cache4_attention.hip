@@ -579,12 +579,13 @@ struct Cache4Plan {
 };
 
 // Rows of a workgroup: 16, 32, 64 or 128. A chunk has as many keys as there are rows at least (its sums are as large as its keys and values in
-// 16 bits then) and 256; up to 16 rows over 512 keys, or over 1024 with heads for half the CUs, take one chunk, without a join. Sequences of the table's
-// length make two workgroups per CU, or three of 64 and 128 rows. Where that makes longer chunks than the shortest (of 16 rows: than twice that),
+// 16 bits then) and 256; up to 16 rows over 512 keys, or over 1024 with heads for half the CUs, and more rows over 384 or 512, take one chunk, without a
+// join. Sequences of the table's length make two workgroups per CU, or three of 64 and 128 rows. Where that makes longer chunks than the shortest (of 16 rows: than twice that),
 // sequences shorter than the table would leave CUs idle: chunks go by the lengths then, for as many workgroups as the card holds at once, or twice as
 // many of 16 rows, which wait for memory.
 // us, 32 / 8 heads of 128: one token over 500 keys, in one chunk and in chunks of 256, 7.2 and 8.2 (32 sequences 8.0 and 10.6); 32 over 1000, in
-// one and in two, 10.5 and 12.9 (1 over 1000 9.9 and 8.2); one over 1000, 128 keys 10.9, 256 9.3. By the table's length and by the sequences':
+// one and in two, 10.5 and 12.9 (1 over 1000 9.9 and 8.2); one over 1000, 128 keys 10.9, 256 9.3; 16 drafts over 8 x 300, in two
+// and in one, 15.9 and 14.3, 4 drafts, 64 / 8 heads, over 32 x 480 21.5 and 12.8. By the table's length and by the sequences':
 // one token over 16 sequences of up to 32768 64 and 60, over 128 of 2000 with tables of 8192 143 and 54, over 16 of 2000 with tables of 2048 13.8 and 15.3; 16 drafts
 // over 8 sequences of 20 to 4000 25 and 17, 29, 32 / 4 heads, over 18191, 17337, 1374 and six short ones 102 and 61, 16, 32 / 4, over 119 thousand keys of 6 84 and 77.
 Cache4Plan cache4_plan(int B, int T, int Hq, int Hkv, int D, long long max_keys) {
@@ -594,7 +595,8 @@ Cache4Plan cache4_plan(int B, int T, int Hq, int Hkv, int D, long long max_keys)
     const long long per_keys = static_cast<long long>(Hkv) * divup(rows, 16 * p.sets), heads = B * per_keys;
     const long long want = std::max<long long>(1, divupll((p.sets >= 4 ? 3 : 2) * default_cu_count(), heads));
     const int least = static_cast<int>(divupll(std::max(rows, 256), 128) * 128);
-    const long long one = p.sets > 1 ? least : 2 * heads >= default_cu_count() ? 1024 : 512;
+    const bool many = 2 * heads >= default_cu_count();
+    const int one = std::max(least, p.sets == 1 ? (many ? 1024 : 512) : many ? 512 : 384);
     const long long chunk = divupll(max_keys <= one ? max_keys : std::max<long long>(divupll(max_keys, want), least), 128) * 128;
     const long long most = std::max<long long>(kCacheMaxChunk, divupll(divupll(max_keys, kGridRows), 128) * 128);
     p.chunk = static_cast<int>(std::min(chunk, most));
@@ -607,7 +609,7 @@ Cache4Plan cache4_plan(int B, int T, int Hq, int Hkv, int D, long long max_keys)
     const long long target = std::max<long long>({1, p.fit ? groups : groups - B / 2, groups / 2, divupll(B * max_keys, kCache4MaxChunk / 2)});
     if (target + B > kGridRows) return p;
     p.target = static_cast<int>(target);
-    p.least = p.sets == 1 && one == 1024 ? 1024 : least;
+    p.least = many ? one : least;
     p.grain = p.sets >= 4 ? 64 : 128;                                // 32 keys of each of a workgroup's waves for the same rows
     p.slots = static_cast<int>(target + B);
     return p;
