@@ -587,7 +587,7 @@ struct Cache4Plan {
 // one and in two, 10.5 and 12.9 (1 over 1000 9.9 and 8.2); one over 1000, 128 keys 10.9, 256 9.3; 16 drafts over 8 x 300, in two
 // and in one, 15.9 and 14.3, 4 drafts, 64 / 8 heads, over 32 x 480 21.5 and 12.8. By the table's length and by the sequences':
 // one token over 16 sequences of up to 32768 64 and 60, over 128 of 2000 with tables of 8192 143 and 54, over 16 of 2000 with tables of 2048 13.8 and 15.3; 16 drafts
-// over 8 sequences of 20 to 4000 25 and 17, 29, 32 / 4 heads, over 18191, 17337, 1374 and six short ones 102 and 61, 16, 32 / 4, over 119 thousand keys of 6 84 and 77.
+// over 8 sequences of 20 to 4000 25 and 17, 29, 32 / 4 heads, over 18191, 17337, 1374 and six short ones 102 and 61, 16, 32 / 4, over 119 thousand keys of 6 84 and 78.
 Cache4Plan cache4_plan(int B, int T, int Hq, int Hkv, int D, long long max_keys) {
     Cache4Plan p = {};
     const int rows = T * (Hq / Hkv);
@@ -647,8 +647,9 @@ int launch_cache4(Cache4Args a, hipStream_t s) {
         cache4_attention_kernel<T, U, RT, RS, KS><<<grid, 64 * RS * KS, lds, s>>>(a);
         int st = launch_status();
         if (st == FORGE_OK && (a.slots || a.chunks > 1)) {
-            // a wave per row where there are few chunks, or rows enough: 4 x 29 rows of 14 heads 4.0 us, and with four 4.9; 6 x 16 of 32 8.6 and 9.5
-            if ((a.slots ? a.slots : a.chunks) > 16 && static_cast<long long>(a.B) * a.T * a.Hq <= 2048)
+            // a wave per row where there are few chunks: 4 x 29 rows of 14 heads, 12 chunks, 4.0 us, with four waves 4.9; 18 x 12 of 32 heads, up to 80
+            // chunks, 11.2 and 8.0 (6 x 16 of 32 heads, up to 33 but most of them, 8.7 and 9.7)
+            if (a.slots ? a.slots > std::max(16, 4 * a.B) : a.chunks > 16)
                 cache4_join_kernel<T, LPR, 4><<<dim3(a.Hq, a.T, a.B), 256, 0, s>>>(a);
             else
                 cache4_join_kernel<T, LPR, 1><<<dim3(divup(a.Hq, 4), a.T, a.B), 256, 0, s>>>(a);
