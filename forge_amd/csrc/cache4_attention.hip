@@ -14,8 +14,8 @@
 // Masked where they are, at bits 0 and 16 too (n 2^-24, of which 2^-14 is dropped), they take one shift for 8 values instead of
 // three, 82.3 for 85.5 us of 6 trees (below).
 // Weights w = p s' are rounded to FP16, in either type, the row's largest at 2^4 or above; sums are FP32. v is taken as (m' + 8 s') + s' (n' - 8):
-// sum w n' less 8 times the sum of the same rounded w, so that a rounding weighs with n' - 8 (a result's error in the 2-norm, FP16 values: 2.4e-4 over
-// long caches; with n' 5.4e-4; rounding the exact result alone 2.0e-4).
+// sum w n' less 8 times the sum of the same rounded w, so that a rounding weighs with n' - 8 (a result's error in the 2-norm, FP16 values: 2.4e-4 to
+// 2.8e-4; with n' 5.4e-4; rounding the exact result alone 2.1e-4).
 //
 // Bound: reading the cache for up to 16 rows: one token over 16 sequences of 278 thousand keys, 32 / 8 heads of 128, 55 us, 5.5 TB/s of 303 MB (and
 // 4.8 for the join of the chunks; 16-bit caches read 3.8 times as much). Many rows: the vector units. 6 trees of 16 drafts, 32 / 4 heads of
