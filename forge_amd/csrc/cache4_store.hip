@@ -116,9 +116,9 @@ __device__ __forceinline__ uint32_t quantize_head(v4u own, bool in, uint32_t* nu
     float n[8], off = s < T::kNormal ? 1.0f : 0.0f;
 #pragma unroll
     for (int e = 0; e < 8; e++) {
-        const float q = (x[e] * 0.5f - m) * inv;
-        n[e] = q + kWhole;
-        off = fmaxf(off, fabsf(q - (n[e] - kWhole)));
+        const float q = x[e] * 0.5f - m;
+        n[e] = __builtin_fmaf(q, inv, kWhole);
+        off = fmaxf(off, fabsf(__builtin_fmaf(q, inv, kWhole - n[e])));
     }
     if (__any(!(off < 0.49999f))) {
         asm volatile("" : "+v"(n[0]));                               // (the compiler would divide in any case)
