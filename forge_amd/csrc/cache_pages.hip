@@ -3,8 +3,9 @@
 // fork_pages: new row r goes on from row p of its group, parents[r] of it (none: the row ends). It names p's full pages again, without a copy;
 // refs counts the names of each page. The page of its next token is p's own where p's first child takes it and nobody else
 // names it, else the lowest free page not yet taken, the next for each row in order; the filled part of p's page is then to be copied (src, dst). Pages that
-// this call frees are not taken by it, so no copied page is written. Counts are added to with integer atomics,
-// whose order does not matter; everything else is in the rows' order.
+// this call frees are not taken by it, so no copied page is written. A row without a free page to copy into has lost the tokens of that page, which
+// its entry of -1 beside a length inside the page says to the next call: rows that would go on from it end there, since the page that they would
+// get is new, or was another row's. Counts are added to with integer atomics, whose order does not matter; everything else is in the rows' order.
 //
 // Bound: latency. Small tables and pools take one workgroup that holds all counts in LDS (4 rows of 40 entries 3.6 us), others two launches:
 // first, a workgroup looks at the rows (first children, places among the takers) while others copy the counts and list the free pages of 1024 pages
@@ -63,6 +64,7 @@ __device__ __forceinline__ ForkRow fork_row(const ForkArgs& a, int parent) {
     row.len = min(max(a.lens[parent], 0), a.width << a.page_shift);
     const int at = row.len >> a.page_shift;
     const int pg = at < a.width ? a.table[static_cast<size_t>(parent) * a.width + at] : -1;
+    if (pg < 0 && (row.len & ((1 << a.page_shift) - 1)) != 0) return {-1, 0, -1, -1};   // its last tokens are lost
     row.last = pg >= 0 && pg < a.pages ? pg : -1;
     return row;
 }
@@ -100,6 +102,7 @@ __global__ __launch_bounds__(kForkThreads) void fork_small_kernel(ForkArgs a)
     __syncthreads();
     if (p >= 0) atomicMin(&first[p], tid);
     ForkRow row = fork_row(a, p);
+    p = row.parent;
     int base = 0;                                                    // the lowest free pages, one a row at most
 #pragma unroll
     for (int i = 0; i < kSmallPages / kForkThreads; i++) {

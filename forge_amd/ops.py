@@ -1087,7 +1087,8 @@ def fork_pages(page_table: torch.Tensor, cache_lens: torch.Tensor, parents: torc
     """forge_fork_pages: the page table (rows, width) after each row went on from another row of its request: parents
     (requests, rows of each) holds their numbers within the request (anything else ends the row), as beam_select returns them. Full
     pages are shared (refs (pages,) counts their names), a page in use is the first child's and copied for the others, and every row has a page for
-    its next token. All int32; the outputs are not the inputs."""
+    its next token, or the slot -1 where none is free; rows that go on from one that had no page to copy its last tokens into end. All
+    int32; the outputs are not the inputs."""
     if out is None and workspace is None:
         made = _fast_new("fork_pages_new", page_table, cache_lens, parents, refs, page_size)
         if made is not None:

@@ -416,7 +416,9 @@ int forge_beam_select(const void* logits, const float* scores, const uint8_t* en
  * the page of its next token (position cache_lens) is the parent's where r is the parent's first child and
  * refs, the number of names of each page, is 1 there; else the lowest page with refs 0 that no row before r takes. Where the parent's
  * page holds tokens, src[r], dst[r] say what is to be copied (-1, -1: nothing). Pages that this call releases
- * are not taken by it. Without room in the table or a free page the row has no page (-1) and no slot. table_out
+ * are not taken by it. Without room in the table or a free page the row has no page (-1) and no slot; where that page is to be
+ * a copy (cache_lens inside a page), its tokens are lost to the row, and rows that go on from one with an entry of -1 there (any negative
+ * one) end, whatever is free then. table_out
  * (rows,table_width), -1 past the row's pages; lens_out: cache_lens of the parents, 0 for rows that end; refs_out (pages): refs less page_table's names
  * and plus table_out's; slots: the next tokens' cache rows, or -1. Entries outside 0..pages-1 name no page.
  * The outputs are not the inputs. workspace: scratch of the size below. */
