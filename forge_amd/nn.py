@@ -336,7 +336,11 @@ class PagedBeams:
 
     After start(), prompts go into the cache at the slots that it returns. Then, again and again, step() takes the logits of each row's newest
     token and the caches, and what it leaves is for the rows' next tokens: `slots` (-1: no page is free), `lens` (their
-    positions, and cache_attention's cache_lens) and `table`. Row w of request b is row b * beams + w. All of it stays on the device."""
+    positions, and cache_attention's cache_lens) and `table`. Row w of request b is row b * beams + w. All of it stays on the device.
+
+    A row without a slot, because no page is free or its table is full, keeps its score and its token, which may be a search's last; it has
+    no continuation, since that token's key and value are nowhere: the next step() gives it the score -inf first. A row that has ended goes
+    on with end_token and takes pages as the others do; without a slot it stays as it is."""
 
     def __init__(self, requests: int, beams: int, pages: int, page_size: int, max_len: int, device):
         if page_size < 1 or page_size & (page_size - 1):
@@ -380,7 +384,10 @@ class PagedBeams:
         """The rows' next tokens from logits (requests, beams, tokens) of their newest ones, and the rows behind them: returns
         tokens and beams (requests, beams) int32, -1 where a request has fewer continuations. caches: the tensors whose pages the rows share."""
         if self._written:
-            self.lens = self.lens + (self.slots >= 0).to(torch.int32)
+            stored = self.slots >= 0
+            self.lens = self.lens + stored
+            live = stored.view_as(self.scores)
+            self.scores = torch.where(live if end_token is None else live | self.ended, self.scores, float("-inf"))
         ended = None if end_token is None else self.ended
         self.scores, beams, tokens = ops.beam_select(logits, self.scores, self.beams, ended, 0 if end_token is None else end_token)
         forked = ops.fork_pages(self.table, self.lens, beams, self.refs, self.page_size)

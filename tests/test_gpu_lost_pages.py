@@ -1,10 +1,12 @@
 """GPU: pools of pages that run out. A row that found no page to copy its last tokens into ends with the next call, however many
-pages are free then; every other row's pages hold its own tokens."""
+pages are free then; every other row's pages hold its own tokens. A search's rows whose newest token found no slot have no continuation."""
 import random
 
 import pytest
 
 from helpers import say
+from test_gpu_beam_select import check as check_selection
+from test_gpu_cache4 import stored
 from test_gpu_cache_pages import on, plain_fork, state
 
 pytestmark = pytest.mark.gpu
@@ -108,3 +110,69 @@ def test_tokens_of_a_pool_that_runs_out(dev, R, G, pages, width, steps):
             parents = [[rng.choice(live[b] + live[b][:1]) for _ in range(G)] for b in range(R)]
             t = [got.table, *on(dev, lens, parents), got.refs]
         assert missed and ended                                      # (the pool did run out)
+
+
+@pytest.mark.parametrize("end", [None, 3])
+@pytest.mark.parametrize("pages,max_len,steps", [(9, 300, 60), (12, 300, 60), (60, 50, 50)])
+def test_search_without_room(dev, end, pages, max_len, steps):
+    """Searches whose pool or whose table runs out: rows go on from rows all of whose tokens are in the cache, and from ended ones."""
+    import torch
+    from forge_amd import ops
+    from forge_amd.nn import PagedBeams
+    B, W, D, page, V = 2, 4, 64, 16, 12
+    dropped = after = 0
+    for seed in range(3):
+        say(f"search without room, {pages} pages, up to {max_len}, end={end} seed={seed}")
+        g = torch.Generator().manual_seed(seed)
+        kinds = torch.randn((2, V, 1, D), generator=g).to(dev)
+        places = torch.randn((2, 300, 1, D), generator=g).to(dev)
+
+        def kv(tokens, at):
+            t, p = tokens.long().clamp_min(0), at.long()
+            return tuple((kinds[i, t] + places[i, p]).half() for i in range(2))
+        prompts = [torch.randint(V, (n,), generator=g).to(dev) for n in (9, 20)]
+        lens = [len(p) for p in prompts]
+        beams = PagedBeams(B, W, pages, page, max_len, dev)
+        cache = torch.zeros(ops.cache4_shape(pages, page, 1, D), dtype=torch.uint8, device=dev)
+        slots = beams.start(lens)
+        ops.cache4_write(*kv(torch.cat(prompts), torch.cat([torch.arange(n, device=dev) for n in lens])), cache, slots)
+        rows = [p.tolist() if w == 0 else None for p in prompts for w in range(W)]
+        for step in range(steps):
+            logits = (torch.randn((B, W, V), generator=g) * 2).half().to(dev)
+            gone = (beams.slots < 0).view(B, W) & ~(beams.ended if end is not None else torch.zeros_like(beams.ended))
+            before, ended = beams.scores.clone(), beams.ended.clone()
+            if step:
+                dropped += int((gone & (before > float("-inf"))).sum())
+                before[gone] = float("-inf")
+            tokens, parents = beams.step(logits, [cache], end)
+            check_selection(logits, before, W, (beams.scores, parents, tokens), None if end is None else ended, end or 0)
+            par, tok = parents.tolist(), tokens.tolist()
+            rows = [rows[b * W + par[b][w]] + [tok[b][w]] if par[b][w] >= 0 else None for b in range(B) for w in range(W)]
+            ops.cache4_write(*kv(tokens.flatten(), beams.lens), cache, beams.slots)
+            done = beams.ended.flatten().tolist()
+            for r, s in enumerate(beams.slots.tolist()):
+                if rows[r] is None or s < 0 or (end is not None and done[r]):
+                    continue
+                after += dropped > 0
+                n = len(rows[r])
+                assert beams.lens[r] == n - 1, (step, r)
+                at = torch.arange(n, device=dev)
+                mine = (beams.table[r, at // page].long() * page + at % page).to(torch.int32)
+                for got, want in zip(ops.cache4_read(cache, mine, D), kv(torch.tensor(rows[r], device=dev), at)):
+                    assert torch.equal(got, stored(want, D, "float16")), (step, r)
+    assert (dropped or end is not None) and (after or max_len < 100)
+
+
+def test_a_table_that_is_full(dev):
+    """The last token needs no slot: its row keeps its score, and is gone with the step after it."""
+    import torch
+    from forge_amd.nn import PagedBeams
+    beams = PagedBeams(1, 2, 20, 16, 20, dev)
+    cache = torch.zeros((20, 16), device=dev)
+    beams.start([20])
+    x = torch.randn((1, 2, 50), generator=torch.Generator().manual_seed(1)).to(dev)
+    for step in range(13):
+        tokens, parents = beams.step(x, [cache])
+        assert (parents >= 0).all() and torch.isfinite(beams.scores).all() and (beams.slots >= 0).all() == (step < 12)
+    tokens, parents = beams.step(x, [cache])
+    assert (parents == -1).all() and (tokens == -1).all() and (beams.scores == float("-inf")).all() and (beams.lens == 0).all()
