@@ -340,12 +340,16 @@ __global__ __launch_bounds__(64 * RS * KS, cache4_waves(U, RT)) void cache4_atte
                 const bool grown = most > r.limit, none = r.limit == -FLT_MAX;
                 const float to = grown ? r.shift - (most + low) : r.shift, d = to - r.shift;
                 const float down = none ? 1.0f : __builtin_amdgcn_exp2f(d);
+                // A shift far from zero is rounded by more than the exponents' own distances: those of this tile are taken relative to its
+                // maximum itself then, or some would lie above every limit (from 2^32 on past FP32). `to` is at most the shift before.
+                const bool far = grown && fabsf(to) > kFar;
+                const float base = far ? most : 0.0f, rest = far ? -low : d;
                 if (grown) r.limit = kRescale - low;
                 r.shift = to;
 #pragma unroll
                 for (int h = 0; h < 2; h++)
 #pragma unroll
-                    for (int e = 0; e < 4; e++) x[rt][h][e] += d;
+                    for (int e = 0; e < 4; e++) x[rt][h][e] = x[rt][h][e] - base + rest;
                 r.l *= down;
                 r.c *= down;
                 r.top *= down;
