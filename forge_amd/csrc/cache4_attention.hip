@@ -308,8 +308,8 @@ __global__ __launch_bounds__(64 * RS * KS, cache4_waves(U, RT)) void cache4_atte
                 vs[h][e] = T::widen(static_cast<uint16_t>(vn & 0xFFFFu));
                 vm[h][e] = __builtin_fmaf(8.0f, vs[h][e], T::widen(static_cast<uint16_t>(vn >> 16)));
 #pragma unroll
-                for (int rt = 0; rt < RT; rt++)
-                    x[rt][h][e] = __builtin_fmaf(s[rt][e] * step, st[rt].unit, __builtin_fmaf(least, st[rt].qsum, st[rt].shift));
+                for (int rt = 0; rt < RT; rt++)                      // (a BF16 key's step times s, up to 2^7, may pass FP32)
+                    x[rt][h][e] = __builtin_fmaf(s[rt][e], step * st[rt].unit, __builtin_fmaf(least, st[rt].qsum, st[rt].shift));
             }
         }
         v4u weights[RT];

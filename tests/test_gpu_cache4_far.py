@@ -2,7 +2,7 @@
 import pytest
 
 from helpers import say
-from test_gpu_cache4 import Cache4
+from test_gpu_cache4 import Cache4, check_all
 from test_gpu_cache_attention import drafts_seen, queries, random_tree
 
 pytestmark = pytest.mark.gpu
@@ -71,3 +71,39 @@ def test_large_scores(dev, dt, q_size, k_size, rising):
                 assert ((got - want).abs() <= room)[alone].all(), (b, h)
                 assert (got.abs() <= v.abs().amax() * (1 + 2.0 ** -7)).all(), (b, h)
     assert said > 50
+
+
+@pytest.mark.parametrize("q_size,k_size", [(1e-37, 1e38), (1e-37, 3e38), (3e-30, 1e30), (1e30, 3e-30), (1e35, 1e-35)])
+def test_large_and_small(dev, q_size, k_size):
+    """BF16 scores of usual size whose factors lie at the ends of the type's range."""
+    import torch
+    from forge_amd import ops
+    top = torch.finfo(torch.bfloat16).max
+    for i, (lens, T, Hq, Hkv, D) in enumerate(CASES):
+        say(f"cache4_attention large and small {q_size} {k_size} lens={lens} T={T} heads={Hq}/{Hkv} D={D}")
+        q = (queries(len(lens), T, Hq, D, "bfloat16", dev, 80 + i).float() * q_size).to(torch.bfloat16)
+        c = Cache4(lens, T, Hkv, D, 16, "bfloat16", dev, 81 + i, change=lambda b, k, v: k.copy_((k.float() / 1.5 * k_size).clamp(-top, top).to(k.dtype)))
+        tree = random_tree(len(lens), T, 82 + i) if T > 1 else None
+        out = ops.cache4_attention(q, c.cache, c.table, c.lens, tree=None if tree is None else tree.to(dev))
+        assert torch.isfinite(out).all()
+        check_all(out, q, c, lens, tree)
+
+
+def test_largest_steps(dev):
+    """Tiny queries of one sign over BF16 keys that span the type: their products with the integers times a step pass FP32."""
+    import torch
+    from forge_amd import ops
+    top = torch.finfo(torch.bfloat16).max
+    for i, (lens, T, Hq, Hkv, D) in enumerate(CASES):
+        say(f"cache4_attention largest steps lens={lens} T={T} heads={Hq}/{Hkv} D={D}")
+        q = ((1.0 + 0.05 * queries(len(lens), T, Hq, D, "bfloat16", dev, 90 + i).float()) * 1e-38).to(torch.bfloat16)
+
+        def change(b, k, v):
+            x = k.float() / 1.5
+            x[:, :, 1::7] /= 3.0
+            k.copy_((torch.where(x > -1.0, 1.0, -1.0) * top * (1.0 - x.abs().clamp_max(2.0) / 4.0)).to(k.dtype))
+        c = Cache4(lens, T, Hkv, D, 16, "bfloat16", dev, 91 + i, change=change)
+        tree = random_tree(len(lens), T, 92 + i) if T > 1 else None
+        out = ops.cache4_attention(q, c.cache, c.table, c.lens, tree=None if tree is None else tree.to(dev))
+        assert torch.isfinite(out).all()
+        check_all(out, q, c, lens, tree)
