@@ -13,7 +13,8 @@
 // their factors, that of a subnormal being 2^-14, and drops what lies 24 bits below: 2^-18 of the largest query, or weight, of the 8.
 // Masked where they are, at bits 0 and 16 too (n 2^-24, of which 2^-14 is dropped), they take one shift for 8 values instead of
 // three, 82.3 for 85.5 us of 6 trees (below).
-// Weights w = p s' are rounded to FP16, in either type, the row's largest at 2^4 or above; sums are FP32. v is taken as (m' + 8 s') + s' (n' - 8):
+// Weights w = p s' are rounded to FP16, in either type, the row's largest at 2^4 or above (as far as a factor of 2^127 brings it there, which for
+// p of 2^-low is up to steps of 2^(low - 123); BF16's smaller ones lose bits); sums are FP32. v is taken as (m' + 8 s') + s' (n' - 8):
 // sum w n' less 8 times the sum of the same rounded w, so that a rounding weighs with n' - 8 (a result's error in the 2-norm, FP16 values: 2.4e-4 to
 // 2.8e-4; with n' 5.4e-4; rounding the exact result alone 2.1e-4).
 //
@@ -126,6 +127,8 @@ struct Block4 {   // a lane's part of 16 keys
     v4u num[2];           // numbers of keys 4 g to 4 g + 3
 };
 
+constexpr int kMostE = 127;   // of a factor 2^e that FP32 holds
+
 // One row tile's softmax state (the lane's column).
 template <int U>
 struct Rows4 {
@@ -235,8 +238,8 @@ __global__ __launch_bounds__(64 * RS * KS, cache4_waves(U, RT)) void cache4_atte
         st[rt].shift = 0.0f;
         st[rt].limit = -FLT_MAX;
         st[rt].l = st[rt].c = st[rt].u = st[rt].top = 0.0f;
-        st[rt].e = 120;
-        st[rt].f = 0x1p120f;
+        st[rt].e = kMostE;
+        st[rt].f = 0x1p127f;
 #pragma unroll
         for (int j = 0; j < Words::kOut; j++) st[rt].o[j] = v4f{0.0f, 0.0f, 0.0f, 0.0f};
     }
@@ -353,7 +356,7 @@ __global__ __launch_bounds__(64 * RS * KS, cache4_waves(U, RT)) void cache4_atte
                 r.l *= down;
                 r.c *= down;
                 r.top *= down;
-                const int e = r.top > 0.0f ? max(-120, min(120, 5 - __builtin_amdgcn_frexp_expf(r.top))) : 120;
+                const int e = r.top > 0.0f ? max(-120, min(kMostE, 5 - __builtin_amdgcn_frexp_expf(r.top))) : kMostE;
                 r.scale(ldexpf(down, e - r.e));
                 r.e = e;
                 r.f = ldexpf(1.0f, e);

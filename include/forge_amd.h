@@ -390,7 +390,8 @@ int forge_cache4_read(const uint8_t* cache, const int32_t* slots, uint16_t* k, u
 
 /* forge_cache_attention over the 4-bit cache, with the same arguments and limits. Keys and values enter as m + s n, not
  * rounded to 16 bits; the softmax weights times the values' steps are rounded to FP16, scaled by a power of two of the row's, in both types. Scores
- * are FP32: finite BF16 inputs give finite results while scale times a row's sum of |q|, and that times its largest |k|, are under 2^120. How
+ * are FP32: finite BF16 inputs give finite results while scale times a row's sum of |q|, and that times its largest |k|, are under 2^120.
+ * Over n keys a result may miss n^2 2^-134, which only BF16 values below some 10^-30 show. How
  * the keys are split over workgroups, and with it a result's last bits, follows from the table's width and the lengths of all sequences. */
 size_t forge_cache4_attention_workspace_size(int B, int T, int Hq, int Hkv, int D, long long max_keys);
 int forge_cache4_attention(const uint16_t* q, const uint8_t* cache, const int32_t* page_table, const int32_t* cache_lens,

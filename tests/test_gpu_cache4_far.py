@@ -107,3 +107,36 @@ def test_largest_steps(dev):
         out = ops.cache4_attention(q, c.cache, c.table, c.lens, tree=None if tree is None else tree.to(dev))
         assert torch.isfinite(out).all()
         check_all(out, q, c, lens, tree)
+
+
+@pytest.mark.parametrize("e", [-60, -100, -108])
+def test_equal_small_values(dev, e):
+    """Means of BF16 values near the lower end of its range keep their bits."""
+    import torch
+    from forge_amd import ops
+    for i, (lens, T, Hq, Hkv, D) in enumerate(CASES):
+        say(f"cache4_attention values of 2^{e} lens={lens} T={T} heads={Hq}/{Hkv} D={D}")
+        c = Cache4(lens, T, Hkv, D, 16, "bfloat16", dev, 100 + i, change=lambda b, k, v: v.fill_(2.0 ** e))
+        out = ops.cache4_attention(queries(len(lens), T, Hq, D, "bfloat16", dev, 101 + i), c.cache, c.table, c.lens)
+        assert (out == 2.0 ** e).all()
+
+
+@pytest.mark.parametrize("e", [-100, -118, -120, -122])
+def test_smallest_steps(dev, e):
+    """Steps 2^e of BF16 values over 30001 keys with equal scores: all weights are 2^-26, and 2^(e - 26 + 127), a number of FP16, behind the row's
+    factor, so that every product and sum is exact. (With a factor of 2^120 the weights of the last two were zero.)"""
+    import torch
+    from forge_amd import ops
+    n, D = 30000, 64
+    say(f"cache4_attention steps of 2^{e}")
+
+    def change(b, k, v):
+        k.zero_()
+        v.fill_(15.0 * 2.0 ** e)
+        v[:, :, 5] = 0.0
+        v[:, :, 60] = 3.0 * 2.0 ** e
+    c = Cache4([n], 1, 1, D, 16, "bfloat16", dev, 110, change=change)
+    out = ops.cache4_attention(queries(1, 1, 3, D, "bfloat16", dev, 111), c.cache, c.table, c.lens)
+    want = torch.full((D,), 15.0 * 2.0 ** e, device=dev).to(torch.bfloat16)
+    want[5], want[60] = 0.0, 3.0 * 2.0 ** e
+    assert torch.equal(out[0, 0], want.expand(3, D))
