@@ -18,7 +18,7 @@ constexpr int kCache4MinPage = 16, kCache4MaxPage = 1 << 20;   // blocks of 16 p
 // A cache of `pages` pages is addressable: its pages' and heads' products stay in range, whatever the device's indices.
 inline bool cache4_shape_ok(int Hkv, int D, int pages, int page_size) {
     return Hkv > 0 && Hkv <= 65535 && D > 0 && D % 8 == 0 && D <= 256 && pages > 0 && page_size >= kCache4MinPage && page_size <= kCache4MaxPage &&
-           (page_size & (page_size - 1)) == 0 && static_cast<long long>(pages) * page_size <= 0x7FFFFFFFLL;
+           (page_size & (page_size - 1)) == 0 && static_cast<long long>(pages) * page_size <= 1LL << 31;
 }
 
 struct Cache4Layout {
