@@ -383,15 +383,18 @@ class PagedBeams:
     def step(self, logits: torch.Tensor, caches, end_token: Optional[int] = None):
         """The rows' next tokens from logits (requests, beams, tokens) of their newest ones, and the rows behind them: returns
         tokens and beams (requests, beams) int32, -1 where a request has fewer continuations. caches: the tensors whose pages the rows share."""
+        lens, scores = self.lens, self.scores
         if self._written:
             stored = self.slots >= 0
-            self.lens = self.lens + stored
-            live = stored.view_as(self.scores)
-            self.scores = torch.where(live if end_token is None else live | self.ended, self.scores, float("-inf"))
+            lens = lens + stored
+            live = stored.view_as(scores)
+            scores = torch.where(live if end_token is None else live | self.ended, scores, float("-inf"))
         ended = None if end_token is None else self.ended
-        self.scores, beams, tokens = ops.beam_select(logits, self.scores, self.beams, ended, 0 if end_token is None else end_token)
-        forked = ops.fork_pages(self.table, self.lens, beams, self.refs, self.page_size)
+        scores, beams, tokens = ops.beam_select(logits, scores, self.beams, ended, 0 if end_token is None else end_token)
+        forked = ops.fork_pages(self.table, lens, beams, self.refs, self.page_size)
         ops.copy_pages(caches, forked.src, forked.dst)
+        # (from here on nothing is refused: a call that raised has left the rows as they were)
+        self.scores = scores
         self.table, self.lens, self.refs, self.slots = forked.table, forked.lens, forked.refs, forked.slots
         if end_token is not None:
             self.ended = self.ended.gather(1, beams.clamp_min(0).long()) | (tokens == end_token)

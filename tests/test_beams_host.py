@@ -1,0 +1,20 @@
+"""CPU: what PagedBeams refuses, and what a refused call leaves."""
+import pytest
+
+
+def beams(**more):
+    from forge_amd.nn import PagedBeams
+    return PagedBeams(**dict(dict(requests=2, beams=3, pages=10, page_size=4, max_len=20, device="cpu"), **more))
+
+
+def test_refused_step():
+    """A step that raises (here for lack of a device) changes nothing, so that it can be made again with what is right."""
+    import torch
+    b = beams()
+    b.start([5, 8])
+    b.slots, b._written = torch.tensor([5, -1, -1, 12, -1, -1], dtype=torch.int32), True
+    was = {k: v.clone() for k, v in vars(b).items() if isinstance(v, torch.Tensor)}
+    for end in (None, 7):
+        with pytest.raises(ValueError, match="device"):
+            b.step(torch.zeros((2, 3, 9)), [torch.zeros((10, 4))], end)
+        assert all(torch.equal(v, getattr(b, k)) for k, v in was.items()) and b._written
