@@ -383,6 +383,9 @@ class PagedBeams:
     def step(self, logits: torch.Tensor, caches, end_token: Optional[int] = None):
         """The rows' next tokens from logits (requests, beams, tokens) of their newest ones, and the rows behind them: returns
         tokens and beams (requests, beams) int32, -1 where a request has fewer continuations. caches: the tensors whose pages the rows share."""
+        for cache in caches[:1]:                    # (copy_pages wants the others to be like it)
+            if cache.shape[0] != self.refs.shape[0]:
+                raise ValueError(f"the caches have {cache.shape[0]} pages, the beams' rows {self.refs.shape[0]}")
         lens, scores = self.lens, self.scores
         if self._written:
             stored = self.slots >= 0

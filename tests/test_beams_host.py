@@ -18,3 +18,13 @@ def test_refused_step():
         with pytest.raises(ValueError, match="device"):
             b.step(torch.zeros((2, 3, 9)), [torch.zeros((10, 4))], end)
         assert all(torch.equal(v, getattr(b, k)) for k, v in was.items()) and b._written
+
+
+def test_other_pages():
+    """Caches of another page count than the rows' are refused: with fewer pages, copies would be left out without a word."""
+    import torch
+    b = beams()
+    b.start([5, 8])
+    for pages in (9, 11):
+        with pytest.raises(ValueError, match="pages"):
+            b.step(torch.zeros((2, 3, 9)), [torch.zeros((pages, 4)), torch.zeros((10, 4))])
