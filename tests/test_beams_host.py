@@ -28,3 +28,12 @@ def test_other_pages():
     for pages in (9, 11):
         with pytest.raises(ValueError, match="pages"):
             b.step(torch.zeros((2, 3, 9)), [torch.zeros((pages, 4)), torch.zeros((10, 4))])
+
+
+def test_limits():
+    """What the operators of a step refuse is refused at once."""
+    beams(beams=64)
+    beams(requests=128, beams=64)
+    for bad in (dict(beams=65), dict(beams=0), dict(requests=129, beams=64), dict(requests=0), dict(pages=0)):
+        with pytest.raises(ValueError):
+            beams(**bad)
