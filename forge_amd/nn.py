@@ -376,9 +376,9 @@ class PagedBeams:
             page += need[b]
         self.table, self.lens = table.to(device), lens.to(device)
         self.refs = (torch.arange(self.refs.shape[0], device=device) < page).to(torch.int32)
-        self.scores.fill_(float("-inf"))
+        self.scores = torch.full_like(self.scores, float("-inf"))    # (the ones before are somebody's results)
         self.scores[:, 0] = 0.0
-        self.ended.zero_()
+        self.ended = torch.zeros_like(self.ended)
         self._written = False
         return torch.cat(slots).to(device) if slots else torch.zeros(0, dtype=torch.int32, device=device)
 

@@ -37,3 +37,15 @@ def test_limits():
     for bad in (dict(beams=65), dict(beams=0), dict(requests=129, beams=64), dict(requests=0), dict(pages=0)):
         with pytest.raises(ValueError):
             beams(**bad)
+
+
+def test_start_keeps_results():
+    """The scores that a search has left are the caller's: the next start() makes others."""
+    import torch
+    b = beams()
+    b.start([5, 8])
+    b.scores, b.ended = torch.full((2, 3), -2.5), torch.ones((2, 3), dtype=torch.bool)
+    scores, ended = b.scores, b.ended
+    b.start([1, 2])
+    assert (scores == -2.5).all() and ended.all()
+    assert b.scores.tolist() == [[0.0, float("-inf"), float("-inf")]] * 2 and not b.ended.any()
