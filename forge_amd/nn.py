@@ -345,8 +345,8 @@ class PagedBeams:
     def __init__(self, requests: int, beams: int, pages: int, page_size: int, max_len: int, device):
         if page_size < 1 or page_size & (page_size - 1):
             raise ValueError(f"page_size must be a power of two, got {page_size}")
-        if not 1 <= beams <= 64 or not 1 <= requests * beams <= 8192 or pages < 1:
-            raise ValueError(f"1 to 64 beams, 1 to 8192 rows of them and a page at least, got {requests} x {beams} over {pages} pages")
+        if not 1 <= beams <= 64 or not 0 <= requests * beams <= 8192 or pages < 1:
+            raise ValueError(f"1 to 64 beams, up to 8192 rows of them and a page at least, got {requests} x {beams} over {pages} pages")
         self.requests, self.beams, self.page_size = requests, beams, page_size
         rows, width = requests * beams, max_len // page_size + 1
         self.table = torch.full((rows, width), -1, dtype=torch.int32, device=device)

@@ -34,7 +34,8 @@ def test_limits():
     """What the operators of a step refuse is refused at once."""
     beams(beams=64)
     beams(requests=128, beams=64)
-    for bad in (dict(beams=65), dict(beams=0), dict(requests=129, beams=64), dict(requests=0), dict(pages=0)):
+    assert beams(requests=0).start([]).shape == (0,)
+    for bad in (dict(beams=65), dict(beams=0), dict(requests=129, beams=64), dict(requests=-1), dict(pages=0)):
         with pytest.raises(ValueError):
             beams(**bad)
 
