@@ -1127,6 +1127,8 @@ def fork_pages(page_table: torch.Tensor, cache_lens: torch.Tensor, parents: torc
     _same_device(page_table, cache_lens, parents, refs, workspace, *out)
     _call("forge_fork_pages", _p(page_table), _p(cache_lens), _p(parents), _p(refs), *(_p(t) for t in out), rows, group, width,
           pages, page_size, _p(workspace), size, _stream())
+    if rows == 0:                                                   # (no work to the library, and the counts are outputs all the same)
+        out.refs.copy_(refs)
     return out
 
 
