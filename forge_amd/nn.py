@@ -356,6 +356,7 @@ class PagedBeams:
         self.scores = torch.full((requests, beams), float("-inf"), dtype=torch.float32, device=device)
         self.ended = torch.zeros((requests, beams), dtype=torch.bool, device=device)
         self._written = False                       # whether the slots' tokens are in the caches
+        self._ends = False                          # whether `ended` may hold any
 
     def start(self, prompt_lens) -> torch.Tensor:
         """Empties all rows and gives each request's first row the pages of a prompt of prompt_lens[b] tokens (integers on the
@@ -384,7 +385,8 @@ class PagedBeams:
 
     def step(self, logits: torch.Tensor, caches, end_token: Optional[int] = None):
         """The rows' next tokens from logits (requests, beams, tokens) of their newest ones, and the rows behind them: returns
-        tokens and beams (requests, beams) int32, -1 where a request has fewer continuations. caches: the tensors whose pages the rows share."""
+        tokens and beams (requests, beams) int32, -1 where a request has fewer continuations. caches: the tensors whose pages the rows share. Without an end_token every row
+        goes on, and none has ended afterwards."""
         for cache in caches[:1]:                    # (copy_pages wants the others to be like it)
             if cache.shape[0] != self.refs.shape[0]:
                 raise ValueError(f"the caches have {cache.shape[0]} pages, the beams' rows {self.refs.shape[0]}")
@@ -403,6 +405,9 @@ class PagedBeams:
         self.table, self.lens, self.refs, self.slots = forked.table, forked.lens, forked.refs, forked.slots
         if end_token is not None:
             self.ended = self.ended.gather(1, beams.clamp_min(0).long()) | (tokens == end_token)
+        elif self._ends:                            # all rows have gone on
+            self.ended = torch.zeros_like(self.ended)
+        self._ends = end_token is not None
         self._written = True
         return tokens, beams
 
