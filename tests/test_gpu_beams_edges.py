@@ -28,6 +28,39 @@ def test_no_rows(dev):
     assert tokens.shape == parents.shape == (0, 3) and (beams.refs == 0).all()
 
 
+@pytest.mark.parametrize("dt,B,W,V,per,piece", [("float16", 40, 8, 16500, 8, 8192), ("bfloat16", 40, 8, 16384, 8, 8192), ("float32", 40, 8, 20000, 4, 8192),
+                                                ("float16", 1, 4, 9001, 8, 2048), ("bfloat16", 2, 1, 2048, 8, 2048)])
+@pytest.mark.parametrize("count", [64, 63])
+def test_a_low_group(dev, dt, B, W, V, per, piece, count):
+    """64 places, and of each 64 vectors of a piece one that holds low logits only: its largest is the first bound, and thousands lie above it."""
+    import torch
+    g = torch.Generator().manual_seed(V + count)
+    x = (torch.randn((B, W, V), generator=g) * 2.5).to(getattr(torch, dt))
+    low = (torch.arange(V) % piece) // per % 64
+    few = low == 17 if count == 64 else (low == 17) | (low == 40)
+    x[:, :, few] = (-25.0 - 5.0 * torch.rand((B, W, int(few.sum())), generator=g)).to(x.dtype)
+    x[:, :, 5::97] = float("-inf")
+    x[0, :, 1000:1040] = 12.0                                        # equal ones at the top
+    x[-1, 0] = x[-1, 0].sort(descending=True).values.float().view(-1).to(x.dtype)
+    x[-1, 0, few] = -28.0
+    run(dev, dt, B, W, V, count, logits=x.to(dev))
+
+
+@pytest.mark.parametrize("B,W,V,low", [(1, 1024, 64, 64), (2, 1024, 100, 128), (1, 1000, 300, 64), (3, 16, 4000, 8), (1, 512, 200, 64)])
+def test_many_rounds(dev, B, W, V, low):
+    """Far more candidates above the first bounds than there is room for, as beams in a fixed stride have low scores; near scores and equal
+    ones among them."""
+    import torch
+    g = torch.Generator().manual_seed(W + V)
+    for kind in range(4):
+        x = torch.randn((B, W, V), generator=g) * (0.01 if kind == 1 else 1.0)
+        if kind == 2:
+            x = x.round()
+        s = torch.rand((B, W), generator=g) * (0.0 if kind == 3 else 1e-2)
+        s[:, 3::low] -= 30.0
+        run(dev, "float32" if kind < 2 else "float16", B, W, V, 64, logits=x.to(torch.float32 if kind < 2 else torch.float16).to(dev), scores=s.to(dev))
+
+
 def test_steps_with_and_without_an_end(dev):
     """A step without an end_token lets every row go on; what it leaves at a row's place is not the one that had ended there."""
     import torch
