@@ -8,7 +8,7 @@
 // The largest of many: of 64 groups' maxima the count-th largest is a bound that at least `count` numbers reach, and what reaches it, few
 // more as a rule, is gathered in LDS and ranked by counting, with ties by place. Where more are found, a better bound comes from those (most lists
 // empty, or many places), or they are equal ones (a mask's lowest value): those above the bound are ranked and the first places that equal
-// it follow. Where LDS has no room even so, the places are filled one after the other.
+// it follow. Where a piece has more of those than LDS has room, its places are filled one after the other.
 //
 // us, pieces + merge: 32 x 8 beams of 131072 FP32 logits, three in ten ended, 18.4 (94 MB at 5.1 TB/s) + 8.2; 4 beams of 32000 FP16 4.6 + 5.7, two chains
 // of dependent steps. In all, 8 x 4 beams of 128000, 16 places: 15; all but 20 tokens at FP16's lowest value 20 (place after place 65), all logits
@@ -328,8 +328,7 @@ __global__ __launch_bounds__(kBeamThreads) void beam_piece_kernel(BeamArgs a)
         __syncthreads();
         last = max(max(part_key[0], part_key[1]), max(part_key[2], part_key[3]));
         __syncthreads();
-        if (tid == 0) put(place, last);
-        if (last == 0) last = 1;                                     // nothing is left: no key is below 1
+        if (tid == 0) put(place, last);                              // (there are more than kBeamRoom)
     }
 }
 
@@ -351,7 +350,6 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a)
     __shared__ float largest[kBeamWidth];
     __shared__ NthGroup<double, kMergeThreads> groups;
     __shared__ BeamCandidate found[kBeamRoom];
-    __shared__ BeamCandidate part[kWaves];
     __shared__ int queue[kBeamRoom];
     __shared__ double bound_of;
     __shared__ int total, waiting, part_count[2][kWaves];
@@ -486,7 +484,8 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a)
             if (place < a.count) put(place, c);
         }
     };
-    for (int round = 0; round < 8; round++) {
+    // (Ends: a bound that has risen leaves out what had the one before, a candidate's score from the first time on. Some five rounds for 64 thousand.)
+    for (;;) {
         collect([&](double x) { return x >= bound; });
         int got = total;
         if (got <= kBeamFew) {
@@ -523,34 +522,6 @@ __global__ __launch_bounds__(kMergeThreads) void beam_merge_kernel(BeamArgs a)
         }
         for (int i = got + tid; i < a.count; i += kMergeThreads) put(i, none);
         return;
-    }
-    BeamCandidate last = {INFINITY, 0ull};
-    for (int place = 0; place < a.count; place++) {
-        BeamCandidate next = none;
-        auto see = [&](const BeamCandidate& c) {
-            if (c.score > -INFINITY && beam_before(last, c) && beam_before(c, next)) next = c;
-        };
-        for (int list = tid; list < lists; list += kMergeThreads)
-            for (int depth = 0; depth < a.count; depth++) {          // (a list's first one after `last` is its best)
-                const BeamCandidate c = candidate(list, depth);
-                see(c);
-                if (!(c.score > -INFINITY) || beam_before(last, c)) break;
-            }
-        if (a.ended)
-            for (int w = tid; w < a.W; w += kMergeThreads) see(own(w));
-#pragma unroll
-        for (int o = 1; o < kWave; o <<= 1) {
-            const BeamCandidate c = {__shfl_xor(next.score, o, kWave), static_cast<unsigned long long>(__shfl_xor(next.place, o, kWave))};
-            if (beam_before(c, next)) next = c;
-        }
-        if (lane == 0) part[wave] = next;
-        __syncthreads();
-        last = part[0];
-#pragma unroll
-        for (int w = 1; w < kWaves; w++)
-            if (beam_before(part[w], last)) last = part[w];
-        __syncthreads();
-        if (tid == 0) put(place, last);
     }
 }
 
