@@ -1,9 +1,12 @@
 """GPU: calls at the edges of a beam search: no rows at all, selections by every path, steps with and without an end, and the
 example's scores against each sequence alone."""
+import types
+
 import pytest
 
 from helpers import say
-from test_gpu_beam_select import run, scores_of
+from test_gpu_beam_select import NEAR, run
+from test_gpu_beams import example  # noqa: F401
 
 pytestmark = pytest.mark.gpu
 
@@ -84,3 +87,49 @@ def test_steps_with_and_without_an_end(dev):
     assert beams.ended.any()
     beams.start([3, 20])
     assert not beams.ended.any()
+
+
+@pytest.mark.parametrize("lens,width,steps,end", [((37, 5, 130), 4, 12, 7), ((16, 1, 31), 5, 40, None), ((64,), 7, 30, 3)])
+def test_example_scores(dev, example, lens, width, steps, end):  # noqa: F811
+    """Every sequence that the example's search returns, run again in a row of its own: pages in order that no other row names, a copy of the
+    prompt's, no selection and no fork. The calls have the same sizes, and a row's result is not its neighbours' matter (fewer keys than
+    are split), so the logits are the same, and the scores but for a selection's error and FP32's rounding in each step."""
+    import torch
+    from forge_amd import ops
+    say(f"the example's search of {lens}, {width} beams, {steps} steps, end={end}")
+    page = 16
+    model = example.Decoder()
+    torch.manual_seed(len(lens))
+    prompts = [torch.randint(1000, (n,)).tolist() for n in lens]
+    found, scores = example.search(model, prompts, width, steps, end, page)
+    B, R = len(lens), len(lens) * width
+    each = (max(lens) + steps) // page + 1                           # pages of a row, and of a prompt
+    of = torch.arange(B).repeat_interleave(width)                    # a row's prompt
+    table = torch.arange(R * each, dtype=torch.int32, device=dev).view(R, each)
+    whole, caches = model.caches(B * each, page), model.caches(R * each, page)
+    at = [torch.arange(n, dtype=torch.int32) for n in lens]
+    cu = torch.tensor([0, *lens], device=dev).cumsum(0).to(torch.int32)
+    logits = model.prompt(torch.tensor(sum(prompts, []), device=dev), cu, torch.cat(at).to(dev), whole,
+                          torch.cat([b * each * page + p for b, p in enumerate(at)]).to(dev))
+    logits = logits[(cu[1:] - 1).long()][of.to(dev)]
+    for a, b in zip(caches, whole):
+        a.view(R, each, -1).copy_(b.view(B, each, -1)[of.to(dev)])
+    n = torch.tensor(lens, dtype=torch.int32)[of].to(dev)
+    total = torch.zeros(R, dtype=torch.float64, device=dev)
+    ended = torch.zeros(R, dtype=torch.bool, device=dev)
+    tokens = found.view(R, steps)
+    assert (tokens >= 0).all() and torch.isfinite(scores).all()
+    for i in range(steps):
+        t = tokens[:, i].contiguous()
+        gain = torch.log_softmax(logits.double(), -1).gather(1, t.long()[:, None])[:, 0]
+        total += torch.where(ended, 0.0, gain)
+        if end is not None:
+            assert (t[ended] == end).all()
+            ended |= t == end
+        slots = table.gather(1, (n // page).long()[:, None])[:, 0] * page + n % page
+        logits = model.next(t, caches, types.SimpleNamespace(lens=n, slots=slots.to(torch.int32), table=table))
+        n = n + 1
+    room = steps * (NEAR + 2.0 ** -24 * scores.abs().max().item())
+    worst = (total.view(B, width) - scores.double()).abs().max().item()
+    assert worst <= room, (worst, room)
+    assert len({tuple(x) for x in tokens.tolist()}) == R             # no sequence twice
