@@ -533,8 +533,8 @@ int beam_vectors(int B, int W, int V) {
 template <class L>
 int beam_splits(int B, int W, int V) { return divup(V, kBeamThreads * beam_vectors<L>(B, W, V) * L::kPer); }
 inline bool beam_shape_ok(int B, int W, int V, int count) {
-    return B > 0 && W > 0 && W <= kBeamWidth && V > 0 && count > 0 && count <= kBeamCount &&
-           static_cast<long long>(B) * W * divup(V, kBeamThreads * 4) <= INT_MAX &&
+    return B > 0 && W > 0 && W <= kBeamWidth && V > 0 && count > 0 && count <= kBeamCount && B <= grid_limit(kMergeThreads) &&
+           static_cast<long long>(B) * W * std::max(beam_splits<Logits16<Fp16>>(B, W, V), beam_splits<Logits32>(B, W, V)) <= grid_limit(kBeamThreads) &&
            static_cast<long long>(W) * (divup(V, kBeamThreads * 4) * static_cast<long long>(count) + 1) <= INT_MAX - kMergeThreads;
 }
 inline size_t beam_bytes(int B, int W, int count, int splits) {

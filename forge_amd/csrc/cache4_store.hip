@@ -8,6 +8,7 @@
 // wave are most of it), read in 14.6.
 #include "cache4.h"
 
+#include <algorithm>
 #include <climits>
 
 namespace forge_amd {
@@ -191,12 +192,28 @@ __global__ __launch_bounds__(256) void cache4_read_kernel(Store4Args a)
 }
 
 template <class T, int LPH>
-int launch_store4(const Store4Args& a, bool write, hipStream_t s) {
-    const long long grid = static_cast<long long>(divup(a.T, 4 * kWave / LPH)) * a.at.Hkv;
-    if (grid > INT_MAX) return FORGE_EINVAL;
-    if (write) cache4_write_kernel<T, LPH><<<static_cast<unsigned>(grid), 256, 0, s>>>(a);
-    else cache4_read_kernel<T, LPH><<<static_cast<unsigned>(grid), 256, 0, s>>>(a);
-    return launch_status();
+int launch_store4(Store4Args a, bool write, hipStream_t s) {
+    // as many tokens at a time as a grid holds
+    constexpr int kTokens = 4 * kWave / LPH;                         // of a workgroup
+    const int total = a.T;
+    const long long most = grid_limit(256) / a.at.Hkv * kTokens;
+    for (long long t = 0; t < total; t += most) {
+        a.T = static_cast<int>(std::min(most, total - t));
+        const unsigned grid = static_cast<unsigned>(divup(a.T, kTokens)) * a.at.Hkv;
+        if (write) cache4_write_kernel<T, LPH><<<grid, 256, 0, s>>>(a);
+        else cache4_read_kernel<T, LPH><<<grid, 256, 0, s>>>(a);
+        const int st = launch_status();
+        if (st != FORGE_OK) return st;
+        a.slots += a.T;
+        if (write) {
+            a.k += static_cast<long long>(a.T) * a.k_token;
+            a.v += static_cast<long long>(a.T) * a.v_token;
+        } else {
+            a.k_out += static_cast<size_t>(a.T) * a.at.Hkv * a.D;
+            a.v_out += static_cast<size_t>(a.T) * a.at.Hkv * a.D;
+        }
+    }
+    return FORGE_OK;
 }
 
 template <class T>

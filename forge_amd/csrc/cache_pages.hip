@@ -229,7 +229,7 @@ constexpr int kCopyTensors = 64;     // of a launch, by value
 struct CopyArgs {
     uint8_t* tensor[kCopyTensors];
     const int32_t *src, *dst;
-    long long page_bytes;
+    long long page_bytes, left;   // left: of a page, from the tensors' addresses on
     int pairs, pages;
 };
 
@@ -240,7 +240,7 @@ __global__ __launch_bounds__(256) void copy_pages_kernel(CopyArgs a)
         const int s = a.src[i], d = a.dst[i];
         if (s < 0 || d < 0 || s >= a.pages || d >= a.pages || s == d) continue;
         const long long at = (static_cast<long long>(blockIdx.x) * 256 + threadIdx.x) * 16;
-        if (at >= a.page_bytes) continue;
+        if (at >= a.left) continue;
         uint8_t* t = a.tensor[blockIdx.z];
         *reinterpret_cast<uint4*>(t + d * a.page_bytes + at) = *reinterpret_cast<const uint4*>(t + s * a.page_bytes + at);
     }
@@ -303,13 +303,18 @@ extern "C" int forge_copy_pages(void* const* caches, int tensors, long long page
     a.page_bytes = page_bytes;
     a.pairs = pairs;
     a.pages = pages;
+    const long long most = grid_limit(256) * 4096;                   // of a page, by a launch
     for (int t = 0; t < tensors; t += kCopyTensors) {
         const int n = std::min(kCopyTensors, tensors - t);
-        for (int i = 0; i < n; i++) a.tensor[i] = static_cast<uint8_t*>(caches[t + i]);
-        const dim3 grid(static_cast<unsigned>(divupll(page_bytes, 4096)), static_cast<unsigned>(std::min(pairs, 65535)), static_cast<unsigned>(n));
-        copy_pages_kernel<<<grid, 256, 0, s>>>(a);
-        const int st = launch_status();
-        if (st != FORGE_OK) return st;
+        for (long long at = 0; at < page_bytes; at += most) {
+            for (int i = 0; i < n; i++) a.tensor[i] = static_cast<uint8_t*>(caches[t + i]) + at;
+            a.left = page_bytes - at;
+            const dim3 grid(static_cast<unsigned>(divupll(std::min(a.left, most), 4096)), static_cast<unsigned>(std::min(pairs, 65535)),
+                            static_cast<unsigned>(n));
+            copy_pages_kernel<<<grid, 256, 0, s>>>(a);
+            const int st = launch_status();
+            if (st != FORGE_OK) return st;
+        }
     }
     return FORGE_OK;
 }

@@ -34,6 +34,9 @@ int default_cu_count();
 // tile/split appended when >= 0 / > 0), read back by forge_last_route.
 void note_route(const char* engine, int tile = -1, int split = 0);
 
+// Workgroups of `threads` that a grid's dimension holds: HIP counts its threads in 32 bits, and launches what is left of more, without an error.
+constexpr long long grid_limit(int threads) { return ((1LL << 32) - 1) / threads; }
+
 inline int divup(int a, int b) { return static_cast<int>((static_cast<long long>(a) + b - 1) / b); }
 constexpr long long divupll(long long a, long long b) { return (a + b - 1) / b; }
 

@@ -405,7 +405,8 @@ int forge_cache4_attention(const uint16_t* q, const uint8_t* cache, const int32_
  * nearer to each other than about 10^-6 may come in either order; equal rows have equal scores). -inf
  * logits are no candidates; neither is a beam whose score is not finite or whose logits hold an infinity or NaN, or -inf only. A beam that has
  * ended (ended[b,w] != 0; NULL: none has) has one candidate, end_token with the beam's score, and its logits are not read. Places
- * that no candidate is left for are -inf, -1, -1. logits: dtype FORGE_FP16, FORGE_BF16 or FORGE_FP32, rows of V contiguous values at
+ * that no candidate is left for are -inf, -1, -1. B is under 2^23 and, with S pieces of 8192 logits (1024 or 2048 for small sizes) to a row, B * W * S
+ * under 2^24. logits: dtype FORGE_FP16, FORGE_BF16 or FORGE_FP32, rows of V contiguous values at
  * b * batch_stride + w * beam_stride elements, at any alignment. workspace: scratch of the size below, 16-byte aligned. */
 #define FORGE_FP32 2
 size_t forge_beam_select_workspace_size(int B, int W, int V, int count);
