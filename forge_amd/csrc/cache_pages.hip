@@ -64,8 +64,10 @@ __device__ __forceinline__ ForkRow fork_row(const ForkArgs& a, int parent) {
     row.len = min(max(a.lens[parent], 0), a.width << a.page_shift);
     const int at = row.len >> a.page_shift;
     const int pg = at < a.width ? a.table[static_cast<size_t>(parent) * a.width + at] : -1;
-    if (pg < 0 && (row.len & ((1 << a.page_shift) - 1)) != 0) return {-1, 0, -1, -1};   // its last tokens are lost
     row.last = pg >= 0 && pg < a.pages ? pg : -1;
+    const bool lost = pg < 0 && (row.len & ((1 << a.page_shift) - 1)) != 0;
+    row.parent = lost ? -1 : parent;
+    row.len = lost ? 0 : row.len;
     return row;
 }
 __device__ __forceinline__ int fork_parent(const ForkArgs& a, int r) {
@@ -169,9 +171,10 @@ __global__ __launch_bounds__(kForkThreads) void fork_rows_kernel(ForkArgs a)
         ForkRow row = {-1, 0, -1, -1};
         bool take = false;
         if (r < a.rows) {
-            row = fork_row(a, fork_parent(a, r));
-            take = row.parent >= 0 && row.len >> a.page_shift < a.width &&
-                   !(row.last >= 0 && first[row.parent] == r && a.refs[row.last] == 1);
+            const int p = fork_parent(a, r);
+            row = fork_row(a, p);
+            const int names = a.refs[max(row.last, 0)], child = first[max(p, 0)];   // (at once, with no branch between)
+            take = row.parent >= 0 && row.len >> a.page_shift < a.width && !(row.last >= 0 && child == r && names == 1);
         }
         const int before = sum_before<kForkThreads>(take, &all, part);
         if (take) row.rank = base + before;
