@@ -9,7 +9,6 @@
 #include "float16_types.h"
 #include "lds_dma.h"
 
-#include <climits>
 
 namespace forge_amd {
 
@@ -331,6 +330,7 @@ __global__ __launch_bounds__(64 * W) void int4_linear_kernel(Int4Args a)
 
 template <class T, int G, int MT, int XR, int NT, int W, int U, int S>
 int launch_int4(const Int4Args& a, hipStream_t s) {
+    if (divup(a.N, 16 * NT) > grid_limit(64 * W)) return FORGE_EINVAL;
     const dim3 grid(static_cast<unsigned>(divup(a.N, 16 * NT)), static_cast<unsigned>(divup(a.M, 16 * MT)));
     int4_linear_kernel<T, G, MT, XR, NT, W, U, S><<<grid, 64 * W, 0, s>>>(a);
     return launch_status();
@@ -365,7 +365,7 @@ template <class T>
 int launch_int4(const Int4Args& a, int group, hipStream_t s) {
     if (a.K < 256) {
         const long long wgs = divupll(static_cast<long long>(a.M) * a.N, 256);
-        if (wgs > INT_MAX) return FORGE_EINVAL;
+        if (wgs > grid_limit(256)) return FORGE_EINVAL;
         int4_short_kernel<T><<<static_cast<unsigned>(wgs), 256, 0, s>>>(a, group);
         return launch_status();
     }
@@ -390,7 +390,7 @@ extern "C" int forge_quantize_weight_int4(const void* w, int w_fp16, uint8_t* w_
     if (!w || !w_int4 || !w_scale || !aligned(w_int4, 16) || !int4_shape_ok(K, group)) return FORGE_EINVAL;
     const int row_words = int4_row_bytes(K) / 4;
     const long long words = static_cast<long long>(N) * row_words, wgs = divupll(words, 256);
-    if (wgs > INT_MAX) return FORGE_EINVAL;
+    if (wgs > grid_limit(256)) return FORGE_EINVAL;
     hipStream_t s = as_stream(stream);
     if (w_fp16)
         quantize_weight_int4_kernel<true><<<static_cast<unsigned>(wgs), 256, 0, s>>>(
@@ -407,7 +407,7 @@ extern "C" int forge_pack_weight_int4(const int8_t* q, uint8_t* w_int4, int N, i
     if (!q || !w_int4 || !aligned(w_int4, 16) || K % 32 != 0) return FORGE_EINVAL;
     const int row_words = int4_row_bytes(K) / 4;
     const long long words = static_cast<long long>(N) * row_words, wgs = divupll(words, 256);
-    if (wgs > INT_MAX) return FORGE_EINVAL;
+    if (wgs > grid_limit(256)) return FORGE_EINVAL;
     pack_weight_int4_kernel<<<static_cast<unsigned>(wgs), 256, 0, as_stream(stream)>>>(
         q, reinterpret_cast<uint32_t*>(w_int4), K, words, row_words);
     return launch_status();

@@ -16,7 +16,6 @@
 #include "attn_tile.h"
 #include "ring_tile.h"
 
-#include <climits>
 
 namespace forge_amd {
 
@@ -178,7 +177,7 @@ int launch_prompt(PromptArgs a, hipStream_t s) {
     const long long tiles = a.tokens / (32 * RS) + static_cast<long long>(a.sequences) + 1;
     const long long units = tiles * a.Hkv, wgs = divupll(units, 8) * 8 * (a.Hq / a.Hkv);
     // udiv_magic's range; 2^31 / 65536 tiles of heads at least
-    if ((units + 8) * a.Hkv >= 1LL << 32 || wgs * a.group >= 1LL << 32 || wgs > INT_MAX) return FORGE_EINVAL;
+    if ((units + 8) * a.Hkv >= 1LL << 32 || wgs * a.group >= 1LL << 32 || wgs > grid_limit(64 * RS * KS)) return FORGE_EINVAL;
     a.mg_group = udiv_multiplier(a.group);
     a.mg_hkv = udiv_multiplier(a.Hkv);
     a.tiles = static_cast<int>(tiles);

@@ -168,7 +168,7 @@ extern "C" int forge_qk_norm_rope(const uint16_t* q, const uint16_t* k, const ui
 {
     if (T <= 0 || D <= 0 || Hq < 0 || Hkv < 0 || Hq + Hkv == 0) return FORGE_OK;
     const bool cache = k_cache || v_cache;
-    if (D % 8 != 0 || D > 256 || R < 0 || R > D || R % 16 != 0 || Hq > 65535 || Hkv > 65535 || !positions ||
+    if (T > grid_limit(256) || D % 8 != 0 || D > 256 || R < 0 || R > D || R % 16 != 0 || Hq > 65535 || Hkv > 65535 || !positions ||
         (R > 0 && (!cos || !sin || table_rows <= 0)) || (Hq > 0 && (!q || !q_out)) || (Hkv > 0 && !k) ||
         (Hkv > 0 && !k_out && !cache) || (cache && (!k_cache || !v_cache || !v || !slots || cache_rows < 0)) ||
         (dtype != FORGE_FP16 && dtype != FORGE_BF16))

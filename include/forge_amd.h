@@ -339,7 +339,7 @@ int forge_int4_linear(const uint16_t* x, const uint8_t* w_int4, const uint16_t* 
  * of the FP32 tables cos, sin (table_rows, R/2); pair i is (y[i], y[i + R/2]), or (y[2i], y[2i + 1]) when
  * interleaved. A position outside the table gives NaN. q_out (T,Hq,D), contiguous; the keys go to k_out (T,Hkv,D)
  * and / or, with v (T,Hkv,D) as it is, to rows slots[t] of k_cache, v_cache (cache_rows, Hkv, D); a slot
- * outside 0..cache_rows-1 writes nothing. q_out may be q itself. */
+ * outside 0..cache_rows-1 writes nothing. q_out may be q itself. T is under 2^24. */
 int forge_qk_norm_rope(const uint16_t* q, const uint16_t* k, const uint16_t* v, const uint16_t* q_weight,
                        const uint16_t* k_weight, const float* cos, const float* sin, const int32_t* positions,
                        uint16_t* q_out, uint16_t* k_out, uint16_t* k_cache, uint16_t* v_cache,
