@@ -10,7 +10,7 @@
 // empty, or many places), or they are equal ones (a mask's lowest value): those above the bound are ranked and the first places that equal
 // it follow. Where a piece has more of those than LDS has room, its places are filled one after the other.
 //
-// us, pieces + merge: 32 x 8 beams of 131072 FP32 logits, three in ten ended, 18.4 (94 MB at 5.1 TB/s) + 8.2; 4 beams of 32000 FP16 4.6 + 5.7, two chains
+// us, pieces + merge: 32 x 8 beams of 131072 FP32 logits, three in ten ended, 18.5 (94 MB at 5.1 TB/s) + 8.5; 4 beams of 32000 FP16 4.6 + 5.5, two chains
 // of dependent steps. In all, 8 x 4 beams of 128000, 16 places: 15; all but 20 tokens at FP16's lowest value 20 (place after place 65), all logits
 // equal 41 (60); 4 x 8 of 50257, 53 places: 25 (ranking all that the first bound leaves 49), one live beam 25 (137), all equal 33 (433).
 #include "float16_types.h"

@@ -5,7 +5,8 @@
 // last ones zeros: word w holds values 8 w to 8 w + 7, of these value 2 i at bits 4 i and value 2 i + 1 at bits 16 + 4 i.
 // A page's KV head is one piece of P (32 U + 8) bytes, P = page size: P rows of a key's words; the values'
 // words, four positions' side by side (position / 4, word, position % 4); P times (key step, key lowest, value step,
-// value lowest). So a lane of cache4_attention has its operands of 16 positions in one 16-byte load each, and the pieces are read whole.
+// value lowest). So a lane of cache4_attention has 4 words of values, of 4 positions, in each of its 16-byte loads, and the U words of a key that it takes
+// lie side by side (in loads of 16 bytes where U is 4 or 8, of 8 where it is 2 or 6, of 4 where it is 3); the pieces are read whole.
 #pragma once
 
 #include "float16_types.h"

@@ -4,8 +4,8 @@
 // passes its largest value, and n = round_half_even((x - m) / s), at most 15 (0 where s is 0). A head that holds an infinity or NaN has none of
 // that: its s and m are NaN, and so is what reads it. Read: m + s n in FP32, rounded once.
 // Bound: memory; a lane has a word of 8 values of a key and its value, a workgroup one head of 8, 16 or 32 neighbouring tokens, whose words and
-// numbers then make whole cache lines. 16384 tokens of 8 heads of 128: written in 22.2 us (67 MB read of 20 KB rows, 18 MB written; 330 vector instructions a
-// wave are most of it), read in 14.6.
+// numbers then make whole cache lines. 16384 tokens of 8 heads of 128: written in 21.6 us (67 MB read of 20 KB rows, 18 MB written; 320 vector instructions a
+// wave are most of it), read in 14.9.
 #include "cache4.h"
 
 #include <algorithm>

@@ -7,9 +7,9 @@
 // its entry of -1 beside a length inside the page says to the next call: rows that would go on from it end there, since the page that they would
 // get is new, or was another row's. Counts are added to with integer atomics, whose order does not matter; everything else is in the rows' order.
 //
-// Bound: latency. Small tables and pools take one workgroup that holds all counts in LDS (4 rows of 40 entries 3.6 us), others two launches:
+// Bound: latency. Small tables and pools take one workgroup that holds all counts in LDS (4 rows of 40 entries 3.7 us), others two launches:
 // first, a workgroup looks at the rows (first children, places among the takers) while others copy the counts and list the free pages of 1024 pages
-// each; then a workgroup per row finds its page and writes its table (512 rows of 128 entries, 4000 pages, 3.7 + 3.6 us). copy_pages: memory; 8 tensors
+// each; then a workgroup per row finds its page and writes its table (512 rows of 128 entries, 4000 pages, 3.9 + 3.6 us). copy_pages: memory; 8 tensors
 // of 16 KB pages, some 300 pairs, 10.8 us.
 #include "common.h"
 

@@ -951,7 +951,8 @@ def cache4_attention(q: torch.Tensor, cache: torch.Tensor, page_table: torch.Ten
                      tree: Optional[torch.Tensor] = None, scale: Optional[float] = None,
                      workspace: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
     """forge_cache4_attention: cache_attention over a 4-bit cache (cache4_shape(pages, page size, Hkv, D)), with the same queries
-    (B, T, Hq, D), tables, lengths and trees. The new tokens' keys and values are in the cache already (cache4_write)."""
+    (B, T, Hq, D), tables, lengths and trees. The new tokens' keys and values are in the cache already (cache4_write). The keys are split
+    over workgroups by all sequences' lengths, so that a result's last bits can depend on the others of its batch."""
     if workspace is None and out is None and isinstance(q, torch.Tensor):
         made = _fast_new("cache4_attention_new", q, cache, page_table, cache_lens, tree, _scale_of(scale, q))
         if made is not None:
