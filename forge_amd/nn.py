@@ -387,9 +387,11 @@ class PagedBeams:
         """The rows' next tokens from logits (requests, beams, tokens) of their newest ones, and the rows behind them: returns
         tokens and beams (requests, beams) int32, -1 where a request has fewer continuations. caches: the tensors whose pages the rows share. Without an end_token every row
         goes on, and none has ended afterwards."""
-        for cache in caches[:1]:                    # (copy_pages wants the others to be like it)
-            if cache.shape[0] != self.refs.shape[0]:
-                raise ValueError(f"the caches have {cache.shape[0]} pages, the beams' rows {self.refs.shape[0]}")
+        if not isinstance(caches, (list, tuple)):
+            caches = list(caches)
+        # (copy_pages wants the others to be like the first, and tensors)
+        if caches and isinstance(caches[0], torch.Tensor) and caches[0].shape[:1] != self.refs.shape:
+            raise ValueError(f"the caches must have {self.refs.shape[0]} pages, got {tuple(caches[0].shape)}")
         lens, scores = self.lens, self.scores
         if self._written:
             stored = self.slots >= 0

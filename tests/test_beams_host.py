@@ -28,6 +28,10 @@ def test_other_pages():
     for pages in (9, 11):
         with pytest.raises(ValueError, match="pages"):
             b.step(torch.zeros((2, 3, 9)), [torch.zeros((pages, 4)), torch.zeros((10, 4))])
+        with pytest.raises(ValueError, match="pages"):
+            b.step(torch.zeros((2, 3, 9)), {0: torch.zeros((pages, 4))}.values())
+    with pytest.raises(ValueError, match="device"):                  # (as far as the operators)
+        b.step(torch.zeros((2, 3, 9)), (torch.zeros((10, 4)) for _ in range(2)))
 
 
 def test_limits():

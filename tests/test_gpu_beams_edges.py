@@ -27,7 +27,7 @@ def test_no_rows(dev):
     assert torch.equal(out.refs, refs)
     beams = PagedBeams(0, 3, 50, 16, 40, dev)
     assert beams.start([]).shape == (0,)
-    tokens, parents = beams.step(torch.zeros((0, 3, 9), device=dev), [torch.zeros((50, 4), device=dev)], 2)
+    tokens, parents = beams.step(torch.zeros((0, 3, 9), device=dev), {0: torch.zeros((50, 4), device=dev)}.values(), 2)
     assert tokens.shape == parents.shape == (0, 3) and (beams.refs == 0).all()
 
 
