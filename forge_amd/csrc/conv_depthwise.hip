@@ -364,7 +364,7 @@ static int launch_dw_rows(const uint16_t* input, const int8_t* weight, const uin
     while (R > 8 && planes * col_waves * divup(Ho, R) < 4096) R >>= 1;
     const int strips = divup(Ho, R);
     const long long waves = planes * col_waves * strips;
-    if (waves > 0x7FFFFFFFLL - 3) return FORGE_EINVAL;
+    if (divupll(waves, 4) > grid_limit(256)) return FORGE_EINVAL;
     const unsigned blocks = static_cast<unsigned>(divupll(waves, 4));
     const int vec = (Wo % 8 == 0 && aligned(output, 16)) ? 1 : 0;
     depthwise_rows_kernel<KH, KW, PW><<<blocks, 256, 0, s>>>(input, weight, w_scale, bias, output, C, H, W, padH,
@@ -442,7 +442,7 @@ extern "C" int forge_int8_depthwise_conv2d_forward(const uint16_t* input, const 
     if (unit && kH <= kDwMaxKH && kW <= kDwMaxKW) {
         const int tiles_h = divup(Ho, kDwTileH), tiles_w = divup(Wo, kDwTileW);
         const long long blocks = planes * tiles_h * tiles_w;
-        if (blocks <= 0x7FFFFFFFLL) {
+        if (blocks <= grid_limit(256)) {
             const int vec = (Wo % kDwPer == 0 && aligned(output, 16)) ? 1 : 0;
             depthwise_tile_kernel<<<static_cast<unsigned>(blocks), 256, 0, s>>>(
                 input, weight, w_scale, bias, output, C, H, W, kH, kW, padH, padW, Ho, Wo, tiles_h, tiles_w, vec);

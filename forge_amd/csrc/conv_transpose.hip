@@ -275,7 +275,7 @@ static int launch_convt_fused(const uint16_t* input, const int8_t* weight, const
 {
     const int tiles = divup(HW, 32);
     const long long blocks = static_cast<long long>(N) * tiles;
-    if (blocks > 0x7FFFFFFFLL) return FORGE_EINVAL;
+    if (blocks > grid_limit(128)) return FORGE_EINVAL;
     convt_fused_kernel<KC><<<static_cast<unsigned>(blocks), 128, 0, s>>>(input, weight, w_scale, bias, output, HW, W,
                                                                         C_out, tiles);
     return launch_status();

@@ -351,7 +351,7 @@ static int launch_quantize_rows(const uint16_t* x, int8_t* q, float* scales, int
     return launch_status();
 }
 
-int launch_quantize(const uint16_t* x, int8_t* q, float* scales, int M, int K, hipStream_t s)
+static int launch_quantize_part(const uint16_t* x, int8_t* q, float* scales, int M, int K, hipStream_t s)
 {
     // Rows under 8 values, and those past the registers, take the two-pass kernel.
     if (K < 8 || K > 8 * 2048) {
@@ -363,12 +363,24 @@ int launch_quantize(const uint16_t* x, int8_t* q, float* scales, int M, int K, h
     return launch_quantize_rows<false>(x, q, scales, M, K, s);
 }
 
+int launch_quantize(const uint16_t* x, int8_t* q, float* scales, int M, int K, hipStream_t s)
+{
+    // As many rows at a time as a grid holds, of a workgroup each at most.
+    constexpr int kRows = 1 << 23;
+    static_assert(kRows <= grid_limit(256), "a launch");
+    for (long long m = 0; m < M; m += kRows) {
+        const int st = launch_quantize_part(x + m * K, q + m * K, scales + m, static_cast<int>(std::min<long long>(kRows, M - m)), K, s);
+        if (st != FORGE_OK) return st;
+    }
+    return FORGE_OK;
+}
+
 int launch_quantize_pixels_nchw(const uint16_t* x, int8_t* q, float* scales, int images, int C, int HW,
                                 hipStream_t s)
 {
     const int tiles = divup(HW, kPixTile);
     const long long blocks = static_cast<long long>(images) * tiles;
-    if (blocks > 0x7FFFFFFFLL) return FORGE_EINVAL;
+    if (blocks > grid_limit(256)) return FORGE_EINVAL;
     const bool g4 = (C % 4 == 0) && aligned(q, 4);
     const bool stash = C <= kPixStashMaxC;
     const size_t lds = stash ? static_cast<size_t>(kPixTile) * (C + 4) * sizeof(uint16_t) : 0;
@@ -406,7 +418,7 @@ extern "C" int forge_quantize_activation_twopass(const uint16_t* x, int8_t* q, f
                                                  int M, int K, int threads, void* stream)
 {
     if (M <= 0 || K <= 0) return FORGE_OK;
-    if (!x || !q || !scales || threads < 1 || threads > 1024) return FORGE_EINVAL;
+    if (!x || !q || !scales || threads < 1 || threads > 1024 || M > grid_limit(threads)) return FORGE_EINVAL;
     forge::quant::fused_quantize_activation_kernel<<<M, threads, 0, as_stream(stream)>>>(
         reinterpret_cast<const __half*>(x), q, scales, K);
     return launch_status();
@@ -427,6 +439,7 @@ extern "C" int forge_dequantize_bias(const int32_t* acc, const float* act_scale,
                                                      w_scale, bias, reinterpret_cast<uint2*>(out),
                                                      static_cast<uint32_t>(N / 4), static_cast<uint32_t>(total4));
     } else {
+        if (M > grid_limit(256)) return FORGE_EINVAL;
         forge::quant::fused_dequantize_bias_kernel<<<M, 256, 0, s>>>(
             acc, act_scale, reinterpret_cast<const __half*>(w_scale),
             reinterpret_cast<const __half*>(bias), reinterpret_cast<__half*>(out), N);

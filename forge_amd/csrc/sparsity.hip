@@ -381,6 +381,7 @@ extern "C" int forge_prune_compress_24(const int8_t* w, int8_t* comp, uint8_t* m
                                                         reinterpret_cast<uint2*>(comp),
                                                         reinterpret_cast<uint32_t*>(meta_raw), n16);
     } else {
+        if (divupll(groups, 256) > grid_limit(256)) return FORGE_EINVAL;
         forge::sparsity::prune_compress_kernel<<<static_cast<unsigned>(divupll(groups, 256)), 256, 0, s>>>(
             w, comp, meta_raw, N, K);
     }
@@ -397,6 +398,7 @@ extern "C" int forge_pack_metadata(const uint8_t* meta_raw, uint32_t* meta_packe
         pack_metadata_out_kernel<<<static_cast<unsigned>(divupll(total, 256)), 256, 0, as_stream(stream)>>>(
             meta_raw, meta_packed, N, K);
     } else {
+        if (divupll(total, 256) > grid_limit(256)) return FORGE_EINVAL;
         forge::sparsity::pack_metadata_kernel<<<static_cast<unsigned>(divupll(total, 256)), 256, 0,
                                                 as_stream(stream)>>>(meta_raw, meta_packed, N, K);
     }
@@ -418,7 +420,7 @@ extern "C" int forge_quantize_weight_rows(const void* w, int w_fp16, int8_t* w_i
                                           void* stream)
 {
     if (N <= 0 || K <= 0) return FORGE_OK;
-    if (!w || !w_int8 || !w_scale) return FORGE_EINVAL;
+    if (!w || !w_int8 || !w_scale || N > grid_limit(256)) return FORGE_EINVAL;
     hipStream_t s = as_stream(stream);
     if (K % 16 == 0 && K <= 4096 && aligned(w, 16) && aligned(w_int8, 16)) {
         if (w_fp16) quantize_weight_rows_vec_kernel<true><<<N, 256, 0, s>>>(w, w_int8, w_scale, K);
@@ -435,7 +437,7 @@ extern "C" int forge_prepare_sparse_weight(const void* w, int w_fp16, int8_t* W_
                                            uint16_t* w_scale, int N, int K, void* stream)
 {
     if (N <= 0 || K <= 0) return FORGE_OK;
-    if (!w || !W_comp || !w_meta || !w_scale || K % 32 != 0 || !aligned(w, 16) || !aligned(W_comp, 16) ||
+    if (!w || !W_comp || !w_meta || !w_scale || N > grid_limit(256) || K % 32 != 0 || !aligned(w, 16) || !aligned(W_comp, 16) ||
         !aligned(w_meta, 4))
         return FORGE_EINVAL;
     hipStream_t s = as_stream(stream);
